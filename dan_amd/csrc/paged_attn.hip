@@ -1,0 +1,571 @@
+// Attention of one new token per sequence over a paged key-value cache on
+// gfx950 (MI355X, CDNA4):  o = sum_j e^{s_j} v_j / sum_j e^{s_j},  s_j = scale q . k_j,
+// over the sequence's first lens[b] keys.
+//
+// HBM-bound: every key and value row is read once. The work is split over
+// (sequence, kv head, range of keys): a work group of 4 waves takes one range, its
+// waves every fourth tile of 32 keys, each with a running maximum and sum of its
+// own; the work group joins them in LDS, and where a sequence spans several
+// ranges a second launch joins those.
+//
+// A tile never passes through LDS. On the matrix core (16 x 16 x 32):
+//   S^T [16 keys x 16 heads] = K [keys x D] Q^T: a lane loads 16 bytes of one key row per
+//     step of 32 dims; the q heads of one kv head (up to 16) are the columns, so grouped
+//     heads cost no second read of the keys;
+//   O^T [D x 16 heads] += V^T [D x 32 keys] P^T: a lane loads D / 16 consecutive dims of
+//     8 keys and takes the transpose in registers (one byte permute for two values).
+// The keys of a lane's 8 contraction slots are the keys whose scores the same lane holds
+// (4 g .. 4 g + 3 of both halves of the tile, g = lane / 16), so P goes from the score
+// registers to the operand without an exchange. P is split into a rounded part and the
+// rounded rest, two products: the output then has the precision of fp32 weights
+// (one rounding of P to bf16 costs about as much as the rounding of the output).
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "cus.h"
+#include "dan_paged.h"
+#include "paged_index.h"
+
+namespace dan {
+int fail(int status, const char *fmt, ...);  // tree_attn.hip: sets the thread's last-error message
+bool finite_positive(float x);                // tree_attn.hip: decided from the float's bits
+extern thread_local char g_err[512];
+}  // namespace dan
+
+namespace dan_pattn {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+#define DAN_GLOBAL __attribute__((address_space(1)))
+
+constexpr int kWaves = 4, kTile = 32, kHeads = 16;
+constexpr int kMaxLen = 1 << 30;  // places are 32-bit
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <typename T>
+struct Ops;
+template <>
+struct Ops<__bf16> {
+  typedef bf16x8 x8;
+  typedef bf16x4 x4;
+  typedef bf16x2 x2;
+  static __device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  template <bool HI>
+  static __device__ inline uint32_t from_e4m3(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  }
+};
+template <>
+struct Ops<_Float16> {
+  typedef f16x8 x8;
+  typedef f16x4 x4;
+  typedef f16x2 x2;
+  static __device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
+  }
+  template <bool HI>
+  static __device__ inline uint32_t from_e4m3(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+  }
+};
+
+// Two fp32 values as one register of T, rounded to nearest even, and back.
+template <typename T>
+__device__ inline uint32_t pack2(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, typename Ops<T>::x2));
+}
+template <typename T>
+__device__ inline f32x2 unpack2(uint32_t w) {
+  return __builtin_convertvector(__builtin_bit_cast(typename Ops<T>::x2, w), f32x2);
+}
+
+// A maximum that keeps a NaN out (v_max_f32): NaN scores reach the sum through their weights.
+__device__ inline float max_across_groups(float x) {  // over the 4 lanes of one head (lane % 16)
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ inline float sum_across_groups(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+struct Params {
+  const void *q, *kc, *vc;
+  void *out;
+  float *lse;
+  float *part;  // [B * H, splits, D] unnormalized outputs, then [B * H, splits, 2] (maximum in log2 units, sum)
+  const float *ks, *vs;
+  dan::PageTable table;
+  const int32_t *lens;
+  int64_t q_ss, q_sh, o_ss, o_sh, kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
+  int32_t B, H, Hkv, G, max_len, chunk, splits, blocks;
+  float scale;
+};
+
+// The keys of sequence b, or -1 where its length is none the launch covers.
+__device__ inline int length_of(const Params &p, int b) {
+  const int n = p.lens[b];
+  return (uint32_t)n <= (uint32_t)p.max_len ? n : -1;
+}
+
+template <typename T, int D, bool FP8>
+struct Tile {
+  static constexpr int VE = D / 16;        // dims of a lane's value rows
+  static constexpr int ES = FP8 ? 1 : 2;   // bytes of a cached value
+  static constexpr int KR = D / 32 * (FP8 ? 2 : 4);  // registers of a 16-key block's K operand, as loaded
+  static constexpr int VR = VE * ES / 4;   // registers of one value row, as loaded
+  uint32_t k[2][KR];
+  uint32_t v[2][4][VR];
+};
+
+// The dim of element j of lane i's (i = lane % 16) piece of a value row. A bf16 row of 256
+// dims is loaded as two 16-byte pieces half a row apart.
+template <int D, bool FP8>
+__device__ inline int value_dim(int i, int j) {
+  if constexpr (D == 256 && !FP8) return (j >> 3) * 128 + 8 * i + (j & 7);
+  else return D / 16 * i + j;
+}
+
+template <typename T, int D, bool FP8>
+__device__ inline void load_k(Tile<T, D, FP8> &t, int u, const uint8_t *base, uint32_t off) {
+  // bf16/fp16: per step of 32 dims 16 bytes at dim 32 s + 8 g; e4m3: per two steps 16 bytes at dim 64 s + 16 g
+#pragma unroll
+  for (int s = 0; s < Tile<T, D, FP8>::KR / 4; ++s) {
+    const u32x4 x = *(const DAN_GLOBAL u32x4 *)(base + off + 64 * s);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) t.k[u][4 * s + c] = x[c];
+  }
+}
+
+template <typename T, int D, bool FP8>
+__device__ inline void load_v(Tile<T, D, FP8> &t, int u, const uint8_t *base, uint32_t off, uint32_t row) {
+  constexpr int VR = Tile<T, D, FP8>::VR;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint8_t *p = base + off + r * row;
+    if constexpr (VR == 8) {
+      const u32x4 a = *(const DAN_GLOBAL u32x4 *)p, b = *(const DAN_GLOBAL u32x4 *)(p + 256);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        t.v[u][r][c] = a[c];
+        t.v[u][r][4 + c] = b[c];
+      }
+    } else if constexpr (VR == 4) {
+      const u32x4 a = *(const DAN_GLOBAL u32x4 *)p;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) t.v[u][r][c] = a[c];
+    } else if constexpr (VR == 2) {
+      const u32x2 a = *(const DAN_GLOBAL u32x2 *)p;
+      t.v[u][r][0] = a[0];
+      t.v[u][r][1] = a[1];
+    } else {
+      t.v[u][r][0] = *(const DAN_GLOBAL uint32_t *)p;
+    }
+  }
+}
+
+// The operand of 32 dims (step s) of a key block.
+template <typename T, int D, bool FP8>
+__device__ inline u32x4 k_operand(const Tile<T, D, FP8> &t, int u, int s) {
+  if constexpr (!FP8) {
+    return (u32x4){t.k[u][4 * s], t.k[u][4 * s + 1], t.k[u][4 * s + 2], t.k[u][4 * s + 3]};
+  } else {
+    const uint32_t a = t.k[u][2 * s], b = t.k[u][2 * s + 1];
+    return (u32x4){Ops<T>::template from_e4m3<false>(a), Ops<T>::template from_e4m3<true>(a), Ops<T>::template from_e4m3<false>(b),
+                   Ops<T>::template from_e4m3<true>(b)};
+  }
+}
+
+// Elements 2 m and 2 m + 1 of a value row.
+template <typename T, int D, bool FP8>
+__device__ inline uint32_t v_pair(const Tile<T, D, FP8> &t, int u, int r, int m) {
+  if constexpr (!FP8) return t.v[u][r][m];
+  else return m & 1 ? Ops<T>::template from_e4m3<true>(t.v[u][r][m >> 1]) : Ops<T>::template from_e4m3<false>(t.v[u][r][m >> 1]);
+}
+
+template <typename T, int D, bool FP8>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
+  typedef Tile<T, D, FP8> Tl;
+  constexpr int VE = Tl::VE, ES = Tl::ES, DP = D + 4;  // DP: a head's row in LDS
+  extern __shared__ __align__(16) float lds[];  // [waves][heads][DP], then maxima and sums [waves][heads]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  // (kv head, block of 16 q heads) fastest, then the sequence, then the range
+  uint32_t at = blockIdx.x;
+  const int hb = at % p.blocks;
+  at /= p.blocks;
+  const int hk = at % p.Hkv;
+  at /= p.Hkv;
+  const int b = at % p.B, split = at / p.B;
+  const int len = length_of(p, b), lo = split * p.chunk;
+  const int heads = min(p.G - hb * kHeads, kHeads);  // of this block
+  const int head0 = hk * p.G + hb * kHeads;
+  const bool direct = p.splits == 1;
+  if (lo >= len) {  // nothing here: the join leaves such ranges out (and takes wrong lengths to NaN)
+    if (direct) {
+      const float none = len < 0 ? __builtin_nanf("") : 0.0f;
+      for (int e = threadIdx.x; e < heads * D; e += 256) {
+        static_cast<T *>(p.out)[b * p.o_ss + (head0 + e / D) * p.o_sh + e % D] = (T)none;
+        if (p.lse && e % D == 0) p.lse[(int64_t)b * p.H + head0 + e / D] = len < 0 ? none : -INFINITY;
+      }
+    }
+    return;
+  }
+  const int hi = min(len, lo + p.chunk);
+  const int tiles = (hi - lo + kTile - 1) / kTile;
+  const int mine = wave < tiles ? (tiles - wave + kWaves - 1) / kWaves : 0;
+
+  f32x4 acc[VE];
+#pragma unroll
+  for (int j = 0; j < VE; ++j) acc[j] = (f32x4){0, 0, 0, 0};
+  float m = -INFINITY, l = 0.f;
+  uint64_t bad = 0;
+
+  if (mine > 0) {
+    // q: column i is head min(i, heads - 1); dims as the key operand has them
+    u32x4 qf[D / 32];
+    {
+      const T *qrow = static_cast<const T *>(p.q) + b * p.q_ss + (head0 + min(i, heads - 1)) * p.q_sh;
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) {
+        const int dim = FP8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+        qf[s] = *(const DAN_GLOBAL u32x4 *)(qrow + dim);
+      }
+    }
+    float c = p.scale * kLog2e;
+    if constexpr (FP8) c *= *p.ks;
+    const uint32_t krow = (uint32_t)(p.kc_st * ES), vrow = (uint32_t)(p.vc_st * ES);
+    const uint32_t koff = i * krow + 16 * g;
+    const uint32_t voff = 4 * g * vrow + (D == 256 && !FP8 ? 16 * i : VE * ES * i);
+
+    // Lane n holds where this wave's 16-key block n (of the next 64) starts in the two caches.
+    uint64_t kadr = 0, vadr = 0;
+    auto find_pages = [&](int first) {
+      const int n = first + (lane >> 1);  // the tile
+      const int key = lo + kTile * (wave + kWaves * n) + 16 * (lane & 1);
+      const bool there = n < mine && key < hi;
+      // Page 0 stands in for a block behind the end and for a page that does not exist. A block starts
+      // at a multiple of 16 rows, as a page's size is one, so all 16 lie in the page.
+      dan::PageRow from = there ? dan::find_row(p.table, b, key) : dan::PageRow{0, 0};
+      bad |= __ballot(from.page < 0);
+      if (from.page < 0) from = {0, 0};
+      kadr = (uint64_t)p.kc + (from.page * p.kc_sp + hk * p.kc_sh + from.row * p.kc_st) * ES;
+      vadr = (uint64_t)p.vc + (from.page * p.vc_sp + hk * p.vc_sh + from.row * p.vc_st) * ES;
+    };
+    auto at_lane = [&](uint64_t x, int n) -> const uint8_t * {
+      const uint32_t a = __builtin_amdgcn_readlane((uint32_t)x, n), h = __builtin_amdgcn_readlane((uint32_t)(x >> 32), n);
+      return (const uint8_t *)((uint64_t)h << 32 | a);
+    };
+    Tl t;
+    auto fetch_k = [&](int n) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) load_k<T, D, FP8>(t, u, at_lane(kadr, 2 * (n & 31) + u), koff);
+    };
+    auto fetch_v = [&](int n) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) load_v<T, D, FP8>(t, u, at_lane(vadr, 2 * (n & 31) + u), voff, vrow);
+    };
+
+    find_pages(0);
+    fetch_k(0);
+    fetch_v(0);
+    for (int n = 0; n < mine; ++n) {
+      const int key0 = lo + kTile * (wave + kWaves * n);
+      // scores of keys key0 + 16 u + 4 g + r and head i
+      f32x4 sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        sc[u] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) sc[u] = Ops<T>::mfma(k_operand<T, D, FP8>(t, u, s), qf[s], sc[u]);
+      }
+      const bool more = n + 1 < mine;
+      if (more) {
+        if (((n + 1) & 31) == 0) find_pages(n + 1);
+        fetch_k(n + 1);
+      }
+      if (key0 + kTile > hi) {  // the sequence's last tile: no weight, and no value either, behind its end
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (key0 + 16 * u + 4 * g + r >= hi) {
+              sc[u][r] = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < Tl::VR; ++e) t.v[u][r][e] = 0;
+            }
+      }
+      float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      top = max_across_groups(top) * c;
+      if (__any(top > m)) {
+        const float to = fmaxf(m, top);
+        const float by = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= by;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) acc[j] *= by;
+      }
+      const float sub = m == -INFINITY ? 0.0f : m;
+      u32x4 ph, pl;  // P rounded, and what the rounding left
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][r], c, -sub));
+          l += w[r];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = pack2<T>(w[2 * h], w[2 * h + 1]);
+          const f32x2 y = unpack2<T>(x);
+          ph[2 * u + h] = x;
+          pl[2 * u + h] = pack2<T>(w[2 * h] - y[0], w[2 * h + 1] - y[1]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VE / 2; ++e) {
+        uint32_t row[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) row[u][r] = v_pair<T, D, FP8>(t, u, r, e);
+        u32x4 even, odd;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            even[2 * u + h] = __builtin_amdgcn_perm(row[u][2 * h + 1], row[u][2 * h], 0x05040100);
+            odd[2 * u + h] = __builtin_amdgcn_perm(row[u][2 * h + 1], row[u][2 * h], 0x07060302);
+          }
+        acc[2 * e] = Ops<T>::mfma(even, pl, acc[2 * e]);
+        acc[2 * e] = Ops<T>::mfma(even, ph, acc[2 * e]);
+        acc[2 * e + 1] = Ops<T>::mfma(odd, pl, acc[2 * e + 1]);
+        acc[2 * e + 1] = Ops<T>::mfma(odd, ph, acc[2 * e + 1]);
+      }
+      if (more) fetch_v(n + 1);
+    }
+    l = sum_across_groups(l);
+    if (bad) l = __builtin_nanf("");
+  }
+
+  // The waves' results into LDS: lane (i, g) holds head i, value lanes 4 g .. 4 g + 3.
+  float *ml = lds + kWaves * heads * DP;
+  if (i < heads) {
+    float *row = lds + (wave * heads + i) * DP;
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+      for (int j = 0; j < VE; j += 4) {
+        const f32x4 x = {acc[j][rr], acc[j + 1][rr], acc[j + 2][rr], acc[j + 3][rr]};
+        *(f32x4 *)(row + value_dim<D, FP8>(4 * g + rr, j)) = x;
+      }
+    if (g == 0) {
+      ml[wave * heads + i] = m;
+      ml[(kWaves + wave) * heads + i] = l;
+    }
+  }
+  __syncthreads();
+  float vscale = 1.0f;
+  if constexpr (FP8) vscale = *p.vs;
+  for (int e = threadIdx.x * 4; e < heads * D; e += 1024) {
+    const int h = e / D, d = e % D;
+    float mw[kWaves], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      mw[w] = ml[w * heads + h];
+      top = fmaxf(top, mw[w]);
+    }
+    const float sub = top == -INFINITY ? 0.0f : top;
+    f32x4 o = {0, 0, 0, 0};
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float by = __builtin_amdgcn_exp2f(mw[w] - sub);
+      sum += by * ml[(kWaves + w) * heads + h];
+      o += by * *(const f32x4 *)(lds + (w * heads + h) * DP + d);
+    }
+    const int64_t row = (int64_t)b * p.H + head0 + h;
+    if (direct) {
+      const float inv = vscale / sum;
+      typename Ops<T>::x4 y = __builtin_convertvector(o * inv, typename Ops<T>::x4);
+      *(DAN_GLOBAL u32x2 *)(static_cast<T *>(p.out) + b * p.o_ss + (head0 + h) * p.o_sh + d) = __builtin_bit_cast(u32x2, y);
+      if (p.lse && d == 0) p.lse[row] = sub * kLn2 + logf(sum);
+    } else {
+      *(DAN_GLOBAL f32x4 *)(p.part + (row * p.splits + split) * D + d) = o * vscale;
+      if (d == 0) {
+        float *s = p.part + (int64_t)p.B * p.H * p.splits * D + (row * p.splits + split) * 2;
+        s[0] = top;
+        s[1] = sum;
+      }
+    }
+  }
+}
+
+// One work group joins the ranges of a (sequence, head).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
+  constexpr int L = D / 4, GR = 256 / L;  // lanes of a row, rows at a time
+  __shared__ float part[GR][D];
+  __shared__ float sums[GR];
+  const int64_t row = blockIdx.x;
+  const int b = row / p.H, h = row % p.H;
+  const int len = length_of(p, b);
+  const int n = len <= 0 ? 0 : (len + p.chunk - 1) / p.chunk;
+  const float *ml = p.part + (int64_t)p.B * p.H * p.splits * D + row * p.splits * 2;
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY;
+  for (int s = lane; s < n; s += 64) top = fmaxf(top, ml[2 * s]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float sub = top == -INFINITY ? 0.0f : top;
+  const int gr = threadIdx.x / L, d = threadIdx.x % L * 4;
+  f32x4 o = {0, 0, 0, 0};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = gr; s < n; s += GR) {
+    const float by = __builtin_amdgcn_exp2f(ml[2 * s] - sub);
+    sum += by * ml[2 * s + 1];
+    o += by * *(const DAN_GLOBAL f32x4 *)(p.part + (row * p.splits + s) * D + d);
+  }
+  *(f32x4 *)&part[gr][d] = o;
+  if (d == 0) sums[gr] = sum;
+  __syncthreads();
+  if (threadIdx.x < L) {
+    o = (f32x4){0, 0, 0, 0};
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < GR; ++w) {
+      o += *(const f32x4 *)&part[w][d];
+      sum += sums[w];
+    }
+    const float inv = len > 0 ? 1.0f / sum : len == 0 ? 0.0f : __builtin_nanf("");
+    typename Ops<T>::x4 y = __builtin_convertvector(o * inv, typename Ops<T>::x4);
+    *(DAN_GLOBAL u32x2 *)(static_cast<T *>(p.out) + b * p.o_ss + h * p.o_sh + d) = __builtin_bit_cast(u32x2, y);
+    if (p.lse && d == 0) p.lse[row] = len > 0 ? sub * kLn2 + logf(sum) : len == 0 ? -INFINITY : __builtin_nanf("");
+  }
+}
+
+// How a launch is split over the keys: ranges of `chunk` keys (whole rounds of the
+// work group's waves), `splits` of them up to max_len.
+struct Split {
+  int chunk, splits;
+};
+Split split_of(int64_t groups, int max_len, int cus) {
+  const int round = kWaves * kTile;
+  const int64_t want = 2 * (int64_t)(cus > 0 ? cus : 256);  // work groups resident at once, two per CU
+  if (groups < 1) groups = 1;  // no sequences
+  int64_t splits = (want + groups - 1) / groups;
+  int64_t chunk = (max_len + splits - 1) / splits;
+  chunk = (chunk + round - 1) / round * round;
+  if (chunk < round) chunk = round;
+  if (chunk > 1024) chunk = 1024;
+  splits = max_len > 0 ? (max_len + chunk - 1) / chunk : 1;
+  return {(int)chunk, (int)splits};
+}
+
+template <typename T, int D, bool FP8>
+void launch(const Params &p, hipStream_t s) {
+  const int heads = p.G < kHeads ? p.G : kHeads;
+  const size_t bytes = sizeof(float) * kWaves * heads * (D + 4 + 2);
+  const unsigned grid = (unsigned)((int64_t)p.splits * p.B * p.Hkv * p.blocks);
+  hipLaunchKernelGGL((paged_attn_kernel<T, D, FP8>), dim3(grid), dim3(256), bytes, s, p);
+  if (p.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)((int64_t)p.B * p.H)), dim3(256), 0, s, p);
+}
+
+template <typename T>
+void by_dim(const Params &p, int d, bool fp8, hipStream_t s) {
+  if (d == 64) fp8 ? launch<T, 64, true>(p, s) : launch<T, 64, false>(p, s);
+  else if (d == 128) fp8 ? launch<T, 128, true>(p, s) : launch<T, 128, false>(p, s);
+  else fp8 ? launch<T, 256, true>(p, s) : launch<T, 256, false>(p, s);
+}
+
+}  // namespace dan_pattn
+
+extern "C" {
+
+int64_t dan_paged_attn_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_len) {
+  using namespace dan_pattn;
+  if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || max_len < 0 || max_len > kMaxLen ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return -1;
+  const int64_t blocks = (num_heads / num_kv_heads + kHeads - 1) / kHeads;
+  const Split sp = split_of((int64_t)num_seqs * num_kv_heads * blocks, max_len, dan::num_cus());
+  return sp.splits > 1 ? (int64_t)num_seqs * num_heads * sp.splits * (head_dim + 2) * 4 : 0;
+}
+
+int dan_paged_attn(const DanPagedAttnArgs *a, void *stream) {
+  using namespace dan_pattn;
+  using dan::fail;
+  dan::g_err[0] = 0;
+  if (!a) return fail(DAN_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->abi_version != DAN_PAGED_ABI_VERSION)
+    return fail(DAN_ERR_VERSION, "abi_version %d, paged cache speaks %d", a->abi_version, DAN_PAGED_ABI_VERSION);
+  const int B = a->num_seqs, H = a->num_heads, Hkv = a->num_kv_heads, D = a->head_dim;
+  if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "need num_seqs >= 0 and num_heads %d a positive multiple of num_kv_heads %d", H, Hkv);
+  if (D != 64 && D != 128 && D != 256) return fail(DAN_ERR_UNSUPPORTED, "head_dim %d: only 64, 128 and 256 are built", D);
+  if (a->dtype != DAN_DTYPE_BF16 && a->dtype != DAN_DTYPE_F16) return fail(DAN_ERR_UNSUPPORTED, "dtype %d: bf16 or f16", a->dtype);
+  const bool fp8 = a->cache_dtype == DAN_DTYPE_E4M3;
+  const int es = fp8 ? 1 : 2;
+  if (!fp8 && a->cache_dtype != a->dtype) return fail(DAN_ERR_UNSUPPORTED, "cache_dtype %d: dtype's own or e4m3", a->cache_dtype);
+  if (a->page_size <= 0 || a->page_size % DAN_PAGED_KEY_BLOCK)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "page_size %d must be a positive multiple of %d", a->page_size, DAN_PAGED_KEY_BLOCK);
+  if (a->num_pages < 0 || a->table_width < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "num_pages and table_width must be >= 0");
+  if (a->max_len < 0 || a->max_len > kMaxLen || a->max_len > (int64_t)a->table_width * a->page_size)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "max_len %d: the table holds %lld keys a sequence", a->max_len, (long long)a->table_width * a->page_size);
+  if (!dan::finite_positive(a->scale)) return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+  if (B == 0) return DAN_OK;
+  if (!a->q || !a->out || !a->lens) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  if (a->max_len > 0 && (!a->k_cache || !a->v_cache || !a->table || a->num_pages == 0))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "a max_len of %d needs a cache with pages and a table", a->max_len);
+  if (fp8 && (!a->k_scale || !a->v_scale)) return fail(DAN_ERR_INVALID_ARGUMENT, "an e4m3 cache needs k_scale and v_scale");
+  for (int64_t st : {a->q_stride_seq, a->q_stride_head, a->o_stride_seq, a->o_stride_head})
+    if (st % 8) return fail(DAN_ERR_INVALID_ARGUMENT, "strides must be multiples of 8 elements (16-byte rows)");
+  for (int64_t st : {a->kc_stride_page, a->kc_stride_head, a->kc_stride_tok, a->vc_stride_page, a->vc_stride_head, a->vc_stride_tok})
+    if (st * es % 16) return fail(DAN_ERR_INVALID_ARGUMENT, "cache strides must be multiples of 16 bytes");
+  for (int64_t st : {a->kc_stride_tok, a->vc_stride_tok})  // offsets inside a 16-key block are 32-bit
+    if (st < D || st > (1 << 26)) return fail(DAN_ERR_INVALID_ARGUMENT, "cache token strides must lie in [head_dim, 2^26]");
+  const void *ptrs[] = {a->q, a->out, a->k_cache, a->v_cache, a->workspace};
+  for (const void *ptr : ptrs)
+    if ((uintptr_t)ptr & 15) return fail(DAN_ERR_INVALID_ARGUMENT, "tensor pointers must be 16-byte aligned");
+
+  Params p;
+  p.q = a->q; p.kc = a->k_cache; p.vc = a->v_cache; p.out = a->out; p.lse = a->lse; p.part = static_cast<float *>(a->workspace);
+  p.ks = a->k_scale; p.vs = a->v_scale; p.table = {a->table, a->table_stride, B, a->table_width, a->page_size, a->num_pages}; p.lens = a->lens;
+  p.q_ss = a->q_stride_seq; p.q_sh = a->q_stride_head; p.o_ss = a->o_stride_seq; p.o_sh = a->o_stride_head;
+  p.kc_sp = a->kc_stride_page; p.kc_sh = a->kc_stride_head; p.kc_st = a->kc_stride_tok;
+  p.vc_sp = a->vc_stride_page; p.vc_sh = a->vc_stride_head; p.vc_st = a->vc_stride_tok;
+  p.B = B; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
+  p.max_len = a->max_len; p.blocks = (p.G + kHeads - 1) / kHeads; p.scale = a->scale;
+  const Split sp = split_of((int64_t)B * Hkv * p.blocks, a->max_len, dan::num_cus());
+  p.chunk = sp.chunk; p.splits = sp.splits;
+  if ((int64_t)sp.splits * B * Hkv * p.blocks >= (int64_t)1 << 31 || (int64_t)B * H >= (int64_t)1 << 31)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "too many work groups");
+  if (sp.splits > 1) {
+    const int64_t need = (int64_t)B * H * sp.splits * (D + 2) * 4;
+    if (!a->workspace || a->workspace_bytes < need)
+      return fail(DAN_ERR_INVALID_ARGUMENT, "workspace of %lld bytes, needs %lld", (long long)a->workspace_bytes, (long long)need);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->dtype == DAN_DTYPE_BF16) by_dim<__bf16>(p, D, fp8, s);
+  else by_dim<_Float16>(p, D, fp8, s);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "paged attention launch failed: %s", hipGetErrorString(err));
+  return DAN_OK;
+}
+
+}  // extern "C"

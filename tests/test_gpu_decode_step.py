@@ -1,0 +1,183 @@
+"""The decode step's operators together: append_paged, attend_paged, token_logprobs, as a serving loop calls
+them token by token, captured into a graph and replayed, and on another stream."""
+import math
+
+import pytest
+import torch
+
+from dan_amd.paged import append_paged, attend_paged
+from dan_amd.readout import token_logprobs
+from oracle import paged as OP
+from oracle import readout as OR
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+H, HKV, D, PAGE, VOCAB = 8, 2, 128, 16, 1003
+
+
+def say(msg):
+    print(f"[gpu-case] {msg}", flush=True)
+
+
+class Layer:
+    """Random weights of one attention layer and a head, and a cache of `seqs` sequences of up to `most` tokens."""
+
+    def __init__(self, gpu, seqs, most, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        self.gpu, self.seqs = gpu, seqs
+        width = -(-most // PAGE)
+        self.table = torch.randperm(seqs * width, generator=g).int().view(seqs, width).to(gpu)
+        self.kc, self.vc = (torch.full((seqs * width, HKV, PAGE, D), math.nan, dtype=BF16, device=gpu) for _ in range(2))
+        inv = 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+        angle = torch.cat((torch.arange(most)[:, None] * inv,) * 2, 1)
+        self.cos, self.sin = angle.cos().float().to(gpu), angle.sin().float().to(gpu)
+        self.wq, self.wk = ((torch.randn(D, generator=g) * 0.2 + 1).to(BF16).to(gpu) for _ in range(2))
+        self.head = (torch.randn(VOCAB, H * D, generator=g) * 0.2).to(BF16).to(gpu)
+
+    def step(self, qkv, places, lens, tokens, seqs=None):
+        n = qkv.shape[0]
+        q, k, v = qkv.view(n, H + 2 * HKV, D).split([H, HKV, HKV], 1)
+        q = append_paged(q, k, v, self.cos, self.sin, self.kc, self.vc, self.table, places, seqs=seqs, rope_rows=places,
+                         q_norm_weight=self.wq, k_norm_weight=self.wk)
+        if seqs is not None:
+            return q
+        o = attend_paged(q, self.kc, self.vc, self.table, lens)
+        logits = o.transpose(0, 1).reshape(n, H * D) @ self.head.t()
+        return (o, logits) + tuple(token_logprobs(logits, tokens, top=5, entropy=True))
+
+
+def ids(x, gpu):
+    return torch.tensor(x, dtype=torch.int32, device=gpu)
+
+
+def test_decode_loop_matches_the_oracle(gpu):
+    """Three prompts of unequal length, then six tokens of each. The cache's own rows (rounded, as any cache holds
+    them) feed the oracle, so each step's output is within one rounding (2^-8) and its weights' fp32 error, far below that."""
+    say("decode loop: prompts, then six steps")
+    lens = [19, 1, 40]
+    m = Layer(gpu, 3, 64)
+    g = torch.Generator().manual_seed(7)
+    rows = sum(lens)
+    prompt = torch.randn(rows, (H + 2 * HKV) * D, generator=g).to(BF16).to(gpu)
+    m.step(prompt, ids([t for n in lens for t in range(n)], gpu), None, None, seqs=ids([s for s, n in enumerate(lens) for _ in range(n)], gpu))
+    for step in range(6):
+        qkv = torch.randn(3, (H + 2 * HKV) * D, generator=g).to(BF16).to(gpu)
+        tokens = torch.randint(0, VOCAB, (3, 2), generator=g)
+        places = [n + step for n in lens]
+        now = [p + 1 for p in places]
+        o, logits, lp, lse, ent, tlp, tid = m.step(qkv, ids(places, gpu), ids(now, gpu), tokens.to(gpu))
+        torch.cuda.synchronize()
+        x = qkv.cpu().view(3, H + 2 * HKV, D)
+        c, s = m.cos.cpu()[places], m.sin.cpu()[places]
+        q = OP.rotate_norm(x[:, :H], m.wq.cpu(), "rms", c, s)
+        k = OP.rotate_norm(x[:, H:H + HKV], m.wk.cpu(), "rms", c, s)
+        table = m.table.cpu()
+        for i, p in enumerate(places):
+            row = m.kc.cpu()[int(table[i, p // PAGE]), :, p % PAGE].double()
+            assert ((row - k[i]).abs() <= k[i].abs() * 2.0 ** -8 + 2.0 ** -18 * 16).all()
+            assert torch.equal(m.vc.cpu()[int(table[i, p // PAGE]), :, p % PAGE], x[i, H + HKV:])
+        ref, _, mag, big = OP.attend(q.to(BF16).transpose(0, 1), m.kc.cpu().double().nan_to_num(), m.vc.cpu().double().nan_to_num(), table, now)
+        # q's own rounding may fall the other way where its fp32 value lies next to a border: 2^-8 of it, in every score
+        tol = 2.0 ** -8 * ref.abs() + (2.0 ** -14 + 2 * 2.0 ** -7 * 2.0 ** -6 * big[..., None] / math.sqrt(D)) * mag
+        assert ((o.cpu().double() - ref).abs() <= tol).all()
+        rlp, rlse, rent, rtlp, rid = OR.token_logprobs(logits.cpu(), tokens, 5)
+        assert torch.equal(tid.cpu(), rid)
+        for got, want in ((lp, rlp), (lse, rlse), (ent, rent), (tlp, rtlp)):
+            assert (got.cpu().double() - want).abs().max() < 2.0 ** -14
+
+
+def test_captured_step_replays_with_changing_lengths(gpu):
+    """One captured step serves every later one: places, lengths, values and tokens change between replays, a row turns
+    idle, and eager work runs in between. Two graphs share nothing: the second is replayed between the first's replays."""
+    say("decode step: two graphs, replayed in turn")
+    places, lens, tokens = ids([300, 5, 77], gpu), ids([301, 6, 78], gpu), torch.zeros(3, 2, dtype=torch.long, device=gpu)
+    qkv = torch.zeros(3, (H + 2 * HKV) * D, dtype=BF16, device=gpu)
+    g = torch.Generator().manual_seed(3)
+    layers = [Layer(gpu, 3, 512, seed=s) for s in (1, 2)]
+    for m in layers:
+        m.kc.normal_()
+        m.vc.normal_()
+    copies = [(m.kc.clone(), m.vc.clone()) for m in layers]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for m in layers:
+            m.step(qkv, places, lens, tokens)
+    torch.cuda.current_stream().wait_stream(side)
+    for m in layers:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(m.step(qkv, places, lens, tokens))
+        graphs.append(graph)
+    for m, (kc, vc) in zip(layers, copies):
+        m.kc.copy_(kc)
+        m.vc.copy_(vc)
+    for step in range(4):
+        at = [300 + 13 * step, 5 + step, 77 + step]
+        n = [p + 1 for p in at]
+        if step == 2:
+            at[1], n[1] = -1, 0  # idle
+        places.copy_(ids(at, gpu))
+        lens.copy_(ids(n, gpu))
+        qkv.copy_(torch.randn(qkv.shape, generator=g).to(BF16))
+        tokens.copy_(torch.randint(-1, VOCAB, tokens.shape, generator=g))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] + [m.kc.clone(), m.vc.clone()] for o, m in zip(outs, layers)]
+        for m, have in zip(layers, got):
+            want = list(m.step(qkv, places, lens, tokens)) + [m.kc, m.vc]  # writes the same rows again
+            torch.cuda.synchronize()
+            assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(have, want))
+            if step == 2:
+                assert (have[0][:, 1] == 0).all()
+
+
+def test_another_stream(gpu):
+    """Everything on a stream of its own, tensors made on it; the default stream works meanwhile."""
+    say("decode step: another stream")
+    m = Layer(gpu, 2, 256)
+    m.kc.normal_()
+    m.vc.normal_()
+    g = torch.Generator().manual_seed(4)
+    qkv = torch.randn(2, (H + 2 * HKV) * D, generator=g).to(BF16).to(gpu)
+    tokens = torch.tensor([3, 4], device=gpu)
+    want = [t.clone() for t in m.step(qkv, ids([200, 9], gpu), ids([201, 10], gpu), tokens)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            got = m.step(qkv, ids([200, 9], gpu), ids([201, 10], gpu), tokens)
+        noise = torch.randn(1 << 20, device=gpu).sum()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.isfinite(noise)
+
+
+def test_gradient_replays(gpu):
+    """Forward and backward of the readout in one captured graph, replayed on changed logits."""
+    say("readout: captured gradient")
+    x = torch.randn(5, 777, device=gpu, requires_grad=True)
+    t = torch.randint(0, 777, (5,), device=gpu)
+    w = torch.randn(5, device=gpu)
+
+    def grad():
+        r = token_logprobs(x, t, entropy=True)
+        return torch.autograd.grad([r.logprobs, r.entropy], x, [w, w])[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grad()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = grad()
+    for _ in range(3):
+        with torch.no_grad():
+            x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        have = out.clone()
+        assert torch.equal(have, grad())
