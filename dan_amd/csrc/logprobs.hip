@@ -16,6 +16,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "dan_readout.h"
 
 namespace dan {
@@ -73,6 +75,17 @@ __device__ inline float wave_sum(float v) {
   v += DAN_DPP(v, 0x141);
   v += DAN_DPP(v, 0x140);
   return (DAN_LANE(v, 0) + DAN_LANE(v, 16)) + (DAN_LANE(v, 32) + DAN_LANE(v, 48));
+}
+
+template <typename F>
+__device__ inline uint32_t wave_fold(uint32_t v, F f) {
+  auto dpp = [](uint32_t x, auto ctrl) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, false); };
+  v = f(v, dpp(v, std::integral_constant<int, 0xB1>()));
+  v = f(v, dpp(v, std::integral_constant<int, 0x4E>()));
+  v = f(v, dpp(v, std::integral_constant<int, 0x141>()));
+  v = f(v, dpp(v, std::integral_constant<int, 0x140>()));
+  auto at = [&](int n) { return (uint32_t)__builtin_amdgcn_readlane((int)v, n); };
+  return f(f(at(0), at(16)), f(at(32), at(48)));
 }
 
 struct Params {
@@ -171,45 +184,59 @@ __global__ __launch_bounds__(256) void chunk_kernel(const Params p) {
   if (lane == 0) *(f32x4 *)(p.part + at * 4) = (f32x4){m, l, a, 0};
 }
 
-// The row's maximum, sum and weighted sum from its chunks', in every lane of a wave.
+// The row's maximum, sum and weighted sum from its chunks', in every lane of a wave; `first` is chunk `lane`'s
+// (-inf, 0, 0 behind the last), loaded ahead.
 struct Row {
   float m, l, a;
 };
-__device__ inline Row join(const Params &p, int64_t r, int lane) {
+__device__ inline f32x4 first_chunk(const Params &p, int64_t r, int lane) {
+  return lane < p.chunks ? ((const f32x4 *)p.part)[r * p.chunks + lane] : (f32x4){-INFINITY, 0, 0, 0};
+}
+__device__ inline Row join(const Params &p, int64_t r, int lane, f32x4 first) {
   const f32x4 *part = (const f32x4 *)p.part + r * p.chunks;
-  float m = -INFINITY;
-  for (int c = lane; c < p.chunks; c += 64) m = fmaxf(m, part[c][0]);
+  float m = first[0];
+  for (int c = lane + 64; c < p.chunks; c += 64) m = fmaxf(m, part[c][0]);
   m = wave_max(m);
   const float sub = m == -INFINITY ? 0.0f : m;
   float l = 0.f, a = 0.f;
-  for (int c = lane; c < p.chunks; c += 64) {
-    const f32x4 q = part[c];
+  auto add = [&](f32x4 q) {
     const float t = fmaxf((q[0] - sub) * kLog2e, -1000.0f), by = __builtin_amdgcn_exp2f(t);  // 0 times -inf else
     l = __builtin_fmaf(by, q[1], l);
     a = __builtin_fmaf(by, __builtin_fmaf(t, q[1], q[2]), a);
-  }
+  };
+  add(first);
+  for (int c = lane + 64; c < p.chunks; c += 64) add(part[c]);
   return {m, wave_sum(l), wave_sum(a)};
 }
 
-// Writes the row's logsumexp, entropy and the given tokens' log probabilities
-// (threads `tid` of `count`); returns what a logit's log probability subtracts: M, then log sum.
+// A thread's first given token and its logit, loaded ahead of the row's sums.
+struct Given {
+  int64_t token;  // -1: padding, or none for this thread
+  float x;
+};
 template <typename T>
-__device__ inline void write_row(const Params &p, int64_t r, const Row &row, int tid, int count, float &m, float &logl) {
-  m = row.m == -INFINITY ? 0.0f : row.m;
-  logl = logf(row.l);
+__device__ inline Given fetch(const Params &p, int64_t r, int l) {
+  Given g = {-1, 0.0f};
+  if (l < p.L) {
+    g.token = p.tokens[r * p.t_st + l];
+    if (g.token >= 0 && g.token < p.V) g.x = (float)static_cast<const T *>(p.x)[r * p.x_st + g.token];
+  }
+  return g;
+}
+
+// Writes the row's logsumexp, entropy and the given tokens' log probabilities (threads `tid` of
+// `count`; the first of each in `g`), x - (M, then log sum).
+template <typename T>
+__device__ inline void write_row(const Params &p, int64_t r, const Row &row, Given g, int tid, int count, float m, float logl) {
   if (tid == 0) {
     p.lse[r] = m + logl;
     if (p.entropy) p.entropy[r] = row.l == 0.0f ? 0.0f : logl - row.a / row.l * kLn2;
   }
-  const T *x = static_cast<const T *>(p.x) + r * p.x_st;
   for (int l = tid; l < p.L; l += count) {
-    const int64_t t = p.tokens[r * p.t_st + l];
+    if (l != tid) g = fetch<T>(p, r, l);
     float y = 0.0f;
-    if (t >= p.V) y = __builtin_nanf("");
-    else if (t >= 0) {
-      const float v = (float)x[t];
-      y = row.l == 0.0f ? -INFINITY : (v - m) - logl;
-    }
+    if (g.token >= p.V) y = __builtin_nanf("");
+    else if (g.token >= 0) y = row.l == 0.0f ? -INFINITY : (g.x - m) - logl;
     p.logprobs[r * p.L + l] = y;
   }
 }
@@ -219,165 +246,284 @@ __global__ __launch_bounds__(256) void row_kernel(const Params p) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= p.N) return;
-  float m, logl;
-  write_row<T>(p, r, join(p, r, lane), lane, 64, m, logl);
+  const f32x4 first = first_chunk(p, r, lane);
+  const Given g = fetch<T>(p, r, lane);
+  const Row row = join(p, r, lane, first);
+  write_row<T>(p, r, row, g, lane, 64, row.m == -INFINITY ? 0.0f : row.m, logf(row.l));
 }
 
-// A value's place among all values as an unsigned number: rising with it, NaN above
-// all, -0 as 0.
+// A value's place among all values as an unsigned number in [0x7fffff, 0xfffffffe]: rising with
+// it, NaN above all, -0 as 0; and the value back.
 __device__ inline uint32_t order(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ inline float value_of(uint32_t o) {
-  return o == 0xffffffffu ? __builtin_nanf("") : __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
-}
+__device__ inline float value_of(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 // Larger for the larger value, and for the lower index of equal ones.
 __device__ inline uint64_t key_of(uint32_t o, uint32_t index) { return (uint64_t)o << 32 | (0xffffffffu - index); }
 
-__device__ inline uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t w = (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)v, o);
-    v = w > v ? w : v;
-  }
-  return v;
+// The bits of a wave's 64-bit lane mask below this lane.
+__device__ inline int below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-constexpr int kGroupKeys = 32;  // group maxima a lane: 2048 groups, rows of DAN_READOUT_MAX_TOP_VOCAB fp32 values
+constexpr int kTaken = 32;   // groups whose values a work group holds: 8 vectors a lane of 4 waves
 constexpr int kCand = 256;
 
-template <typename T>
-__global__ __launch_bounds__(256) void top_kernel(const Params p) {
-  constexpr int n = Vec<T>::n, kRegs = DAN_READOUT_MAX_TOP / 4;  // vectors a lane: 64 of each group, 4 waves
-  __shared__ int group[DAN_READOUT_MAX_TOP];
-  __shared__ uint64_t cand[kCand];
-  __shared__ uint32_t quad[64];
-  __shared__ uint64_t best_of[2][4];
-  __shared__ int count;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
-  const Row row = join(p, r, lane);
-  float m, logl;
-  write_row<T>(p, r, row, tid, 256, m, logl);
-  const bool empty = row.l == 0.0f;  // every logit is -inf
+// Raises `bound` by bisection, between what K or more of a set's keys reach and `over`, which
+// fewer do, until at most `most` reach it or the two are neighbours; `have` is how many
+// do, reach(x) how many reach x.
+template <typename F>
+__device__ inline void bisect(uint32_t &bound, uint32_t &over, int &have, int k, int most, F reach) {
+  while (have > most && over - bound > 1) {
+    const uint32_t mid = bound + (over - bound) / 2;
+    const int c = reach(mid);
+    if (c >= k) bound = mid, have = c;
+    else over = mid;
+  }
+}
 
-  // The K groups of largest maximum, by one wave: each lane keeps its best.
-  const int vectors = (p.V + n - 1) / n, groups = (vectors + 63) / 64, taken = min(p.K, groups);
+// The K largest values of a row, one work group.
+//  1. Each wave finds by bisection a bound that K and not many more of the group maxima reach, or,
+//     where too many are equal at it, that value itself. K values of the row reach it, so the row's K
+//     largest do, and they lie in these groups (of those whose maximum is the bound itself, in
+//     the first that make up K).
+//  2. The work group loads these groups and collects the values that reach the bound: in rows of
+//     ordinary logits few more than K. Of values equal to a bound that too many reach (masked rows: the
+//     masked value) each wave collects its first K. Where more than 256 come together (no more
+//     groups than K; most of the largest side by side) the bound is raised by bisection over the
+//     lanes' maxima, and if need be over the values.
+//  3. Each collected value's rank among them is its place in the result.
+// KEYS: group maxima a lane, 64 KEYS >= groups.
+template <typename T, int KEYS>
+__global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
+  constexpr int n = Vec<T>::n, kRegs = kTaken / 4;
+  __shared__ int group[4][kTaken];
+  __shared__ uint64_t cand[kCand];
+  __shared__ uint32_t lane_max[256];
+  __shared__ int count, sums[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t r = blockIdx.x;
+  const int vectors = (p.V + n - 1) / n, groups = (vectors + 63) / 64;
+  const float *gm = p.part + (int64_t)p.N * p.chunks * 4 + r * p.chunks * kVecs;
+  const f32x4 first = first_chunk(p, r, lane);
+  float g[KEYS];
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) g[i] = lane + 64 * i < groups ? gm[lane + 64 * i] : 0.0f;
+  const Given given = fetch<T>(p, r, tid);
   if (tid == 0) count = 0;
-  if (wave == 0) {
-    const float *gm = p.part + (int64_t)p.N * p.chunks * 4 + r * p.chunks * kVecs;
-    uint32_t o[kGroupKeys];
+  uint32_t o[KEYS];
 #pragma unroll
-    for (int i = 0; i < kGroupKeys; ++i) o[i] = lane + 64 * i < groups ? order(gm[lane + 64 * i]) : 0;
-    uint64_t best = 0;
+  for (int i = 0; i < KEYS; ++i) o[i] = lane + 64 * i < groups ? order(g[i]) : 0;
+
+  // 1.
+  auto reach = [&](uint32_t x) {
+    int c = 0;
 #pragma unroll
-    for (int i = 0; i < kGroupKeys; ++i) {
-      const uint64_t k = lane + 64 * i < groups ? key_of(o[i], lane + 64 * i) : 0;
-      best = k > best ? k : best;
-    }
-    for (int k = 0; k < taken; ++k) {
-      const uint64_t top = wave_max64(best);
-      if (lane == 0) group[k] = (int)(0xffffffffu - (uint32_t)top);
-      if (best == top) {  // one lane: its next
-        best = 0;
+    for (int i = 0; i < KEYS; ++i) c += __builtin_popcountll(__ballot(o[i] >= x));
+    return c;
+  };
+  const int most = min(kTaken, p.K + p.K / 4 + 2);
+  uint32_t best = o[0];
 #pragma unroll
-        for (int i = 0; i < kGroupKeys; ++i) {
-          const uint64_t q = lane + 64 * i < groups ? key_of(o[i], lane + 64 * i) : 0;
-          best = q < top && q > best ? q : best;
-        }
+  for (int i = 1; i < KEYS; ++i) best = max(best, o[i]);
+  // The smallest of the lanes' largest (of lanes that have one) is reached by each of them.
+  uint32_t bound = wave_fold(best ? best : 0xffffffffu, [](uint32_t x, uint32_t y) { return min(x, y); });
+  uint32_t over = wave_fold(best, [](uint32_t x, uint32_t y) { return max(x, y); }) + 1;
+  int have = reach(bound);
+  if (have > p.K) bisect(bound, over, have, p.K, most, reach);
+  if (groups <= p.K) bound = 1, have = groups;  // all of them (of one maximum or of many)
+  bool equal = have > kTaken;  // then over = bound + 1
+  const int left = equal ? p.K - reach(over) : 0, taken = equal ? p.K : have;
+  {
+    int at = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      bool in = o[i] >= (equal ? over : bound);
+      if (equal) {
+        const uint64_t same = __ballot(o[i] == bound);
+        in = in || (o[i] == bound && before + below(same) < left);
+        before += __builtin_popcountll(same);
       }
+      const uint64_t mask = __ballot(in);
+      if (in) group[wave][at + below(mask)] = lane + 64 * i;
+      at += __builtin_popcountll(mask);
     }
   }
-  __syncthreads();
+  __builtin_amdgcn_wave_barrier();  // a wave reads its own list
 
-  // Those groups again, wave w taking groups w, w + 4, ..
+  // 2. Wave w takes groups w, w + 4, ..; rising ones, so that of equal values the first come first.
   const T *x = static_cast<const T *>(p.x) + r * p.x_st;
-  const int whole = p.V / n;
+  const int whole = p.V / n, mine = (taken - wave + 3) / 4;
   typename Vec<T>::type raw[kRegs];
   int at[kRegs];
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int k = wave + 4 * i;
-    at[i] = k < taken ? group[k] * 64 + lane : vectors;
-    if (whole > 0) raw[i] = *(const DAN_GLOBAL typename Vec<T>::loose *)(x + (int64_t)n * min(at[i], whole - 1));
+    at[i] = i < mine ? group[wave][wave + 4 * i] * 64 + lane : vectors;
+    if (whole > 0 && i < mine) raw[i] = *(const DAN_GLOBAL typename Vec<T>::loose *)(x + (int64_t)n * min(at[i], whole - 1));
   }
-  uint32_t o[kRegs][n];
-  uint32_t most = 0;
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i)
-#pragma unroll
-    for (int e = 0; e < n; ++e) {
-      const bool there = at[i] < vectors && n * at[i] + e < p.V;
-      o[i][e] = !there ? 0 : order(at[i] < whole ? (float)raw[i][e] : (float)x[n * at[i] + e]);  // order() of a value is never 0
-      most = max(most, o[i][e]);
-    }
-
-  // A bound that at least K values reach: the K-th largest of the 64 maxima of four lanes each.
-  uint32_t q4 = max(most, (uint32_t)__shfl_xor((int)most, 1));
-  q4 = max(q4, (uint32_t)__shfl_xor((int)q4, 2));
-  if ((lane & 3) == 0) quad[tid >> 2] = q4;
-  __syncthreads();
-  const uint32_t mine = quad[lane];
-  int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < 64; ++i) {
-    const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-    above += other > mine || (other == mine && i < lane);
-  }
-  const uint64_t kth = __ballot(above == p.K - 1);
-  const uint32_t bound = max(1u, (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(kth)));
-  int have = 0;
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i)
-#pragma unroll
-    for (int e = 0; e < n; ++e) have += o[i][e] >= bound;
-  int start = have ? atomicAdd(&count, have) : 0;  // where they go does not change the result: keys differ
-  if (have && start + have <= kCand) {
+  if (p.V != whole * n) {  // the row's last values fill no vector: one lane reads them one by one
 #pragma unroll
     for (int i = 0; i < kRegs; ++i)
+      if (at[i] == whole) {
 #pragma unroll
-      for (int e = 0; e < n; ++e)
-        if (o[i][e] >= bound) cand[start++] = key_of(o[i][e], n * at[i] + e);
+        for (int e = 0; e < n; ++e)
+          if (n * whole + e < p.V) raw[i][e] = x[n * whole + e];
+      }
   }
-  __syncthreads();
-  const int total = count;
-  auto write = [&](int k, uint64_t key) {
-    const float v = value_of((uint32_t)(key >> 32));
-    p.top_logprobs[r * p.K + k] = empty ? -INFINITY : (v - m) - logl;
-    p.top_ids[r * p.K + k] = 0xffffffffu - (uint32_t)key;
-  };
-  if (total <= kCand) {  // each candidate's rank among them
-    if (tid < total) {
-      const uint64_t k = cand[tid];
-      int rank = 0;
-      for (int i = 0; i < total; ++i) rank += cand[i] > k;
-      if (rank < p.K) write(rank, k);
+
+  const Row row = join(p, r, lane, first);
+  const float m = row.m == -INFINITY ? 0.0f : row.m, logl = logf(row.l);
+  write_row<T>(p, r, row, given, tid, 256, m, logl);
+  if (!(row.l >= 0.0f)) {  // NaN: the row has no order
+    if (tid < p.K) {
+      p.top_logprobs[r * p.K + tid] = __builtin_nanf("");
+      p.top_ids[r * p.K + tid] = tid;
     }
     return;
   }
-  // Too many reach the bound (a row of equal values, or its largest side by side): K rounds of the largest left.
-  uint64_t last = ~0ull, best = 0;
-  for (int k = 0; k < p.K; ++k) {
-    if (k == 0 || best == last) {
-      best = 0;
+
+  auto is_there = [&](int i, int e) { return at[i] < whole || (at[i] == whole && n * whole + e < p.V); };
+  auto values = [&](int i) { return __builtin_convertvector(raw[i], typename Vec<T>::f32); };
+  auto largest = [&](int i) {
+    const typename Vec<T>::f32 f = values(i);
+    float y = f[0];
+#pragma unroll
+    for (int e = 1; e < n; ++e) y = fmaxf(y, f[e]);
+    return y;
+  };
+  int total = 0;
+  for (int stage = groups > p.K ? 0 : 1;; ++stage) {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) asm("" : "+v"(raw[i]), "+v"(at[i]));  // what a turn makes of them is not kept over the turns
+    if (stage == 1) {  // K or more of the lanes' maxima reach it, so as many values do
+      uint32_t mx = 0, q[4];
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) {
+        if (at[i] < whole) mx = max(mx, order(largest(i)));
+        if (at[i] == whole) {
+#pragma unroll
+          for (int e = 0; e < n; ++e)
+            if (is_there(i, e)) mx = max(mx, order((float)raw[i][e]));
+        }
+      }
+      lane_max[tid] = mx;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = lane_max[lane + 64 * i];
+      auto reach_lanes = [&](uint32_t y) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c += __builtin_popcountll(__ballot(q[i] >= y));
+        return c;
+      };
+      over = wave_fold(max(max(q[0], q[1]), max(q[2], q[3])), [](uint32_t y, uint32_t z) { return max(y, z); }) + 1;
+      have = reach_lanes(bound);
+      if (have > p.K) bisect(bound, over, have, p.K, most, reach_lanes);
+      equal = have > most;
+    } else if (stage == 2) {
+      int turn = 0;
+      auto reach_values = [&](uint32_t y) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) {
+          const typename Vec<T>::f32 f = values(i);
+#pragma unroll
+          for (int e = 0; e < n; ++e) c += __builtin_popcountll(__ballot(is_there(i, e) && order(f[e]) >= y));
+        }
+        if (lane == 0) sums[turn & 1][wave] = c;
+        __syncthreads();
+        c = sums[turn & 1][0] + sums[turn & 1][1] + sums[turn & 1][2] + sums[turn & 1][3];
+        ++turn;
+        return c;
+      };
+      total = reach_values(bound);
+      over = 0xffffffffu;
+      bisect(bound, over, total, p.K, kCand, reach_values);
+      equal = total > kCand;
+    }
+    // Values that reach the bound (NaN at bound 1, which every value then does), or that lie above
+    // it where `equal`, into cand[]; where in it does not change the result, since keys differ.
+    const float v = value_of(equal ? over : bound);
+    int c = 0;
+    bool hit[kRegs];
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      hit[i] = false;
+      if (i < mine) {
+        hit[i] = at[i] == whole || (at[i] < whole && !(largest(i) < v));
+        if (hit[i]) {
+          const typename Vec<T>::f32 f = values(i);
+#pragma unroll
+          for (int e = 0; e < n; ++e) c += !(f[e] < v) && is_there(i, e);
+        }
+      }
+    }
+    int start = c ? atomicAdd(&count, c) : 0;
+    if (c && start + c <= kCand) {
 #pragma unroll
       for (int i = 0; i < kRegs; ++i)
+        if (hit[i]) {
+          const typename Vec<T>::f32 f = values(i);
 #pragma unroll
-        for (int e = 0; e < n; ++e) {
-          const uint64_t q = o[i][e] ? key_of(o[i][e], n * at[i] + e) : 0;
-          best = q < last && q > best ? q : best;
+          for (int e = 0; e < n; ++e)
+            if (!(f[e] < v) && is_there(i, e)) cand[start++] = key_of(order(f[e]), n * at[i] + e);
         }
     }
-    const uint64_t w = wave_max64(best);
-    if (lane == 0) best_of[k & 1][wave] = w;
-    __syncthreads();
-    last = best_of[k & 1][0];
+    if (equal) {  // over = bound + 1: the wave's first K of those equal to the bound
+      const float w = value_of(bound);
+      int room = p.K;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) last = best_of[k & 1][i] > last ? best_of[k & 1][i] : last;
-    if (tid == 0) write(k, last);
+      for (int i = 0; i < kRegs; ++i)
+        if (i < mine && room > 0) {
+          const typename Vec<T>::f32 f = values(i);
+          int before = 0, all = 0;
+          bool same[n];
+#pragma unroll
+          for (int e = 0; e < n; ++e) {
+            same[e] = is_there(i, e) && f[e] == w;
+            const uint64_t mask = __ballot(same[e]);
+            before += below(mask);
+            all += __builtin_popcountll(mask);
+          }
+#pragma unroll
+          for (int e = 0; e < n; ++e)
+            if (same[e] && before++ < room) {
+              const int to = atomicAdd(&count, 1);
+              if (to < kCand) cand[to] = key_of(bound, n * at[i] + e);
+            }
+          room -= min(room, all);
+        }
+    }
+    __syncthreads();
+    total = count;
+    if (total <= kCand) break;  // at stage 2 at the latest: fewer than K above the bound, and 4 K at it
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
   }
+
+  // 3.
+  if (tid < total) {
+    const uint64_t k = cand[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < total; ++i) rank += cand[i] > k;
+    if (rank < p.K) {
+      const float y = value_of((uint32_t)(k >> 32));
+      p.top_logprobs[r * p.K + rank] = row.l == 0.0f ? -INFINITY : (y - m) - logl;
+      p.top_ids[r * p.K + rank] = 0xffffffffu - (uint32_t)k;
+    }
+  }
+}
+
+template <typename T>
+void launch_top(const Params &p, hipStream_t s) {
+  const int groups = ((p.V + Vec<T>::n - 1) / Vec<T>::n + 63) / 64;
+  if (groups <= 64 * 4) hipLaunchKernelGGL((top_kernel<T, 4>), dim3((unsigned)p.N), dim3(256), 0, s, p);
+  else if (groups <= 64 * 8) hipLaunchKernelGGL((top_kernel<T, 8>), dim3((unsigned)p.N), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((top_kernel<T, 32>), dim3((unsigned)p.N), dim3(256), 0, s, p);  // up to DAN_READOUT_MAX_TOP_VOCAB fp32 values
 }
 
 struct GradParams {
@@ -481,7 +627,7 @@ void forward(const Params &p, hipStream_t s) {
     if (p.K > 0) hipLaunchKernelGGL((chunk_kernel<T, false, true>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((chunk_kernel<T, false, false>), grid, dim3(256), 0, s, p);
   }
-  if (p.K > 0) hipLaunchKernelGGL((top_kernel<T>), dim3((unsigned)p.N), dim3(256), 0, s, p);
+  if (p.K > 0) launch_top<T>(p, s);
   else hipLaunchKernelGGL((row_kernel<T>), dim3((unsigned)((p.N + 3) / 4)), dim3(256), 0, s, p);
 }
 

@@ -26,34 +26,53 @@ import torch
 
 from . import _decode, _native
 from .attention import _DTYPES, E4M3, has_tangent
-from .front import NORMS, _row_ok, _view
+from .front import NORMS
+
+
+def _rows(t):
+    """t (16-bit, three-dimensional) or a fresh contiguous copy where its rows are not 16-byte aligned or of unit
+    stride, with its address and its first two strides."""
+    s0, s1, s2 = t.stride()
+    at = t.data_ptr()
+    if s2 != 1 or ((s0 | s1) * 2 | at) & 15:
+        t = torch.empty_like(t, memory_format=torch.contiguous_format).copy_(t)
+        (s0, s1, _), at = t.stride(), t.data_ptr()
+    return t, at, s0, s1
+
+
+def _cache_rows(t):
+    """A cache's address and first three strides; its rows are written and read in place."""
+    s0, s1, s2, s3 = t.stride()
+    at = t.data_ptr()
+    if s3 != 1 or ((s0 | s1 | s2) * t.element_size() | at) & 15:
+        raise ValueError("the cache's rows must have unit stride and be 16-byte aligned (they are written and read in place)")
+    return at, s0, s1, s2
 
 
 def _check_cache(k_cache, v_cache, k_scale, v_scale, table, dtype, device):
     """Refuses a cache or table that the kernels cannot read; returns
-    (pages, Hkv, page size, D) and the scales' addresses."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must both be [pages, Hkv, page, D]")
-    if k_cache.dtype != v_cache.dtype or (k_cache.dtype != dtype and k_cache.dtype != E4M3):
-        raise ValueError(f"k_cache and v_cache must share q's {dtype} or {E4M3}; got {k_cache.dtype}, {v_cache.dtype}")
+    [pages, Hkv, page size, D] and the scales' addresses."""
+    shape, kind = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)} must both be [pages, Hkv, page, D]")
+    if kind != v_cache.dtype or (kind != dtype and kind != E4M3):
+        raise ValueError(f"k_cache and v_cache must share q's {dtype} or {E4M3}; got {kind}, {v_cache.dtype}")
     if not (k_cache.device == v_cache.device == table.device == device):
         raise ValueError(f"k_cache, v_cache and table must be on {device}")
-    if not (_row_ok(k_cache) and _row_ok(v_cache)):
-        raise ValueError("the cache's rows must have unit stride and be 16-byte aligned (they are written and read in place)")
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
         raise ValueError(f"table must be int32 [sequences, width] with unit stride; got {table.dtype} {tuple(table.shape)}")
-    if k_cache.dtype != E4M3:
+    if kind != E4M3:
         if k_scale is not None or v_scale is not None:
             raise ValueError("k_scale and v_scale belong to an e4m3 cache")
-        return k_cache.shape, 0, 0
+        return shape, 0, 0
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         if not (isinstance(t, torch.Tensor) and t.numel() == 1 and t.dtype == torch.float32 and t.device == device):
             raise ValueError(f"an e4m3 cache needs {name}: a one-element fp32 tensor on {device}")
-    return k_cache.shape, k_scale.data_ptr(), v_scale.data_ptr()
+    return shape, k_scale.data_ptr(), v_scale.data_ptr()
 
 
 def _check_index(t, name, count, device):
-    if t.dtype != torch.int32 or t.shape != (count,) or t.device != device or (count > 1 and t.stride(0) != 1):
+    if t.dtype != torch.int32 or t.shape != (count,) or t.device != device or (t.stride(0) != 1 and count > 1):
         raise ValueError(f"{name} must be a contiguous int32 [{count}] on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -91,61 +110,77 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
             return append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, seqs=seqs, rope_rows=rope_rows,
                                 q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, eps=eps, norm=norm, k_scale=k_scale,
                                 v_scale=v_scale)
-    inputs = [t for t in (q, k, v, k_cache, v_cache) if t is not None]
+    inputs = (k, v, k_cache, v_cache) if q is None else (q, k, v, k_cache, v_cache)
     if (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)) or has_tangent(*inputs):
         raise NotImplementedError("append_paged is forward-only")
-    if k.dim() != 3 or v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, Hkv, D]")
-    n, hkv, d = k.shape
-    h = 0
-    if q is not None:
-        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype or q.device != dev:
-            raise ValueError(f"q {tuple(q.shape)} {q.dtype} must be [{n}, H, {d}] {k.dtype} on {dev}")
-        h = q.shape[1]
-    if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or v.device != dev:
-        raise ValueError(f"q, k, v must share bf16 or fp16 on {dev}; got {k.dtype}, {v.dtype} on {v.device}")
-    if norm not in NORMS:
-        raise ValueError(f"norm {norm!r}: one of {list(NORMS)}")
-    (pages, chkv, page, cd), ks, vs = _check_cache(k_cache, v_cache, k_scale, v_scale, table, k.dtype, dev)
-    if (chkv, cd) != (hkv, d):
+    dtype, shape = k.dtype, k.shape
+    if len(shape) != 3 or v.shape != shape:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must both be [N, Hkv, D]")
+    n, hkv, d = shape
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or v.dtype != dtype or v.device != dev:
+        raise ValueError(f"q, k, v must share bf16 or fp16 on {dev}; got {dtype}, {v.dtype} on {v.device}")
+    (pages, chkv, page, cd), ks, vs = _check_cache(k_cache, v_cache, k_scale, v_scale, table, dtype, dev)
+    if chkv != hkv or cd != d:
         raise ValueError(f"a cache of {chkv} heads x {cd} for k of {hkv} x {d}")
-    if any(s == 0 and c > 1 for t in (k_cache, v_cache) for s, c in zip(t.stride(), t.shape)):
+    kc, vc = _cache_rows(k_cache), _cache_rows(v_cache)
+    if (0 in kc or 0 in vc) and any(s == 0 and c > 1 for t in (k_cache, v_cache) for s, c in zip(t.stride(), t.shape)):
         raise ValueError("an expanded cache cannot be written")
+    seqs_of_table, width = table.shape
+    if seqs is None and seqs_of_table < n:
+        raise ValueError(f"{n} tokens without seqs need a table of as many rows; got {seqs_of_table}")
     place_p = _check_index(places, "places", n, dev)
     seq_p = 0 if seqs is None else _check_index(seqs, "seqs", n, dev)
     rope_p = 0 if rope_rows is None else _check_index(rope_rows, "rope_rows", n, dev)
-    if seqs is None and table.shape[0] < n:
-        raise ValueError(f"{n} tokens without seqs need a table of as many rows; got {table.shape[0]}")
-    r = 0 if cos is None else cos.shape[-1]
-    if r:
-        rows = cos.shape[0]
-        if cos.dim() != 2 or sin is None or sin.shape != cos.shape or (rows != n and rope_rows is None):
+
+    r = rows = cs_p = sn_p = cs_st = 0
+    cs_type = dtype
+    if cos is not None and cos.shape[-1]:
+        rows, r = cos.shape if cos.dim() == 2 else (0, 0)
+        if not r or sin is None or sin.shape != cos.shape or (rows != n and rope_rows is None):
             raise ValueError(f"cos and sin must both be [{n}, R] ([any, R] with rope_rows)")
-        if cos.dtype not in (k.dtype, torch.float32) or sin.dtype != cos.dtype or not (cos.device == sin.device == dev):
-            raise ValueError(f"cos and sin must share {k.dtype} or fp32 on {dev}; got {cos.dtype}, {sin.dtype}")
-        if cos.stride() != sin.stride() or not (_row_ok(cos) and _row_ok(sin)) or cos.stride(0) < r:
+        cs_type = cos.dtype
+        if (cs_type != dtype and cs_type != torch.float32) or sin.dtype != cs_type or not (cos.device == sin.device == dev):
+            raise ValueError(f"cos and sin must share {dtype} or fp32 on {dev}; got {cs_type}, {sin.dtype}")
+        cs_st, one = cos.stride()
+        cs_p, sn_p = cos.data_ptr(), sin.data_ptr()
+        if one != 1 or sin.stride() != (cs_st, one) or cs_st < r or (cs_st * cos.element_size() | cs_p | sn_p) & 15:
             cos, sin = (torch.empty_like(t, memory_format=torch.contiguous_format).copy_(t) for t in (cos, sin))
-        elif rows == 1:
-            cos, sin = cos.contiguous(), sin.contiguous()
+            cs_st, cs_p, sn_p = r, cos.data_ptr(), sin.data_ptr()
     elif sin is not None and sin.shape[-1]:
         raise ValueError("sin without cos")
-    qw = kw = None
+
+    if norm not in NORMS:
+        raise ValueError(f"norm {norm!r}: one of {list(NORMS)}")
+    qw_p = kw_p = 0
     if norm is not None:
-        for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
-            if (name[0] == "k" or q is not None) and not (isinstance(w, torch.Tensor) and w.shape == (d,) and w.device == dev):
-                raise ValueError(f"norm {norm!r} needs {name}: a [{d}] tensor on {dev}")
-        qw, kw = (None if w is None else _view(w.detach().to(k.dtype)) for w in (q_norm_weight if q is not None else None, k_norm_weight))
-    q_in, k_in, v_in = None if q is None else _view(q), _view(k), _view(v)
-    q_out = None if q is None else torch.empty((n, h, d), dtype=k.dtype, device=dev)
+        qw, kw = (_weight(w, name, norm, dtype, d, dev) for w, name in ((k_norm_weight if q is None else q_norm_weight, "q_norm_weight"),
+                                                                        (k_norm_weight, "k_norm_weight")))
+        qw_p, kw_p = qw.data_ptr(), kw.data_ptr()
+    h = q_p = q_st = q_sh = out_p = 0
+    out = None
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != dtype or q.device != dev:
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} must be [{n}, H, {d}] {dtype} on {dev}")
+        h = q.shape[1]
+        q, q_p, q_st, q_sh = _rows(q)
+        out = torch.empty((n, h, d), dtype=dtype, device=dev)
+        out_p = out.data_ptr()
+    k, k_p, k_st, k_sh = _rows(k)
+    v, v_p, v_st, v_sh = _rows(v)
     _decode.call_append(
-        _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[k.dtype], _DTYPES[k_cache.dtype], _DTYPES[cos.dtype if r else k.dtype],
-        n, h, hkv, d, r, NORMS[norm], page, pages, table.shape[1], table.shape[0], rows if r else 0, _native.f32(float(eps)),
-        *((0, 0, 0) if q is None else (q_in.data_ptr(), *q_in.stride()[:2])), k_in.data_ptr(), *k_in.stride()[:2], v_in.data_ptr(),
-        *v_in.stride()[:2], cos.data_ptr() if r else 0, sin.data_ptr() if r else 0, cos.stride(0) if r else 0,
-        0 if qw is None else qw.data_ptr(), 0 if kw is None else kw.data_ptr(), *((0, 0, 0) if q is None else (q_out.data_ptr(), h * d, d)),
-        k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], ks, vs, table.data_ptr(), table.stride(0),
-        place_p, seq_p, rope_p)
-    return None if q is None else q_out.transpose(0, 1)
+        _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[dtype], _DTYPES[k_cache.dtype], _DTYPES[cs_type], n, h, hkv, d, r, NORMS[norm],
+        page, pages, width, seqs_of_table, rows, _native.f32(float(eps)), q_p, q_st, q_sh, k_p, k_st, k_sh, v_p, v_st, v_sh,
+        cs_p, sn_p, cs_st, qw_p, kw_p, out_p, h * d, d, *kc, *vc, ks, vs, table.data_ptr(), table.stride(0), place_p, seq_p, rope_p)
+    return None if out is None else out.transpose(0, 1)
+
+
+def _weight(w, name, norm, dtype, d, device):
+    """A norm weight in the model dtype, contiguous and 16-byte aligned."""
+    if not (isinstance(w, torch.Tensor) and w.shape == (d,) and w.device == device):
+        raise ValueError(f"norm {norm!r} needs {name}: a [{d}] tensor on {device}")
+    if w.dtype == dtype and w.stride(0) == 1 and not w.data_ptr() & 15:
+        return w
+    return torch.empty(d, dtype=dtype, device=device).copy_(w.detach())
 
 
 def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, v_scale=None, max_len=None, return_lse=False):
@@ -175,31 +210,33 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
                                 return_lse=return_lse)
     if (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)) or has_tangent(q, k_cache, v_cache):
         raise NotImplementedError("attend_paged is forward-only")
-    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"q must be [H, B, D] in bf16 or fp16; got {tuple(q.shape)} {q.dtype}")
-    h, b, d = q.shape
-    (pages, hkv, page, cd), ks, vs = _check_cache(k_cache, v_cache, k_scale, v_scale, table, q.dtype, dev)
+    dtype, shape = q.dtype, q.shape
+    if len(shape) != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
+        raise ValueError(f"q must be [H, B, D] in bf16 or fp16; got {tuple(shape)} {dtype}")
+    h, b, d = shape
+    (pages, hkv, page, cd), ks, vs = _check_cache(k_cache, v_cache, k_scale, v_scale, table, dtype, dev)
     if cd != d or hkv == 0 or h == 0 or h % hkv:
         raise ValueError(f"q of {h} heads x {d} on a cache of {hkv} x {cd}: the heads must be a multiple, head_dim the same")
-    if table.shape[0] != b:
-        raise ValueError(f"a table of {table.shape[0]} sequences for {b} tokens")
+    rows, width = table.shape
+    if rows != b:
+        raise ValueError(f"a table of {rows} sequences for {b} tokens")
     len_p = _check_index(lens, "lens", b, dev)
-    most = table.shape[1] * page if max_len is None else int(max_len)
-    if not 0 <= most <= table.shape[1] * page:
-        raise ValueError(f"max_len {max_len}: the table holds {table.shape[1] * page} keys a sequence")
+    most = width * page if max_len is None else int(max_len)
+    if not 0 <= most <= width * page:
+        raise ValueError(f"max_len {max_len}: the table holds {width * page} keys a sequence")
     if scale is None:
-        scale = 1.0 / math.sqrt(d)
+        scale = d ** -0.5
     elif not (float(scale) > 0 and math.isfinite(float(scale))):
         raise ValueError(f"scale {scale}: the kernel needs a finite positive softmax scale")
-    q = _view(q)
-    out = torch.empty((b, h, d), dtype=q.dtype, device=dev)
+    q, q_p, q_sh, q_ss = _rows(q)
+    out = torch.empty((b, h, d), dtype=dtype, device=dev)
     lse = torch.empty((b, h), dtype=torch.float32, device=dev) if return_lse else None
     need = _decode.paged_attn_workspace_size(dev.index, b, h, hkv, d, most)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _decode.call_paged_attn(
-        _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[q.dtype], _DTYPES[k_cache.dtype], b, h, hkv, d, page, pages,
-        table.shape[1], most, _native.f32(float(scale)), q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), h * d, d,
-        0 if lse is None else lse.data_ptr(), k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3],
-        ks, vs, table.data_ptr(), table.stride(0), len_p, 0 if ws is None else ws.data_ptr(), max(need, 0))
+        _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[dtype], _DTYPES[k_cache.dtype], b, h, hkv, d, page, pages, width, most,
+        _native.f32(float(scale)), q_p, q_ss, q_sh, out.data_ptr(), h * d, d, 0 if lse is None else lse.data_ptr(),
+        *_cache_rows(k_cache), *_cache_rows(v_cache), ks, vs, table.data_ptr(), table.stride(0), len_p,
+        0 if ws is None else ws.data_ptr(), max(need, 0))
     out = out.transpose(0, 1)
     return (out, lse.transpose(0, 1)) if return_lse else out

@@ -28,19 +28,23 @@ class TokenLogprobs(NamedTuple):
 
 def _forward(logits, tokens, top, entropy):
     n, vocab = logits.shape
-    labels, dev = tokens.shape[1], logits.device
-    f32 = dict(dtype=torch.float32, device=dev)
-    logprobs, lse = torch.empty((n, labels), **f32), torch.empty(n, **f32)
-    ent = torch.empty(n, **f32) if entropy else None
-    top_lp = torch.empty((n, top), **f32) if top else None
-    top_ids = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
-    dtype = _DTYPES[logits.dtype]
+    dev, dtype = logits.device, _DTYPES[logits.dtype]
+    labels = tokens.shape[1] if tokens.dim() == 2 else 1
+    logprobs, lse = torch.empty(tokens.shape, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+    ent = top_lp = top_ids = None
+    ent_p = lp_p = id_p = 0
+    if entropy:
+        ent = torch.empty(n, dtype=torch.float32, device=dev)
+        ent_p = ent.data_ptr()
+    if top:
+        top_lp = torch.empty((n, top), dtype=torch.float32, device=dev)
+        top_ids = torch.empty((n, top), dtype=torch.int64, device=dev)
+        lp_p, id_p = top_lp.data_ptr(), top_ids.data_ptr()
     need = _decode.logprobs_workspace_size(dtype, n, vocab, top)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _decode.call_logprobs(
         _native.stream(dev), _decode.READOUT_ABI_VERSION, dtype, n, vocab, labels, top, logits.data_ptr(), logits.stride(0),
-        tokens.data_ptr(), tokens.stride(0), logprobs.data_ptr(), lse.data_ptr(), 0 if ent is None else ent.data_ptr(),
-        0 if top_lp is None else top_lp.data_ptr(), 0 if top_ids is None else top_ids.data_ptr(), ws.data_ptr(), need)
+        tokens.data_ptr(), tokens.stride(0), logprobs.data_ptr(), lse.data_ptr(), ent_p, lp_p, id_p, ws.data_ptr(), need)
     return logprobs, lse, ent, top_lp, top_ids
 
 
@@ -59,19 +63,23 @@ class _Logprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logprobs, g_lse, g_entropy, g_top, _g_ids):
         logits, tokens, lse, ent, top_ids = ctx.saved_tensors
-        grads = [None if g is None else g.contiguous() for g in (g_logprobs, g_lse, g_entropy, g_top)]
-        if not any(g is not None for g in grads):
-            return None, None, None, None
-        with torch.cuda.device(logits.device):
-            n, vocab = logits.shape
-            grad = torch.empty((n, vocab), dtype=logits.dtype, device=logits.device)
-            p_logp, p_lse, p_ent, p_top = (0 if g is None else g.data_ptr() for g in grads)
-            _decode.call_logprobs_grad(
-                _native.stream(logits.device), _decode.READOUT_ABI_VERSION, _DTYPES[logits.dtype], n, vocab, tokens.shape[1], ctx.top,
-                logits.data_ptr(), logits.stride(0), tokens.data_ptr(), tokens.stride(0), lse.data_ptr(),
-                0 if ent is None else ent.data_ptr(), 0 if top_ids is None else top_ids.data_ptr(), p_logp, p_lse, p_ent, p_top,
-                grad.data_ptr(), vocab)
-        return grad, None, None, None
+        if torch._C._cuda_getDevice() != logits.device.index:  # (the engine's thread is on the gradients' device)
+            with torch.cuda.device(logits.device):
+                return _backward(logits, tokens, lse, ent, top_ids, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
+        return _backward(logits, tokens, lse, ent, top_ids, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
+
+
+def _backward(logits, tokens, lse, ent, top_ids, top, *grads):
+    grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+    n, vocab = logits.shape
+    dtype = logits.dtype
+    grad = torch.empty((n, vocab), dtype=dtype, device=logits.device)
+    g_logp, g_lse, g_ent, g_top = (0 if g is None else g.data_ptr() for g in grads)
+    _decode.call_logprobs_grad(
+        _native.stream(logits.device), _decode.READOUT_ABI_VERSION, _DTYPES[dtype], n, vocab, tokens.shape[1] if tokens.dim() == 2 else 1, top,
+        logits.data_ptr(), logits.stride(0), tokens.data_ptr(), tokens.stride(0), lse.data_ptr(), 0 if ent is None else ent.data_ptr(),
+        0 if top_ids is None else top_ids.data_ptr(), g_logp, g_lse, g_ent, g_top, grad.data_ptr(), vocab)
+    return grad
 
 
 def token_logprobs(logits, tokens, *, top=0, entropy=False):
@@ -111,14 +119,11 @@ def token_logprobs(logits, tokens, *, top=0, entropy=False):
         raise ValueError(f"top {top}: at most {_decode.MAX_TOP} and the vocabulary's {vocab}, for at most {_decode.MAX_TOP_VOCAB} values")
     if has_tangent(logits):
         raise NotImplementedError("token_logprobs has no forward-mode derivative")
-    flat = tokens.dim() == 1
-    tokens = tokens.long()
-    if flat:
-        tokens = tokens.contiguous()[:, None]
-    elif tokens.shape[1] > 1 and tokens.stride(1) != 1:
+    if tokens.dtype != torch.int64:
+        tokens = tokens.long()
+    if tokens.dim() == 2 and tokens.stride(1) != 1 and tokens.shape[1] > 1:
         tokens = tokens.contiguous()
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
-    call = _Logprobs.apply if torch.is_grad_enabled() and logits.requires_grad else _forward
-    logprobs, *rest = call(logits, tokens, int(top), bool(entropy))
-    return TokenLogprobs(logprobs[:, 0] if flat else logprobs, *rest)
+    call = _Logprobs.apply if logits.requires_grad and torch.is_grad_enabled() else _forward
+    return TokenLogprobs(*call(logits, tokens, int(top), bool(entropy)))
