@@ -74,9 +74,9 @@ def _sized(name, *types):
 
 
 @functools.lru_cache(maxsize=1024)
-def paged_attn_workspace_size(device_index, num_seqs, num_heads, num_kv_heads, head_dim, max_len):
+def paged_attn_workspace_size(device_index, cache_dtype, num_seqs, num_heads, num_kv_heads, head_dim, max_len):
     """Bytes of workspace of one attention call on the (current) device (0: none; -1: invalid arguments)."""
-    return _sized("dan_paged_attn_workspace_size", *[_i32] * 5)(num_seqs, num_heads, num_kv_heads, head_dim, max_len)
+    return _sized("dan_paged_attn_workspace_size", *[_i32] * 6)(cache_dtype, num_seqs, num_heads, num_kv_heads, head_dim, max_len)
 
 
 @functools.lru_cache(maxsize=1024)

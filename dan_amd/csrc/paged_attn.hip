@@ -23,6 +23,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "cus.h"
 #include "dan_paged.h"
 #include "paged_index.h"
@@ -48,7 +50,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 #define DAN_GLOBAL __attribute__((address_space(1)))
 
-constexpr int kWaves = 4, kTile = 32, kHeads = 16;
+constexpr int kTile = 32, kHeads = 16;
 constexpr int kMaxLen = 1 << 30;  // places are 32-bit
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -102,6 +104,10 @@ __device__ inline float sum_across_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+constexpr int kMaxChunk = 2048;            // keys of a range, at most
+constexpr int kWideChunk = 768;            // from here on a range takes 8 waves
+constexpr int kDirectBytes = 192 * 1024;   // keys and values of one range without a join
+
 struct Params {
   const void *q, *kc, *vc;
   void *out;
@@ -111,7 +117,7 @@ struct Params {
   dan::PageTable table;
   const int32_t *lens;
   int64_t q_ss, q_sh, o_ss, o_sh, kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
-  int32_t B, H, Hkv, G, max_len, chunk, splits, blocks;
+  int32_t B, H, Hkv, G, max_len, target, splits, waves, blocks, chunk;  // chunk: of a sequence of max_len
   float scale;
 };
 
@@ -119,6 +125,16 @@ struct Params {
 __device__ inline int length_of(const Params &p, int b) {
   const int n = p.lens[b];
   return (uint32_t)n <= (uint32_t)p.max_len ? n : -1;
+}
+
+// Keys of a range of a sequence of `len`: a `target`-th of it, within limits, in whole rounds of the work
+// group's tiles. By its own length alone, so that a sequence's result does not change with its
+// neighbours', and a launch sized for max_len splits shorter ones well, too.
+__host__ __device__ inline int chunk_of(int len, int target, int splits, int waves) {
+  if (splits == 1) return len < 1 ? 1 : len;
+  const int round = kTile * waves, share = (int)(((uint32_t)(len < 0 ? 0 : len) + (uint32_t)target - 1) / (uint32_t)target);
+  const int chunk = (share + round - 1) / round * round;
+  return chunk < round ? round : chunk > kMaxChunk ? kMaxChunk : chunk;
 }
 
 template <typename T, int D, bool FP8>
@@ -196,11 +212,14 @@ __device__ inline uint32_t v_pair(const Tile<T, D, FP8> &t, int u, int r, int m)
   else return m & 1 ? Ops<T>::template from_e4m3<true>(t.v[u][r][m >> 1]) : Ops<T>::template from_e4m3<false>(t.v[u][r][m >> 1]);
 }
 
-template <typename T, int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
+// W waves. LDS: the waves' results [W][heads][D + 4], their maxima and sums [2][W][heads];
+// before that (D = 256) the q operand, in the order its steps read it.
+template <typename T, int D, bool FP8, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   typedef Tile<T, D, FP8> Tl;
-  constexpr int VE = Tl::VE, ES = Tl::ES, DP = D + 4;  // DP: a head's row in LDS
-  extern __shared__ __align__(16) float lds[];  // [waves][heads][DP], then maxima and sums [waves][heads]
+  constexpr int VE = Tl::VE, ES = Tl::ES, DP = D + 4, S = D / 32;
+  constexpr bool kQLds = D == 256;  // 32 registers that the tile needs
+  extern __shared__ __align__(16) float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4;
   // (kv head, block of 16 q heads) fastest, then the sequence, then the range
@@ -210,99 +229,104 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
   const int hk = at % p.Hkv;
   at /= p.Hkv;
   const int b = at % p.B, split = at / p.B;
-  const int len = length_of(p, b), lo = split * p.chunk;
   const int heads = min(p.G - hb * kHeads, kHeads);  // of this block
   const int head0 = hk * p.G + hb * kHeads;
   const bool direct = p.splits == 1;
+
+  // The length, q, and the pages that are this wave's if the sequence is of max_len, or this its first
+  // range, are loaded side by side: lane n takes the wave's 16-key block n.
+  const int mykey = kTile * (wave + W * (lane >> 1)) + 16 * (lane & 1);
+  dan::PageRow from = dan::find_row(p.table, b, split * p.chunk + mykey);
+  // q: column i is head min(i, heads - 1); dims as the key operand has them
+  const T *qrow = static_cast<const T *>(p.q) + b * p.q_ss + (head0 + min(i, heads - 1)) * p.q_sh;
+  auto q_step = [&](int s) { return *(const DAN_GLOBAL u32x4 *)(qrow + (FP8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g)); };
+  u32x4 qf[kQLds ? 1 : S];
+  u32x4 *ql = (u32x4 *)lds + lane;
+  if constexpr (kQLds) {
+    for (int s = wave; s < S; s += W) ql[64 * s] = q_step(s);
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; ++s) qf[s] = q_step(s);
+  }
+  float c = p.scale * kLog2e, vscale = 1.0f;
+  if constexpr (FP8) {
+    c *= *p.ks;
+    vscale = *p.vs;
+  }
+  const int len = length_of(p, b), chunk = chunk_of(len, p.target, p.splits, W), lo = split * chunk;
   if (lo >= len) {  // nothing here: the join leaves such ranges out (and takes wrong lengths to NaN)
     if (direct) {
       const float none = len < 0 ? __builtin_nanf("") : 0.0f;
-      for (int e = threadIdx.x; e < heads * D; e += 256) {
+      for (int e = threadIdx.x; e < heads * D; e += 64 * W) {
         static_cast<T *>(p.out)[b * p.o_ss + (head0 + e / D) * p.o_sh + e % D] = (T)none;
         if (p.lse && e % D == 0) p.lse[(int64_t)b * p.H + head0 + e / D] = len < 0 ? none : -INFINITY;
       }
     }
     return;
   }
-  const int hi = min(len, lo + p.chunk);
+  const int hi = min(len, lo + chunk);
   const int tiles = (hi - lo + kTile - 1) / kTile;
-  const int mine = wave < tiles ? (tiles - wave + kWaves - 1) / kWaves : 0;
+  const int mine = wave < tiles ? (tiles - wave + W - 1) / W : 0;  // at most 16 (kMaxChunk, kDirectBytes)
 
   f32x4 acc[VE];
 #pragma unroll
   for (int j = 0; j < VE; ++j) acc[j] = (f32x4){0, 0, 0, 0};
   float m = -INFINITY, l = 0.f;
-  uint64_t bad = 0;
 
   if (mine > 0) {
-    // q: column i is head min(i, heads - 1); dims as the key operand has them
-    u32x4 qf[D / 32];
-    {
-      const T *qrow = static_cast<const T *>(p.q) + b * p.q_ss + (head0 + min(i, heads - 1)) * p.q_sh;
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) {
-        const int dim = FP8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-        qf[s] = *(const DAN_GLOBAL u32x4 *)(qrow + dim);
-      }
-    }
-    float c = p.scale * kLog2e;
-    if constexpr (FP8) c *= *p.ks;
+    // Where the lane's block starts in the two caches. Page 0 stands in for a
+    // block behind the end and for a page that does not exist. A block starts at a multiple of 16
+    // rows, as a page's size is one, so all 16 lie in the page.
+    if (lo != split * p.chunk) from = dan::find_row(p.table, b, lo + mykey);
+    const bool there = lane < 2 * mine && lo + mykey < hi;
+    const uint64_t bad = __ballot(there && from.page < 0);
+    if (!there || from.page < 0) from = {0, 0};
+    const uint64_t kadr = (uint64_t)p.kc + (from.page * p.kc_sp + hk * p.kc_sh + from.row * p.kc_st) * ES;
+    const uint64_t vadr = (uint64_t)p.vc + (from.page * p.vc_sp + hk * p.vc_sh + from.row * p.vc_st) * ES;
     const uint32_t krow = (uint32_t)(p.kc_st * ES), vrow = (uint32_t)(p.vc_st * ES);
     const uint32_t koff = i * krow + 16 * g;
     const uint32_t voff = 4 * g * vrow + (D == 256 && !FP8 ? 16 * i : VE * ES * i);
-
-    // Lane n holds where this wave's 16-key block n (of the next 64) starts in the two caches.
-    uint64_t kadr = 0, vadr = 0;
-    auto find_pages = [&](int first) {
-      const int n = first + (lane >> 1);  // the tile
-      const int key = lo + kTile * (wave + kWaves * n) + 16 * (lane & 1);
-      const bool there = n < mine && key < hi;
-      // Page 0 stands in for a block behind the end and for a page that does not exist. A block starts
-      // at a multiple of 16 rows, as a page's size is one, so all 16 lie in the page.
-      dan::PageRow from = there ? dan::find_row(p.table, b, key) : dan::PageRow{0, 0};
-      bad |= __ballot(from.page < 0);
-      if (from.page < 0) from = {0, 0};
-      kadr = (uint64_t)p.kc + (from.page * p.kc_sp + hk * p.kc_sh + from.row * p.kc_st) * ES;
-      vadr = (uint64_t)p.vc + (from.page * p.vc_sp + hk * p.vc_sh + from.row * p.vc_st) * ES;
-    };
     auto at_lane = [&](uint64_t x, int n) -> const uint8_t * {
       const uint32_t a = __builtin_amdgcn_readlane((uint32_t)x, n), h = __builtin_amdgcn_readlane((uint32_t)(x >> 32), n);
       return (const uint8_t *)((uint64_t)h << 32 | a);
     };
     Tl t;
-    auto fetch_k = [&](int n) {
+    auto fetch_k = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) load_k<T, D, FP8>(t, u, at_lane(kadr, 2 * (n & 31) + u), koff);
+      for (int u = 0; u < 2; ++u) load_k<T, D, FP8>(t, u, at_lane(kadr, 2 * n + u), koff);
     };
-    auto fetch_v = [&](int n) {
+    auto fetch_v = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) load_v<T, D, FP8>(t, u, at_lane(vadr, 2 * (n & 31) + u), voff, vrow);
+      for (int u = 0; u < 2; ++u) load_v<T, D, FP8>(t, u, at_lane(vadr, 2 * n + u), voff, vrow);
     };
-
-    find_pages(0);
     fetch_k(0);
+    __builtin_amdgcn_sched_barrier(0);
     fetch_v(0);
-    for (int n = 0; n < mine; ++n) {
-      const int key0 = lo + kTile * (wave + kWaves * n);
-      // scores of keys key0 + 16 u + 4 g + r and head i
-      f32x4 sc[2];
+    __builtin_amdgcn_sched_barrier(0);
+
+    // One tile; the next one's keys are loaded once its own are spent, and its values likewise. The last tile
+    // is a copy of its own: a load under a condition would make the wait in front of each product
+    // one for all loads.
+    auto tile = [&](int n, auto last) __attribute__((always_inline)) {
+      f32x4 sc[2];  // scores of keys 16 u + 4 g + r and head i
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         sc[u] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) sc[u] = Ops<T>::mfma(k_operand<T, D, FP8>(t, u, s), qf[s], sc[u]);
+        for (int s = 0; s < S; ++s) sc[u] = Ops<T>::mfma(k_operand<T, D, FP8>(t, u, s), kQLds ? ql[64 * s] : qf[kQLds ? 0 : s], sc[u]);
       }
-      const bool more = n + 1 < mine;
-      if (more) {
-        if (((n + 1) & 31) == 0) find_pages(n + 1);
+      if constexpr (!last.value) {
         fetch_k(n + 1);
+        __builtin_amdgcn_sched_barrier(0);  // the scheduler would mix these loads with those of the values
       }
-      if (key0 + kTile > hi) {  // the sequence's last tile: no weight, and no value either, behind its end
+      if constexpr (last.value) {  // no weight, and no value either, behind the sequence's end
+        const int key0 = lo + kTile * (wave + W * n) + 4 * g;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (key0 + 16 * u + 4 * g + r >= hi) {
+            if (key0 + 16 * u + r >= hi) {
               sc[u][r] = -INFINITY;
 #pragma unroll
               for (int e = 0; e < Tl::VR; ++e) t.v[u][r][e] = 0;
@@ -356,14 +380,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
         acc[2 * e + 1] = Ops<T>::mfma(odd, pl, acc[2 * e + 1]);
         acc[2 * e + 1] = Ops<T>::mfma(odd, ph, acc[2 * e + 1]);
       }
-      if (more) fetch_v(n + 1);
-    }
+      if constexpr (!last.value) {
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_v(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for (int n = 0; n < mine - 1; ++n) tile(n, std::false_type());
+    tile(mine - 1, std::true_type());
     l = sum_across_groups(l);
     if (bad) l = __builtin_nanf("");
   }
 
   // The waves' results into LDS: lane (i, g) holds head i, value lanes 4 g .. 4 g + 3.
-  float *ml = lds + kWaves * heads * DP;
+  if constexpr (kQLds) __syncthreads();
+  float *ml = lds + W * heads * DP;
   if (i < heads) {
     float *row = lds + (wave * heads + i) * DP;
 #pragma unroll
@@ -375,17 +406,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
       }
     if (g == 0) {
       ml[wave * heads + i] = m;
-      ml[(kWaves + wave) * heads + i] = l;
+      ml[(W + wave) * heads + i] = l;
     }
   }
   __syncthreads();
-  float vscale = 1.0f;
-  if constexpr (FP8) vscale = *p.vs;
-  for (int e = threadIdx.x * 4; e < heads * D; e += 1024) {
+  for (int e = threadIdx.x * 4; e < heads * D; e += 256 * W) {
     const int h = e / D, d = e % D;
-    float mw[kWaves], top = -INFINITY;
+    float mw[W], top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       mw[w] = ml[w * heads + h];
       top = fmaxf(top, mw[w]);
     }
@@ -393,9 +422,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
     f32x4 o = {0, 0, 0, 0};
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float by = __builtin_amdgcn_exp2f(mw[w] - sub);
-      sum += by * ml[(kWaves + w) * heads + h];
+      sum += by * ml[(W + w) * heads + h];
       o += by * *(const f32x4 *)(lds + (w * heads + h) * DP + d);
     }
     const int64_t row = (int64_t)b * p.H + head0 + h;
@@ -415,42 +444,49 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Params p) {
   }
 }
 
-// One work group joins the ranges of a (sequence, head).
+// One work group joins the ranges of a (sequence, head): D / 4 lanes take every GR-th range with a running
+// maximum, so a range's maximum, sum and row are loaded side by side, and the GR results meet in LDS.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
-  constexpr int L = D / 4, GR = 256 / L;  // lanes of a row, rows at a time
+  constexpr int L = D / 4, GR = 256 / L;
   __shared__ float part[GR][D];
-  __shared__ float sums[GR];
+  __shared__ float tops[GR], sums[GR];
   const int64_t row = blockIdx.x;
   const int b = row / p.H, h = row % p.H;
-  const int len = length_of(p, b);
-  const int n = len <= 0 ? 0 : (len + p.chunk - 1) / p.chunk;
-  const float *ml = p.part + (int64_t)p.B * p.H * p.splits * D + row * p.splits * 2;
-  const int lane = threadIdx.x & 63;
-  float top = -INFINITY;
-  for (int s = lane; s < n; s += 64) top = fmaxf(top, ml[2 * s]);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float sub = top == -INFINITY ? 0.0f : top;
   const int gr = threadIdx.x / L, d = threadIdx.x % L * 4;
+  const float *ml = p.part + (int64_t)p.B * p.H * p.splits * D + row * p.splits * 2;
+  const float *rows = p.part + row * p.splits * D + d;
+  const int len = length_of(p, b);
+  const int chunk = chunk_of(len, p.target, p.splits, p.waves), n = len <= 0 ? 0 : (len + chunk - 1) / chunk;
   f32x4 o = {0, 0, 0, 0};
-  float sum = 0.f;
+  float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
   for (int s = gr; s < n; s += GR) {
-    const float by = __builtin_amdgcn_exp2f(ml[2 * s] - sub);
-    sum += by * ml[2 * s + 1];
-    o += by * *(const DAN_GLOBAL f32x4 *)(p.part + (row * p.splits + s) * D + d);
+    const f32x2 q = *(const DAN_GLOBAL f32x2 *)(ml + 2 * s);
+    const f32x4 x = *(const DAN_GLOBAL f32x4 *)(rows + (int64_t)s * D);
+    const float to = fmaxf(top, q[0]), sub = to == -INFINITY ? 0.0f : to;
+    const float was = __builtin_amdgcn_exp2f(top - sub), by = __builtin_amdgcn_exp2f(q[0] - sub);
+    top = to;
+    sum = __builtin_fmaf(by, q[1], was * sum);
+    o = was * o + by * x;
   }
   *(f32x4 *)&part[gr][d] = o;
-  if (d == 0) sums[gr] = sum;
+  if (d == 0) {
+    tops[gr] = top;
+    sums[gr] = sum;
+  }
   __syncthreads();
   if (threadIdx.x < L) {
+#pragma unroll
+    for (int w = 0; w < GR; ++w) top = fmaxf(top, tops[w]);
+    const float sub = top == -INFINITY ? 0.0f : top;
     o = (f32x4){0, 0, 0, 0};
     sum = 0.f;
 #pragma unroll
     for (int w = 0; w < GR; ++w) {
-      o += *(const f32x4 *)&part[w][d];
-      sum += sums[w];
+      const float by = __builtin_amdgcn_exp2f(tops[w] - sub);
+      o += by * *(const f32x4 *)&part[w][d];
+      sum += by * sums[w];
     }
     const float inv = len > 0 ? 1.0f / sum : len == 0 ? 0.0f : __builtin_nanf("");
     typename Ops<T>::x4 y = __builtin_convertvector(o * inv, typename Ops<T>::x4);
@@ -459,30 +495,48 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
   }
 }
 
-// How a launch is split over the keys: ranges of `chunk` keys (whole rounds of the
-// work group's waves), `splits` of them up to max_len.
+// How a launch is split over the keys: work groups of `waves` waves, `splits` ranges of a
+// sequence of max_len keys.
 struct Split {
-  int chunk, splits;
+  int waves, target, splits, chunk;
 };
-Split split_of(int64_t groups, int max_len, int cus) {
-  const int round = kWaves * kTile;
-  const int64_t want = 2 * (int64_t)(cus > 0 ? cus : 256);  // work groups resident at once, two per CU
+Split split_of(int64_t seqs, int64_t groups, int max_len, int head_dim, int key_bytes, int cus) {
+  if (cus <= 0) cus = 256;
   if (groups < 1) groups = 1;  // no sequences
-  int64_t splits = (want + groups - 1) / groups;
-  int64_t chunk = (max_len + splits - 1) / splits;
-  chunk = (chunk + round - 1) / round * round;
-  if (chunk < round) chunk = round;
-  if (chunk > 1024) chunk = 1024;
-  splits = max_len > 0 ? (max_len + chunk - 1) / chunk : 1;
-  return {(int)chunk, (int)splits};
+  if ((int64_t)max_len * key_bytes <= kDirectBytes) return {4, 1, 1, chunk_of(max_len, 1, 1, 4)};
+  const int64_t want = (seqs == 1 ? 1 : head_dim == 256 ? 2 : 4) * (int64_t)cus, shares = (want + groups - 1) / groups;
+  auto of = [&](int waves) {
+    const int64_t most = (max_len + kTile * waves - 1) / (kTile * waves);  // ranges of the shortest length
+    const int target = (int)(shares < most ? shares : most), least = (max_len + kMaxChunk - 1) / kMaxChunk;
+    const int splits = target > least ? target : least;
+    return Split{waves, target, splits, chunk_of(max_len, target, splits, waves)};
+  };
+  const Split s = of(4);
+  return s.chunk >= kWideChunk && head_dim <= 128 ? of(8) : s;
+}
+
+template <typename T, int D, bool FP8, int W>
+void launch_waves(const Params &p, hipStream_t s) {
+  const int heads = p.G < kHeads ? p.G : kHeads;
+  const size_t out = sizeof(float) * W * heads * (D + 4 + 2), q = D == 256 ? 16 * 64 * (D / 32) : 0;
+  constexpr int kMost = (int)sizeof(float) * W * kHeads * (D + 4 + 2);
+  auto kernel = paged_attn_kernel<T, D, FP8, W>;
+  if constexpr (kMost > 64 * 1024) {  // beyond what a launch may have unasked; an error is the launch's
+    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    (void)allowed;
+  }
+  const unsigned grid = (unsigned)((int64_t)p.splits * p.B * p.Hkv * p.blocks);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * W), out > q ? out : q, s, p);
 }
 
 template <typename T, int D, bool FP8>
 void launch(const Params &p, hipStream_t s) {
-  const int heads = p.G < kHeads ? p.G : kHeads;
-  const size_t bytes = sizeof(float) * kWaves * heads * (D + 4 + 2);
-  const unsigned grid = (unsigned)((int64_t)p.splits * p.B * p.Hkv * p.blocks);
-  hipLaunchKernelGGL((paged_attn_kernel<T, D, FP8>), dim3(grid), dim3(256), bytes, s, p);
+  if constexpr (D <= 128) {
+    if (p.waves == 8) launch_waves<T, D, FP8, 8>(p, s);
+    else launch_waves<T, D, FP8, 4>(p, s);
+  } else {
+    launch_waves<T, D, FP8, 4>(p, s);
+  }
   if (p.splits > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)((int64_t)p.B * p.H)), dim3(256), 0, s, p);
 }
 
@@ -497,13 +551,15 @@ void by_dim(const Params &p, int d, bool fp8, hipStream_t s) {
 
 extern "C" {
 
-int64_t dan_paged_attn_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_len) {
+int64_t dan_paged_attn_workspace_size(int32_t cache_dtype, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      int32_t max_len) {
   using namespace dan_pattn;
   if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || max_len < 0 || max_len > kMaxLen ||
-      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
+      (cache_dtype != DAN_DTYPE_BF16 && cache_dtype != DAN_DTYPE_F16 && cache_dtype != DAN_DTYPE_E4M3))
     return -1;
   const int64_t blocks = (num_heads / num_kv_heads + kHeads - 1) / kHeads;
-  const Split sp = split_of((int64_t)num_seqs * num_kv_heads * blocks, max_len, dan::num_cus());
+  const Split sp = split_of(num_seqs, (int64_t)num_seqs * num_kv_heads * blocks, max_len, head_dim, head_dim * (cache_dtype == DAN_DTYPE_E4M3 ? 2 : 4), dan::num_cus());
   return sp.splits > 1 ? (int64_t)num_seqs * num_heads * sp.splits * (head_dim + 2) * 4 : 0;
 }
 
@@ -551,8 +607,8 @@ int dan_paged_attn(const DanPagedAttnArgs *a, void *stream) {
   p.vc_sp = a->vc_stride_page; p.vc_sh = a->vc_stride_head; p.vc_st = a->vc_stride_tok;
   p.B = B; p.H = H; p.Hkv = Hkv; p.G = H / Hkv;
   p.max_len = a->max_len; p.blocks = (p.G + kHeads - 1) / kHeads; p.scale = a->scale;
-  const Split sp = split_of((int64_t)B * Hkv * p.blocks, a->max_len, dan::num_cus());
-  p.chunk = sp.chunk; p.splits = sp.splits;
+  const Split sp = split_of(B, (int64_t)B * Hkv * p.blocks, a->max_len, D, 2 * D * es, dan::num_cus());
+  p.target = sp.target; p.splits = sp.splits; p.waves = sp.waves; p.chunk = sp.chunk;
   if ((int64_t)sp.splits * B * Hkv * p.blocks >= (int64_t)1 << 31 || (int64_t)B * H >= (int64_t)1 << 31)
     return fail(DAN_ERR_INVALID_ARGUMENT, "too many work groups");
   if (sp.splits > 1) {

@@ -199,8 +199,8 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
     zeros and -inf. A length outside [0, max_len], or a page outside the
     cache, gives NaN for its sequence.
 
-    The keys are split between work groups by B, Hkv and ``max_len`` alone, so a
-    sequence's result does not depend on its neighbours' lengths."""
+    How a sequence's keys are split between work groups follows from its own length,
+    B, Hkv and ``max_len``: its result does not depend on its neighbours' lengths."""
     dev = q.device
     if not q.is_cuda:
         raise RuntimeError(f"dan_amd.attend_paged runs on a gfx950 GPU only; got tensors on {dev}")
@@ -231,10 +231,11 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
     q, q_p, q_sh, q_ss = _rows(q)
     out = torch.empty((b, h, d), dtype=dtype, device=dev)
     lse = torch.empty((b, h), dtype=torch.float32, device=dev) if return_lse else None
-    need = _decode.paged_attn_workspace_size(dev.index, b, h, hkv, d, most)
+    kind = _DTYPES[k_cache.dtype]
+    need = _decode.paged_attn_workspace_size(dev.index, kind, b, h, hkv, d, most)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _decode.call_paged_attn(
-        _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[dtype], _DTYPES[k_cache.dtype], b, h, hkv, d, page, pages, width, most,
+        _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[dtype], kind, b, h, hkv, d, page, pages, width, most,
         _native.f32(float(scale)), q_p, q_ss, q_sh, out.data_ptr(), h * d, d, 0 if lse is None else lse.data_ptr(),
         *_cache_rows(k_cache), *_cache_rows(v_cache), ks, vs, table.data_ptr(), table.stride(0), len_p,
         0 if ws is None else ws.data_ptr(), max(need, 0))

@@ -102,7 +102,8 @@ int dan_paged_attn(const DanPagedAttnArgs *args, void *stream);
 
 /* Bytes of workspace of such a call on the current device (0: none is
  * needed; -1: invalid arguments). */
-int64_t dan_paged_attn_workspace_size(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_len);
+int64_t dan_paged_attn_workspace_size(int32_t cache_dtype, int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      int32_t max_len);
 
 /* DAN_PAGED_ABI_VERSION of the loaded library. */
 int dan_paged_abi_version(void);

@@ -126,8 +126,10 @@ def test_nothing_to_do_is_no_error(lib):
 def test_workspace_sizes(lib):
     """None for no sequences or keys; -1 (0 for the readout) for what the calls refuse."""
     size = _decode.paged_attn_workspace_size
-    assert size(-1, 0, 8, 2, 128, 4096) == 0 and size(-1, 3, 8, 2, 128, 0) == 0 and size(-1, 1, 8, 2, 128, 1 << 20) > 0
-    assert all(size(-1, *a) == -1 for a in ((1, 9, 2, 128, 16), (1, 8, 0, 128, 16), (1, 8, 2, 96, 16), (1, 8, 2, 128, -1), (-1, 8, 2, 128, 1), (1, 8, 2, 128, (1 << 30) + 1)))
+    assert size(-1, 0, 0, 8, 2, 128, 4096) == 0
+    assert size(-1, 0, 3, 8, 2, 128, 0) == 0 and size(-1, 0, 1, 8, 2, 128, 1 << 20) > 0 and size(-1, 3, 1, 8, 2, 128, 1 << 20) > 0
+    assert all(size(-1, *a) == -1 for a in ((0, 1, 9, 2, 128, 16), (0, 1, 8, 0, 128, 16), (1, 1, 8, 2, 96, 16), (0, 1, 8, 2, 128, -1),
+                                            (0, -1, 8, 2, 128, 1), (0, 1, 8, 2, 128, (1 << 30) + 1), (2, 1, 8, 2, 128, 1)))
     assert _decode.logprobs_workspace_size(0, 0, 100, 0) == 16 and _decode.logprobs_workspace_size(3, 1, 100, 0) == 0
 
 

@@ -319,6 +319,15 @@ def test_attend_long_and_many(gpu):
     run_attend(gpu, [1] * 300, 8, 2, 64)
 
 
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attend_many_heads_of_one_group(gpu, d, cache):
+    """16 and more q heads of a kv head (the largest work group memory), in ranges of four and of eight waves."""
+    run_attend(gpu, [60, 3001, 0, 1], 16, 1, d, cache=cache)
+    run_attend(gpu, [1 + 17 * (i % 60) for i in range(300)], 18, 1, d, cache=cache, seed=1)
+    run_attend(gpu, [2500] * 20 + [900, 2499, 0], 32, 16, d, cache=cache, seed=2)
+
+
 def test_attend_scales_layouts_and_capacity(gpu):
     run_attend(gpu, [33, 500], 8, 2, 128, std=20.0)  # peaked weights
     run_attend(gpu, [33, 500], 8, 2, 128, scale=0.013)
