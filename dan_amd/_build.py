@@ -1,6 +1,7 @@
-"""Build recipe for the gfx950 shared library (hipcc, in-tree).
+"""Build recipe for the gfx950 shared library (hipcc, in-tree) and the host
+module of the decode step's calls (g++).
 
-    python -m dan_amd._build          # -> dan_amd/_lib/libdan_tree_attn.so
+    python -m dan_amd._build          # -> dan_amd/_lib/libdan_tree_attn.so, _decode_calls.so
 
 Flags:
   --offload-arch=gfx950            CDNA4 only, no other targets.
@@ -36,6 +37,9 @@ SRC_FLAGS = {"tree_attn.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"]}
 # accumulators per lane live in the accumulation registers (AGPRs).
 MFMA_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 ACC_IN_AGPRS = {"fp8_gemm.hip"}
+# The host side of the decode step's plain calls: a CPython module on torch's headers (g++).
+CALLS_SRC = os.path.join(HERE, "csrc", "decode_calls.cpp")
+CALLS_NAME = "_decode_calls.so"
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(OUT_DIR, "libdan_tree_attn.so")
@@ -55,6 +59,19 @@ def hipcc():
     return path
 
 
+def calls_command(out):
+    import sysconfig
+
+    import torch
+
+    home = os.path.dirname(torch.__file__)
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I", INCLUDE,
+            *(f for d in (os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
+                          sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")) for f in ("-isystem", d)),
+            CALLS_SRC, "-o", out, "-L", os.path.join(home, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+
+
 def _run(cmd, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
@@ -63,7 +80,7 @@ def _run(cmd, verbose):
     noise = "is not a recognized feature for this target"
     diag = "\n".join(line for line in (res.stderr or "").splitlines() if noise not in line)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{diag}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{diag}")
     if diag.strip() and verbose:
         print(diag, file=sys.stderr)
 
@@ -81,12 +98,15 @@ def build(out=OUT, extra=(), verbose=False):
         return [*HIPCC_FLAGS, *([] if name in ACC_IN_AGPRS else MFMA_VGPR_FORM), *SRC_FLAGS.get(name, [])]
 
     cmds = [[hipcc(), *flags(src), *extra, "-I", INCLUDE, "-c", src, "-o", obj] for src, obj in zip(SRCS, objs)]
+    calls = os.path.join(os.path.dirname(out), CALLS_NAME)
+    cmds.insert(0, calls_command(calls + ".tmp"))
     with ThreadPoolExecutor(max_workers=min(len(cmds), max(1, (os.cpu_count() or 1)))) as pool:
         for f in [pool.submit(_run, c, verbose) for c in cmds]:
             f.result()
     tmp = out + ".tmp"
     _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", tmp], verbose)
     os.replace(tmp, out)
+    os.replace(calls + ".tmp", calls)
     return out
 
 

@@ -3,6 +3,9 @@ structures and entry points of a decode step's operators, in the library that
 ``_native`` loads."""
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
+import os
 
 from . import _native
 
@@ -83,3 +86,19 @@ def paged_attn_workspace_size(device_index, cache_dtype, num_seqs, num_heads, nu
 def logprobs_workspace_size(dtype, rows, vocab, top):
     """Bytes of workspace of one forward call (0: invalid arguments)."""
     return _sized("dan_logprobs_workspace_size", *[_i32] * 4)(dtype, rows, vocab, top)
+
+
+@functools.lru_cache(maxsize=None)
+def calls():
+    """The host module of the plain calls (csrc/decode_calls.cpp), bound to the library. Like the
+    library it has to be there: there is no fallback for a missing one."""
+    lib, path = _native.load(), os.path.join(_native.LIB_DIR, "_decode_calls.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is not built; run __graft_entry__.build()")
+    loader = importlib.machinery.ExtensionFileLoader("_decode_calls", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_decode_calls", loader))
+    loader.exec_module(module)
+    module.bind(*(ctypes.cast(lib[name], ctypes.c_void_p).value for name in (
+        "dan_paged_append", "dan_paged_attn", "dan_paged_attn_workspace_size", "dan_logprobs_fwd", "dan_logprobs_bwd",
+        "dan_logprobs_workspace_size", "dan_tree_attn_last_error")))
+    return module

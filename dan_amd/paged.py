@@ -102,6 +102,10 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
     without q). All arithmetic is fp32, rounded once at each store (an e4m3
     cache: ``x / scale`` clamped to +-448), where ``qkv_front`` rounds after each of the
     reference's eager ops; the two differ by up to two roundings of the dtype."""
+    out = _decode.calls().append(q, k, v, cos, sin, k_cache, v_cache, table, places, seqs, rope_rows, q_norm_weight, k_norm_weight,
+                                 eps, NORMS.get(norm, -1), k_scale, v_scale)
+    if out is not None:  # a plain call, made
+        return out
     dev = k.device
     if not k.is_cuda:
         raise RuntimeError(f"dan_amd.append_paged runs on a gfx950 GPU only; got tensors on {dev}")
@@ -201,6 +205,9 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
 
     How a sequence's keys are split between work groups follows from its own length,
     B, Hkv and ``max_len``: its result does not depend on its neighbours' lengths."""
+    made = _decode.calls().attend(q, k_cache, v_cache, table, lens, scale, k_scale, v_scale, max_len, return_lse)
+    if made is not None:  # a plain call
+        return made
     dev = q.device
     if not q.is_cuda:
         raise RuntimeError(f"dan_amd.attend_paged runs on a gfx950 GPU only; got tensors on {dev}")

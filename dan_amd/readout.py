@@ -104,6 +104,9 @@ def token_logprobs(logits, tokens, *, top=0, entropy=False):
     Where ``logits`` requires grad, every output but ``top_ids`` is
     differentiable (once): the gradient has the logits' dtype, computed in fp32
     and rounded once; a token given twice adds up."""
+    made = _decode.calls().logprobs(logits, tokens, top, entropy)
+    if made is not None:  # a plain call
+        return TokenLogprobs._make(made)
     dev = logits.device
     if not logits.is_cuda:
         raise RuntimeError(f"dan_amd.token_logprobs runs on a gfx950 GPU only; got tensors on {dev}")

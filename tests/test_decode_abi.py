@@ -147,6 +147,14 @@ def test_cpu_tensors_are_refused():
         token_logprobs(torch.zeros(2, 5), torch.zeros(2, dtype=torch.long))
 
 
+def test_host_module(lib):
+    calls = _decode.calls()
+    assert _decode.calls() is calls
+    for addresses in ((), (1,) * 6, (0,) * 7):
+        with pytest.raises((TypeError, ValueError)):
+            calls.bind(*addresses)
+
+
 def test_wrong_places_and_pages_find_no_row(tmp_path):
     """find_row: every value that a table, a place or a sequence may hold, against the oracle; the table lies
     between guard values that would be valid pages."""

@@ -181,3 +181,77 @@ def test_gradient_replays(gpu):
         torch.cuda.synchronize()
         have = out.clone()
         assert torch.equal(have, grad())
+
+
+class _Rest:
+    """Stands for the host module: makes no call, so that the Python functions make every one."""
+
+    append = attend = logprobs = staticmethod(lambda *args: None)
+
+
+def test_both_host_paths_make_the_same_calls(gpu, monkeypatch):
+    """Plain calls go through the host module, all others through Python: here the same calls through either."""
+    say("decode step: host module and Python")
+    from dan_amd import _decode
+
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(3, (H + 2 * HKV) * D, generator=g).to(BF16).to(gpu)
+    tokens = torch.randint(-1, VOCAB, (3, 2), generator=g).to(gpu)
+    x = torch.randn(4, VOCAB, generator=g).to(gpu).requires_grad_()
+
+    def run():
+        m = Layer(gpu, 3, 700, seed=3)
+        m.kc.zero_()
+        m.vc.zero_()
+        out = list(m.step(qkv, ids([650, 0, -1], gpu), ids([651, 1, 0], gpu), tokens)) + [m.kc, m.vc]
+        cache8 = m.kc.to(torch.float8_e4m3fn)
+        scale = torch.full((1,), 0.5, device=gpu)
+        out += attend_paged(out[0], cache8, cache8, m.table, ids([651, 1, 0], gpu), 0.1, k_scale=scale, v_scale=scale, max_len=660, return_lse=True)
+        r = token_logprobs(x, torch.arange(4, device=gpu), top=3, entropy=True)
+        out += list(r) + [torch.autograd.grad([r.logprobs, r.logsumexp, r.entropy, r.top_logprobs], x, [torch.ones_like(t) for t in (r.logprobs, r.logsumexp, r.entropy, r.top_logprobs)])[0]]
+        torch.cuda.synchronize()
+        return out
+
+    made = []
+    real = _decode.calls()
+
+    class Watch:
+        append, attend, logprobs = (staticmethod(lambda *a, f=f: made.append(f(*a)) or made[-1]) for f in (real.append, real.attend, real.logprobs))
+
+    monkeypatch.setattr(_decode, "calls", lambda: Watch)
+    first = run()
+    assert len(made) == 5 and all(m is not None for m in made)
+    monkeypatch.setattr(_decode, "calls", lambda: _Rest)
+    for a, b in zip(first, run(), strict=True):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and torch.equal(a, b)
+
+
+def test_what_is_not_plain_is_left_to_python(gpu):
+    """The host module makes no call on other types, layouts, sizes, or where a gradient or tangent is to be refused."""
+    say("host module: calls it leaves")
+    from dan_amd import _decode
+
+    c = _decode.calls()
+    m = Layer(gpu, 2, 64)
+    q, k = torch.zeros(2, H, D, dtype=BF16, device=gpu), torch.zeros(2, HKV, D, dtype=BF16, device=gpu)
+    places, lens, norm = ids([0, 1], gpu), ids([1, 2], gpu), 0
+    a = lambda **w: c.append(*{**dict(q=q, k=k, v=k, cos=None, sin=None, kc=m.kc, vc=m.vc, t=m.table, p=places, s=None, r=None, qw=None, kw=None, e=1e-6,
+                                      n=norm, ks=None, vs=None), **w}.values())
+    t = lambda **w: c.attend(*{**dict(q=q.transpose(0, 1), kc=m.kc, vc=m.vc, t=m.table, l=lens, s=None, ks=None, vs=None, m=None, r=False), **w}.values())
+    x, tok = torch.zeros(2, 50, device=gpu), torch.zeros(2, dtype=torch.long, device=gpu)
+    r = lambda **w: c.logprobs(*{**dict(x=x, t=tok, top=1, e=False), **w}.values())
+    assert a() is not None and t() is not None and r() is not None
+    odd = torch.zeros(2 * HKV * D + 1, dtype=BF16, device=gpu)[1:].view(2, HKV, D)
+    dual = torch.autograd.forward_ad
+    for w in (dict(q=None), dict(k=odd), dict(q=q.cpu()), dict(k=k.clone().requires_grad_()), dict(p=places.long()), dict(n=1), dict(n=-1), dict(n=3),
+              dict(t=m.table.t()), dict(kc=m.kc[:, :, :, :64]), dict(kc=m.kc[:1].expand(m.kc.shape)), dict(ks=x[:1, 0]), dict(cos=x), dict(sin=x), dict(e=1),
+              dict(q=5), dict(s=places[:1]), dict(vc=m.vc.half()), dict(p=m.table[:, 0].cpu())):
+        assert a(**w) is None, w
+    for w in (dict(q=q), dict(m=10 ** 30), dict(m=-1), dict(m=65), dict(s=0.0), dict(s=math.nan), dict(s=1), dict(l=lens.long()), dict(q=q.float().transpose(0, 1)),
+              dict(q=q.transpose(0, 1)[:7]), dict(t=m.table[:1]), dict(kc=None), dict(q=q.transpose(0, 1).clone().requires_grad_())):
+        assert t(**w) is None, w
+    for w in (dict(top=33), dict(top=-1), dict(top=10 ** 30), dict(t=tok.int()), dict(x=x.double()), dict(x=x.t()[:, :0]), dict(x=x[0]), dict(t=None), dict(top=None), dict(x=x.cpu())):
+        assert r(**w) is None, w
+    with dual.dual_level():
+        assert r(x=dual.make_dual(x, x)) is None and t(q=dual.make_dual(q, q).transpose(0, 1)) is None
+    assert c.append() is None and c.attend(1) is None and c.logprobs() is None
