@@ -30,6 +30,7 @@ namespace dan_logp {
 #define DAN_GLOBAL __attribute__((address_space(1)))
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kVecs = 8;               // vectors a lane
 constexpr int kChunk = 64 * kVecs;     // vectors a wave
@@ -268,8 +269,9 @@ __device__ inline int below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-constexpr int kTaken = 32;   // groups whose values a work group holds: 8 vectors a lane of 4 waves
-constexpr int kCand = 256;
+constexpr int kTaken = 32;    // groups whose values a work group holds: 8 vectors a lane of 4 waves
+constexpr int kCand = 64;     // values that a wave collects
+constexpr uint32_t kLowest = 0x007fffffu;  // order(-inf): every value reaches it
 
 // Raises `bound` by bisection, between what K or more of a set's keys reach and `over`, which
 // fewer do, until at most `most` reach it or the two are neighbours; `have` is how many
@@ -289,9 +291,9 @@ __device__ inline void bisect(uint32_t &bound, uint32_t &over, int &have, int k,
 //     where too many are equal at it, that value itself. K values of the row reach it, so the row's K
 //     largest do, and they lie in these groups (of those whose maximum is the bound itself, in
 //     the first that make up K).
-//  2. The work group loads these groups and collects the values that reach the bound: in rows of
-//     ordinary logits few more than K. Of values equal to a bound that too many reach (masked rows: the
-//     masked value) each wave collects its first K. Where more than 256 come together (no more
+//  2. The work group loads these groups and each wave collects its values that reach the bound: in
+//     rows of ordinary logits few more than K in all. Of values equal to a bound that too many reach (masked
+//     rows: the masked value) each wave collects its first K. Where a wave has more than 64 (no more
 //     groups than K; most of the largest side by side) the bound is raised by bisection over the
 //     lanes' maxima, and if need be over the values.
 //  3. Each collected value's rank among them is its place in the result.
@@ -300,9 +302,10 @@ template <typename T, int KEYS>
 __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
   constexpr int n = Vec<T>::n, kRegs = kTaken / 4;
   __shared__ int group[4][kTaken];
-  __shared__ uint64_t cand[kCand];
+  __shared__ u32x4 kept[4][kRegs][64];
+  __shared__ uint64_t cand[4][kCand];
   __shared__ uint32_t lane_max[256];
-  __shared__ int count, sums[2][4];
+  __shared__ int counts[4], sums[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t r = blockIdx.x;
   const int vectors = (p.V + n - 1) / n, groups = (vectors + 63) / 64;
@@ -312,7 +315,6 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) g[i] = lane + 64 * i < groups ? gm[lane + 64 * i] : 0.0f;
   const Given given = fetch<T>(p, r, tid);
-  if (tid == 0) count = 0;
   uint32_t o[KEYS];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) o[i] = lane + 64 * i < groups ? order(g[i]) : 0;
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
     for (int i = 0; i < KEYS; ++i) c += __builtin_popcountll(__ballot(o[i] >= x));
     return c;
   };
-  const int most = min(kTaken, p.K + p.K / 4 + 2);
+  const int most = min(kTaken, p.K + p.K / 2 + 4);
   uint32_t best = o[0];
 #pragma unroll
   for (int i = 1; i < KEYS; ++i) best = max(best, o[i]);
@@ -333,8 +335,8 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
   uint32_t over = wave_fold(best, [](uint32_t x, uint32_t y) { return max(x, y); }) + 1;
   int have = reach(bound);
   if (have > p.K) bisect(bound, over, have, p.K, most, reach);
-  if (groups <= p.K) bound = 1, have = groups;  // all of them (of one maximum or of many)
-  bool equal = have > kTaken;  // then over = bound + 1
+  if (groups <= p.K) bound = kLowest, have = groups;  // all of them
+  bool equal = have > kTaken;                         // then over = bound + 1
   const int left = equal ? p.K - reach(over) : 0, taken = equal ? p.K : have;
   {
     int at = 0, before = 0;
@@ -346,6 +348,7 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
         in = in || (o[i] == bound && before + below(same) < left);
         before += __builtin_popcountll(same);
       }
+      in = in && lane + 64 * i < groups;
       const uint64_t mask = __ballot(in);
       if (in) group[wave][at + below(mask)] = lane + 64 * i;
       at += __builtin_popcountll(mask);
@@ -354,24 +357,32 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
   __builtin_amdgcn_wave_barrier();  // a wave reads its own list
 
   // 2. Wave w takes groups w, w + 4, ..; rising ones, so that of equal values the first come first.
+  // What lies behind the row's end is NaN, which reaches no bound.
   const T *x = static_cast<const T *>(p.x) + r * p.x_st;
   const int whole = p.V / n, mine = (taken - wave + 3) / 4;
-  typename Vec<T>::type raw[kRegs];
+  // They are kept in LDS (a wave's own part), where loops over them need few registers.
+  u32x4 raw[kRegs];
   int at[kRegs];
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
     at[i] = i < mine ? group[wave][wave + 4 * i] * 64 + lane : vectors;
-    if (whole > 0 && i < mine) raw[i] = *(const DAN_GLOBAL typename Vec<T>::loose *)(x + (int64_t)n * min(at[i], whole - 1));
+    if (whole > 0 && i < mine) raw[i] = __builtin_bit_cast(u32x4, *(const DAN_GLOBAL typename Vec<T>::loose *)(x + (int64_t)n * min(at[i], whole - 1)));
   }
-  if (p.V != whole * n) {  // the row's last values fill no vector: one lane reads them one by one
+  u32x4 tail = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // NaN in every type
+  if (p.V != whole * n) {                                           // the row's last values fill no vector: one by one
+    const uint16_t *last = (const uint16_t *)(x + (int64_t)n * whole);
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      if (at[i] == whole) {
-#pragma unroll
-        for (int e = 0; e < n; ++e)
-          if (n * whole + e < p.V) raw[i][e] = x[n * whole + e];
-      }
+    for (int e = 0; e < 8; ++e)
+      if ((int)sizeof(T) * (p.V - n * whole) > 2 * e) tail[e / 2] = e % 2 ? (tail[e / 2] & 0xffffu) | (uint32_t)last[e] << 16 : (tail[e / 2] & 0xffff0000u) | last[e];
   }
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i)
+    if (i < mine) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) raw[i][c] = at[i] < whole ? raw[i][c] : at[i] == whole ? tail[c] : 0x7fff7fffu;
+      kept[wave][i][lane] = raw[i];
+    }
+  __builtin_amdgcn_wave_barrier();
 
   const Row row = join(p, r, lane, first);
   const float m = row.m == -INFINITY ? 0.0f : row.m, logl = logf(row.l);
@@ -384,29 +395,19 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
     return;
   }
 
-  auto is_there = [&](int i, int e) { return at[i] < whole || (at[i] == whole && n * whole + e < p.V); };
-  auto values = [&](int i) { return __builtin_convertvector(raw[i], typename Vec<T>::f32); };
-  auto largest = [&](int i) {
-    const typename Vec<T>::f32 f = values(i);
+  auto values = [&](int i) { return __builtin_convertvector(__builtin_bit_cast(typename Vec<T>::type, kept[wave][i][lane]), typename Vec<T>::f32); };
+  auto largest = [&](typename Vec<T>::f32 f) {
     float y = f[0];
 #pragma unroll
     for (int e = 1; e < n; ++e) y = fmaxf(y, f[e]);
     return y;
   };
-  int total = 0;
   for (int stage = groups > p.K ? 0 : 1;; ++stage) {
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) asm("" : "+v"(raw[i]), "+v"(at[i]));  // what a turn makes of them is not kept over the turns
     if (stage == 1) {  // K or more of the lanes' maxima reach it, so as many values do
       uint32_t mx = 0, q[4];
-#pragma unroll
-      for (int i = 0; i < kRegs; ++i) {
-        if (at[i] < whole) mx = max(mx, order(largest(i)));
-        if (at[i] == whole) {
-#pragma unroll
-          for (int e = 0; e < n; ++e)
-            if (is_there(i, e)) mx = max(mx, order((float)raw[i][e]));
-        }
+      for (int i = 0; i < mine; ++i) {
+        const float y = largest(values(i));
+        mx = y == y ? max(mx, order(y)) : mx;
       }
       lane_max[tid] = mx;
       __syncthreads();
@@ -425,12 +426,12 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
     } else if (stage == 2) {
       int turn = 0;
       auto reach_values = [&](uint32_t y) {
+        const float v = value_of(y);  // NaN above +inf's place: reached by none
         int c = 0;
-#pragma unroll
-        for (int i = 0; i < kRegs; ++i) {
+        for (int i = 0; i < mine; ++i) {
           const typename Vec<T>::f32 f = values(i);
 #pragma unroll
-          for (int e = 0; e < n; ++e) c += __builtin_popcountll(__ballot(is_there(i, e) && order(f[e]) >= y));
+          for (int e = 0; e < n; ++e) c += __builtin_popcountll(__ballot(f[e] >= v));
         }
         if (lane == 0) sums[turn & 1][wave] = c;
         __syncthreads();
@@ -438,83 +439,73 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
         ++turn;
         return c;
       };
-      total = reach_values(bound);
+      int total = reach_values(bound);
       over = 0xffffffffu;
       bisect(bound, over, total, p.K, kCand, reach_values);
       equal = total > kCand;
     }
-    // Values that reach the bound (NaN at bound 1, which every value then does), or that lie above
-    // it where `equal`, into cand[]; where in it does not change the result, since keys differ.
+    // The wave's values that reach the bound, or the next one where `equal`.
     const float v = value_of(equal ? over : bound);
     int c = 0;
-    bool hit[kRegs];
+    for (int i = 0; i < mine; ++i) {
+      const typename Vec<T>::f32 f = values(i);
+      const uint32_t index = n * (group[wave][wave + 4 * i] * 64 + lane);
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i) {
-      hit[i] = false;
-      if (i < mine) {
-        hit[i] = at[i] == whole || (at[i] < whole && !(largest(i) < v));
-        if (hit[i]) {
-          const typename Vec<T>::f32 f = values(i);
-#pragma unroll
-          for (int e = 0; e < n; ++e) c += !(f[e] < v) && is_there(i, e);
+      for (int e = 0; e < n; ++e) {
+        const uint64_t mask = __ballot(f[e] >= v);
+        if (mask) {  // (most have none)
+          const int to = c + below(mask);
+          if (f[e] >= v && to < kCand) cand[wave][to] = key_of(order(f[e]), index + e);
+          c += __builtin_popcountll(mask);
         }
       }
     }
-    int start = c ? atomicAdd(&count, c) : 0;
-    if (c && start + c <= kCand) {
-#pragma unroll
-      for (int i = 0; i < kRegs; ++i)
-        if (hit[i]) {
-          const typename Vec<T>::f32 f = values(i);
-#pragma unroll
-          for (int e = 0; e < n; ++e)
-            if (!(f[e] < v) && is_there(i, e)) cand[start++] = key_of(order(f[e]), n * at[i] + e);
-        }
-    }
-    if (equal) {  // over = bound + 1: the wave's first K of those equal to the bound
+    if (equal) {  // over = bound + 1: the first K of those equal to the bound
       const float w = value_of(bound);
       int room = p.K;
+      for (int i = 0; i < mine && room > 0; ++i) {
+        const typename Vec<T>::f32 f = values(i);
+        const uint32_t index = n * (group[wave][wave + 4 * i] * 64 + lane);
+        int before = 0, all = 0;
 #pragma unroll
-      for (int i = 0; i < kRegs; ++i)
-        if (i < mine && room > 0) {
-          const typename Vec<T>::f32 f = values(i);
-          int before = 0, all = 0;
-          bool same[n];
-#pragma unroll
-          for (int e = 0; e < n; ++e) {
-            same[e] = is_there(i, e) && f[e] == w;
-            const uint64_t mask = __ballot(same[e]);
-            before += below(mask);
-            all += __builtin_popcountll(mask);
-          }
-#pragma unroll
-          for (int e = 0; e < n; ++e)
-            if (same[e] && before++ < room) {
-              const int to = atomicAdd(&count, 1);
-              if (to < kCand) cand[to] = key_of(bound, n * at[i] + e);
-            }
-          room -= min(room, all);
+        for (int e = 0; e < n; ++e) {
+          const uint64_t mask = __ballot(f[e] == w);
+          before += below(mask);
+          all += __builtin_popcountll(mask);
         }
+#pragma unroll
+        for (int e = 0; e < n; ++e)
+          if (f[e] == w) {
+            if (before < room && c + before < kCand) cand[wave][c + before] = key_of(bound, index + e);
+            ++before;
+          }
+        all = min(all, room);
+        c += all;
+        room -= all;
+      }
     }
+    if (lane == 0) counts[wave] = c;
     __syncthreads();
-    total = count;
-    if (total <= kCand) break;  // at stage 2 at the latest: fewer than K above the bound, and 4 K at it
-    __syncthreads();
-    if (tid == 0) count = 0;
+    if (max(max(counts[0], counts[1]), max(counts[2], counts[3])) <= kCand) break;  // at stage 2 at the latest: 64 in all, or fewer than K and K
     __syncthreads();
   }
 
   // 3.
-  if (tid < total) {
-    const uint64_t k = cand[tid];
-    int rank = 0;
-#pragma unroll 4
-    for (int i = 0; i < total; ++i) rank += cand[i] > k;
-    if (rank < p.K) {
-      const float y = value_of((uint32_t)(k >> 32));
-      p.top_logprobs[r * p.K + rank] = row.l == 0.0f ? -INFINITY : (y - m) - logl;
-      p.top_ids[r * p.K + rank] = 0xffffffffu - (uint32_t)k;
+  uint64_t other[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) other[w] = lane < counts[w] ? cand[w][lane] : 0;
+  const uint64_t k = cand[wave][lane];
+  int rank = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    for (int i = 0, c = counts[w]; i < c; ++i) {
+      const uint64_t q = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(other[w] >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)other[w], i);
+      rank += q > k;
     }
+  if (lane < counts[wave] && rank < p.K) {
+    const float y = value_of((uint32_t)(k >> 32));
+    p.top_logprobs[r * p.K + rank] = row.l == 0.0f ? -INFINITY : (y - m) - logl;
+    p.top_ids[r * p.K + rank] = 0xffffffffu - (uint32_t)k;
   }
 }
 
