@@ -240,15 +240,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   // q: column i is head min(i, heads - 1); dims as the key operand has them
   const T *qrow = static_cast<const T *>(p.q) + b * p.q_ss + (head0 + min(i, heads - 1)) * p.q_sh;
   auto q_step = [&](int s) { return *(const DAN_GLOBAL u32x4 *)(qrow + (FP8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g)); };
-  u32x4 qf[kQLds ? 1 : S];
+  u32x4 qf[kQLds ? S / W : S];  // in LDS: this wave's share of the steps, until it is written there
   u32x4 *ql = (u32x4 *)lds + lane;
-  if constexpr (kQLds) {
-    for (int s = wave; s < S; s += W) ql[64 * s] = q_step(s);
-    __syncthreads();
-  } else {
 #pragma unroll
-    for (int s = 0; s < S; ++s) qf[s] = q_step(s);
-  }
+  for (int s = 0; s < (kQLds ? S / W : S); ++s) qf[s] = q_step(kQLds ? W * s + wave : s);
   float c = p.scale * kLog2e, vscale = 1.0f;
   if constexpr (FP8) {
     c *= *p.ks;
@@ -274,37 +269,45 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   for (int j = 0; j < VE; ++j) acc[j] = (f32x4){0, 0, 0, 0};
   float m = -INFINITY, l = 0.f;
 
+  Tl t;
+  uint64_t bad = 0, kadr = 0, vadr = 0;
+  const uint32_t krow = (uint32_t)(p.kc_st * ES), vrow = (uint32_t)(p.vc_st * ES);
+  const uint32_t koff = i * krow + 16 * g;
+  const uint32_t voff = 4 * g * vrow + (D == 256 && !FP8 ? 16 * i : VE * ES * i);
+  auto at_lane = [&](uint64_t x, int n) -> const uint8_t * {
+    const uint32_t a = __builtin_amdgcn_readlane((uint32_t)x, n), h = __builtin_amdgcn_readlane((uint32_t)(x >> 32), n);
+    return (const uint8_t *)((uint64_t)h << 32 | a);
+  };
+  auto fetch_k = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_k<T, D, FP8>(t, u, at_lane(kadr, 2 * n + u), koff);
+  };
+  auto fetch_v = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_v<T, D, FP8>(t, u, at_lane(vadr, 2 * n + u), voff, vrow);
+  };
   if (mine > 0) {
     // Where the lane's block starts in the two caches. Page 0 stands in for a
     // block behind the end and for a page that does not exist. A block starts at a multiple of 16
     // rows, as a page's size is one, so all 16 lie in the page.
     if (lo != split * p.chunk) from = dan::find_row(p.table, b, lo + mykey);
     const bool there = lane < 2 * mine && lo + mykey < hi;
-    const uint64_t bad = __ballot(there && from.page < 0);
+    bad = __ballot(there && from.page < 0);
     if (!there || from.page < 0) from = {0, 0};
-    const uint64_t kadr = (uint64_t)p.kc + (from.page * p.kc_sp + hk * p.kc_sh + from.row * p.kc_st) * ES;
-    const uint64_t vadr = (uint64_t)p.vc + (from.page * p.vc_sp + hk * p.vc_sh + from.row * p.vc_st) * ES;
-    const uint32_t krow = (uint32_t)(p.kc_st * ES), vrow = (uint32_t)(p.vc_st * ES);
-    const uint32_t koff = i * krow + 16 * g;
-    const uint32_t voff = 4 * g * vrow + (D == 256 && !FP8 ? 16 * i : VE * ES * i);
-    auto at_lane = [&](uint64_t x, int n) -> const uint8_t * {
-      const uint32_t a = __builtin_amdgcn_readlane((uint32_t)x, n), h = __builtin_amdgcn_readlane((uint32_t)(x >> 32), n);
-      return (const uint8_t *)((uint64_t)h << 32 | a);
-    };
-    Tl t;
-    auto fetch_k = [&](int n) __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) load_k<T, D, FP8>(t, u, at_lane(kadr, 2 * n + u), koff);
-    };
-    auto fetch_v = [&](int n) __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) load_v<T, D, FP8>(t, u, at_lane(vadr, 2 * n + u), voff, vrow);
-    };
+    kadr = (uint64_t)p.kc + (from.page * p.kc_sp + hk * p.kc_sh + from.row * p.kc_st) * ES;
+    vadr = (uint64_t)p.vc + (from.page * p.vc_sp + hk * p.vc_sh + from.row * p.vc_st) * ES;
     fetch_k(0);
     __builtin_amdgcn_sched_barrier(0);
     fetch_v(0);
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if constexpr (kQLds) {
+#pragma unroll
+    for (int s = 0; s < S / W; ++s) ql[64 * (W * s + wave)] = qf[s];
+    __syncthreads();
+  }
 
+  if (mine > 0) {
     // One tile; the next one's keys are loaded once its own are spent, and its values likewise. The last tile
     // is a copy of its own: a load under a condition would make the wait in front of each product
     // one for all loads.
