@@ -91,7 +91,7 @@ REFUSED = [
     (0, APPEND, dict(page_size=0), "page_size"), (0, APPEND, dict(num_rope_rows=3), "rows of cos"), (0, APPEND, dict(k=0), "NULL"),
     (0, APPEND, dict(places=0), "NULL"), (0, APPEND, dict(cache_dtype=3), "k_scale"), (0, APPEND, dict(k_stride_tok=132), "multiples of 8"),
     (0, APPEND, dict(kc_stride_tok=132), "16 bytes"), (0, APPEND, dict(v_cache=BUF + 8), "aligned"), (0, APPEND, dict(cs_stride_tok=32), "cs_stride"),
-    (0, APPEND, dict(num_tokens=-1), "num_tokens"), (0, APPEND, dict(num_tokens=1 << 28, num_rope_rows=1 << 28), "too many"),
+    (0, APPEND, dict(num_tokens=-1), "num_tokens"), (0, APPEND, dict(num_heads=1 << 30), "too many"),
     (1, ATTN, dict(abi_version=0), "abi_version"), (1, ATTN, dict(num_heads=9), "multiple"), (1, ATTN, dict(head_dim=80), "head_dim"),
     (1, ATTN, dict(dtype=3), "dtype"), (1, ATTN, dict(cache_dtype=2), "cache_dtype"), (1, ATTN, dict(page_size=24), "page_size"),
     (1, ATTN, dict(max_len=65), "max_len"), (1, ATTN, dict(max_len=-1), "max_len"), (1, ATTN, dict(scale=0.0), "scale"),
