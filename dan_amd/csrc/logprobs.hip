@@ -99,8 +99,9 @@ struct Params {
   int32_t N, V, L, K, chunks;
 };
 
-// The row's vector `at` (from its first value on; what lies past its end is -inf). Vectors past
-// the last whole one load that instead, or the row's start where there is none.
+// A lane's vectors of a chunk; what lies past the row's end is -inf. (A vector past the last whole one
+// loads that instead.) The loads pass the caches by, which rows of a few hundred MB only
+// sweep: 2039 x 128256 bf16 91 -> 80 us, forward and backward of 4096 rows 548 -> 521.
 template <typename T>
 __device__ inline void load_chunk(typename Vec<T>::f32 (&x)[kVecs], const T *row, int vocab, int first, int lane) {
   constexpr int n = Vec<T>::n;
@@ -109,7 +110,7 @@ __device__ inline void load_chunk(typename Vec<T>::f32 (&x)[kVecs], const T *row
   if (whole > 0) {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k)
-      raw[k] = *(const DAN_GLOBAL typename Vec<T>::loose *)(row + (int64_t)n * min(first + 64 * k + lane, whole - 1));
+      raw[k] = __builtin_nontemporal_load((const DAN_GLOBAL typename Vec<T>::loose *)(row + (int64_t)n * min(first + 64 * k + lane, whole - 1)));
   }
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
@@ -532,8 +533,9 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t work = (int64_t)blockIdx.x * 4 + wave;
   if (work >= (int64_t)p.N * p.chunks) return;
-  const int64_t r = work / p.chunks;
-  const int first = (int)(work - r * p.chunks) * kChunk;
+  // The rows from the last to the first: the forward, if it has just run, has left the last ones in cache.
+  const int64_t turn = work / p.chunks, r = p.N - 1 - turn;
+  const int first = (int)(work - turn * p.chunks) * kChunk;
   typename Vec<T>::f32 x[kVecs];
   load_chunk<T>(x, static_cast<const T *>(p.x) + r * p.x_st, p.V, first, lane);
   const float lse = p.lse[r];
@@ -593,7 +595,9 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradParams p) {
     }
     const typename Vec<T>::type z = __builtin_convertvector(y, typename Vec<T>::type);
     if ((int64_t)n * at + n <= p.V) {
-      *(DAN_GLOBAL typename Vec<T>::loose *)(out + (int64_t)n * at) = z;
+      // past the caches, which the logits still to come then keep: forward and backward of 4096 x 128256 bf16
+      // 584 -> 545 us (and 537 with the rows reversed); a product that reads the gradient next is no slower
+      __builtin_nontemporal_store((typename Vec<T>::loose)z, (DAN_GLOBAL typename Vec<T>::loose *)(out + (int64_t)n * at));
     } else {
 #pragma unroll
       for (int e = 0; e < n; ++e)
