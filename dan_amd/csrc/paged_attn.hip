@@ -155,51 +155,98 @@ __device__ inline int value_dim(int i, int j) {
   else return D / 16 * i + j;
 }
 
-template <typename T, int D, bool FP8>
-__device__ inline void load_k(Tile<T, D, FP8> &t, int u, const uint8_t *base, uint32_t off) {
-  // bf16/fp16: per step of 32 dims 16 bytes at dim 32 s + 8 g; e4m3: per two steps 16 bytes at dim 64 s + 16 g
+// Keys. A unit is 64 bytes of a row: one step of 32 dims in 16 bits, two in 8. Where a row has
+// several units they are loaded in pairs, 128 bytes of 8 rows in one instruction (whole cache lines, so
+// the loads may pass the caches by), and dealt out to the lanes by key_unit. Offsets of a lane:
+// first and second load of a pair.
+struct KeyOffsets {
+  uint32_t a, b;
+};
+// A load from the cache; STREAM: past the processor's caches.
+template <bool STREAM, typename V>
+__device__ inline V load(const uint8_t *p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load((const DAN_GLOBAL V *)p);
+  else return *(const DAN_GLOBAL V *)p;
+}
+__device__ inline KeyOffsets key_offsets(int lane, uint32_t row, bool pairs) {
+  const uint32_t i = lane & 15, g = lane >> 4, up = i >> 3;
+  if (!pairs) return {i * row + 16 * g, 0};
+  return {(i & 7) * row + 16 * g + 64 * up, (8 + (i & 7)) * row + 16 * g + 64 * (1 - up)};
+}
+
+template <bool STREAM, typename T, int D, bool FP8>
+__device__ inline void load_k(Tile<T, D, FP8> &t, int u, const uint8_t *base, KeyOffsets off) {
+  constexpr int KR = Tile<T, D, FP8>::KR;
+  if constexpr (KR == 4) {
+    const u32x4 x = load<STREAM, u32x4>(base + off.a);
 #pragma unroll
-  for (int s = 0; s < Tile<T, D, FP8>::KR / 4; ++s) {
-    const u32x4 x = *(const DAN_GLOBAL u32x4 *)(base + off + 64 * s);
+    for (int c = 0; c < 4; ++c) t.k[u][c] = x[c];
+  } else {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) t.k[u][4 * s + c] = x[c];
+    for (int s = 0; s < KR / 8; ++s) {
+      const u32x4 x = load<STREAM, u32x4>(base + off.a + 128 * s);
+      const u32x4 y = load<STREAM, u32x4>(base + off.b + 128 * s);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        t.k[u][8 * s + c] = x[c];
+        t.k[u][8 * s + 4 + c] = y[c];
+      }
+    }
   }
 }
 
+// Unit m of the lane's row i: of a pair, lanes 0 to 7 of each 16 have the first load's low half and
+// lanes 8 to 15 the second's; the other halves belong to the lanes 8 further.
 template <typename T, int D, bool FP8>
+__device__ inline u32x4 key_unit(const Tile<T, D, FP8> &t, int u, int m, bool low) {
+  u32x4 x;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if constexpr (Tile<T, D, FP8>::KR == 4) {
+      x[c] = t.k[u][c];
+    } else {
+      const uint32_t a = t.k[u][8 * (m / 2) + c], b = t.k[u][8 * (m / 2) + 4 + c];
+      x[c] = m % 2 == 0 ? (low ? a : b) : (uint32_t)__builtin_amdgcn_mov_dpp((int)(low ? b : a), 0x128, 0xF, 0xF, false);  // row_ror:8
+    }
+  }
+  return x;
+}
+
+template <bool STREAM, typename T, int D, bool FP8>
 __device__ inline void load_v(Tile<T, D, FP8> &t, int u, const uint8_t *base, uint32_t off, uint32_t row) {
   constexpr int VR = Tile<T, D, FP8>::VR;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const uint8_t *p = base + off + r * row;
     if constexpr (VR == 8) {
-      const u32x4 a = *(const DAN_GLOBAL u32x4 *)p, b = *(const DAN_GLOBAL u32x4 *)(p + 256);
+      const u32x4 a = load<STREAM, u32x4>(p), b = load<STREAM, u32x4>(p + 256);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         t.v[u][r][c] = a[c];
         t.v[u][r][4 + c] = b[c];
       }
     } else if constexpr (VR == 4) {
-      const u32x4 a = *(const DAN_GLOBAL u32x4 *)p;
+      const u32x4 a = load<STREAM, u32x4>(p);
 #pragma unroll
       for (int c = 0; c < 4; ++c) t.v[u][r][c] = a[c];
     } else if constexpr (VR == 2) {
-      const u32x2 a = *(const DAN_GLOBAL u32x2 *)p;
+      const u32x2 a = load<STREAM, u32x2>(p);
       t.v[u][r][0] = a[0];
       t.v[u][r][1] = a[1];
     } else {
-      t.v[u][r][0] = *(const DAN_GLOBAL uint32_t *)p;
+      t.v[u][r][0] = load<STREAM, uint32_t>(p);
     }
   }
 }
 
 // The operand of 32 dims (step s) of a key block.
 template <typename T, int D, bool FP8>
-__device__ inline u32x4 k_operand(const Tile<T, D, FP8> &t, int u, int s) {
+__device__ inline u32x4 k_operand(const Tile<T, D, FP8> &t, int u, int s, bool low) {
   if constexpr (!FP8) {
-    return (u32x4){t.k[u][4 * s], t.k[u][4 * s + 1], t.k[u][4 * s + 2], t.k[u][4 * s + 3]};
+    return key_unit<T, D, FP8>(t, u, s, low);
   } else {
-    const uint32_t a = t.k[u][2 * s], b = t.k[u][2 * s + 1];
+    const u32x4 x = key_unit<T, D, FP8>(t, u, s / 2, low);
+    const uint32_t a = x[s % 2 * 2], b = x[s % 2 * 2 + 1];
     return (u32x4){Ops<T>::template from_e4m3<false>(a), Ops<T>::template from_e4m3<true>(a), Ops<T>::template from_e4m3<false>(b),
                    Ops<T>::template from_e4m3<true>(b)};
   }
@@ -214,7 +261,7 @@ __device__ inline uint32_t v_pair(const Tile<T, D, FP8> &t, int u, int r, int m)
 
 // W waves. LDS: the waves' results [W][heads][D + 4], their maxima and sums [2][W][heads];
 // before that (D = 256) the q operand, in the order its steps read it.
-template <typename T, int D, bool FP8, int W>
+template <typename T, int D, bool FP8, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   typedef Tile<T, D, FP8> Tl;
   constexpr int VE = Tl::VE, ES = Tl::ES, DP = D + 4, S = D / 32;
@@ -272,7 +319,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   Tl t;
   uint64_t bad = 0, kadr = 0, vadr = 0;
   const uint32_t krow = (uint32_t)(p.kc_st * ES), vrow = (uint32_t)(p.vc_st * ES);
-  const uint32_t koff = i * krow + 16 * g;
+  const KeyOffsets koff = key_offsets(lane, krow, Tl::KR > 4);
+  const bool low = i < 8;
   const uint32_t voff = 4 * g * vrow + (D == 256 && !FP8 ? 16 * i : VE * ES * i);
   auto at_lane = [&](uint64_t x, int n) -> const uint8_t * {
     const uint32_t a = __builtin_amdgcn_readlane((uint32_t)x, n), h = __builtin_amdgcn_readlane((uint32_t)(x >> 32), n);
@@ -280,11 +328,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   };
   auto fetch_k = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_k<T, D, FP8>(t, u, at_lane(kadr, 2 * n + u), koff);
+    for (int u = 0; u < 2; ++u) load_k<STREAM, T, D, FP8>(t, u, at_lane(kadr, 2 * n + u), koff);
   };
   auto fetch_v = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) load_v<T, D, FP8>(t, u, at_lane(vadr, 2 * n + u), voff, vrow);
+    for (int u = 0; u < 2; ++u) load_v<STREAM, T, D, FP8>(t, u, at_lane(vadr, 2 * n + u), voff, vrow);
   };
   if (mine > 0) {
     // Where the lane's block starts in the two caches. Page 0 stands in for a
@@ -317,7 +365,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
       for (int u = 0; u < 2; ++u) {
         sc[u] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < S; ++s) sc[u] = Ops<T>::mfma(k_operand<T, D, FP8>(t, u, s), kQLds ? ql[64 * s] : qf[kQLds ? 0 : s], sc[u]);
+        for (int s = 0; s < S; ++s) sc[u] = Ops<T>::mfma(k_operand<T, D, FP8>(t, u, s, low), kQLds ? ql[64 * s] : qf[kQLds ? 0 : s], sc[u]);
       }
       if constexpr (!last.value) {
         fetch_k(n + 1);
@@ -518,18 +566,31 @@ Split split_of(int64_t seqs, int64_t groups, int max_len, int head_dim, int key_
   return s.chunk >= kWideChunk && head_dim <= 128 ? of(8) : s;
 }
 
-template <typename T, int D, bool FP8, int W>
-void launch_waves(const Params &p, hipStream_t s) {
+template <typename T, int D, bool FP8, int W, bool STREAM>
+void launch_kernel(const Params &p, hipStream_t s) {
   const int heads = p.G < kHeads ? p.G : kHeads;
   const size_t out = sizeof(float) * W * heads * (D + 4 + 2), q = D == 256 ? 16 * 64 * (D / 32) : 0;
   constexpr int kMost = (int)sizeof(float) * W * kHeads * (D + 4 + 2);
-  auto kernel = paged_attn_kernel<T, D, FP8, W>;
+  auto kernel = paged_attn_kernel<T, D, FP8, W, STREAM>;
   if constexpr (kMost > 64 * 1024) {  // beyond what a launch may have unasked; an error is the launch's
     static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
     (void)allowed;
   }
   const unsigned grid = (unsigned)((int64_t)p.splits * p.B * p.Hkv * p.blocks);
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * W), out > q ? out : q, s, p);
+}
+
+// Keys and values of a launch that may read more than the last-level cache holds pass the caches by, which they would
+// only sweep. us, through the caches / past them: 64 to 8192 (32/8 x 128; up to 2.1 GB) 216 / 194, 1 of 131072 99 / 88,
+// 100 to 1000 (32/32) 146 / 132, 16 to 8000 (524 MB) 65 / 59; a smaller launch gains by the caches
+// where a few layers' caches fit them (37 to 4099, 16/2 x 256 e4m3, 155 MB: 22.0 / 24.0 over 3 layers)
+// and loses a little where they do not (25.6 / 24.7 over 12).
+constexpr int64_t kStreamBytes = (int64_t)256 << 20;
+
+template <typename T, int D, bool FP8, int W>
+void launch_waves(const Params &p, hipStream_t s) {
+  if ((int64_t)p.B * p.max_len * p.Hkv * (2 * D * Tile<T, D, FP8>::ES) >= kStreamBytes) launch_kernel<T, D, FP8, W, true>(p, s);
+  else launch_kernel<T, D, FP8, W, false>(p, s);
 }
 
 template <typename T, int D, bool FP8>
