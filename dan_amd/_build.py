@@ -69,7 +69,7 @@ def calls_command(out):
             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I", INCLUDE,
             *(f for d in (os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
                           sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")) for f in ("-isystem", d)),
-            CALLS_SRC, "-o", out, "-L", os.path.join(home, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+            CALLS_SRC, "-o", out, "-L", os.path.join(home, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-lamdhip64"]
 
 
 def _run(cmd, verbose):

@@ -59,10 +59,10 @@ void check(int rc, const char *name) {
 // A plain tensor on device `index`: nothing wraps it, and it carries no tangent.
 bool plain(const Tensor &t, int index) {
   return t.defined() && t.is_cuda() && t.get_device() == index && t.layout() == at::kStrided && !at::isTensorSubclassLike(t) &&
-         !t.is_neg() && !t._fw_grad(0).defined();
+         !t.is_neg() && !t._is_zerotensor() && !t._fw_grad(0).defined();
 }
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
-void *at_of(const Tensor &t) { return t.defined() ? const_cast<void *>(t.const_data_ptr()) : nullptr; }
+void *at_of(const Tensor &t) { return t.defined() ? const_cast<void *>(t.const_data_ptr()) : nullptr; }  // read, or new
 
 // Rows that the kernels read in place: unit stride, 16-byte aligned.
 bool rows_ok(const Tensor &t) {
@@ -174,8 +174,8 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   a.v = at_of(v); a.v_stride_tok = v.stride(0); a.v_stride_head = v.stride(1);
   a.cos = at_of(cos); a.sin = at_of(sin);
   a.q_out = at_of(out); a.qo_stride_tok = h * d; a.qo_stride_head = d;
-  a.k_cache = at_of(kc); a.kc_stride_page = kc.stride(0); a.kc_stride_head = kc.stride(1); a.kc_stride_tok = kc.stride(2);
-  a.v_cache = at_of(vc); a.vc_stride_page = vc.stride(0); a.vc_stride_head = vc.stride(1); a.vc_stride_tok = vc.stride(2);
+  a.k_cache = kc.mutable_data_ptr(); a.kc_stride_page = kc.stride(0); a.kc_stride_head = kc.stride(1); a.kc_stride_tok = kc.stride(2);
+  a.v_cache = vc.mutable_data_ptr(); a.vc_stride_page = vc.stride(0); a.vc_stride_head = vc.stride(1); a.vc_stride_tok = vc.stride(2);
   a.k_scale = static_cast<const float *>(at_of(ks));
   a.v_scale = static_cast<const float *>(at_of(vs));
   a.table = static_cast<const int32_t *>(at_of(table)); a.table_stride = table.stride(0);
@@ -210,7 +210,8 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   if (!fits(h) || !fits(b) || b == 0 || kc.size(3) != d || hkv == 0 || h == 0 || h % hkv || table.size(0) != b || !index_ok(lens, b, index) ||
       overflow || most < 0 || most > holds || !fits(most) || !(scale > 0) || !std::isfinite(scale))
     Py_RETURN_NONE;
-  const bool want = PyObject_IsTrue(args[9]);
+  const int want = PyObject_IsTrue(args[9]);
+  if (want < 0) return nullptr;
   const int kind = code_of(kc.scalar_type());
   const Tensor out = at::empty_strided({h, b, d}, {d, h * d, 1}, q.options().requires_grad(false));
   Tensor lse, ws;
@@ -285,6 +286,23 @@ Outputs logprobs_forward(const Tensor &x, const Tensor &tokens, int64_t top, boo
   return o;
 }
 
+// A backward in a stream capture whose result goes to a node that lives on a stream outside of it, as the
+// accumulator of a leaf does while an eager graph of the same leaf is alive: the engine would make that
+// stream wait for the capture, which ends the process where it is the default one.
+bool leaves_capture(int index) {
+  const auto node = torch::autograd::get_current_node();
+  if (!node || node->num_outputs() == 0 || !node->next_edge(0).function) return false;
+  const auto to = node->next_edge(0).function->stream();
+  const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(index);
+  if (!to || to->device_index() != index || to->id() == here.id()) return false;
+  const c10::hip::HIPStream there(c10::Stream(c10::Stream::UNSAFE, here.unwrap().device(), to->id()));
+  auto captures = [](hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return s && hipStreamIsCapturing(s, &status) == hipSuccess && status != hipStreamCaptureStatusNone;  // never the default one
+  };
+  return captures(here.stream()) && !captures(there.stream());
+}
+
 struct Logprobs : torch::autograd::Function<Logprobs> {
   static variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &tokens, int64_t top, bool entropy) {
     const Outputs o = logprobs_forward(x, tokens, top, entropy);
@@ -315,6 +333,8 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
       again |= g[i].defined() && g[i].requires_grad();
     }
     if (!any) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    TORCH_CHECK(!leaves_capture(x.get_device()), "token_logprobs: a captured backward whose logits were first used outside of the capture; "
+                "drop every earlier result that holds their graph before the capture");
     again = (again || x.requires_grad()) && at::GradMode::is_enabled();
     Tensor grad;
     {
@@ -369,7 +389,8 @@ PyObject *logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       (tokens.dim() == 2 && (!fits(tokens.size(1)) || tokens.stride(1) != 1)) || overflow || top < 0 || top > DAN_READOUT_MAX_TOP || top > vocab ||
       (top && vocab > DAN_READOUT_MAX_TOP_VOCAB))
     Py_RETURN_NONE;
-  const bool entropy = PyObject_IsTrue(args[3]);
+  const int entropy = PyObject_IsTrue(args[3]);
+  if (entropy < 0) return nullptr;
   Outputs o;
   if (grads_of({&x})) {
     const variable_list out = Logprobs::apply(x, tokens, top, entropy);

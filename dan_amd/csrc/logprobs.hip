@@ -270,6 +270,12 @@ __device__ inline int below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+// What a lane wrote to LDS is there for the other lanes of its wave.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 constexpr int kTaken = 32;    // groups whose values a work group holds: 8 vectors a lane of 4 waves
 constexpr int kCand = 64;     // values that a wave collects
 constexpr uint32_t kLowest = 0x007fffffu;  // order(-inf): every value reaches it
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
       at += __builtin_popcountll(mask);
     }
   }
-  __builtin_amdgcn_wave_barrier();  // a wave reads its own list
+  wave_sync();  // a wave reads its own list
 
   // 2. Wave w takes groups w, w + 4, ..; rising ones, so that of equal values the first come first.
   // What lies behind the row's end is NaN, which reaches no bound.
@@ -383,7 +389,7 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
       for (int c = 0; c < 4; ++c) raw[i][c] = at[i] < whole ? raw[i][c] : at[i] == whole ? tail[c] : 0x7fff7fffu;
       kept[wave][i][lane] = raw[i];
     }
-  __builtin_amdgcn_wave_barrier();
+  wave_sync();
 
   const Row row = join(p, r, lane, first);
   const float m = row.m == -INFINITY ? 0.0f : row.m, logl = logf(row.l);
@@ -644,7 +650,9 @@ int check(int abi, int dtype, int rows, int vocab, int labels, int top, int64_t 
   if (top > 0 && vocab > DAN_READOUT_MAX_TOP_VOCAB)
     return fail(DAN_ERR_UNSUPPORTED, "top tokens of %d values: rows of at most %d", vocab, DAN_READOUT_MAX_TOP_VOCAB);
   if (stride < 0 || tokens_stride < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "row strides must be >= 0");
-  if (((int64_t)rows * chunks_of(dtype, vocab) + 3) / 4 >= (int64_t)1 << 31) return fail(DAN_ERR_INVALID_ARGUMENT, "too many rows");
+  // A launch has fewer than 2^32 threads: 64 a chunk, and for the top tokens 256 a row.
+  if (((int64_t)rows * chunks_of(dtype, vocab) + 3) / 4 * 256 >= (int64_t)1 << 32 || (top > 0 && rows >= 1 << 24))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "%d rows: too many for one launch", rows);
   return 0;
 }
 

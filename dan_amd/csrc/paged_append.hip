@@ -193,10 +193,15 @@ __global__ __launch_bounds__(256) void append_kernel(const Params p) {
   }
 }
 
+// Of a token's work group.
+int threads_of(int h, int hkv, int d) {
+  const int64_t lanes = ((int64_t)h + 2 * (int64_t)hkv) * (d / 8);
+  return lanes < 256 ? (int)(lanes + 63) / 64 * 64 : 256;
+}
+
 template <typename T, int D, bool FP8, bool CS32>
 void by_norm(const Params &p, int norm, hipStream_t s) {
-  const int64_t lanes = ((int64_t)p.H + 2 * (int64_t)p.Hkv) * (D / 8);
-  const dim3 grid((unsigned)p.N), block(lanes < 256 ? (unsigned)(lanes + 63) / 64 * 64 : 256);
+  const dim3 grid((unsigned)p.N), block(threads_of(p.H, p.Hkv, D));
   if (norm == DAN_FRONT_NORM_RMS) hipLaunchKernelGGL((append_kernel<T, D, DAN_FRONT_NORM_RMS, FP8, CS32>), grid, block, 0, s, p);
   else if (norm == DAN_FRONT_NORM_RMS_ZERO_CENTERED)
     hipLaunchKernelGGL((append_kernel<T, D, DAN_FRONT_NORM_RMS_ZERO_CENTERED, FP8, CS32>), grid, block, 0, s, p);
@@ -264,6 +269,7 @@ int dan_paged_append(const DanPagedAppendArgs *a, void *stream) {
   for (const void *ptr : ptrs)
     if ((uintptr_t)ptr & 15) return fail(DAN_ERR_INVALID_ARGUMENT, "tensor pointers must be 16-byte aligned");
   if ((int64_t)H + 2 * (int64_t)Hkv >= (int64_t)1 << 30) return fail(DAN_ERR_INVALID_ARGUMENT, "too many heads");
+  if ((int64_t)N * threads_of(H, Hkv, D) >= (int64_t)1 << 32) return fail(DAN_ERR_INVALID_ARGUMENT, "%d tokens: too many for one launch", N);
 
   Params p;
   p.q = a->q; p.k = a->k; p.v = a->v; p.cos = a->cos; p.sin = a->sin; p.qw = a->q_norm_weight; p.kw = a->k_norm_weight;

@@ -570,12 +570,9 @@ template <typename T, int D, bool FP8, int W, bool STREAM>
 void launch_kernel(const Params &p, hipStream_t s) {
   const int heads = p.G < kHeads ? p.G : kHeads;
   const size_t out = sizeof(float) * W * heads * (D + 4 + 2), q = D == 256 ? 16 * 64 * (D / 32) : 0;
-  constexpr int kMost = (int)sizeof(float) * W * kHeads * (D + 4 + 2);
   auto kernel = paged_attn_kernel<T, D, FP8, W, STREAM>;
-  if constexpr (kMost > 64 * 1024) {  // beyond what a launch may have unasked; an error is the launch's
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
-    (void)allowed;
-  }
+  // Beyond what a launch may have unasked, of 16 heads x 128 in 8 waves: asked of the current device each time.
+  if (out > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)out);
   const unsigned grid = (unsigned)((int64_t)p.splits * p.B * p.Hkv * p.blocks);
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * W), out > q ? out : q, s, p);
 }
@@ -589,7 +586,7 @@ constexpr int64_t kStreamBytes = (int64_t)256 << 20;
 
 template <typename T, int D, bool FP8, int W>
 void launch_waves(const Params &p, hipStream_t s) {
-  if ((int64_t)p.B * p.max_len * p.Hkv * (2 * D * Tile<T, D, FP8>::ES) >= kStreamBytes) launch_kernel<T, D, FP8, W, true>(p, s);
+  if ((double)p.B * p.max_len * p.Hkv * (2 * D * Tile<T, D, FP8>::ES) >= (double)kStreamBytes) launch_kernel<T, D, FP8, W, true>(p, s);
   else launch_kernel<T, D, FP8, W, false>(p, s);
 }
 
@@ -665,7 +662,7 @@ int dan_paged_attn(const DanPagedAttnArgs *a, void *stream) {
 
   Params p;
   p.q = a->q; p.kc = a->k_cache; p.vc = a->v_cache; p.out = a->out; p.lse = a->lse; p.part = static_cast<float *>(a->workspace);
-  p.ks = a->k_scale; p.vs = a->v_scale; p.table = {a->table, a->table_stride, B, a->table_width, a->page_size, a->num_pages}; p.lens = a->lens;
+  p.ks = a->k_scale; p.vs = a->v_scale; p.table = {a->table, a->table_stride, B, a->table ? a->table_width : 0, a->page_size, a->num_pages}; p.lens = a->lens;
   p.q_ss = a->q_stride_seq; p.q_sh = a->q_stride_head; p.o_ss = a->o_stride_seq; p.o_sh = a->o_stride_head;
   p.kc_sp = a->kc_stride_page; p.kc_sh = a->kc_stride_head; p.kc_st = a->kc_stride_tok;
   p.vc_sp = a->vc_stride_page; p.vc_sh = a->vc_stride_head; p.vc_st = a->vc_stride_tok;
@@ -673,8 +670,9 @@ int dan_paged_attn(const DanPagedAttnArgs *a, void *stream) {
   p.max_len = a->max_len; p.blocks = (p.G + kHeads - 1) / kHeads; p.scale = a->scale;
   const Split sp = split_of(B, (int64_t)B * Hkv * p.blocks, a->max_len, D, 2 * D * es, dan::num_cus());
   p.target = sp.target; p.splits = sp.splits; p.waves = sp.waves; p.chunk = sp.chunk;
-  if ((int64_t)sp.splits * B * Hkv * p.blocks >= (int64_t)1 << 31 || (int64_t)B * H >= (int64_t)1 << 31)
-    return fail(DAN_ERR_INVALID_ARGUMENT, "too many work groups");
+  const int64_t threads = (int64_t)1 << 32;  // a launch has fewer
+  if ((int64_t)sp.splits * B >= threads || (int64_t)sp.splits * B * Hkv * p.blocks * 64 * sp.waves >= threads || (int64_t)B * H * 256 >= threads)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "too many sequences and heads for one launch");
   if (sp.splits > 1) {
     const int64_t need = (int64_t)B * H * sp.splits * (D + 2) * 4;
     if (!a->workspace || a->workspace_bytes < need)

@@ -103,7 +103,10 @@ def token_logprobs(logits, tokens, *, top=0, entropy=False):
 
     Where ``logits`` requires grad, every output but ``top_ids`` is
     differentiable (once): the gradient has the logits' dtype, computed in fp32
-    and rounded once; a token given twice adds up."""
+    and rounded once; a token given twice adds up. A backward that is captured into
+    a HIP graph must have its forward in the same capture, and no earlier, eager
+    result that holds the graph of the same leaves may be alive (torch's engine would join
+    the two streams): where ``logits`` is such a leaf itself, that raises."""
     made = _decode.calls().logprobs(logits, tokens, top, entropy)
     if made is not None:  # a plain call
         return TokenLogprobs._make(made)
@@ -122,11 +125,8 @@ def token_logprobs(logits, tokens, *, top=0, entropy=False):
         raise ValueError(f"top {top}: at most {_decode.MAX_TOP} and the vocabulary's {vocab}, for at most {_decode.MAX_TOP_VOCAB} values")
     if has_tangent(logits):
         raise NotImplementedError("token_logprobs has no forward-mode derivative")
-    if tokens.dtype != torch.int64:
-        tokens = tokens.long()
-    if tokens.dim() == 2 and tokens.stride(1) != 1 and tokens.shape[1] > 1:
-        tokens = tokens.contiguous()
-    if logits.stride(1) != 1 and vocab > 1:
-        logits = logits.contiguous()
+    spread = logits.stride(1) != 1 and vocab > 1
+    if spread or tokens.dtype != torch.int64 or (tokens.dim() == 2 and tokens.stride(1) != 1 and tokens.shape[1] > 1):
+        return token_logprobs(logits.contiguous() if spread else logits, tokens.long().contiguous(), top=top, entropy=entropy)
     call = _Logprobs.apply if logits.requires_grad and torch.is_grad_enabled() else _forward
     return TokenLogprobs(*call(logits, tokens, int(top), bool(entropy)))

@@ -106,6 +106,10 @@ REFUSED = [
     (3, GRAD, dict(abi_version=7), "abi_version"), (3, GRAD, dict(grad=0), "NULL"), (3, GRAD, dict(g_entropy=BUF), "NULL"),
     (3, GRAD, dict(top=3, g_top=BUF), "NULL"), (3, GRAD, dict(tokens=0), "NULL"), (3, GRAD, dict(grad_stride=99), "grad_stride"),
     (3, GRAD, dict(dtype=2, grad=BUF + 2), "aligned"),
+    # more threads than a launch has
+    (0, APPEND, dict(num_tokens=1 << 25, num_rope_rows=1 << 25), "one launch"), (1, ATTN, dict(num_seqs=1 << 24, num_heads=2), "one launch"),
+    (1, ATTN, dict(num_seqs=1 << 21, num_heads=16, num_kv_heads=1), "one launch"), (2, LOGP, dict(rows=1 << 24), "one launch"),
+    (2, LOGP, dict(rows=1 << 26, top=0), "one launch"), (3, GRAD, dict(rows=1 << 26), "one launch"),
 ]
 
 

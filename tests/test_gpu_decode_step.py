@@ -255,3 +255,107 @@ def test_what_is_not_plain_is_left_to_python(gpu):
     with dual.dual_level():
         assert r(x=dual.make_dual(x, x)) is None and t(q=dual.make_dual(q, q).transpose(0, 1)) is None
     assert c.append() is None and c.attend(1) is None and c.logprobs() is None
+
+
+def test_without_keys_no_table_is_read(gpu):
+    """max_len 0 needs no cache and no table, whatever width is given for one."""
+    say("attend: no table")
+    from dan_amd import _decode
+
+    q, lens = torch.ones(2, H, D, dtype=BF16, device=gpu), ids([0, 1], gpu)
+    out, lse = torch.ones_like(q), torch.ones(2, H, device=gpu)
+    fields = dict(abi_version=_decode.PAGED_ABI_VERSION, num_seqs=2, num_heads=H, num_kv_heads=HKV, head_dim=D, page_size=16, num_pages=4, table_width=4,
+                  scale=1.0, q=q.data_ptr(), q_stride_seq=H * D, q_stride_head=D, out=out.data_ptr(), o_stride_seq=H * D, o_stride_head=D,
+                  lse=lse.data_ptr(), kc_stride_tok=D, vc_stride_tok=D, table_stride=4, lens=lens.data_ptr())
+    _decode.call_paged_attn(torch.cuda.current_stream().cuda_stream, *(fields.get(n, 0) for n, _ in _decode.DanPagedAttnArgs._fields_))
+    torch.cuda.synchronize()
+    assert not out[0].any() and (lse[0] == -math.inf).all() and out[1].isnan().all() and lse[1].isnan().all()
+
+
+def test_inference_mode_and_two_threads(gpu):
+    """The same step from two threads at once, each on a stream of its own, in inference mode."""
+    say("decode step: two threads in inference mode")
+    import threading
+
+    g = torch.Generator().manual_seed(6)
+    qkv = torch.randn(2, (H + 2 * HKV) * D, generator=g).to(BF16).to(gpu)
+    tokens = torch.tensor([3, 4], device=gpu)
+    got, wrong = {}, []
+
+    def run(i):
+        try:
+            with torch.inference_mode(), torch.cuda.stream(torch.cuda.Stream()):
+                m = Layer(gpu, 2, 256, seed=2)
+                m.kc.fill_(0.25)
+                m.vc.fill_(0.5)
+                for _ in range(20):
+                    out = m.step(qkv, ids([200, 9], gpu), ids([201, 10], gpu), tokens)
+                torch.cuda.current_stream().synchronize()
+                got[i] = [t.clone() for t in out]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # shown by the test's own thread
+            wrong.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and all(torch.equal(a, b) and a.is_inference() for a, b in zip(got[0], got[1], strict=True))
+
+
+def test_compiled_step(gpu):
+    """A compiled function that calls the operators gives what the plain one does."""
+    say("decode step: torch.compile")
+    m = Layer(gpu, 2, 256, seed=2)
+    m.kc.fill_(0.25)
+    m.vc.fill_(0.5)
+    qkv = torch.randn(2, (H + 2 * HKV) * D, generator=torch.Generator().manual_seed(6)).to(BF16).to(gpu)
+    args = qkv, ids([200, 9], gpu), ids([201, 10], gpu), torch.tensor([3, 4], device=gpu)
+    with torch.no_grad():
+        want = m.step(*args)
+        got = torch.compile(m.step, backend="eager")(*args)
+    assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+def test_an_appended_copy_on_write_cache_leaves_its_source(gpu):
+    say("append: copy on write")
+    m = Layer(gpu, 2, 64)
+    m.kc.zero_()
+    m.vc.zero_()
+    kc, vc = m.kc, m.vc
+    m.kc, m.vc = torch._lazy_clone(kc), torch._lazy_clone(vc)
+    qkv = torch.ones(2, (H + 2 * HKV) * D, dtype=BF16, device=gpu)
+    m.step(qkv, ids([0, 1], gpu), ids([1, 2], gpu), torch.tensor([3, 4], device=gpu))
+    assert not kc.any() and not vc.any() and m.kc.any() and (m.vc == 1).sum() == 2 * HKV * D
+
+
+@pytest.mark.parametrize("tokens", [torch.int64, torch.int32])
+def test_a_capture_that_an_eager_graph_would_join_is_refused(gpu, tokens):
+    """While an eager result holds the graph of a leaf, a captured backward to the same leaf raises, and both go on."""
+    say(f"readout: captured gradient beside an eager graph, {tokens}")
+    x = torch.randn(4, 300, device=gpu, requires_grad=True)
+    t = torch.tensor([1, 2, 3, -1], device=gpu, dtype=tokens)
+
+    def grad(r):
+        return torch.autograd.grad(r.logprobs, x, torch.ones_like(r.logprobs), retain_graph=True)[0]
+
+    side = torch.cuda.Stream()
+    eager = token_logprobs(x, t)  # alive, with its graph
+    want = grad(eager)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured backward"):
+        with torch.cuda.graph(graph, stream=side):
+            grad(token_logprobs(x, t))
+    torch.cuda.synchronize()
+    assert torch.equal(grad(eager), want)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = grad(token_logprobs(x, t))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
