@@ -12,6 +12,11 @@
 // the chunk kernel also leaves the maximum of each group of 64 consecutive vectors, and the K
 // largest values of a row lie in the K groups of largest maximum (of equal ones those
 // of lowest index), which alone are read again.
+//
+// Measured, us: 2039 rows x 128256 bf16 with 5 top tokens and entropy 104 to 109 (the chunk kernel 80 to 92: 523 MB at
+// 5.7 to 6.5 TB/s; the top kernel 15 to 18), without top tokens 87; 1 row 4.8 + 7.4 with 20 top tokens, of which
+// about 4 each are a launch and its first loads; 45 rows x 50257 fp32 with 10, 4.6 + 6. Forward with entropy and gradient of
+// 4096 x 128256 bf16 (3.15 GB) 517: 6.1 TB/s, where a large copy moves 4.9.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -516,6 +521,9 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
   }
 }
 
+// By how many group maxima a lane keeps in registers: the fewest that hold the row's, for each
+// adds an operation to every step of the search. 128256 bf16 values (251 groups), a whole call of 1 row with 20 top
+// tokens / of 2039 rows with 5, us: 4 a lane 12.8 / 108.7, 8 13.6 / 111.9, 32 18.7 / 118.9.
 template <typename T>
 void launch_top(const Params &p, hipStream_t s) {
   const int groups = ((p.V + Vec<T>::n - 1) / Vec<T>::n + 63) / 64;

@@ -3,13 +3,15 @@
 // over the sequence's first lens[b] keys.
 //
 // HBM-bound: every key and value row is read once. The work is split over
-// (sequence, kv head, range of keys): a work group of 4 waves takes one range, its
-// waves every fourth tile of 32 keys, each with a running maximum and sum of its
+// (sequence, kv head, range of keys): a work group of 4 or 8 waves takes one range, each
+// of its waves every 4th or 8th tile of 32 keys, with a running maximum and sum of its
 // own; the work group joins them in LDS, and where a sequence spans several
-// ranges a second launch joins those.
+// ranges a second launch joins those (3 to 4 us: a launch behind another. The last work group of
+// a sequence could join instead, but a counter that tells it so would have to be cleared
+// for the next replay of a graph, and its partners' rows fetched from other dies' caches).
 //
 // A tile never passes through LDS. On the matrix core (16 x 16 x 32):
-//   S^T [16 keys x 16 heads] = K [keys x D] Q^T: a lane loads 16 bytes of one key row per
+//   S^T [16 keys x 16 heads] = K [keys x D] Q^T: a lane's operand is 16 bytes of one key row per
 //     step of 32 dims; the q heads of one kv head (up to 16) are the columns, so grouped
 //     heads cost no second read of the keys;
 //   O^T [D x 16 heads] += V^T [D x 32 keys] P^T: a lane loads D / 16 consecutive dims of
@@ -19,6 +21,14 @@
 // registers to the operand without an exchange. P is split into a rounded part and the
 // rounded rest, two products: the output then has the precision of fp32 weights
 // (one rounding of P to bf16 costs about as much as the rounding of the output).
+//
+// Measured, us and TB/s of keys and values, 32/8 heads x 128 in bf16 if not said: 1 sequence of 277 keys
+// 6.4 (of which 4 are a launch and its chain of dependent loads: length, page, keys), 1 of 131072 87
+// (6.2), 64 of up to 8192 194 (5.6), 100 of up to 1000 (32/32 fp16) 133 (6.2), 37 of up to 4099 (16/2 x 256, e4m3) 24
+// (2.6: a CU draws about 60 GB/s from HBM however many waves ask, so what holds a short launch of unequal
+// sequences is the CU with the most keys, and then the join). A large copy moves 4.9.
+// Two tiles in flight a wave (240 registers, 2 waves a SIMD) were 1 to 40 % slower; the two parts
+// of P in one product for up to 8 heads 0 to 3 %: the products are not what bounds it.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -104,9 +114,17 @@ __device__ inline float sum_across_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-constexpr int kMaxChunk = 2048;            // keys of a range, at most
-constexpr int kWideChunk = 768;            // from here on a range takes 8 waves
-constexpr int kDirectBytes = 192 * 1024;   // keys and values of one range without a join
+// The limits of a split (us on either side, 32/8 heads x 128 in bf16 if not said):
+// - a range has at most kMaxChunk keys (a lane holds the address of one of a wave's 32 blocks of 16 keys):
+//   64 sequences of up to 8192 194 with 2048, 199 with 1024; 128 of up to 2000 93 / 100; 1 of 131072 88 / 92;
+// - one of kWideChunk keys or more takes 8 waves, 4 / 8: 64 of up to 8192 205 / 194, 128 of up to 2000
+//   97 / 93, 100 of up to 1000 (32/32) 138 / 132, 16 of up to 8000 57 / 59; below it 4 to 8000 21 / 26, 16 to 1000
+//   13.5 / 15.2 (few work groups: a range of 8 waves is twice as long);
+// - keys and values of kDirectBytes or less are one range, one launch / several and the join: 1 of 277 6.4 / 7.5,
+//   1 of 384 (192 KB) 7.0 / 7.5, 64 of up to 380 12.7 / 17.5.
+constexpr int kMaxChunk = 2048;
+constexpr int kWideChunk = 768;
+constexpr int kDirectBytes = 192 * 1024;
 
 struct Params {
   const void *q, *kc, *vc;
@@ -547,7 +565,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
 }
 
 // How a launch is split over the keys: work groups of `waves` waves, `splits` ranges of a
-// sequence of max_len keys.
+// sequence of max_len keys, a sequence's own number in proportion to its length up to `target`.
+// Equal sequences would have one range for each CU in all; in a batch of unequal ones the long ones need
+// more, the shorter the better, but each costs a work group's start and its row in the join. us with ranges
+// for 1 / 2 / 4 times the CUs (32/8 x 128 in bf16 if not said): 1 of 131072 88 / 89 / 92, 1 of 32768 30 / 31 / 33;
+// few sequences, 2: 4 to 8000 19.5 / 20.0 / 21.0, 2 to 20000 29.6 / 30.2 / 33.0, 32 to 3000 (8/2 x 64) 11.7 / 11.7 / 12.7;
+// more, 4: 16 to 8000 63.6 / 58.3 / 58.6, 16 to 3000 27.7 / 27.4 / 24.7, 48 to 6000 120 / 118 / 116; of 256 dims, 2:
+// 37 to 4099 (16/2, e4m3) 27.4 / 23.7 / 26.2, 64 to 4000 61.2 / 61.5 / 63.5. Where every CU has a sequence and a head
+// and none is longer than a range may be, no join: 64 to 500 15.8 / 15.7 / 20.2, 64 to 1000 32 / 32 / 37,
+// 32 to 1500 24.5 / 28.8 / 26.8 (a single sequence of 2000 among short ones then takes some 20 us of its own).
 struct Split {
   int waves, target, splits, chunk;
 };
@@ -555,7 +581,8 @@ Split split_of(int64_t seqs, int64_t groups, int max_len, int head_dim, int key_
   if (cus <= 0) cus = 256;
   if (groups < 1) groups = 1;  // no sequences
   if ((int64_t)max_len * key_bytes <= kDirectBytes) return {4, 1, 1, chunk_of(max_len, 1, 1, 4)};
-  const int64_t want = (seqs == 1 ? 1 : head_dim == 256 ? 2 : 4) * (int64_t)cus, shares = (want + groups - 1) / groups;
+  const bool even = seqs == 1 || (groups >= cus && max_len <= kMaxChunk);
+  const int64_t want = (even ? 1 : head_dim == 256 || 2 * groups < cus ? 2 : 4) * (int64_t)cus, shares = (want + groups - 1) / groups;
   auto of = [&](int waves) {
     const int64_t most = (max_len + kTile * waves - 1) / (kTile * waves);  // ranges of the shortest length
     const int target = (int)(shares < most ? shares : most), least = (max_len + kMaxChunk - 1) / kMaxChunk;
