@@ -523,12 +523,14 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
 
 // By how many group maxima a lane keeps in registers: the fewest that hold the row's, for each
 // adds an operation to every step of the search. 128256 bf16 values (251 groups), a whole call of 1 row with 20 top
-// tokens / of 2039 rows with 5, us: 4 a lane 12.8 / 108.7, 8 13.6 / 111.9, 32 18.7 / 118.9.
+// tokens / of 2039 rows with 5, us: 4 a lane 12.8 / 108.7, 8 13.6 / 111.9, 32 18.7 / 118.9. 151936 fp32 values (594 groups),
+// 1 row with 20 / 500 rows with 5: 16 a lane 14.2 / 60, 32 17.9 / 65.
 template <typename T>
 void launch_top(const Params &p, hipStream_t s) {
   const int groups = ((p.V + Vec<T>::n - 1) / Vec<T>::n + 63) / 64;
   if (groups <= 64 * 4) hipLaunchKernelGGL((top_kernel<T, 4>), dim3((unsigned)p.N), dim3(256), 0, s, p);
   else if (groups <= 64 * 8) hipLaunchKernelGGL((top_kernel<T, 8>), dim3((unsigned)p.N), dim3(256), 0, s, p);
+  else if (groups <= 64 * 16) hipLaunchKernelGGL((top_kernel<T, 16>), dim3((unsigned)p.N), dim3(256), 0, s, p);
   else hipLaunchKernelGGL((top_kernel<T, 32>), dim3((unsigned)p.N), dim3(256), 0, s, p);  // up to DAN_READOUT_MAX_TOP_VOCAB fp32 values
 }
 
