@@ -96,7 +96,8 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
     marks a row without a token (a batch padded to a fixed size), whose k and v are not
     stored. ``seqs`` (int32 [N]): its row of ``table``; None: token n belongs to
     sequence n (a decode step). Tokens whose page the table does not name (past its width,
-    or outside the cache) are not stored either. No two tokens may share a place.
+    or outside the cache) are not stored either. No two tokens may share a place, and
+    q, k and v may not lie in rows of the cache that the call writes.
 
     Returns q [H, N, D], a view of a new token-major [N, H, D] tensor (None
     without q). All arithmetic is fp32, rounded once at each store (an e4m3
@@ -201,7 +202,8 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
     with ``return_lse`` also the fp32 [H, B] log of the sum of e^score (a merge with other
     keys' attention takes it, dan/fused.py:94-101). A sequence of no keys gives
     zeros and -inf. A length outside [0, max_len], or a page outside the
-    cache, gives NaN for its sequence.
+    cache, gives NaN for its sequence. An infinite value among a sequence's own may give NaN where
+    the sum would be infinite (weights are held in two parts).
 
     How a sequence's keys are split between work groups follows from its own length,
     B, Hkv and ``max_len``: its result does not depend on its neighbours' lengths."""

@@ -328,6 +328,37 @@ def test_attend_many_heads_of_one_group(gpu, d, cache):
     run_attend(gpu, [2500] * 20 + [900, 2499, 0], 32, 16, d, cache=cache, seed=2)
 
 
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attend_a_launch_sized_past_the_caches(gpu, d, cache):
+    """A table that could hold more than 256 MB of keys and values: their loads pass the caches by."""
+    run_attend(gpu, [60, 3001, 0, 1], 16, 1, d, cache=cache, extra=(1 << 28) // (4 * 16 * 2 * d * (2 if cache == BF16 else 1)) + 1)
+
+
+def test_attend_short_ranges_past_the_caches(gpu):
+    run_attend(gpu, [2100] + [3 * i for i in range(31)], 32, 8, 128)
+
+
+def test_attend_captured_with_the_largest_work_groups(gpu):
+    """16 heads of one kv head in ranges of eight waves take more LDS than a launch has unasked: asked for inside the capture too."""
+    say("attend: captured, 16/1 x 128, 256 sequences of up to 1024 keys")
+    g = gen(9)
+    kc, vc = (torch.randn(64, 1, 16, 128, generator=g).to(BF16).to(gpu) for _ in range(2))
+    table = torch.randperm(64, generator=g).int().to(gpu).expand(256, 64)  # all sequences share their pages
+    q, lens = torch.zeros(16, 256, 128, dtype=BF16, device=gpu), torch.zeros(256, dtype=torch.int32, device=gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = attend_paged(q, kc, vc, table, lens, return_lse=True)
+    for _ in range(3):
+        q.copy_(torch.randn(16, 256, 128, generator=g))
+        lens.copy_(torch.randint(0, 1025, (256,), generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), lse.clone()
+        want = attend_paged(q, kc, vc, table, lens, return_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and (got[1] > 0).sum() > 3000
+
+
 def test_attend_scales_layouts_and_capacity(gpu):
     run_attend(gpu, [33, 500], 8, 2, 128, std=20.0)  # peaked weights
     run_attend(gpu, [33, 500], 8, 2, 128, scale=0.013)
