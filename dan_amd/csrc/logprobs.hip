@@ -8,7 +8,7 @@
 // much). A row is cut into chunks of 512 vectors of 16 bytes; a wave takes one chunk, 8
 // vectors a lane, all loaded before any math, and leaves the chunk's maximum, sum and
 // weighted sum, so no wave waits for another and a single row still fills many CUs. A second
-// launch joins a row's chunks, looks up the given tokens and finds the top ones:
+// launch (short rows: the same, in_one) joins a row's chunks, looks up the given tokens and finds the top ones:
 // the chunk kernel also leaves the maximum of each group of 64 consecutive vectors, and the K
 // largest values of a row lie in the K groups of largest maximum (of equal ones those
 // of lowest index), which alone are read again.
@@ -23,6 +23,7 @@
 
 #include <type_traits>
 
+#include "cus.h"
 #include "dan_readout.h"
 
 namespace dan {
@@ -39,6 +40,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kVecs = 8;               // vectors a lane
 constexpr int kChunk = 64 * kVecs;     // vectors a wave
+constexpr int kWhole = 8;              // chunks of a row that one work group takes whole
 
 // A vector of 16 bytes at an address that only the type's own alignment holds for
 // (rows of an odd number of values): the hardware reads it in one piece.
@@ -129,16 +131,12 @@ __device__ inline void load_chunk(typename Vec<T>::f32 (&x)[kVecs], const T *row
   }
 }
 
+// A chunk's maximum, sum and weighted sum (and 0), in every lane; TOP: with lane k's `mine` the maximum of group k.
 template <typename T, bool ENTROPY, bool TOP>
-__global__ __launch_bounds__(256) void chunk_kernel(const Params p) {
+__device__ __forceinline__ f32x4 chunk_sums(const T *row, int vocab, int first, int lane, float &mine) {
   constexpr int n = Vec<T>::n;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t at = (int64_t)blockIdx.x * 4 + wave;
-  if (at >= (int64_t)p.N * p.chunks) return;
-  const int64_t r = at / p.chunks;
-  const int c = (int)(at - r * p.chunks);
   typename Vec<T>::f32 x[kVecs];
-  load_chunk<T>(x, static_cast<const T *>(p.x) + r * p.x_st, p.V, c * kChunk, lane);
+  load_chunk<T>(x, row, vocab, first, lane);
   float most[kVecs];
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
@@ -149,14 +147,12 @@ __global__ __launch_bounds__(256) void chunk_kernel(const Params p) {
   float m;
   if constexpr (TOP) {
     m = -INFINITY;
-    float mine = 0.f;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const float w = wave_max(most[k]);
       m = fmaxf(m, w);
       mine = lane == k ? w : mine;
     }
-    if (lane < kVecs) p.part[(int64_t)p.N * p.chunks * 4 + at * kVecs + lane] = mine;
   } else {
 #pragma unroll
     for (int k = 1; k < kVecs; ++k) most[0] = fmaxf(most[0], most[k]);
@@ -188,7 +184,19 @@ __global__ __launch_bounds__(256) void chunk_kernel(const Params p) {
   }
   l = wave_sum(l);
   if constexpr (ENTROPY) a = wave_sum(a);
-  if (lane == 0) *(f32x4 *)(p.part + at * 4) = (f32x4){m, l, a, 0};
+  return {m, l, a, 0};
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(256) void chunk_kernel(const Params p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t at = (int64_t)blockIdx.x * 4 + wave;
+  if (at >= (int64_t)p.N * p.chunks) return;
+  const int64_t r = at / p.chunks;
+  float mine = 0.f;
+  const f32x4 sums = chunk_sums<T, ENTROPY, TOP>(static_cast<const T *>(p.x) + r * p.x_st, p.V, (int)(at - r * p.chunks) * kChunk, lane, mine);
+  if (TOP && lane < kVecs) p.part[(int64_t)p.N * p.chunks * 4 + at * kVecs + lane] = mine;
+  if (lane == 0) *(f32x4 *)(p.part + at * 4) = sums;
 }
 
 // The row's maximum, sum and weighted sum from its chunks', in every lane of a wave; `first` is chunk `lane`'s
@@ -196,13 +204,10 @@ __global__ __launch_bounds__(256) void chunk_kernel(const Params p) {
 struct Row {
   float m, l, a;
 };
-__device__ inline f32x4 first_chunk(const Params &p, int64_t r, int lane) {
-  return lane < p.chunks ? ((const f32x4 *)p.part)[r * p.chunks + lane] : (f32x4){-INFINITY, 0, 0, 0};
-}
-__device__ inline Row join(const Params &p, int64_t r, int lane, f32x4 first) {
-  const f32x4 *part = (const f32x4 *)p.part + r * p.chunks;
+__device__ inline f32x4 first_chunk(const f32x4 *part, int chunks, int lane) { return lane < chunks ? part[lane] : (f32x4){-INFINITY, 0, 0, 0}; }
+__device__ inline Row join(const f32x4 *part, int chunks, int lane, f32x4 first) {
   float m = first[0];
-  for (int c = lane + 64; c < p.chunks; c += 64) m = fmaxf(m, part[c][0]);
+  for (int c = lane + 64; c < chunks; c += 64) m = fmaxf(m, part[c][0]);
   m = wave_max(m);
   const float sub = m == -INFINITY ? 0.0f : m;
   float l = 0.f, a = 0.f;
@@ -212,7 +217,7 @@ __device__ inline Row join(const Params &p, int64_t r, int lane, f32x4 first) {
     a = __builtin_fmaf(by, __builtin_fmaf(t, q[1], q[2]), a);
   };
   add(first);
-  for (int c = lane + 64; c < p.chunks; c += 64) add(part[c]);
+  for (int c = lane + 64; c < chunks; c += 64) add(part[c]);
   return {m, wave_sum(l), wave_sum(a)};
 }
 
@@ -253,10 +258,37 @@ __global__ __launch_bounds__(256) void row_kernel(const Params p) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= p.N) return;
-  const f32x4 first = first_chunk(p, r, lane);
+  const f32x4 *part = (const f32x4 *)p.part + r * p.chunks;
+  const f32x4 first = first_chunk(part, p.chunks, lane);
   const Given g = fetch<T>(p, r, lane);
-  const Row row = join(p, r, lane, first);
+  const Row row = join(part, p.chunks, lane, first);
   write_row<T>(p, r, row, g, lane, 64, row.m == -INFINITY ? 0.0f : row.m, logf(row.l));
+}
+
+// Short rows in one launch: ONE: a wave takes a row of one chunk; else a work group takes a row of up to kWhole, whose
+// sums meet in LDS.
+template <typename T, bool ENTROPY, bool ONE>
+__global__ __launch_bounds__(256) void whole_kernel(const Params p) {
+  __shared__ f32x4 part[kWhole];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t r = ONE ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (ONE && r >= p.N) return;
+  const T *x = static_cast<const T *>(p.x) + r * p.x_st;
+  const Given g = fetch<T>(p, r, ONE ? lane : tid);
+  float none = 0.f;
+  Row row;
+  if constexpr (ONE) {
+    const f32x4 sums = chunk_sums<T, ENTROPY, false>(x, p.V, 0, lane, none);
+    row = join(part, 1, lane, lane == 0 ? sums : (f32x4){-INFINITY, 0, 0, 0});
+  } else {
+    for (int c = wave; c < p.chunks; c += 4) {
+      const f32x4 sums = chunk_sums<T, ENTROPY, false>(x, p.V, c * kChunk, lane, none);
+      if (lane == 0) part[c] = sums;
+    }
+    __syncthreads();
+    row = join(part, p.chunks, lane, first_chunk(part, p.chunks, lane));
+  }
+  write_row<T>(p, r, row, g, ONE ? lane : tid, ONE ? 64 : 256, row.m == -INFINITY ? 0.0f : row.m, logf(row.l));
 }
 
 // A value's place among all values as an unsigned number in [0x7fffff, 0xfffffffe]: rising with
@@ -309,9 +341,10 @@ __device__ inline void bisect(uint32_t &bound, uint32_t &over, int &have, int k,
 //     groups than K; most of the largest side by side) the bound is raised by bisection over the
 //     lanes' maxima, and if need be over the values.
 //  3. Each collected value's rank among them is its place in the result.
-// KEYS: group maxima a lane, 64 KEYS >= groups.
+// KEYS: group maxima a lane, 64 KEYS >= groups. `part` and `gm` are the row's chunks' sums and its group
+// maxima, `given` the thread's first token.
 template <typename T, int KEYS>
-__global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
+__device__ __forceinline__ void top_row(const Params &p, const int64_t r, const f32x4 *part, const float *gm, const Given given) {
   constexpr int n = Vec<T>::n, kRegs = kTaken / 4;
   __shared__ int group[4][kTaken];
   __shared__ u32x4 kept[4][kRegs][64];
@@ -319,14 +352,11 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
   __shared__ uint32_t lane_max[256];
   __shared__ int counts[4], sums[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t r = blockIdx.x;
   const int vectors = (p.V + n - 1) / n, groups = (vectors + 63) / 64;
-  const float *gm = p.part + (int64_t)p.N * p.chunks * 4 + r * p.chunks * kVecs;
-  const f32x4 first = first_chunk(p, r, lane);
+  const f32x4 first = first_chunk(part, p.chunks, lane);
   float g[KEYS];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) g[i] = lane + 64 * i < groups ? gm[lane + 64 * i] : 0.0f;
-  const Given given = fetch<T>(p, r, tid);
   uint32_t o[KEYS];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) o[i] = lane + 64 * i < groups ? order(g[i]) : 0;
@@ -396,7 +426,7 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
     }
   wave_sync();
 
-  const Row row = join(p, r, lane, first);
+  const Row row = join(part, p.chunks, lane, first);
   const float m = row.m == -INFINITY ? 0.0f : row.m, logl = logf(row.l);
   write_row<T>(p, r, row, given, tid, 256, m, logl);
   if (!(row.l >= 0.0f)) {  // NaN: the row has no order
@@ -521,6 +551,31 @@ __global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
   }
 }
 
+template <typename T, int KEYS>
+__global__ __launch_bounds__(256, 4) void top_kernel(const Params p) {
+  const int64_t r = blockIdx.x;
+  const Given given = fetch<T>(p, r, threadIdx.x);
+  top_row<T, KEYS>(p, r, (const f32x4 *)p.part + r * p.chunks, p.part + (int64_t)p.N * p.chunks * 4 + r * p.chunks * kVecs, given);
+}
+
+// A short row (kWhole) with its top tokens in one launch.
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(256, 4) void whole_top_kernel(const Params p) {
+  __shared__ f32x4 part[kWhole];
+  __shared__ float gm[kWhole * kVecs];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t r = blockIdx.x;
+  const Given given = fetch<T>(p, r, tid);
+  for (int c = wave; c < p.chunks; c += 4) {
+    float mine = 0.f;
+    const f32x4 sums = chunk_sums<T, ENTROPY, true>(static_cast<const T *>(p.x) + r * p.x_st, p.V, c * kChunk, lane, mine);
+    if (lane == 0) part[c] = sums;
+    if (lane < kVecs) gm[c * kVecs + lane] = mine;
+  }
+  __syncthreads();
+  top_row<T, kWhole * kVecs / 64>(p, r, part, gm, given);
+}
+
 // By how many group maxima a lane keeps in registers: the fewest that hold the row's, for each
 // adds an operation to every step of the search. 128256 bf16 values (251 groups), a whole call of 1 row with 20 top
 // tokens / of 2039 rows with 5, us: 4 a lane 12.8 / 108.7, 8 13.6 / 111.9, 32 18.7 / 118.9. 151936 fp32 values (594 groups),
@@ -628,8 +683,26 @@ inline int chunks_of(int dtype, int vocab) {
   return (int)(((int64_t)vocab + (int64_t)n * kChunk - 1) / ((int64_t)n * kChunk));
 }
 
+template <typename T, bool ENTROPY>
+void forward_whole(const Params &p, hipStream_t s) {
+  if (p.K > 0) hipLaunchKernelGGL((whole_top_kernel<T, ENTROPY>), dim3((unsigned)p.N), dim3(256), 0, s, p);
+  else if (p.chunks == 1) hipLaunchKernelGGL((whole_kernel<T, ENTROPY, true>), dim3((unsigned)((p.N + 3) / 4)), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((whole_kernel<T, ENTROPY, false>), dim3((unsigned)p.N), dim3(256), 0, s, p);
+}
+
+// Whether rows go through one launch, whose work groups take a row (or four of one chunk) whole. us in two
+// launches / in one, bf16 with entropy: 1 row of 4000 4.9 / 3.6, 500 rows of 16000 7.2 / 5.2, 8000 of 4000 17.4 / 15.0,
+// but 2000 of 16000 16.1 / 16.6 and 8000 47 / 55, 100 of 32000 7.0 / 7.4 (work groups wait on their own join); with 5 top tokens 1 of
+// 16000 8.2 / 6.3, 500 of 32000 15.4 / 13.2, 8000 of 10000 85 / 70, but 8000 of 1000 64 / 71 (three waves of four have no
+// chunk); 1 of 50257 (13 chunks) 9.9 / 13.8.
+bool in_one(int rows, int chunks, bool top, int cus) {
+  const bool few = rows <= 4 * (cus > 0 ? cus : 256);
+  return top ? chunks <= kWhole && (few || chunks > 1) : chunks == 1 || (chunks <= 4 && few);
+}
+
 template <typename T>
 void forward(const Params &p, hipStream_t s) {
+  if (in_one(p.N, p.chunks, p.K > 0, dan::num_cus())) return p.entropy ? forward_whole<T, true>(p, s) : forward_whole<T, false>(p, s);
   const dim3 grid((unsigned)(((int64_t)p.N * p.chunks + 3) / 4));
   if (p.entropy) {
     if (p.K > 0) hipLaunchKernelGGL((chunk_kernel<T, true, true>), grid, dim3(256), 0, s, p);
@@ -660,8 +733,9 @@ int check(int abi, int dtype, int rows, int vocab, int labels, int top, int64_t 
   if (top > 0 && vocab > DAN_READOUT_MAX_TOP_VOCAB)
     return fail(DAN_ERR_UNSUPPORTED, "top tokens of %d values: rows of at most %d", vocab, DAN_READOUT_MAX_TOP_VOCAB);
   if (stride < 0 || tokens_stride < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "row strides must be >= 0");
-  // A launch has fewer than 2^32 threads: 64 a chunk, and for the top tokens 256 a row.
-  if (((int64_t)rows * chunks_of(dtype, vocab) + 3) / 4 * 256 >= (int64_t)1 << 32 || (top > 0 && rows >= 1 << 24))
+  // A launch has fewer than 2^32 threads: 64 a chunk, and 256 a row but for rows of one chunk without top tokens.
+  const int64_t chunks = chunks_of(dtype, vocab);
+  if ((rows * chunks + 3) / 4 * 256 >= (int64_t)1 << 32 || ((top > 0 || chunks > 1) && rows >= 1 << 24))
     return fail(DAN_ERR_INVALID_ARGUMENT, "%d rows: too many for one launch", rows);
   return 0;
 }
