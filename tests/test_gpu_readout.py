@@ -88,6 +88,21 @@ def test_many_rows(gpu):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [300, 2048, 4096, 5001, 16384, 16385, 32768, 32769])
+def test_few_and_many_rows_agree(gpu, vocab, dtype):
+    """Short rows go through one launch or two, by how many there are: to the same bits."""
+    g = gen(vocab)
+    x = (torch.randn(40, vocab, generator=g) * 2.5).to(dtype)
+    t = torch.randint(0, vocab, (40, 2), generator=g)
+    xd, td = x.to(gpu).repeat(28, 1), t.to(gpu).repeat(28, 1)
+    for top in (0, 5, 32):
+        few = check_forward(x, t, top, gpu)
+        many = token_logprobs(xd, td, top=top, entropy=True)
+        for a, b in zip(few, many):
+            assert a is None and b is None or torch.equal(a.repeat(28, *[1] * (a.dim() - 1)), b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("vocab", [20, 300, 9000, 40000])
 def test_equal_and_clustered_logits(gpu, vocab, dtype):
     """Rows of one value, of few values, sorted up and down, signed zeros: ties to the lowest id."""
