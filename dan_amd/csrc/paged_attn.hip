@@ -18,17 +18,21 @@
 //     8 keys and takes the transpose in registers (one byte permute for two values).
 // The keys of a lane's 8 contraction slots are the keys whose scores the same lane holds
 // (4 g .. 4 g + 3 of both halves of the tile, g = lane / 16), so P goes from the score
-// registers to the operand without an exchange. P is split into a rounded part and the
-// rounded rest, two products: the output then has the precision of fp32 weights
-// (one rounding of P to bf16 costs about as much as the rounding of the output).
+// registers to the operand without an exchange. P keeps the bits of its fp32 weights: against bf16 values it is
+// cut into three bf16 parts, which hold all 24 bits of a weight; against fp16 ones (e4m3 codes become
+// fp16, which holds each of them) it is scaled by 2^15, so that small weights stay clear of fp16's subnormals, and
+// is a rounded part and the rounded rest, off by 2^-24 of a weight. One product for each part. (Two bf16 parts
+// leave 2^-17 of a weight: outputs next to a border of their own rounding then fall to the other side twice as
+// often as fp32's own errors let them.)
 //
 // Measured, us and TB/s of keys and values, 32/8 heads x 128 in bf16 if not said: 1 sequence of 277 keys
 // 6.4 (of which 4 are a launch and its chain of dependent loads: length, page, keys), 1 of 131072 87
 // (6.2), 64 of up to 8192 194 (5.6), 100 of up to 1000 (32/32 fp16) 133 (6.2), 37 of up to 4099 (16/2 x 256, e4m3) 24
 // (2.6: a CU draws about 60 GB/s from HBM however many waves ask, so what holds a short launch of unequal
 // sequences is the CU with the most keys, and then the join). A large copy moves 4.9.
-// Two tiles in flight a wave (240 registers, 2 waves a SIMD) were 1 to 40 % slower; the two parts
-// of P in one product for up to 8 heads 0 to 3 %: the products are not what bounds it.
+// Two tiles in flight a wave (240 registers, 2 waves a SIMD) were 1 to 40 % slower; two parts
+// of P in one product for up to 8 heads 0 to 3 %, and a third part costs nothing but 0.1 us of the shortest calls: the
+// products are not what bounds it.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -102,6 +106,35 @@ __device__ inline uint32_t pack2(float a, float b) {
 template <typename T>
 __device__ inline f32x2 unpack2(uint32_t w) {
   return __builtin_convertvector(__builtin_bit_cast(typename Ops<T>::x2, w), f32x2);
+}
+
+// The type that values and weights are multiplied in, the parts of a weight, and what the weights are scaled by.
+template <typename T, bool FP8>
+struct Weights {
+  typedef typename std::conditional<FP8, _Float16, T>::type type;
+  static constexpr bool bf16 = std::is_same<type, __bf16>::value;
+  static constexpr int parts = bf16 ? 3 : 2;
+  static constexpr float unit = bf16 ? 1.0f : 32768.0f;
+};
+// Two weights' parts, the largest last.
+template <typename T, bool FP8>
+__device__ inline void split_weights(float a, float b, uint32_t (&part)[Weights<T, FP8>::parts]) {
+  typedef Weights<T, FP8> Wt;
+  if constexpr (Wt::bf16) {
+#pragma unroll
+    for (int n = 2; n >= 0; --n) {
+      const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+      part[n] = __builtin_amdgcn_perm(y, x, 0x07060302);
+      a -= __builtin_bit_cast(float, x & 0xffff0000u);
+      b -= __builtin_bit_cast(float, y & 0xffff0000u);
+    }
+  } else {
+    a *= Wt::unit;
+    b *= Wt::unit;
+    part[1] = pack2<_Float16>(a, b);
+    const f32x2 y = unpack2<_Float16>(part[1]);
+    part[0] = pack2<_Float16>(a - y[0], b - y[1]);
+  }
 }
 
 // A maximum that keeps a NaN out (v_max_f32): NaN scores reach the sum through their weights.
@@ -270,11 +303,11 @@ __device__ inline u32x4 k_operand(const Tile<T, D, FP8> &t, int u, int s, bool l
   }
 }
 
-// Elements 2 m and 2 m + 1 of a value row.
+// Elements 2 m and 2 m + 1 of a value row, as the weights' type has them.
 template <typename T, int D, bool FP8>
 __device__ inline uint32_t v_pair(const Tile<T, D, FP8> &t, int u, int r, int m) {
   if constexpr (!FP8) return t.v[u][r][m];
-  else return m & 1 ? Ops<T>::template from_e4m3<true>(t.v[u][r][m >> 1]) : Ops<T>::template from_e4m3<false>(t.v[u][r][m >> 1]);
+  else return m & 1 ? Ops<_Float16>::from_e4m3<true>(t.v[u][r][m >> 1]) : Ops<_Float16>::from_e4m3<false>(t.v[u][r][m >> 1]);
 }
 
 // W waves. LDS: the waves' results [W][heads][D + 4], their maxima and sums [2][W][heads];
@@ -282,6 +315,7 @@ __device__ inline uint32_t v_pair(const Tile<T, D, FP8> &t, int u, int r, int m)
 template <typename T, int D, bool FP8, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   typedef Tile<T, D, FP8> Tl;
+  typedef Weights<T, FP8> Wt;
   constexpr int VE = Tl::VE, ES = Tl::ES, DP = D + 4, S = D / 32;
   constexpr bool kQLds = D == 256;  // 32 registers that the tile needs
   extern __shared__ __align__(16) float lds[];
@@ -309,10 +343,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   u32x4 *ql = (u32x4 *)lds + lane;
 #pragma unroll
   for (int s = 0; s < (kQLds ? S / W : S); ++s) qf[s] = q_step(kQLds ? W * s + wave : s);
-  float c = p.scale * kLog2e, vscale = 1.0f;
+  float c = p.scale * kLog2e, vscale = 1.0f / Wt::unit;
   if constexpr (FP8) {
     c *= *p.ks;
-    vscale = *p.vs;
+    vscale *= *p.vs;
   }
   const int len = length_of(p, b), chunk = chunk_of(len, p.target, p.splits, W), lo = split * chunk;
   if (lo >= len) {  // nothing here: the join leaves such ranges out (and takes wrong lengths to NaN)
@@ -412,7 +446,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
         for (int j = 0; j < VE; ++j) acc[j] *= by;
       }
       const float sub = m == -INFINITY ? 0.0f : m;
-      u32x4 ph, pl;  // P rounded, and what the rounding left
+      u32x4 pw[Wt::parts];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float w[4];
@@ -423,10 +457,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t x = pack2<T>(w[2 * h], w[2 * h + 1]);
-          const f32x2 y = unpack2<T>(x);
-          ph[2 * u + h] = x;
-          pl[2 * u + h] = pack2<T>(w[2 * h] - y[0], w[2 * h + 1] - y[1]);
+          uint32_t part[Wt::parts];
+          split_weights<T, FP8>(w[2 * h], w[2 * h + 1], part);
+#pragma unroll
+          for (int n = 0; n < Wt::parts; ++n) pw[n][2 * u + h] = part[n];
         }
       }
 #pragma unroll
@@ -444,10 +478,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
             even[2 * u + h] = __builtin_amdgcn_perm(row[u][2 * h + 1], row[u][2 * h], 0x05040100);
             odd[2 * u + h] = __builtin_amdgcn_perm(row[u][2 * h + 1], row[u][2 * h], 0x07060302);
           }
-        acc[2 * e] = Ops<T>::mfma(even, pl, acc[2 * e]);
-        acc[2 * e] = Ops<T>::mfma(even, ph, acc[2 * e]);
-        acc[2 * e + 1] = Ops<T>::mfma(odd, pl, acc[2 * e + 1]);
-        acc[2 * e + 1] = Ops<T>::mfma(odd, ph, acc[2 * e + 1]);
+#pragma unroll
+        for (int n = 0; n < Wt::parts; ++n) {
+          acc[2 * e] = Ops<typename Wt::type>::mfma(even, pw[n], acc[2 * e]);
+          acc[2 * e + 1] = Ops<typename Wt::type>::mfma(odd, pw[n], acc[2 * e + 1]);
+        }
       }
       if constexpr (!last.value) {
         __builtin_amdgcn_sched_barrier(0);

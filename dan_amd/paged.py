@@ -203,7 +203,7 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
     keys' attention takes it, dan/fused.py:94-101). A sequence of no keys gives
     zeros and -inf. A length outside [0, max_len], or a page outside the
     cache, gives NaN for its sequence. An infinite value among a sequence's own may give NaN where
-    the sum would be infinite (weights are held in two parts).
+    the sum would be infinite (weights are held in parts).
 
     How a sequence's keys are split between work groups follows from its own length,
     B, Hkv and ``max_len``: its result does not depend on its neighbours' lengths."""
