@@ -171,14 +171,15 @@ __device__ __forceinline__ f32x4 chunk_sums(const T *row, int vocab, int first, 
         if constexpr (ENTROPY) a = __builtin_fmaf(w, fmaxf(t, -1000.0f), a);  // 0 times -inf else
       }
   };
-  if (fabsf(m) < 1e38f) {
-    // One operation a value: t + d, d being what the product's rounding adds to all of them, taken back below.
+  if (fabsf(m) < 0x1p20f) {
+    // One operation a value: t + d, d being what the product's rounding adds to all of them, taken back below. d is at most
+    // half a unit of m log2 e: 2^-4 here, but past m = 3e9 more than the 127 that an exponent holds.
     const float sub = -m * kLog2e, d = __builtin_fmaf(m, kLog2e, sub);
     sums([&](float v) { return __builtin_fmaf(v, kLog2e, sub); });
     const float by = __builtin_amdgcn_exp2f(-d);
     a = by * __builtin_fmaf(-d, l, a);
     l *= by;
-  } else {  // m log2 e overflows (a chunk of the type's lowest value), or nothing is finite here
+  } else {  // a chunk of large values (as a mask's), or one that nothing finite is in
     const float sub = m == -INFINITY ? 0.0f : m;
     sums([&](float v) { return (v - sub) * kLog2e; });
   }
