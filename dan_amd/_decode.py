@@ -13,7 +13,7 @@ _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c
 
 PAGED_ABI_VERSION = 1
 KEY_BLOCK = 16  # DAN_PAGED_KEY_BLOCK
-READOUT_ABI_VERSION = 1
+READOUT_ABI_VERSION = 2
 MAX_TOP, MAX_TOP_VOCAB = 32, 524288  # DAN_READOUT_MAX_TOP, DAN_READOUT_MAX_TOP_VOCAB
 
 
@@ -50,7 +50,7 @@ class DanLogprobsArgs(ctypes.Structure):
     _fields_ = [("abi_version", _i32), ("dtype", _i32), ("rows", _i32), ("vocab", _i32), ("labels", _i32), ("top", _i32),
                 ("logits", _vp), ("logits_stride", _i64), ("tokens", _vp), ("tokens_stride", _i64),
                 ("logprobs", _vp), ("logsumexp", _vp), ("entropy", _vp), ("top_logprobs", _vp), ("top_ids", _vp),
-                ("workspace", _vp), ("workspace_bytes", _i64)]
+                ("workspace", _vp), ("workspace_bytes", _i64), ("logsumexp_rest", _vp)]
 
 
 class DanLogprobsGradArgs(ctypes.Structure):
@@ -58,7 +58,7 @@ class DanLogprobsGradArgs(ctypes.Structure):
                 ("logits", _vp), ("logits_stride", _i64), ("tokens", _vp), ("tokens_stride", _i64),
                 ("logsumexp", _vp), ("entropy", _vp), ("top_ids", _vp),
                 ("g_logprobs", _vp), ("g_logsumexp", _vp), ("g_entropy", _vp), ("g_top", _vp),
-                ("grad", _vp), ("grad_stride", _i64)]
+                ("grad", _vp), ("grad_stride", _i64), ("logsumexp_rest", _vp)]
 
 
 EXPORTS = ("dan_paged_append", "dan_paged_attn", "dan_paged_attn_workspace_size", "dan_paged_abi_version",

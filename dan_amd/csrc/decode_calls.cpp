@@ -248,17 +248,18 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// What forward gives: undefined where it was not asked for.
+// What forward gives: undefined where it was not asked for. rest: what rounding took from lse.
 struct Outputs {
-  Tensor logprobs, lse, entropy, top_logprobs, top_ids;
+  Tensor logprobs, lse, rest, entropy, top_logprobs, top_ids;
 };
 
-Outputs logprobs_forward(const Tensor &x, const Tensor &tokens, int64_t top, bool entropy) {
+Outputs logprobs_forward(const Tensor &x, const Tensor &tokens, int64_t top, bool entropy, bool rest) {
   const int64_t n = x.size(0), vocab = x.size(1);
   const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
   Outputs o;
   o.logprobs = at::empty(tokens.sizes(), f32);
   o.lse = at::empty({n}, f32);
+  if (rest) o.rest = at::empty({n}, f32);
   if (entropy) o.entropy = at::empty({n}, f32);
   if (top) {
     o.top_logprobs = at::empty({n, top}, f32);
@@ -282,6 +283,7 @@ Outputs logprobs_forward(const Tensor &x, const Tensor &tokens, int64_t top, boo
   a.top_logprobs = static_cast<float *>(at_of(o.top_logprobs));
   a.top_ids = static_cast<int64_t *>(at_of(o.top_ids));
   a.workspace = at_of(ws); a.workspace_bytes = need;
+  a.logsumexp_rest = static_cast<float *>(at_of(o.rest));
   check(lib.logprobs(&a, c10::hip::getCurrentHIPStream(x.get_device()).stream()), "dan_logprobs_fwd");
   return o;
 }
@@ -305,8 +307,8 @@ bool leaves_capture(int index) {
 
 struct Logprobs : torch::autograd::Function<Logprobs> {
   static variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &tokens, int64_t top, bool entropy) {
-    const Outputs o = logprobs_forward(x, tokens, top, entropy);
-    ctx->save_for_backward({x, tokens, o.lse, o.entropy, o.top_ids});
+    const Outputs o = logprobs_forward(x, tokens, top, entropy, true);
+    ctx->save_for_backward({x, tokens, o.lse, o.entropy, o.top_ids, o.rest});
     ctx->saved_data["top"] = top;
     ctx->saved_data["entropy"] = entropy;
     ctx->set_materialize_grads(false);
@@ -360,6 +362,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
       a.g_entropy = static_cast<const float *>(at_of(g[2]));
       a.g_top = static_cast<const float *>(at_of(g[3]));
       a.grad = at_of(grad); a.grad_stride = vocab;
+      a.logsumexp_rest = static_cast<const float *>(at_of(saved[5]));
       // (the engine has made the gradients' device the thread's)
       check(lib.grad(&a, c10::hip::getCurrentHIPStream(x.get_device()).stream()), "dan_logprobs_bwd");
     }
@@ -402,7 +405,7 @@ PyObject *logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       o.top_ids = out[3 + entropy];
     }
   } else {
-    o = logprobs_forward(x, tokens, top, entropy);
+    o = logprobs_forward(x, tokens, top, entropy, false);
   }
   THPObjectPtr tuple(PyTuple_New(5));
   if (!tuple) return nullptr;

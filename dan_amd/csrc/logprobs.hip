@@ -3,6 +3,7 @@
 //
 //   lse = M + log sum e^{x - M};  logp_t = x_t - lse;  H = log sum e^{x - M} - sum (x - M) e^{x - M} / sum e^{x - M}
 //   grad_j = sum_l g_l [t_l = j] + sum_k h_k [i_k = j] + p_j (g_lse - sum g - sum h - g_H (x_j - lse + H))
+// (lse rounded to fp32, and what that took from it, which log p_j = (x_j - lse) - rest needs)
 //
 // HBM-bound: the rows are read once (the backward reads them once more and writes as
 // much). A row is cut into chunks of 512 vectors of 16 bytes; a wave takes one chunk, 8
@@ -99,7 +100,7 @@ __device__ inline uint32_t wave_fold(uint32_t v, F f) {
 struct Params {
   const void *x;
   const int64_t *tokens;
-  float *logprobs, *lse, *entropy, *top_logprobs;
+  float *logprobs, *lse, *rest, *entropy, *top_logprobs;  // rest: of lse, or NULL
   int64_t *top_ids;
   float *part;  // [N, chunks, 4]: maximum, sum e, sum e t (t in log2 units); then [N, chunks * kVecs] group maxima
   int64_t x_st, t_st;
@@ -242,7 +243,12 @@ __device__ inline Given fetch(const Params &p, int64_t r, int l) {
 template <typename T>
 __device__ inline void write_row(const Params &p, int64_t r, const Row &row, Given g, int tid, int count, float m, float logl) {
   if (tid == 0) {
-    p.lse[r] = m + logl;
+    const float lse = m + logl;
+    p.lse[r] = lse;
+    if (p.rest) {  // m + logl = lse + rest exactly, whichever of the two is larger
+      const float back = lse - m;
+      p.rest[r] = fabsf(lse) < INFINITY ? (m - (lse - back)) + (logl - back) : 0.0f;
+    }
     if (p.entropy) p.entropy[r] = row.l == 0.0f ? 0.0f : logl - row.a / row.l * kLn2;
   }
   for (int l = tid; l < p.L; l += count) {
@@ -593,7 +599,7 @@ void launch_top(const Params &p, hipStream_t s) {
 struct GradParams {
   const void *x;
   const int64_t *tokens, *top_ids;
-  const float *lse, *entropy, *g_logp, *g_lse, *g_entropy, *g_top;
+  const float *lse, *rest, *entropy, *g_logp, *g_lse, *g_entropy, *g_top;
   void *grad;
   int64_t x_st, t_st, g_st;
   int32_t N, V, L, K, chunks;
@@ -611,7 +617,7 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradParams p) {
   typename Vec<T>::f32 x[kVecs];
   load_chunk<T>(x, static_cast<const T *>(p.x) + r * p.x_st, p.V, first, lane);
   const float lse = p.lse[r];
-  const float sub = lse == -INFINITY ? 0.0f : lse;
+  const float sub = lse == -INFINITY ? 0.0f : lse, rest = p.rest ? p.rest[r] : 0.0f;
   // The ids of the row that take a gradient of their own (the labels, then the top tokens;
   // none where every logit is -inf), and its sum.
   const int labels = p.g_logp ? p.L : 0, ids = lse == -INFINITY ? 0 : labels + (p.g_top ? p.K : 0);
@@ -643,7 +649,7 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradParams p) {
     typename Vec<T>::f32 y;
 #pragma unroll
     for (int e = 0; e < n; ++e) {
-      const float lp = x[k][e] - sub;
+      const float lp = (x[k][e] - sub) - rest;
       const float w = __builtin_amdgcn_exp2f(lp * kLog2e);
       float f = sum;
       if constexpr (ENTROPY) f = __builtin_fmaf(-ge, fmaxf(lp, -1000.0f) + h, f);  // 0 times -inf else
@@ -726,7 +732,7 @@ void backward(const GradParams &p, hipStream_t s) {
 // What both calls check alike; 0 when all is well.
 int check(int abi, int dtype, int rows, int vocab, int labels, int top, int64_t stride, int64_t tokens_stride) {
   using dan::fail;
-  if (abi != DAN_READOUT_ABI_VERSION) return fail(DAN_ERR_VERSION, "abi_version %d, readout speaks %d", abi, DAN_READOUT_ABI_VERSION);
+  if (abi != DAN_READOUT_ABI_VERSION && abi != 1) return fail(DAN_ERR_VERSION, "abi_version %d, readout speaks %d and 1", abi, DAN_READOUT_ABI_VERSION);
   if (dtype != DAN_DTYPE_BF16 && dtype != DAN_DTYPE_F16 && dtype != DAN_DTYPE_F32) return fail(DAN_ERR_UNSUPPORTED, "dtype %d: bf16, f16 or f32", dtype);
   if (rows < 0 || vocab < 1 || vocab > (1 << 30) || labels < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "need rows >= 0, vocab in [1, 2^30] and labels >= 0");
   if (top < 0 || top > DAN_READOUT_MAX_TOP || top > vocab)
@@ -769,6 +775,7 @@ int dan_logprobs_fwd(const DanLogprobsArgs *a, void *stream) {
     return fail(DAN_ERR_INVALID_ARGUMENT, "workspace: %lld bytes, 16-byte aligned; got %lld", (long long)need, (long long)a->workspace_bytes);
   Params p;
   p.x = a->logits; p.tokens = a->tokens; p.logprobs = a->logprobs; p.lse = a->logsumexp; p.entropy = a->entropy;
+  p.rest = a->abi_version == 1 ? nullptr : a->logsumexp_rest;
   p.top_logprobs = a->top_logprobs; p.top_ids = a->top_ids; p.part = static_cast<float *>(a->workspace);
   p.x_st = a->logits_stride; p.t_st = a->tokens_stride;
   p.N = a->rows; p.V = a->vocab; p.L = a->labels; p.K = a->top; p.chunks = chunks_of(a->dtype, a->vocab);
@@ -796,6 +803,7 @@ int dan_logprobs_bwd(const DanLogprobsGradArgs *a, void *stream) {
   if (a->grad_stride < a->vocab) return fail(DAN_ERR_INVALID_ARGUMENT, "grad_stride %lld < vocab", (long long)a->grad_stride);
   GradParams p;
   p.x = a->logits; p.tokens = a->tokens; p.top_ids = a->top_ids; p.lse = a->logsumexp; p.entropy = a->entropy;
+  p.rest = a->abi_version == 1 ? nullptr : a->logsumexp_rest;
   p.g_logp = a->g_logprobs; p.g_lse = a->g_logsumexp; p.g_entropy = a->g_entropy; p.g_top = a->g_top; p.grad = a->grad;
   p.x_st = a->logits_stride; p.t_st = a->tokens_stride; p.g_st = a->grad_stride;
   p.N = a->rows; p.V = a->vocab; p.L = a->labels; p.K = a->top; p.chunks = chunks_of(a->dtype, a->vocab);

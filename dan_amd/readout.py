@@ -26,7 +26,8 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]  # int64 [N, top]
 
 
-def _forward(logits, tokens, top, entropy):
+def _forward(logits, tokens, top, entropy, rest=None):
+    """The five outputs; what rounding took from logsumexp into ``rest`` (fp32 [N])."""
     n, vocab = logits.shape
     dev, dtype = logits.device, _DTYPES[logits.dtype]
     labels = tokens.shape[1] if tokens.dim() == 2 else 1
@@ -44,15 +45,17 @@ def _forward(logits, tokens, top, entropy):
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _decode.call_logprobs(
         _native.stream(dev), _decode.READOUT_ABI_VERSION, dtype, n, vocab, labels, top, logits.data_ptr(), logits.stride(0),
-        tokens.data_ptr(), tokens.stride(0), logprobs.data_ptr(), lse.data_ptr(), ent_p, lp_p, id_p, ws.data_ptr(), need)
+        tokens.data_ptr(), tokens.stride(0), logprobs.data_ptr(), lse.data_ptr(), ent_p, lp_p, id_p, ws.data_ptr(), need,
+        0 if rest is None else rest.data_ptr())
     return logprobs, lse, ent, top_lp, top_ids
 
 
 class _Logprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, entropy):
-        logprobs, lse, ent, top_lp, top_ids = _forward(logits, tokens, top, entropy)
-        ctx.save_for_backward(logits, tokens, lse, ent, top_ids)
+        rest = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        logprobs, lse, ent, top_lp, top_ids = _forward(logits, tokens, top, entropy, rest)
+        ctx.save_for_backward(logits, tokens, lse, rest, ent, top_ids)
         ctx.top = top
         ctx.set_materialize_grads(False)
         if top:
@@ -62,14 +65,14 @@ class _Logprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logprobs, g_lse, g_entropy, g_top, _g_ids):
-        logits, tokens, lse, ent, top_ids = ctx.saved_tensors
+        saved, logits = ctx.saved_tensors, ctx.saved_tensors[0]
         if torch._C._cuda_getDevice() != logits.device.index:  # (the engine's thread is on the gradients' device)
             with torch.cuda.device(logits.device):
-                return _backward(logits, tokens, lse, ent, top_ids, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
-        return _backward(logits, tokens, lse, ent, top_ids, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
+                return _backward(*saved, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
+        return _backward(*saved, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
 
 
-def _backward(logits, tokens, lse, ent, top_ids, top, *grads):
+def _backward(logits, tokens, lse, rest, ent, top_ids, top, *grads):
     grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
     n, vocab = logits.shape
     dtype = logits.dtype
@@ -78,7 +81,7 @@ def _backward(logits, tokens, lse, ent, top_ids, top, *grads):
     _decode.call_logprobs_grad(
         _native.stream(logits.device), _decode.READOUT_ABI_VERSION, _DTYPES[dtype], n, vocab, tokens.shape[1] if tokens.dim() == 2 else 1, top,
         logits.data_ptr(), logits.stride(0), tokens.data_ptr(), tokens.stride(0), lse.data_ptr(), 0 if ent is None else ent.data_ptr(),
-        0 if top_ids is None else top_ids.data_ptr(), g_logp, g_lse, g_ent, g_top, grad.data_ptr(), vocab)
+        0 if top_ids is None else top_ids.data_ptr(), g_logp, g_lse, g_ent, g_top, grad.data_ptr(), vocab, rest.data_ptr())
     return grad
 
 

@@ -21,14 +21,15 @@
 extern "C" {
 #endif
 
-#define DAN_READOUT_ABI_VERSION 1
+/* 2. The calls take version 1 as well: the structures without their last field, logsumexp_rest. */
+#define DAN_READOUT_ABI_VERSION 2
 
 /* At most so many top tokens, and so many values in a row whose top tokens are asked for. */
 #define DAN_READOUT_MAX_TOP 32
 #define DAN_READOUT_MAX_TOP_VOCAB 524288
 
 typedef struct {
-  int32_t abi_version; /* DAN_READOUT_ABI_VERSION */
+  int32_t abi_version; /* DAN_READOUT_ABI_VERSION, or 1 */
   int32_t dtype;       /* DanDtype of the logits (and of their gradient): bf16, f16 or f32 */
   int32_t rows;        /* N */
   int32_t vocab;       /* V >= 1 */
@@ -42,6 +43,7 @@ typedef struct {
   float *top_logprobs; /* [N, K] */
   int64_t *top_ids;    /* [N, K] */
   void *workspace; int64_t workspace_bytes; /* dan_logprobs_workspace_size bytes, 16-byte aligned */
+  float *logsumexp_rest; /* [N] or NULL: what rounding to fp32 took from logsumexp (0 where that is not finite) */
 } DanLogprobsArgs;
 
 /* logprobs[n, l] = x[n, tokens[n, l]] - logsumexp[n]; a negative token is
@@ -55,7 +57,7 @@ int dan_logprobs_fwd(const DanLogprobsArgs *args, void *stream);
 int64_t dan_logprobs_workspace_size(int32_t dtype, int32_t rows, int32_t vocab, int32_t top);
 
 typedef struct {
-  int32_t abi_version;
+  int32_t abi_version; /* DAN_READOUT_ABI_VERSION, or 1 */
   int32_t dtype, rows, vocab, labels, top;
   const void *logits; int64_t logits_stride;
   const int64_t *tokens; int64_t tokens_stride;
@@ -67,6 +69,8 @@ typedef struct {
   const float *g_entropy;     /* [N] or NULL */
   const float *g_top;         /* [N, K] contiguous, or NULL */
   void *grad; int64_t grad_stride; /* [N, V] of dtype */
+  const float *logsumexp_rest; /* [N], of the forward call; NULL: zeros, which leaves each p off by half a unit of logsumexp
+                                  (2^-24 |logsumexp| of p: all of it where that is 2^24 and more) */
 } DanLogprobsGradArgs;
 
 /* grad[n, j] = sum_l g_l [tokens_l = j] + sum_k h_k [top_k = j]

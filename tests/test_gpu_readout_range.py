@@ -103,3 +103,78 @@ def test_finite_logits_fp16(gpu, offset):
     x[:4, 100:] = offset
     x[4:] += offset / 2
     check(x.to(F16), torch.randint(0, 9000, (9, 4), generator=gen(4)), 5, gpu)
+
+
+# ------------------------------------------------------------------ gradients
+
+
+class _Rest:
+    """Stands for the host module: makes no call, so that the Python functions make every one."""
+
+    append = attend = logprobs = staticmethod(lambda *args: None)
+
+
+def check_gradient(x, tokens, top, gpu, seed=0):
+    """Against the formula in 64 bits with x - M - log(sum) for log p. p is off by 2^-17 for the sum in it, 2^-24 |log p| < 2^-17 for the
+    exponent's rounding: 2^-16 of p (|pull| + |g_H| (|log p| + H)), as in test_gpu_readout.py, whatever the logits' size.
+    A p below 2^-126, fp32's smallest normal value, is 0 on the hardware: off by less than 2^-126 of what it is a factor of."""
+    g = gen(seed)
+    n, vocab = x.shape
+    leaf = x.to(gpu).requires_grad_()
+    r = token_logprobs(leaf, tokens.to(gpu), top=top, entropy=True)
+    w = [torch.randn(s, generator=g) for s in (tokens.shape, (n,), (n,), (n, top))]
+    outs = [r.logprobs, r.logsumexp, r.entropy] + ([r.top_logprobs] if top else [])
+    got = torch.autograd.grad(outs, leaf, [t.to(gpu) for t, _ in zip(w, outs)])[0]
+    torch.cuda.synchronize()
+    logp, _, _, ent = exact(x)
+    p = logp.exp()
+    own, mag = torch.zeros_like(logp), torch.zeros_like(logp)
+    for ids, h in ((tokens, w[0]), (ordered(x, top), w[3])):
+        own.scatter_add_(1, ids, h.double())
+        mag.scatter_add_(1, ids, h.double().abs())
+    weight = torch.where(p > 0, logp + ent[:, None], 0.0)
+    ge = w[2].double()[:, None]
+    ref = own + p * (w[1].double()[:, None] - own.sum(1, keepdim=True) - ge * weight)
+    pull = w[1].double().abs()[:, None] + mag.sum(1, keepdim=True) + ge.abs() * (torch.where(p > 0, logp.abs(), 0.0) + ent[:, None])
+    tol = torch.finfo(x.dtype).eps / 2 * ref.abs() + (2.0 ** -16 * p + 2.0 ** -126) * pull + 2.0 ** -22 * mag + (2.0 ** -25 if x.dtype == F16 else 1e-37)
+    worst = ((got.double().cpu() - ref).abs() / tol).max().item()
+    say(f"gradient {tuple(x.shape)} {x.dtype} top={top}: {worst:.3f} of the tolerance")
+    assert worst <= 1.0
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1e3, 1e5] + SIZES + [3.3e38])
+@pytest.mark.parametrize("vocab", [300, 5000, 33333])
+def test_gradient_of_finite_logits_of_any_size(gpu, vocab, size, dtype):
+    g = gen(vocab + 1)
+    x = rows_of(vocab, size, dtype, g)
+    tokens = torch.stack([torch.randint(0, vocab, (9,), generator=g), torch.full((9,), 5)], 1)
+    check_gradient(x, tokens, 0, gpu)
+    check_gradient(x, tokens, 4, gpu)
+
+
+@pytest.mark.parametrize("offset", [-1e6, -1e4, -300.0, 77.0, 1e4, 1e6, 1.6e7])
+def test_gradient_at_an_offset(gpu, offset):
+    """Logits of ordinary spread around an offset, and one value in all places: sum p is 1, not e^(what rounding takes from logsumexp)."""
+    vocab = 32000
+    x = torch.randn(4, vocab, generator=gen(7)) * 2 + offset
+    x[3] = offset
+    t = torch.randint(0, vocab, (4, 1), generator=gen(8))
+    check_gradient(x, t, 0, gpu)
+    leaf = x.to(gpu).requires_grad_()
+    (grad,) = torch.autograd.grad(token_logprobs(leaf, t.to(gpu)).logsumexp.sum(), leaf)
+    assert (grad.double().sum(1) - 1).abs().max() <= 2.0 ** -16
+
+
+def test_gradient_of_lowest_rows_through_python(gpu, monkeypatch):
+    """The calls that go on in Python keep the same two parts of logsumexp."""
+    from dan_amd import _decode
+
+    x = torch.full((3, 700), torch.finfo(F32).min)
+    x[1] = 1e6
+    x[2, :5] = -1e10
+    t = torch.tensor([[3, 200], [0, 699], [4, 9]])
+    first = check_gradient(x, t, 2, gpu)
+    monkeypatch.setattr(_decode, "calls", lambda: _Rest)
+    assert torch.equal(first, check_gradient(x, t, 2, gpu))
