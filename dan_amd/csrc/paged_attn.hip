@@ -66,7 +66,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32, kHeads = 16;
 constexpr int kMaxLen = 1 << 30;  // places are 32-bit
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 struct Ops;
@@ -163,7 +163,7 @@ struct Params {
   const void *q, *kc, *vc;
   void *out;
   float *lse;
-  float *part;  // [B * H, splits, D] unnormalized outputs, then [B * H, splits, 2] (maximum in log2 units, sum)
+  float *part;  // [B * H, splits, D] unnormalized outputs, then [B * H, splits, 2] (maximum q . k, sum)
   const float *ks, *vs;
   dan::PageTable table;
   const int32_t *lens;
@@ -177,6 +177,11 @@ __device__ inline int length_of(const Params &p, int b) {
   const int n = p.lens[b];
   return (uint32_t)n <= (uint32_t)p.max_len ? n : -1;
 }
+
+// What a product q . k (of codes, from an e4m3 cache) is multiplied by to be a score. The largest product is subtracted
+// before that, so that its weight is 1 whatever its size: the rounding of a maximum that is multiplied first would be part of every
+// exponent, and at scores of 1e9 that is more than fp32 or fp16 hold.
+__device__ inline float score_of(const Params &p) { return p.scale * (p.ks ? *p.ks : 1.0f); }
 
 // Keys of a range of a sequence of `len`: a `target`-th of it, within limits, in whole rounds of the work
 // group's tiles. By its own length alone, so that a sequence's result does not change with its
@@ -343,11 +348,9 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   u32x4 *ql = (u32x4 *)lds + lane;
 #pragma unroll
   for (int s = 0; s < (kQLds ? S / W : S); ++s) qf[s] = q_step(kQLds ? W * s + wave : s);
-  float c = p.scale * kLog2e, vscale = 1.0f / Wt::unit;
-  if constexpr (FP8) {
-    c *= *p.ks;
-    vscale *= *p.vs;
-  }
+  const float to_score = score_of(p), c = to_score * kLog2e;
+  float vscale = 1.0f / Wt::unit;
+  if constexpr (FP8) vscale *= *p.vs;
   const int len = length_of(p, b), chunk = chunk_of(len, p.target, p.splits, W), lo = split * chunk;
   if (lo >= len) {  // nothing here: the join leaves such ranges out (and takes wrong lengths to NaN)
     if (direct) {
@@ -436,10 +439,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
             }
       }
       float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-      top = max_across_groups(top) * c;
+      top = max_across_groups(top);
       if (__any(top > m)) {
         const float to = fmaxf(m, top);
-        const float by = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        const float by = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
         m = to;
         l *= by;
 #pragma unroll
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
         float w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][r], c, -sub));
+          w[r] = __builtin_amdgcn_exp2f((sc[u][r] - sub) * c);
           l += w[r];
         }
 #pragma unroll
@@ -527,7 +530,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float by = __builtin_amdgcn_exp2f(mw[w] - sub);
+      const float by = __builtin_amdgcn_exp2f((mw[w] - sub) * c);
       sum += by * ml[(W + w) * heads + h];
       o += by * *(const f32x4 *)(lds + (w * heads + h) * DP + d);
     }
@@ -536,7 +539,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
       const float inv = vscale / sum;
       typename Ops<T>::x4 y = __builtin_convertvector(o * inv, typename Ops<T>::x4);
       *(DAN_GLOBAL u32x2 *)(static_cast<T *>(p.out) + b * p.o_ss + (head0 + h) * p.o_sh + d) = __builtin_bit_cast(u32x2, y);
-      if (p.lse && d == 0) p.lse[row] = sub * kLn2 + logf(sum);
+      if (p.lse && d == 0) p.lse[row] = sub * to_score + logf(sum);
     } else {
       *(DAN_GLOBAL f32x4 *)(p.part + (row * p.splits + split) * D + d) = o * vscale;
       if (d == 0) {
@@ -562,14 +565,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
   const float *rows = p.part + row * p.splits * D + d;
   const int len = length_of(p, b);
   const int chunk = chunk_of(len, p.target, p.splits, p.waves), n = len <= 0 ? 0 : (len + chunk - 1) / chunk;
+  const float to_score = score_of(p), c = to_score * kLog2e;
   f32x4 o = {0, 0, 0, 0};
-  float top = -INFINITY, sum = 0.f;
+  float top = -INFINITY, sum = 0.f;  // top: in products
 #pragma unroll 4
   for (int s = gr; s < n; s += GR) {
     const f32x2 q = *(const DAN_GLOBAL f32x2 *)(ml + 2 * s);
     const f32x4 x = *(const DAN_GLOBAL f32x4 *)(rows + (int64_t)s * D);
     const float to = fmaxf(top, q[0]), sub = to == -INFINITY ? 0.0f : to;
-    const float was = __builtin_amdgcn_exp2f(top - sub), by = __builtin_amdgcn_exp2f(q[0] - sub);
+    const float was = __builtin_amdgcn_exp2f((top - sub) * c), by = __builtin_amdgcn_exp2f((q[0] - sub) * c);
     top = to;
     sum = __builtin_fmaf(by, q[1], was * sum);
     o = was * o + by * x;
@@ -588,14 +592,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
     sum = 0.f;
 #pragma unroll
     for (int w = 0; w < GR; ++w) {
-      const float by = __builtin_amdgcn_exp2f(tops[w] - sub);
+      const float by = __builtin_amdgcn_exp2f((tops[w] - sub) * c);
       o += by * *(const f32x4 *)&part[w][d];
       sum += by * sums[w];
     }
     const float inv = len > 0 ? 1.0f / sum : len == 0 ? 0.0f : __builtin_nanf("");
     typename Ops<T>::x4 y = __builtin_convertvector(o * inv, typename Ops<T>::x4);
     *(DAN_GLOBAL u32x2 *)(static_cast<T *>(p.out) + b * p.o_ss + h * p.o_sh + d) = __builtin_bit_cast(u32x2, y);
-    if (p.lse && d == 0) p.lse[row] = len > 0 ? sub * kLn2 + logf(sum) : len == 0 ? -INFINITY : __builtin_nanf("");
+    if (p.lse && d == 0) p.lse[row] = len > 0 ? sub * to_score + logf(sum) : len == 0 ? -INFINITY : __builtin_nanf("");
   }
 }
 
@@ -724,7 +728,7 @@ int dan_paged_attn(const DanPagedAttnArgs *a, void *stream) {
 
   Params p;
   p.q = a->q; p.kc = a->k_cache; p.vc = a->v_cache; p.out = a->out; p.lse = a->lse; p.part = static_cast<float *>(a->workspace);
-  p.ks = a->k_scale; p.vs = a->v_scale; p.table = {a->table, a->table_stride, B, a->table ? a->table_width : 0, a->page_size, a->num_pages}; p.lens = a->lens;
+  p.ks = fp8 ? a->k_scale : nullptr; p.vs = a->v_scale; p.table = {a->table, a->table_stride, B, a->table ? a->table_width : 0, a->page_size, a->num_pages}; p.lens = a->lens;
   p.q_ss = a->q_stride_seq; p.q_sh = a->q_stride_head; p.o_ss = a->o_stride_seq; p.o_sh = a->o_stride_head;
   p.kc_sp = a->kc_stride_page; p.kc_sh = a->kc_stride_head; p.kc_st = a->kc_stride_tok;
   p.vc_sp = a->vc_stride_page; p.vc_sh = a->vc_stride_head; p.vc_st = a->vc_stride_tok;

@@ -89,3 +89,39 @@ def test_many_small_weights_beside_a_large_one(gpu, n, dtype, cache):
     worst = (out - ref).abs().max().item() / tol
     say(f"small weights {dtype} cache={cache} n={n}: {worst:.3f} of the tolerance")
     assert worst <= 1.0 and (lse - math.log1p(total)).abs().max() <= (n + 64) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("d,n", [(64, 5), (128, 40), (256, 40), (64, 3001), (128, 9000), (256, 9000)])
+def test_finite_scores_of_any_size(gpu, d, n, dtype, cache):
+    """Scores of up to 2^29 (fp16) to 2^40, far apart: the largest takes all, equal ones share, in one range and in several. Products are single and
+    exact; the weights are 1 and 0, so that only the output rounds (a sum of two and a quotient by 2 are exact: u |o|), and the logsumexp by 2^-22."""
+    g = gen(n + d)
+    b, h = 6, 8
+    size = 2.0 ** (15 if dtype == F16 else 20)
+    q = torch.zeros(b, h, d, dtype=dtype)
+    q[..., 7] = torch.where(torch.arange(h) % 2 == 0, size, -size).to(dtype)
+    k = torch.zeros(b, n, 2, d)
+    steps = torch.randint(-100, 100, (b, n, 2), generator=g).float()
+    steps = torch.where(steps == 0, 1.0, steps)
+    steps[0, 0], steps[0, n - 1] = 110, 110       # two at the top
+    steps[1, n // 2] = 120
+    steps[2] = 96                                  # all alike
+    steps[3] = -steps[3].abs() - 1                 # all of one sign
+    unit = 1.0 if cache == E4M3 else 2.0 ** 8 if dtype == F16 else 2.0 ** 13
+    k[..., 7] = (steps * unit).to(cache).float()
+    v = torch.randint(-8, 9, (b, n, 2, d), generator=g).float()
+    ks = 2.0 ** 12
+    out, lse = call(q, k, v, gpu, cache, ks=ks, vs=1.0)
+    s = torch.einsum("bhd,bnhd->bhn", q.double(), k.double().repeat_interleave(h // 2, 2)) * (ks if cache == E4M3 else 1.0)
+    p = torch.softmax(s, -1)
+    assert s.abs().max() >= 2.0 ** 29
+    ref = torch.einsum("bhn,bnhd->bhd", p, v.double().repeat_interleave(h // 2, 2))
+    some = (p > 0).sum(-1).double()[..., None]     # of many equal ones the sum's quotient by their number rounds, too
+    tol = HALF[dtype] * ref.abs() + torch.where(some > 2, 2.0 ** -21, 0.0) * 8
+    worst = torch.where(out == ref, 0.0, (out - ref).abs() / tol)
+    assert not worst.isnan().any()
+    rl = torch.logsumexp(s, -1)
+    lerr = ((lse - rl).abs() / (rl.abs() * 2.0 ** -22 + 2.0 ** -21)).max().item()
+    say(f"scores to {s.abs().max().item():.3g} {dtype} cache={cache} x {d}, {n} keys: {worst.max().item():.3f} of the tolerance, lse {lerr:.3f}")
+    assert worst.max() <= 1.0 and lerr <= 1.0
