@@ -183,6 +183,8 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   a.seqs = static_cast<const int32_t *>(at_of(seqs));
   a.rope_rows = static_cast<const int32_t *>(at_of(rope));
   check(lib.append(&a, c10::hip::getCurrentHIPStream(index).stream()), "dan_paged_append");
+  for (const Tensor *t : {&kc, &vc})  // a backward that has saved a cache must not take the new rows for the old
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }

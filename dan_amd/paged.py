@@ -97,7 +97,8 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
     stored. ``seqs`` (int32 [N]): its row of ``table``; None: token n belongs to
     sequence n (a decode step). Tokens whose page the table does not name (past its width,
     or outside the cache) are not stored either. No two tokens may share a place, and
-    q, k and v may not lie in rows of the cache that the call writes.
+    q, k and v may not lie in rows of the cache that the call writes. To autograd it is an in-place
+    operation on both caches.
 
     Returns q [H, N, D], a view of a new token-major [N, H, D] tensor (None
     without q). All arithmetic is fp32, rounded once at each store (an e4m3
@@ -176,6 +177,8 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
         _native.stream(dev), _decode.PAGED_ABI_VERSION, _DTYPES[dtype], _DTYPES[k_cache.dtype], _DTYPES[cs_type], n, h, hkv, d, r, NORMS[norm],
         page, pages, width, seqs_of_table, rows, _native.f32(float(eps)), q_p, q_st, q_sh, k_p, k_st, k_sh, v_p, v_st, v_sh,
         cs_p, sn_p, cs_st, qw_p, kw_p, out_p, h * d, d, *kc, *vc, ks, vs, table.data_ptr(), table.stride(0), place_p, seq_p, rope_p)
+    if n:  # a backward that has saved a cache must not take the new rows for the old
+        torch.autograd.graph.increment_version([k_cache, v_cache])
     return None if out is None else out.transpose(0, 1)
 
 
