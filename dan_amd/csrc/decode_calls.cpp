@@ -124,7 +124,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   const int64_t norm = PyLong_AsLong(args[14]);
   if (norm < DAN_FRONT_NORM_NONE || norm > DAN_FRONT_NORM_RMS_ZERO_CENTERED) Py_RETURN_NONE;
   if (!is16(dtype) || k.dim() != 3 || q.dim() != 3 || v.sizes() != k.sizes() || q.size(0) != k.size(0) || q.size(2) != k.size(2) ||
-      q.scalar_type() != dtype || v.scalar_type() != dtype || grads_of({&q, &k, &v, &kc, &vc}))
+      q.scalar_type() != dtype || v.scalar_type() != dtype || grads_of({&q, &k, &v, &kc, &vc, &cos, &sin, &ks, &vs}))
     Py_RETURN_NONE;
   const int64_t n = k.size(0), h = q.size(1), hkv = k.size(1), d = k.size(2);
   if (!fits(n) || !fits(h) || !fits(hkv) || n == 0 || !cache_ok(kc, vc, ks, vs, table, dtype, index) || kc.size(1) != hkv || kc.size(3) != d)
@@ -149,6 +149,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
   }
   if (norm != DAN_FRONT_NORM_NONE) {
+    if (grads_of({&qw, &kw})) Py_RETURN_NONE;
     for (const Tensor *t : {&qw, &kw})
       if (!t->defined() || t->dim() != 1 || t->size(0) != d || t->scalar_type() != dtype || !plain(*t, index) || !rows_ok(*t)) Py_RETURN_NONE;
     a.q_norm_weight = at_of(qw);
@@ -203,7 +204,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
   const int index = q.get_device();
   const auto dtype = q.scalar_type();
-  if (!is16(dtype) || q.dim() != 3 || !plain(q, index) || !rows_ok(q) || grads_of({&q, &kc, &vc}) || !cache_ok(kc, vc, ks, vs, table, dtype, index))
+  if (!is16(dtype) || q.dim() != 3 || !plain(q, index) || !rows_ok(q) || grads_of({&q, &kc, &vc, &ks, &vs}) || !cache_ok(kc, vc, ks, vs, table, dtype, index))
     Py_RETURN_NONE;
   const int64_t h = q.size(0), b = q.size(1), d = q.size(2), hkv = kc.size(1), page = kc.size(2), holds = table.size(1) * page;
   int overflow = 0;

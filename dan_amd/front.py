@@ -76,7 +76,8 @@ def qkv_front(q, k, v, cos, sin, *, q_norm_weight=None, k_norm_weight=None, eps=
     (R: rotary dims, a multiple of 16 up to D; the reference's tables).
     ``norm``: None (no q/k norm), "rms" (dan/fused.py:36-40) or
     "zero_centered" (dan/fused.py:44-48), with ``q_norm_weight``,
-    ``k_norm_weight`` [D] and ``eps``.
+    ``k_norm_weight`` [D] and ``eps``. Forward only: q and k that require grad
+    are refused, weights and tables are taken as constants.
 
     Returns ``(q [H, N, D], k [Hkv, N, D], v [Hkv, N, D])``: the first two
     are views of new token-major [N, H, D] / [N, Hkv, D] tensors, v is the

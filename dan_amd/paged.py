@@ -71,6 +71,13 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale, table, dtype, device):
     return shape, k_scale.data_ptr(), v_scale.data_ptr()
 
 
+def _forward_only(name, *inputs):
+    """Refuses inputs that a derivative is wanted of."""
+    inputs = [t for t in inputs if isinstance(t, torch.Tensor)]
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)) or has_tangent(*inputs):
+        raise NotImplementedError(f"{name} is forward-only")
+
+
 def _check_index(t, name, count, device):
     if t.dtype != torch.int32 or t.shape != (count,) or t.device != device or (t.stride(0) != 1 and count > 1):
         raise ValueError(f"{name} must be a contiguous int32 [{count}] on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -116,9 +123,7 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
             return append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, seqs=seqs, rope_rows=rope_rows,
                                 q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, eps=eps, norm=norm, k_scale=k_scale,
                                 v_scale=v_scale)
-    inputs = (k, v, k_cache, v_cache) if q is None else (q, k, v, k_cache, v_cache)
-    if (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)) or has_tangent(*inputs):
-        raise NotImplementedError("append_paged is forward-only")
+    _forward_only("append_paged", q, k, v, cos, sin, k_cache, v_cache, k_scale, v_scale, *((q_norm_weight, k_norm_weight) if norm is not None else ()))
     dtype, shape = k.dtype, k.shape
     if len(shape) != 3 or v.shape != shape:
         raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must both be [N, Hkv, D]")
@@ -220,8 +225,7 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
         with torch.cuda.device(dev):
             return attend_paged(q, k_cache, v_cache, table, lens, scale, k_scale=k_scale, v_scale=v_scale, max_len=max_len,
                                 return_lse=return_lse)
-    if (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)) or has_tangent(q, k_cache, v_cache):
-        raise NotImplementedError("attend_paged is forward-only")
+    _forward_only("attend_paged", q, k_cache, v_cache, k_scale, v_scale)
     dtype, shape = q.dtype, q.shape
     if len(shape) != 3 or (dtype != torch.bfloat16 and dtype != torch.float16):
         raise ValueError(f"q must be [H, B, D] in bf16 or fp16; got {tuple(shape)} {dtype}")

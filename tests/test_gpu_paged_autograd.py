@@ -75,3 +75,34 @@ def test_inference_tensors_are_written(gpu, path):
     with torch.inference_mode():
         append(q, k, v, kc, vc, table, places)  # caches made outside
     assert kc._version == 1 and (vc == 1).sum() == 2 * HKV * D
+
+
+def test_every_input_that_wants_a_derivative_is_refused(gpu, path):
+    """Both are forward-only: no input loses its gradient or tangent without a word, the norm's weights, tables and scales among them. Without grad
+    mode, and where the call does not use them, they pass."""
+    say(f"paged: inputs that require grad, {path}")
+    q, k, v, kc, vc, table, places = inputs(gpu)
+    one, cs = torch.ones(D, dtype=BF16, device=gpu), torch.ones(2, D, device=gpu)
+    e4m3, scale = torch.zeros(3, HKV, PAGE, D, device=gpu).to(torch.float8_e4m3fn), torch.ones(1, device=gpu)
+    plain = dict(q=q, k=k, v=v, kc=kc, vc=vc, table=table, places=places, norm="rms", q_norm_weight=one, k_norm_weight=one, cos=cs, sin=cs)
+    coded = dict(plain, kc=e4m3, vc=e4m3.clone(), k_scale=scale, v_scale=scale)
+    dual = torch.autograd.forward_ad
+    for base, names in ((plain, ("q", "k", "v", "kc", "vc", "q_norm_weight", "k_norm_weight", "cos", "sin")), (coded, ("k_scale", "v_scale"))):
+        append(**base)
+        for name in names:
+            wants = dict(base, **{name: base[name].clone().requires_grad_()})
+            with pytest.raises(NotImplementedError):
+                append(**wants)
+            with torch.no_grad():
+                append(**wants)
+            with dual.dual_level(), pytest.raises(NotImplementedError):
+                append(**dict(base, **{name: dual.make_dual(base[name], torch.ones_like(base[name]))}))
+    append(**dict(plain, norm=None, q_norm_weight=one.clone().requires_grad_()))  # not used
+    heads, lens = q.transpose(0, 1), torch.tensor([1, 1], dtype=torch.int32, device=gpu)
+    for cache, scales in ((kc, {}), (e4m3, dict(k_scale=scale, v_scale=scale))):
+        attend_paged(heads, cache, cache, table, lens, **scales)
+        for name in scales:
+            with pytest.raises(NotImplementedError):
+                attend_paged(heads, cache, cache, table, lens, **dict(scales, **{name: scale.clone().requires_grad_()}))
+            with dual.dual_level(), pytest.raises(NotImplementedError):
+                attend_paged(heads, cache, cache, table, lens, **dict(scales, **{name: dual.make_dual(scale, scale)}))
