@@ -102,3 +102,11 @@ def calls():
         "dan_paged_append", "dan_paged_attn", "dan_paged_attn_workspace_size", "dan_logprobs_fwd", "dan_logprobs_bwd",
         "dan_logprobs_workspace_size", "dan_tree_attn_last_error")))
     return module
+
+
+_host = calls
+
+
+def check_capture(device_index):
+    """Inside a backward: refuses to run in a capture that torch's engine would make the stream of an eager graph wait for."""
+    _host().check_capture(device_index)

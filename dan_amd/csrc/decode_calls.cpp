@@ -308,6 +308,20 @@ bool leaves_capture(int index) {
   return captures(here.stream()) && !captures(there.stream());
 }
 
+void check_capture(int index) {
+  TORCH_CHECK(!leaves_capture(index), "token_logprobs: a captured backward whose logits were first used outside of the capture; "
+              "drop every earlier result that holds their graph before the capture");
+}
+// check_capture(device index), for a backward that runs in Python
+PyObject *py_check_capture(PyObject *, PyObject *arg) {
+  HANDLE_TH_ERRORS
+  const long index = PyLong_AsLong(arg);
+  if (index == -1 && PyErr_Occurred()) return nullptr;
+  check_capture((int)index);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 struct Logprobs : torch::autograd::Function<Logprobs> {
   static variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &tokens, int64_t top, bool entropy) {
     const Outputs o = logprobs_forward(x, tokens, top, entropy, true);
@@ -338,8 +352,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
       again |= g[i].defined() && g[i].requires_grad();
     }
     if (!any) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    TORCH_CHECK(!leaves_capture(x.get_device()), "token_logprobs: a captured backward whose logits were first used outside of the capture; "
-                "drop every earlier result that holds their graph before the capture");
+    check_capture(x.get_device());
     again = (again || x.requires_grad()) && at::GradMode::is_enabled();
     Tensor grad;
     {
@@ -442,7 +455,8 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 }
 
 #define DAN_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {DAN_METHOD(append), DAN_METHOD(attend), DAN_METHOD(logprobs), DAN_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {DAN_METHOD(append), DAN_METHOD(attend), DAN_METHOD(logprobs), DAN_METHOD(bind),
+                         {"check_capture", py_check_capture, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decode_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -65,7 +65,9 @@ class _Logprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logprobs, g_lse, g_entropy, g_top, _g_ids):
-        saved, logits = ctx.saved_tensors, ctx.saved_tensors[0]
+        saved = ctx.saved_tensors
+        logits = saved[0]
+        _decode.check_capture(logits.device.index)
         if torch._C._cuda_getDevice() != logits.device.index:  # (the engine's thread is on the gradients' device)
             with torch.cuda.device(logits.device):
                 return _backward(*saved, ctx.top, g_logprobs, g_lse, g_entropy, g_top), None, None, None
