@@ -10,7 +10,8 @@ sequence that goes on token by token keeps its keys and values in pages instead:
   e4m3 with one fp32 scale each (``x ~ xq * scale``, as ``attend`` takes it);
 - ``table``: int32 ``[sequences, width]``; the key at place ``t`` of a sequence lies
   in page ``table[sequence, t // page_size]``, row ``t % page_size``. Entries
-  behind a sequence's last page are not read.
+  behind a sequence's last page may be loaded (the whole table has to be
+  readable), but nothing follows from what they hold.
 
 ``append_paged`` stands beside ``dan_amd.front.qkv_front`` (norm and rotary of q
 and k, dan/models/llama.py:78-86, with the cache as the destination) and
@@ -201,8 +202,8 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
 
     q: [H, B, D] (rotary applied; what ``append_paged`` returns), bf16 or fp16,
     H a multiple of Hkv. ``lens`` (int32 [B]): how many keys each sequence has,
-    the new token's own among them; places behind them are not read (they may hold
-    anything). ``max_len``: the most that any entry of ``lens`` reaches while this
+    the new token's own among them; rows behind them, and page 0, may be loaded, but
+    whatever they hold changes no result. ``max_len``: the most that any entry of ``lens`` reaches while this
     call (or a graph that captured it) runs, by default all that the table can
     hold; the launch is sized for it, so a tight one saves time.
 

@@ -97,7 +97,9 @@ typedef struct {
 
 /* out[b, h] = softmax(scale q[b, h] . k) v over the sequence's first lens[b]
  * keys; zeros (lse -inf) where lens[b] is 0; NaN where lens[b] lies outside
- * [0, max_len] or one of its pages outside the cache. */
+ * [0, max_len] or one of its pages outside the cache. The whole table
+ * [B, table_width], rows behind a sequence's end in its last page, and page 0
+ * may be loaded; no result depends on what they hold. */
 int dan_paged_attn(const DanPagedAttnArgs *args, void *stream);
 
 /* Bytes of workspace of such a call on the current device (0: none is
