@@ -91,8 +91,9 @@ def append_paged(q, k, v, cos, sin, k_cache, v_cache, table, places, *, seqs=Non
     rotation, v as it is, and returns q after the same norm and rotation.
 
     q: [N, H, D]; k, v: [N, Hkv, D] (views of the projection output: any strides
-    with a unit-stride head_dim), bf16 or fp16; q may be None (a prefix moved
-    into the cache: pass its k with ``norm=None`` and no cos and sin).
+    with a unit-stride head_dim), bf16 or fp16; q may be None (keys that ``qkv_front`` has
+    made for ``attend``, or a prefix, moved into the cache as they are: pass them with
+    ``norm=None`` and no cos and sin).
     ``norm``, ``q_norm_weight``, ``k_norm_weight``, ``eps``: as in ``qkv_front``.
     cos, sin: [N, R] or None, in the model dtype or fp32 (R: rotary dims, a
     multiple of 16 up to D); with ``rope_rows`` (int32 [N]) token n takes row
