@@ -253,7 +253,8 @@ int dan_paged_append(const DanPagedAppendArgs *a, void *stream) {
   if (R > 0 && !a->rope_rows && a->num_rope_rows < N)
     return fail(DAN_ERR_INVALID_ARGUMENT, "%d rows of cos and sin for %d tokens", a->num_rope_rows, N);
   if (N == 0) return DAN_OK;
-  if ((H > 0 && (!a->q || !a->q_out)) || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->table || !a->places || (R > 0 && (!a->cos || !a->sin)))
+  if ((H > 0 && (!a->q || !a->q_out)) || !a->k || !a->v || !a->places || (R > 0 && (!a->cos || !a->sin)) ||
+      (a->num_pages > 0 && (!a->k_cache || !a->v_cache)) || (a->table_width > 0 && a->num_seqs > 0 && !a->table))
     return fail(DAN_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
   if (R > 0 && a->num_rope_rows == 0) return fail(DAN_ERR_INVALID_ARGUMENT, "cos and sin have no rows");
   if (fp8 && (!a->k_scale || !a->v_scale)) return fail(DAN_ERR_INVALID_ARGUMENT, "an e4m3 cache needs k_scale and v_scale");

@@ -53,3 +53,23 @@ def test_prompts_go_on_token_by_token(gpu, dtype):
     ref, _, mag, _ = OP.attend(qn.cpu(), kc.cpu().double().nan_to_num(), vc.cpu().double().nan_to_num(), table.cpu(), whole)
     assert ((out - ref).abs() <= HALF[dtype] * ref.abs() + 2.0 ** -14 * mag).all()
     assert (out - whole_read[:, last].cpu().double()).abs().max() <= 2e-2 + 2.0 ** -7
+
+
+@pytest.mark.parametrize("pages,seqs_of_table,width", [(0, 3, 2), (4, 3, 0), (0, 0, 0), (4, 0, 2)])
+def test_a_cache_or_table_without_pages_stores_nothing(gpu, pages, seqs_of_table, width, monkeypatch):
+    """No token has a page then: q comes back, nothing is written, through the host module and through Python."""
+    print(f"[gpu-case] append: {pages} pages, a table of {seqs_of_table} x {width}", flush=True)
+    from dan_amd import _decode
+
+    x = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(0)).bfloat16().to(gpu)
+    guard = torch.zeros(pages + 2, 2, PAGE, 64, dtype=torch.bfloat16, device=gpu)
+    cache = guard[1:pages + 1] if pages else torch.empty(0, 2, PAGE, 64, dtype=torch.bfloat16, device=gpu)
+    table = torch.zeros(seqs_of_table, width, dtype=torch.int32, device=gpu)
+    places, seqs = (torch.tensor(t, dtype=torch.int32, device=gpu) for t in ([0, 17, -1], [0, 1, 2]))
+    rest = type("Rest", (), dict(append=staticmethod(lambda *a: None)))
+    for real in (True, False):
+        if not real:
+            monkeypatch.setattr(_decode, "calls", lambda: rest)
+        q = append_paged(x, x, x, None, None, cache, cache.clone(), table, places, seqs=seqs, norm=None)
+        torch.cuda.synchronize()
+        assert torch.equal(q, x.transpose(0, 1)) and not guard.any()
