@@ -5,14 +5,18 @@ import math
 import torch
 
 
+def log_softmax(x):
+    """(log p, logsumexp [N]) of float64 rows. The maximum is subtracted first, so that log p keeps its bits whatever the rows' offset."""
+    m = x.amax(1, keepdim=True)
+    m = torch.where(m == -math.inf, 0.0, m)
+    z = torch.log(torch.exp(x - m).sum(1, keepdim=True))
+    return torch.where(z == -math.inf, -math.inf, (x - m) - z), (m + z)[:, 0]
+
+
 def token_logprobs(logits, tokens, top=0):
     """(logprobs [N, L], logsumexp, entropy, top_logprobs, top_ids); rows of -inf only: -inf, -inf, 0."""
     x = logits.double()
-    m = x.amax(1, keepdim=True)
-    m = torch.where(m == -math.inf, 0.0, m)
-    e = torch.exp(x - m)
-    lse = m[:, 0] + torch.log(e.sum(1))
-    logp = torch.where(lse[:, None] == -math.inf, -math.inf, x - lse[:, None])
+    logp, lse = log_softmax(x)
     p = logp.exp()
     entropy = -torch.where(p == 0, 0.0, p * logp).sum(1)
     given = torch.where(tokens < 0, 0.0, logp.gather(1, tokens.clamp(0, x.shape[1] - 1)))
@@ -25,8 +29,8 @@ def gradient(logits, tokens, top_ids=None, g=None, g_lse=None, g_entropy=None, g
     """The logits' gradient by the formula (finite logits or -inf)."""
     x = logits.double()
     n, vocab = x.shape
-    _, lse, entropy, _, _ = token_logprobs(x, tokens[:, :0])
-    logp = torch.where(lse[:, None] == -math.inf, -math.inf, x - lse[:, None])
+    _, _, entropy, _, _ = token_logprobs(x, tokens[:, :0])
+    logp, lse = log_softmax(x)
     p = logp.exp()
     grad = torch.zeros_like(x)
     pull = torch.zeros(n, 1, dtype=torch.float64)
