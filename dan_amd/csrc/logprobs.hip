@@ -14,10 +14,10 @@
 // largest values of a row lie in the K groups of largest maximum (of equal ones those
 // of lowest index), which alone are read again.
 //
-// Measured, us: 2039 rows x 128256 bf16 with 5 top tokens and entropy 104 to 109 (the chunk kernel 80 to 92: 523 MB at
-// 5.7 to 6.5 TB/s; the top kernel 15 to 18), without top tokens 87; 1 row 4.8 + 7.4 with 20 top tokens, of which
-// about 4 each are a launch and its first loads; 45 rows x 50257 fp32 with 10, 4.6 + 6. Forward with entropy and gradient of
-// 4096 x 128256 bf16 (3.15 GB) 517: 6.1 TB/s, where a large copy moves 4.9.
+// Measured, us: 2039 rows x 128256 bf16 with 5 top tokens and entropy 104 (the chunk kernel 86: 523 MB at 6.1 TB/s; the
+// top kernel 16), without top tokens 87; 1 row 5.0 + 7.8 with 20 top tokens, of which
+// about 4 each are a launch and its first loads; 45 rows x 50257 fp32 with 5, 5.4 + 6.7. Forward with entropy and gradient of
+// 4096 x 128256 bf16 (3.15 GB) 520: 6.0 TB/s, where a large copy moves 4.9.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

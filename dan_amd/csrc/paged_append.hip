@@ -16,8 +16,8 @@
 // each lane takes up to kVecs of them at a time, all loaded before any math. (Vectors dealt out over work
 // groups whatever their token, as the front end does, cost about 200 vector instructions each,
 // most of them addresses and a 64-bit division, and were bound by those.) 8192 tokens of 32 + 2 x 8
-// heads of 128 with norm: 38.2 us (205 MB, 5.4 TB/s; a large copy reaches 4.9), dealt out 47.2; on an
-// e4m3 cache 40.0 against 49.4; one token 2.7.
+// heads of 128 with norm: 41.7 us (205 MB, 4.9 TB/s, as a large copy); where every call's q goes into the same memory 38.2, dealt
+// out 47.2, on an e4m3 cache 40.0 against 49.4. One token: 3.1.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

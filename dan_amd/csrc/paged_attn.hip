@@ -25,10 +25,10 @@
 // leave 2^-17 of a weight: outputs next to a border of their own rounding then fall to the other side twice as
 // often as fp32's own errors let them.)
 //
-// Measured, us and TB/s of keys and values, 32/8 heads x 128 in bf16 if not said: 1 sequence of 277 keys
-// 6.4 (of which 4 are a launch and its chain of dependent loads: length, page, keys), 1 of 131072 87
-// (6.2), 64 of up to 8192 194 (5.6), 100 of up to 1000 (32/32 fp16) 133 (6.2), 37 of up to 4099 (16/2 x 256, e4m3) 24
-// (2.6: a CU draws about 60 GB/s from HBM however many waves ask, so what holds a short launch of unequal
+// Measured, whole calls, us and TB/s of keys and values, 32/8 heads x 128 in bf16 if not said: 1 sequence of 277 keys
+// 6.4 (of which 4 are a launch and its chain of dependent loads: length, page, keys), 1 of 131072 84.8
+// (6.3), 64 of up to 8192 186 (6.0), 100 of up to 1000 (32/32 fp16) 128 (6.5), 37 of up to 4099 (16/2 x 256, e4m3) 22.4
+// (2.9: a CU draws about 60 GB/s from HBM however many waves ask, so what holds a short launch of unequal
 // sequences is the CU with the most keys, and then the join). A large copy moves 4.9.
 // Two tiles in flight a wave (240 registers, 2 waves a SIMD) were 1 to 40 % slower; two parts
 // of P in one product for up to 8 heads 0 to 3 %, and a third part costs nothing but 0.1 us of the shortest calls: the
@@ -147,7 +147,8 @@ __device__ inline float sum_across_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// The limits of a split (us on either side, 32/8 heads x 128 in bf16 if not said):
+// The limits of a split (us on either side, 32/8 heads x 128 in bf16 if not said; here and at the rules below the sides of a pair
+// ran on the same lengths, different pairs on different ones):
 // - a range has at most kMaxChunk keys (a lane holds the address of one of a wave's 32 blocks of 16 keys):
 //   64 sequences of up to 8192 194 with 2048, 199 with 1024; 128 of up to 2000 93 / 100; 1 of 131072 88 / 92;
 // - one of kWideChunk keys or more takes 8 waves, 4 / 8: 64 of up to 8192 205 / 194, 128 of up to 2000
