@@ -66,7 +66,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32, kHeads = 16;
 constexpr int kMaxLen = 1 << 30;  // places are 32-bit
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 struct Ops;
@@ -183,6 +182,9 @@ __device__ inline int length_of(const Params &p, int b) {
 // before that, so that its weight is 1 whatever its size: the rounding of a maximum that is multiplied first would be part of every
 // exponent, and at scores of 1e9 that is more than fp32 or fp16 hold.
 __device__ inline float score_of(const Params &p) { return p.scale * (p.ks ? *p.ks : 1.0f); }
+// The same for exponents of 2. A cache of scale 0 has scores of 0 and equal weights: a smallest value in place of 0, as what is
+// masked has -inf to be multiplied.
+__device__ inline float exponent_of(float to_score) { return to_score == 0.0f ? 0x1p-126f : to_score * 1.4426950408889634f; }
 
 // Keys of a range of a sequence of `len`: a `target`-th of it, within limits, in whole rounds of the work
 // group's tiles. By its own length alone, so that a sequence's result does not change with its
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(const Params p) {
   u32x4 *ql = (u32x4 *)lds + lane;
 #pragma unroll
   for (int s = 0; s < (kQLds ? S / W : S); ++s) qf[s] = q_step(kQLds ? W * s + wave : s);
-  const float to_score = score_of(p), c = to_score * kLog2e;
+  const float to_score = score_of(p), c = exponent_of(to_score);
   float vscale = 1.0f / Wt::unit;
   if constexpr (FP8) vscale *= *p.vs;
   const int len = length_of(p, b), chunk = chunk_of(len, p.target, p.splits, W), lo = split * chunk;
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
   const float *rows = p.part + row * p.splits * D + d;
   const int len = length_of(p, b);
   const int chunk = chunk_of(len, p.target, p.splits, p.waves), n = len <= 0 ? 0 : (len + chunk - 1) / chunk;
-  const float to_score = score_of(p), c = to_score * kLog2e;
+  const float to_score = score_of(p), c = exponent_of(to_score);
   f32x4 o = {0, 0, 0, 0};
   float top = -INFINITY, sum = 0.f;  // top: in products
 #pragma unroll 4

@@ -125,3 +125,19 @@ def test_finite_scores_of_any_size(gpu, d, n, dtype, cache):
     lerr = ((lse - rl).abs() / (rl.abs() * 2.0 ** -22 + 2.0 ** -21)).max().item()
     say(f"scores to {s.abs().max().item():.3g} {dtype} cache={cache} x {d}, {n} keys: {worst.max().item():.3f} of the tolerance, lse {lerr:.3f}")
     assert worst.max() <= 1.0 and lerr <= 1.0
+
+
+@pytest.mark.parametrize("n", [5, 64, 700, 9000])
+@pytest.mark.parametrize("d", [64, 256])
+def test_a_cache_of_scale_zero(gpu, d, n):
+    """k_scale 0 makes every score 0: the mean of the values, whole numbers of up to 8 whose sums are exact; u |o| for the output, 2^-23 for the quotient.
+    v_scale 0 makes every output 0."""
+    g = gen(n)
+    q = torch.randn(2, 4, d, generator=g).to(BF16)
+    k, v = torch.randint(-8, 9, (2, n, 2, d), generator=g).float(), torch.randint(-8, 9, (2, n, 2, d), generator=g).float()
+    out, lse = call(q, k, v, gpu, E4M3, ks=0.0)
+    ref = v.double().mean(1).repeat_interleave(2, 1)
+    say(f"k_scale 0, {n} keys x {d}: {(out - ref).abs().max().item():.3g}")
+    assert ((out - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -20).all() and (lse - math.log(n)).abs().max() <= 2.0 ** -20
+    out, lse = call(q, k, v, gpu, E4M3, ks=0.25, vs=0.0)
+    assert (out == 0).all() and lse.isfinite().all()
