@@ -206,8 +206,8 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
     the new token's own among them; rows behind them, and page 0, may be loaded, but
     whatever they hold changes no result. ``max_len``: the most that any entry of ``lens`` reaches while this
     call (or a graph that captured it) runs, by default all that the table can
-    hold. The launch and its workspace are sized for it: up to about twice the longest length costs nothing,
-    far more does (64 sequences of up to 1000 keys: 33 us, 155 for a table of 131072).
+    hold. The launch and its workspace are sized for it: up to about twice the longest length costs a short
+    sequence a second launch and others nothing, far more does (64 sequences of up to 1000 keys: 33 us, 155 for a table of 131072).
 
     Returns [H, B, D], a view of token-major [B, H, D] storage, in q's dtype;
     with ``return_lse`` also the fp32 [H, B] log of the sum of e^score (a merge with other
