@@ -126,6 +126,8 @@ def token_logprobs(logits, tokens, *, top=0, entropy=False):
     n, vocab = logits.shape
     if tokens.dim() not in (1, 2) or tokens.shape[0] != n or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != dev:
         raise ValueError(f"tokens must be int64 or int32 [{n}] or [{n}, L] on {dev}; got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
+    if top != int(top):
+        raise ValueError(f"top {top}: a whole number")
     if not 0 <= top <= min(vocab, _decode.MAX_TOP) or (top and vocab > _decode.MAX_TOP_VOCAB):
         raise ValueError(f"top {top}: at most {_decode.MAX_TOP} and the vocabulary's {vocab}, for at most {_decode.MAX_TOP_VOCAB} values")
     if has_tangent(logits):

@@ -6,6 +6,7 @@ test_gpu_readout.py: 128 roundings of 2^-24 of it), which the logarithm makes ab
 entropy's sum has terms of weight |log p|: 2^-17 (1 + H + log V)."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -103,6 +104,18 @@ def test_finite_logits_fp16(gpu, offset):
     x[:4, 100:] = offset
     x[4:] += offset / 2
     check(x.to(F16), torch.randint(0, 9000, (9, 4), generator=gen(4)), 5, gpu)
+
+
+def test_top_is_a_whole_number(gpu):
+    """A fraction is refused, not cut; whole numbers of any type are taken."""
+    say("logprobs: top of other types")
+    x, t = torch.randn(2, 50, device=gpu), torch.tensor([3, 4], device=gpu)
+    want = token_logprobs(x, t, top=3)
+    for top in (np.int64(3), torch.tensor(3), 3.0):
+        assert torch.equal(token_logprobs(x, t, top=top).top_ids, want.top_ids)
+    for top in (2.5, "3", None):
+        with pytest.raises((TypeError, ValueError)):
+            token_logprobs(x, t, top=top)
 
 
 # ------------------------------------------------------------------ gradients
