@@ -713,7 +713,8 @@ int dan_paged_attn(const DanPagedAttnArgs *a, void *stream) {
   if (a->num_pages < 0 || a->table_width < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "num_pages and table_width must be >= 0");
   if (a->max_len < 0 || a->max_len > kMaxLen || a->max_len > (int64_t)a->table_width * a->page_size)
     return fail(DAN_ERR_INVALID_ARGUMENT, "max_len %d: the table holds %lld keys a sequence", a->max_len, (long long)a->table_width * a->page_size);
-  if (!dan::finite_positive(a->scale)) return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+  if (!dan::finite_positive(a->scale) || a->scale > 0x1p127f)  // (times log2 e it has to be finite, too)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be finite, > 0 and at most 2^127");
   if (B == 0) return DAN_OK;
   if (!a->q || !a->out || !a->lens) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
   if (a->max_len > 0 && (!a->k_cache || !a->v_cache || !a->table || a->num_pages == 0))

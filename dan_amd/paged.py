@@ -212,7 +212,7 @@ def attend_paged(q, k_cache, v_cache, table, lens, scale=None, *, k_scale=None, 
     Returns [H, B, D], a view of token-major [B, H, D] storage, in q's dtype;
     with ``return_lse`` also the fp32 [H, B] log of the sum of e^score (a merge with other
     keys' attention takes it, dan/fused.py:94-101). A sequence of no keys gives
-    zeros and -inf. A length outside [0, max_len], or a page outside the
+    zeros and -inf. ``scale``: positive, at most 2^127. A length outside [0, max_len], or a page outside the
     cache, gives NaN for its sequence. An infinite value among a sequence's own may give NaN where
     the sum would be infinite (weights are held in parts).
 

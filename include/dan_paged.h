@@ -82,7 +82,7 @@ typedef struct {
   int32_t num_heads, num_kv_heads, head_dim;
   int32_t page_size, num_pages, table_width;
   int32_t max_len;      /* the longest sequence that the launch covers, <= table_width * page_size */
-  float scale;          /* of the scores, finite and > 0 */
+  float scale;          /* of the scores, > 0 and at most 2^127 */
 
   const void *q; int64_t q_stride_seq, q_stride_head; /* [B, H, D] */
   void *out; int64_t o_stride_seq, o_stride_head;     /* [B, H, D] */
