@@ -1,12 +1,16 @@
 """The operators of adapter training and serving as measurable cases: their plain forms in
 elementary torch operations, and the calls that a user makes of the framework's own.
 
-Two operators, the trained part of a model that is otherwise left as it is:
+Three operators, what a decoder layer runs where its own weights stay as they are and
+adapters are trained beside them, or served:
 
 - ``attend``: tree attention of packed reads with its gradient, the output and the gradients of
   q, k and v (``dan_amd.attention.attend_train``);
 - ``adapt``: the low-rank adapters of many requests added to a shared projection's output
-  (``dan_amd.adapters.adapt``), and with ``grad`` the gradients of the input and of the adapters too.
+  (``dan_amd.adapters.adapt``), and with ``grad`` the gradients of the input and of the adapters too;
+- ``norm``: the residual's addition and the root-mean-square norm in front of a projection, its
+  result in 16 bits or in 8 bits with a scale for each row (``dan_amd.norm.add_norm``), and with
+  ``grad`` the gradients of the addends and of the weight too.
 
 ``own`` selects: false, the plain forms (fp32 whatever the inputs' type, rounded once at
 the end); true, the framework's calls. Values come from the seed given to ``prepare``, the
@@ -23,6 +27,7 @@ own = False
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 LAYOUTS = ((32, 8, 128), (32, 8, 128), (16, 2, 256), (8, 2, 64), (32, 32, 128))  # q heads, kv heads, head_dim
 LLAMA3_8B_LINEARS = ((6144, 4096), (4096, 4096), (28672, 4096), (4096, 14336))  # qkv, o, gate_up, down: (out, in)
+E4M3_MAX = 448.0
 BUDGET = 8192  # packed tokens of a full serving batch
 
 
@@ -43,29 +48,27 @@ def listed():
         dict(name="attend_requests_fp16", kind="attend", dtype="fp16", **_heads(32, 8, 128), **_tree(2, 3413, 4, (3, 6), (16, 64))),
         # Hybrid models' gated layers (head_dim 256) behind a shared, cached prompt, which has no gradient.
         dict(name="attend_prefix_d256", kind="attend", dtype="bf16", **_heads(16, 2, 256), **_tree(3, 4099, 5, (3, 12), (16, 96), 1024)),
-        # A training step of a full budget of requests.
-        dict(name="attend_budget", kind="attend", dtype="bf16", **_heads(32, 8, 128), **_tree(4, BUDGET, 6, (3, 12), (16, 96))),
-        # One long document with 32 questions.
+        # A training step of one long document with 32 questions, a full budget.
         dict(name="attend_document", kind="attend", dtype="bf16", **_heads(32, 8, 128), **_tree(5, BUDGET, 1, (32, 32), (16, 16))),
         # One user's next token: a single row beside the fused qkv projection, where latency counts.
         dict(name="adapt_token", kind="adapt", dtype="bf16", rows=1, n_in=4096, n_out=6144, rank=16, adapters=1, mixed=True, grad=False),
         # The next tokens of a batch whose requests have adapters of their own, or none.
         dict(name="adapt_batch", kind="adapt", dtype="bf16", rows=64, n_in=4096, n_out=4096, rank=16, adapters=24, mixed=True, grad=False),
-        # A larger batch of higher rank, half precision, at the widest input.
-        dict(name="adapt_batch_fp16", kind="adapt", dtype="fp16", rows=237, n_in=14336, n_out=4096, rank=64, adapters=32, mixed=True,
-             grad=False),
         # The packed prompts of a full budget, each request with its adapter.
         dict(name="adapt_prompts", kind="adapt", dtype="bf16", rows=BUDGET, n_in=4096, n_out=6144, rank=16, adapters=7, mixed=False,
              grad=False),
-        # A training step of one small request, half precision.
-        dict(name="adapt_train_request", kind="adapt", dtype="fp16", rows=384, n_in=2048, n_out=2048, rank=8, adapters=1, mixed=False,
-             grad=True),
-        # Several adapters trained at once on packed requests.
-        dict(name="adapt_train_many", kind="adapt", dtype="bf16", rows=4099, n_in=4096, n_out=4096, rank=64, adapters=5, mixed=False,
+        # Several adapters of high rank trained at once on packed requests, half precision.
+        dict(name="adapt_train_fp16", kind="adapt", dtype="fp16", rows=1037, n_in=4096, n_out=4096, rank=64, adapters=5, mixed=False,
              grad=True),
         # A training step of a full budget beside the widest projection.
         dict(name="adapt_train_budget", kind="adapt", dtype="bf16", rows=BUDGET, n_in=4096, n_out=28672, rank=16, adapters=1, mixed=False,
              grad=True),
+        # The next tokens of a few users, in 8 bits for the quantised projection behind.
+        dict(name="norm_batch_e4m3", kind="norm", dtype="bf16", rows=7, cols=4096, norm="rms", codes=True, grad=False),
+        # A full budget of prompts, in 8 bits.
+        dict(name="norm_prompts_e4m3", kind="norm", dtype="bf16", rows=BUDGET, cols=4096, norm="rms", codes=True, grad=False),
+        # A training step's norm of a hybrid model (zero-centered weights), half precision.
+        dict(name="norm_train_fp16", kind="norm", dtype="fp16", rows=4099, cols=2048, norm="zero_centered", codes=False, grad=True),
     ]
 
 
@@ -76,7 +79,12 @@ def _log(rng, lo, hi):
 
 def draw(rng):
     dtype = rng.choice(("bf16", "bf16", "fp16"))
-    if rng.random() < 0.5:
+    kind = rng.choice(("attend", "attend", "adapt", "adapt", "norm"))
+    if kind == "norm":
+        codes = rng.random() < 0.5
+        return dict(kind=kind, dtype=dtype, rows=_log(rng, 1, BUDGET), cols=rng.choice((1024, 2048, 4096, 14336, 16 * rng.randint(4, 384))),
+                    norm=rng.choice(("rms", "zero_centered")), codes=codes, grad=not codes and rng.random() < 0.6)
+    if kind == "attend":
         h, hkv, d = rng.choice(LAYOUTS)
         tokens = _log(rng, 16, BUDGET)
         requests = rng.randint(1, 8) if tokens >= 512 else rng.randint(1, 2)
@@ -166,8 +174,21 @@ def _prepare_adapt(case, seed):
     return s
 
 
+def _prepare_norm(case, seed):
+    g = _gen(seed)
+    n, cols = case["rows"], case["cols"]
+    dt = DTYPES[case["dtype"]]
+    s = dict(x=_randn(g, n, cols, dtype=dt), stream=_randn(g, n, cols, std=3.0, dtype=dt), norm=case["norm"], codes=case["codes"],
+             w=(_randn(g, cols, std=0.2) + (case["norm"] == "rms")).to(dt))
+    if case["grad"]:
+        for f in ("x", "stream", "w"):
+            s[f].requires_grad_()
+        s["g"], s["gs"] = _randn(g, n, cols, dtype=dt), _randn(g, n, cols, dtype=dt)
+    return s
+
+
 def prepare(case, seed):
-    make = {"attend": _prepare_attend, "adapt": _prepare_adapt}[case["kind"]]
+    make = {"attend": _prepare_attend, "adapt": _prepare_adapt, "norm": _prepare_norm}[case["kind"]]
     return SimpleNamespace(kind=case["kind"], grad=case.get("grad", True), **make(case, seed))
 
 
@@ -230,12 +251,41 @@ def _plain_adapt(s):
             db.view(count, r, n_out).transpose(1, 2).to(s.b.dtype))
 
 
+def _plain_norm(s, eps=1e-6):
+    dt = s.x.dtype
+    t = s.x.detach().float() + s.stream.detach().float()
+    w = s.w.detach().float() + (s.norm == "zero_centered")
+    r = torch.rsqrt(t.square().mean(1, keepdim=True) + eps)
+    hat = t * r
+    y = hat * w
+    if s.codes:
+        scale = y.abs().amax(1, keepdim=True).clamp(min=1e-12) / E4M3_MAX
+        return t.to(dt), (y / scale).to(torch.float8_e4m3fn), scale
+    if not s.grad:
+        return t.to(dt), y.to(dt)
+    g = s.g.float()
+    dw = (g * hat).sum(0)
+    g = g * w
+    dt_ = r * (g - hat * (g * hat).mean(1, keepdim=True)) + s.gs.float()  # of both addends
+    return t.to(dt), y.to(dt), dt_.to(dt), dw.to(dt)
+
+
 # ------------------------------------------------------------------ one pass
 
 
 def run(s):
     if not own:
-        return _plain_attend(s) if s.kind == "attend" else _plain_adapt(s)
+        return {"attend": _plain_attend, "adapt": _plain_adapt, "norm": _plain_norm}[s.kind](s)
+    if s.kind == "norm":
+        from dan_amd.norm import add_norm
+
+        r = add_norm(s.x, s.stream, s.w, norm=s.norm, fp8="rows" if s.codes else None)
+        if s.codes:
+            return r.stream, r.codes, r.scale
+        if not s.grad:
+            return r.stream, r.out
+        dx, dw = torch.autograd.grad((r.out, r.stream), (s.x, s.w), (s.g, s.gs))
+        return r.stream.detach(), r.out.detach(), dx, dw
     if s.kind == "attend":
         from dan_amd.attention import attend_train
 
@@ -264,6 +314,11 @@ def work(case):
         pairs, past = _pairs(case)
         # Forward: scores and output. Backward: scores again, the probabilities' gradient, dq, dk and dv (no dk, dv of a prefix).
         return {"bytes": 2 * d * (n * (4 * h + 4 * hkv) + 2 * hkv * case["past"]), "flops": 2 * d * h * (7 * pairs + 5 * past)}
+    if case["kind"] == "norm":
+        n, cols = case["rows"], case["cols"]
+        if case["grad"]:  # the addends, the two gradients; the sum, the norm, the addends' gradient
+            return {"bytes": 2 * cols * (7 * n + 2), "flops": 15 * n * cols}
+        return {"bytes": 2 * cols * (3 * n + 1) + n * (cols + 4 if case["codes"] else 2 * cols), "flops": n * cols * (7 if case["codes"] else 5)}
     n, n_in, n_out, r = (case[f] for f in ("rows", "n_in", "n_out", "rank"))
     used = min(n, case["adapters"])
     rows = n - (len(range(4, n, 9)) if case["mixed"] else 0)
@@ -321,6 +376,23 @@ def _exact_adapt(s):
     return (out, dx, da, db) if s.grad else out
 
 
+def _exact_norm(s):
+    t = s.x.detach().double() + s.stream.detach().double()
+    w = s.w.detach().double()
+    if s.norm == "zero_centered":
+        w = 1.0 + w
+    rms = torch.sqrt((t * t).sum(1) / t.shape[1] + 1e-6)[:, None]
+    y = t / rms * w
+    if s.codes:
+        scale = torch.clip(y.abs().max(1, keepdim=True).values, min=1e-12) / E4M3_MAX
+        return t, y / scale, scale
+    if not s.grad:
+        return t, y
+    g = s.g.double()
+    dt = g * w / rms - t * ((g * w * t).sum(1, keepdim=True) / (t.shape[1] * rms ** 3)) + s.gs.double()
+    return t, y, dt, (g * t / rms).sum(0)
+
+
 def exact(case, seed):
     s = prepare(case, seed)
-    return _exact_attend(s) if s.kind == "attend" else _exact_adapt(s)
+    return {"attend": _exact_attend, "adapt": _exact_adapt, "norm": _exact_norm}[s.kind](s)
