@@ -9,9 +9,9 @@ token by token behind its read: ``append_paged`` (norm, rotary and a paged
 key-value cache), ``attend_paged`` (one new token over that cache) and
 ``token_logprobs`` (log probabilities of given tokens, with their gradient).
 """
-from .attention import Batch, Segment, attend, branch_rows_mask, repeat_heads, segment, to_device, tree_mask
+from .attention import Batch, Segment, attend, attend_train, branch_rows_mask, repeat_heads, segment, to_device, tree_mask
 from .paged import append_paged, attend_paged
 from .readout import TokenLogprobs, token_logprobs
 
-__all__ = ["Batch", "Segment", "TokenLogprobs", "append_paged", "attend", "attend_paged", "branch_rows_mask", "repeat_heads", "segment",
+__all__ = ["Batch", "Segment", "TokenLogprobs", "append_paged", "attend", "attend_paged", "attend_train", "branch_rows_mask", "repeat_heads", "segment",
            "to_device", "token_logprobs", "tree_mask"]

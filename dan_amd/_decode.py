@@ -107,6 +107,6 @@ def calls():
 _host = calls
 
 
-def check_capture(device_index):
-    """Inside a backward: refuses to run in a capture that torch's engine would make the stream of an eager graph wait for."""
-    _host().check_capture(device_index)
+def check_capture(device_index, name="token_logprobs"):
+    """Inside a backward of ``name``: refuses to run in a capture that torch's engine would make the stream of an eager graph wait for."""
+    _host().check_capture(device_index, name)

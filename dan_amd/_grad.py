@@ -1,0 +1,199 @@
+"""The gradient of tree attention (include/dan_tree_grad.h): its argument
+structure, its tables, and the autograd function behind
+``dan_amd.attention.attend_train``."""
+import ctypes
+import functools
+
+import numpy as np
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _decode, _native
+
+_i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+
+GRAD_ABI_VERSION = 1
+TILE = 32  # rows or keys of one step
+
+
+class DanTreeGradArgs(ctypes.Structure):
+    _fields_ = [("abi_version", _i32), ("dtype", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+                ("num_tokens", _i32), ("scale", _f32), ("key_rows", _i32),
+                ("q", _vp), ("q_stride_tok", _i64), ("q_stride_head", _i64),
+                ("k", _vp), ("k_stride_tok", _i64), ("k_stride_head", _i64),
+                ("v", _vp), ("v_stride_tok", _i64), ("v_stride_head", _i64),
+                ("out", _vp), ("o_stride_tok", _i64), ("o_stride_head", _i64),
+                ("grad", _vp), ("g_stride_tok", _i64), ("g_stride_head", _i64),
+                ("lse", _vp),
+                ("dq", _vp), ("dq_stride_tok", _i64), ("dq_stride_head", _i64),
+                ("dk", _vp), ("dk_stride_tok", _i64), ("dk_stride_head", _i64),
+                ("dv", _vp), ("dv_stride_tok", _i64), ("dv_stride_head", _i64),
+                ("key_units", _vp), ("num_key_units", _i32), ("query_units", _vp), ("num_query_units", _i32),
+                ("row_lo", _vp), ("row_end", _vp), ("pasts", _vp), ("num_pasts", _i32),
+                ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
+EXPORTS = ("dan_tree_attn_fwd_lse", "dan_tree_attn_bwd", "dan_tree_grad_key_rows", "dan_tree_grad_query_rows",
+           "dan_tree_grad_workspace_size", "dan_tree_grad_abi_version")
+
+call_backward = _native.Entry("dan_tree_attn_bwd", DanTreeGradArgs)
+
+
+class _ForwardLse(_native.Entry):
+    """``dan_tree_attn_fwd_lse``: the forward entry with one more argument."""
+
+    def __call__(self, lse, stream, *fields):
+        if self.fn is None:
+            fn = _native.load()[self.name]
+            fn.argtypes, fn.restype = [ctypes.c_char_p, _vp, _vp], ctypes.c_int
+            self.fn = fn
+        rc = self.fn(self.pack(*fields), lse, stream)
+        if rc != _native.OK:
+            raise RuntimeError(f"{self.name} failed (status {rc}): {_native.last_error(_native.load())}")
+
+
+call_forward_lse = _ForwardLse("dan_tree_attn_fwd_lse", _native.DanTreeAttnArgs)
+
+
+@functools.lru_cache(maxsize=None)
+def _rows(h, hkv, d, small):
+    """(keys of a key unit, rows of a query unit) of a head layout."""
+    lib = _native.load()
+    return lib["dan_tree_grad_key_rows"](d, int(small)), lib["dan_tree_grad_query_rows"](h, hkv, d)
+
+
+@functools.lru_cache(maxsize=256)
+def workspace_size(h, n):
+    fn = _native.load()["dan_tree_grad_workspace_size"]
+    fn.argtypes, fn.restype = [_i32, _i32], _i64
+    return fn(h, n)
+
+
+def build_units(segs, spans, num_tokens, key_rows, query_rows):
+    """The backward pass's tables: (key units int32 [K, 8], query units int32
+    [Q, 8], row_lo int32 [N], row_end int32 [N]) as DanTreeGradArgs takes them.
+    ``segs``: rows whose first fields are (start, n, trunk, past_len, past
+    index); ``spans``: each segment's branches (a, b) in packed rows. Units are
+    sorted by the steps they take, longest first: the hardware starts work
+    groups in order."""
+    row_lo, row_end = np.zeros(num_tokens, np.int32), np.zeros(num_tokens, np.int32)
+    taken = np.zeros(num_tokens, bool)
+    keys, queries = [], []
+    for seg, branches in zip(segs, spans):
+        start, n, trunk, past, pidx = (int(x) for x in seg[:5])
+        if taken[start:start + n].any():
+            raise ValueError(f"segment at row {start}: its rows belong to another segment, too")
+        taken[start:start + n] = True
+        row_end[start:start + trunk] = n
+        for a, b in branches:
+            row_lo[a:b], row_end[a:b] = a - start, b - start
+        at = np.arange(0, n, key_rows)
+        end = np.minimum(at + key_rows, n)
+        q_end = np.array([row_end[start + a:start + b].max() for a, b in zip(at, end)])
+        u = np.zeros((len(at), 9), np.int64)
+        u[:, 0], u[:, 1], u[:, 2], u[:, 3], u[:, 4], u[:, 5] = start, n, trunk, at, end - at, q_end
+        u[:, 8] = -(-(q_end - at) // TILE)
+        keys.append(u)
+        at = np.arange(0, n, query_rows)
+        end = np.minimum(at + query_rows, n)
+        mixed = end > trunk  # holds branch rows
+        b0 = np.where(mixed, row_lo[start + np.minimum(np.maximum(at, trunk), n - 1)], 0)
+        u = np.zeros((len(at), 9), np.int64)
+        u[:, 0], u[:, 1], u[:, 2], u[:, 3], u[:, 4], u[:, 5], u[:, 6], u[:, 7] = start, n, trunk, at, end - at, past, pidx, b0
+        u[:, 8] = -(-past // TILE) + -(-np.minimum(trunk, end) // TILE) + np.where(mixed, -(-(end - b0) // TILE), 0)
+        queries.append(u)
+    out = []
+    for units in (keys, queries):
+        u = np.concatenate(units) if units else np.zeros((0, 9), np.int64)
+        out.append(u[np.argsort(-u[:, 8], kind="stable"), :8].astype(np.int32))
+    return (*out, row_lo, row_end, bool(taken.all()))
+
+
+class Tables:
+    """Device copy of ``build_units``' arrays for one head layout."""
+
+    def __init__(self, segments, plan, h, hkv, d, num_cus):
+        from .plan import _upload
+
+        self.device, n = plan.device, plan.num_tokens
+        spans = [s.branches for s in segments]
+        whole, rows = _rows(h, hkv, d, False)
+        count = int((-(-plan.segs[:, 1] // whole)).sum()) * hkv
+        self.key_rows = _rows(h, hkv, d, count < num_cus)[0]
+        keys, queries, row_lo, row_end, self.covered = build_units(plan.segs, spans, n, self.key_rows, rows)
+        self.num_keys, self.num_queries = len(keys), len(queries)
+        self.blob = _upload(np.concatenate([keys.ravel(), queries.ravel(), row_lo, row_end]), self.device)
+        at = self.blob.data_ptr()
+        self.keys, self.queries = at, at + keys.nbytes
+        self.row_lo = self.queries + queries.nbytes
+        self.row_end = self.row_lo + row_lo.nbytes
+        self.stream = _native.stream(self.device)
+        self.ready = torch.cuda.Event()
+        self.ready.record(torch.cuda.current_stream(self.device))
+
+    def use(self):
+        """Orders the current stream behind the upload (a capture begins with the device idle)."""
+        if _native.stream(self.device) != self.stream and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(self.device)
+            stream.wait_event(self.ready)
+            self.blob.record_stream(stream)
+
+
+def tables(segments, plan, h, hkv, d, num_cus):
+    """The batch's tables, kept on its plan with the forward pass's."""
+    if (h, hkv, d) not in plan.grad_tables:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attend_train: run the batch once before a capture (its tables are uploaded then)")
+        plan.grad_tables[h, hkv, d] = Tables(segments, plan, h, hkv, d, num_cus)
+    t = plan.grad_tables[h, hkv, d]
+    t.use()
+    return t
+
+
+class TreeAttention(torch.autograd.Function):
+    """Tree attention with its gradient: q [H, N, D], k and v [Hkv, N, D] -> [H, N, D]."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, segments, layer, scale):
+        from . import attention as A
+
+        args, pasts_host, plan = A._call_args(q, k, v, segments, layer, scale, None, _native.PHASES_ALL, False, upload=False)
+        (h, n, d), hkv = q.shape, k.shape[0]
+        t = tables(segments, plan, h, hkv, d, A._num_cus(q.device))
+        lse = torch.empty((h, n), dtype=torch.float32, device=q.device)
+        out = A._launch_tree_attn(*args, None, pasts_host, launch=functools.partial(call_forward_lse, lse.data_ptr()), zero=not t.covered)
+        # The prefix's own tensors are saved, too: what the backward pass reads has to be what the forward pass read.
+        pasts = [x for entry in plan.past_dicts for x in entry[layer][:2]]
+        ctx.save_for_backward(q, k, v, out, lse, *pasts)
+        ctx.tables, ctx.past = t, plan.past_tables[layer]
+        ctx.num_pasts, ctx.scale = len(plan.past_dicts), args[6]
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse = ctx.saved_tensors[:5]
+        _decode.check_capture(q.device.index, "attend_train")
+        if torch._C._cuda_getDevice() != q.device.index:  # (the engine's thread is on the gradient's device)
+            with torch.cuda.device(q.device):
+                return *_backward(ctx, q, k, v, out, lse, grad), None, None, None
+        return *_backward(ctx, q, k, v, out, lse, grad), None, None, None
+
+
+def _backward(ctx, q, k, v, out, lse, grad):
+    from . import attention as A
+
+    (h, n, d), hkv, t = q.shape, k.shape[0], ctx.tables
+    new = torch.empty if t.covered else torch.zeros  # rows of no segment have no gradient
+    dq, dk, dv = (new((n, x.shape[0], d), dtype=q.dtype, device=q.device).transpose(0, 1) for x in (q, k, v))
+    if n:
+        t.use()
+        q, k, v, grad = (A._kernel_view(x) for x in (q, k, v, grad))
+        nbytes = workspace_size(h, n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rows = [f for x in (q, k, v, out, grad) for f in (x.data_ptr(), x.stride(1), x.stride(0))]
+        grads = [f for x in (dq, dk, dv) for f in (x.data_ptr(), x.stride(1), x.stride(0))]
+        call_backward(_native.stream(q.device), GRAD_ABI_VERSION, A._DTYPES[q.dtype], h, hkv, d, n, _native.f32(ctx.scale), t.key_rows,
+                      *rows, lse.data_ptr(), *grads, t.keys, t.num_keys, t.queries, t.num_queries, t.row_lo, t.row_end,
+                      ctx.past[0].data_ptr(), ctx.num_pasts, ws.data_ptr(), nbytes)
+    return tuple(x if need else None for x, need in zip((dq, dk, dv), ctx.needs_input_grad))

@@ -165,6 +165,45 @@ def attend(q, k, v, segments, layer, scale=None, *, q_scale=None, k_scale=None, 
     return _attend_fused(q, k, v, segments, layer, scale, (q_scale, k_scale, v_scale) if fp8 else None)
 
 
+def attend_train(q, k, v, segments, layer, scale=None):
+    """``attend`` with its gradient, for training through reads
+    (dan/tuning.py:82-133): q [H, N, D], k and v [Hkv, N, D], bf16 or fp16,
+    -> [H, N, D], differentiable (once) in q, k and v.
+
+    The forward pass is ``attend``'s kernel, which also writes each row's
+    logsumexp; the backward pass computes the probabilities again from it
+    (dan_amd/csrc/tree_attn_grad.hip). A kv head's gradients are summed over
+    the heads that share it. Sums are fp32 in an order that the batch alone
+    fixes; P and dS are rounded to the inputs' type for the matrix core, dS
+    after a power-of-2 scaling where that is fp16.
+
+    Prefix-cache entries are constants (one that requires grad raises); a
+    segment with ``save`` > 0 keeps detached copies, as ``attend`` does. Rows of
+    no segment give zeros and have no gradient. Segments must not overlap.
+    k and v of finite values: a hidden key's weight is zero, its products are not
+    left out. The first call on a ``Batch`` uploads its tables, so it cannot be
+    captured into a HIP graph; later ones can, forward and backward in the same
+    capture and with no earlier, eager result alive that holds the graph of the
+    same leaves (where q, k or v is such a leaf itself, that raises)."""
+    from . import _grad
+
+    if torch.is_grad_enabled() and any(x.requires_grad for s in segments if s.past for x in s.past[layer] if isinstance(x, torch.Tensor)):
+        raise NotImplementedError("attend_train: prefix-cache entries are constants; got one that requires grad")
+    if has_tangent(q, k, v):
+        raise NotImplementedError("attend_train has no forward-mode derivative")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"attend_train takes bf16 or fp16; got {q.dtype}")
+    if q.is_cuda and q.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(q.device):
+            return attend_train(q, k, v, segments, layer, scale)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return attend(q, k, v, segments, layer, scale)
+    for s in segments:
+        if s.save:
+            s.saved[layer] = tuple(x[:, s.start:s.start + s.save].detach().clone() for x in (k, v))
+    return _grad.TreeAttention.apply(q, k, v, segments, layer, scale)
+
+
 def has_tangent(*tensors):
     """Whether one of the tensors carries a forward-mode tangent, which torch's
     operators pass on and a kernel that writes in their place would drop
@@ -552,15 +591,17 @@ def tree_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tables: List[to
     return _launch_tree_attn(q, k, v, tables, scales, meta, scale, workspace)
 
 
-def _launch_tree_attn(q, k, v, tables, scales, meta, scale, workspace, pasts_host=None, saves=None):
+def _launch_tree_attn(q, k, v, tables, scales, meta, scale, workspace, pasts_host=None, saves=None, launch=None, zero=False):
     """The body of ``tree_attn``; ``pasts_host`` (uint8, on the host): the
     prefix-cache table's entries, which the launch writes to the table;
-    ``saves``: ``DanTreeAttnSave`` entries it fills, and their layout bits."""
+    ``saves``: ``DanTreeAttnSave`` entries it fills, and their layout bits;
+    ``launch``: another entry of the same arguments (the training forward's);
+    ``zero``: rows of no segment are zeros."""
     lib = _native.load()
     h, n, d = q.shape
     hkv = k.shape[0]
     num_segments, num_pasts, num_work, tile_q, vt_cols, slots, phases, noalloc = meta
-    out = torch.empty((n, h, d), dtype=_out_dtype(q, v), device=q.device)
+    out = (torch.zeros if zero else torch.empty)((n, h, d), dtype=_out_dtype(q, v), device=q.device)
     if num_work:
         segs_d, work_d, key_lo_d, col_seg_d, past_table, units, sched_off = tables[:7]
         counts = tables[7] if len(tables) > 7 else None  # budget mode: the batch's device counts
@@ -572,7 +613,7 @@ def _launch_tree_attn(q, k, v, tables, scales, meta, scale, workspace, pasts_hos
                 raise ValueError(f"workspace: a contiguous uint8 tensor of >= {nbytes} bytes on {q.device}")
         scale_ptrs = [t.data_ptr() for t in scales] + [0] * (3 - len(scales))  # e4m3: q, k, v; fp32 staged to fp16: q, k
         (q_head, q_tok, _), (k_head, k_tok, _), (v_head, v_tok, _), (o_tok, o_head, _) = q.stride(), k.stride(), v.stride(), out.stride()
-        launch = _native.call_forward_noalloc if noalloc else _native.call_forward
+        launch = launch or (_native.call_forward_noalloc if noalloc else _native.call_forward)
         launch(_native.stream(q.device),
                _native.ABI_VERSION, _DTYPES[q.dtype], _DTYPES[out.dtype], _DTYPES[v.dtype], h, hkv, d, n, _native.f32(scale),
                q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head, out.data_ptr(), o_tok, o_head,

@@ -296,28 +296,35 @@ Outputs logprobs_forward(const Tensor &x, const Tensor &tokens, int64_t top, boo
 // stream wait for the capture, which ends the process where it is the default one.
 bool leaves_capture(int index) {
   const auto node = torch::autograd::get_current_node();
-  if (!node || node->num_outputs() == 0 || !node->next_edge(0).function) return false;
-  const auto to = node->next_edge(0).function->stream();
+  if (!node) return false;
   const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(index);
-  if (!to || to->device_index() != index || to->id() == here.id()) return false;
-  const c10::hip::HIPStream there(c10::Stream(c10::Stream::UNSAFE, here.unwrap().device(), to->id()));
   auto captures = [](hipStream_t s) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     return s && hipStreamIsCapturing(s, &status) == hipSuccess && status != hipStreamCaptureStatusNone;  // never the default one
   };
-  return captures(here.stream()) && !captures(there.stream());
+  for (const auto &edge : node->next_edges()) {
+    if (!edge.function) continue;
+    const auto to = edge.function->stream();
+    if (!to || to->device_index() != index || to->id() == here.id()) continue;
+    const c10::hip::HIPStream there(c10::Stream(c10::Stream::UNSAFE, here.unwrap().device(), to->id()));
+    if (captures(here.stream()) && !captures(there.stream())) return true;
+  }
+  return false;
 }
 
-void check_capture(int index) {
-  TORCH_CHECK(!leaves_capture(index), "token_logprobs: a captured backward whose logits were first used outside of the capture; "
+void check_capture(int index, const char *name = "token_logprobs") {
+  TORCH_CHECK(!leaves_capture(index), name, ": a captured backward whose inputs were first used outside of the capture; "
               "drop every earlier result that holds their graph before the capture");
 }
-// check_capture(device index), for a backward that runs in Python
-PyObject *py_check_capture(PyObject *, PyObject *arg) {
+// check_capture(device index, name), for a backward that runs in Python
+PyObject *py_check_capture(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  const long index = PyLong_AsLong(arg);
+  if (nargs != 2) return PyErr_Format(PyExc_TypeError, "check_capture takes a device index and a name");
+  const long index = PyLong_AsLong(args[0]);
   if (index == -1 && PyErr_Occurred()) return nullptr;
-  check_capture((int)index);
+  const char *name = PyUnicode_AsUTF8(args[1]);
+  if (!name) return nullptr;
+  check_capture((int)index, name);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -456,7 +463,7 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 
 #define DAN_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {DAN_METHOD(append), DAN_METHOD(attend), DAN_METHOD(logprobs), DAN_METHOD(bind),
-                         {"check_capture", py_check_capture, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         {"check_capture", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_check_capture)), METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decode_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -61,6 +61,7 @@
 #include <mutex>
 
 #include "dan_tree_attn.h"
+#include "dan_tree_grad.h"
 
 namespace dan {
 
@@ -147,6 +148,9 @@ struct KParams {
   const DanUnit *units;
   const int32_t *sched_off;
   int32_t num_units;
+  // Forward for a gradient only: log2 of each row's sum of exponentials, [heads][lse_rows].
+  float *lse;
+  int64_t lse_rows;
 };
 
 typedef const __attribute__((address_space(4))) KParams *KArgPtr;
@@ -768,7 +772,7 @@ __global__ __launch_bounds__(256) void vt_pack_kernel(const PackParams p) {
 // 36.0; 8/2 heads x 64, 2048 tokens 39.9 -> 26.8. With more units than that the
 // doubled loads lose (2776 tokens in 4 requests, 352 units: 29.8 -> 34.5). All
 // eight waves issuing the loads: 5 to 12 % slower than waves 0-3.
-template <typename TQK, typename TOut, int D, int KH>
+template <typename TQK, typename TOut, int D, int KH, bool LS = false>
 __global__ __attribute__((amdgpu_flat_work_group_size(Shape<D>::threads, Shape<D>::threads),
                           amdgpu_waves_per_eu(Shape<D>::waves_per_simd, Shape<D>::waves_per_simd)))
 void tree_attn_kernel(const KParams args) {
@@ -1413,6 +1417,8 @@ void tree_attn_kernel(const KParams args) {
       if (qvalid) {
 #pragma unroll
         for (int db = 0; db < NDB; ++db) store4<TOut>(orow + 16 * db + 4 * q4, o4[db] * linv);
+        if constexpr (LS)
+          if (q4 == 0) *gbl_mut(p.lse + head * p.lse_rows + cur.start + ql) = __builtin_amdgcn_logf(l) - mneg;
       }
       nn = 0;
     } else {
@@ -1543,7 +1549,8 @@ void tree_attn_kernel(const KParams args) {
       // r4 of block db holds d = 32 db + 8 r4 + 4 hl + (0..3); lanes l and
       // l ^ 32 (the same query) trade halves so that each stores 8 contiguous
       // d: lane hl = 0 the even groups, hl = 1 the odd ones.
-      float l = lsum + __shfl_xor(lsum, 32);
+      float l = lsum + __shfl_xor(lsum, 32), lse = 0.f;
+      if constexpr (LS) lse = __builtin_amdgcn_logf(l) - mneg;
       if constexpr (KH == 2) {
         // Merge the halves: the waves of keys 32-63 hand m, l, the V scale and
         // O (kRound d blocks at a time) to their partners over LDS, past the
@@ -1577,6 +1584,7 @@ void tree_attn_kernel(const KParams args) {
               const float lm = l * e0 + word(stat + 256) * e1, inv = lm > 0.f ? 1.0f / lm : 0.f;
               f0 = e0 * exp2i(vE) * inv;
               f1 = e1 * word(stat + 512) * inv;
+              if constexpr (LS) lse = __builtin_amdgcn_logf(lm) + m;
             }
 #pragma unroll
             for (int b = 0; b < kRound; ++b)
@@ -1591,6 +1599,8 @@ void tree_attn_kernel(const KParams args) {
         }
       }
       const float linv = KH == 2 ? 1.0f : l > 0.f ? exp2i(vE) / l : 0.f;
+      if constexpr (LS)
+        if (qvalid && khalf == 0 && hl == 0) *gbl_mut(p.lse + head * p.lse_rows + cur.start + ql) = lse;
       TOut *orow = static_cast<TOut *>(p.o) + (int64_t)(cur.start + ql) * p.o_st + (int64_t)head * p.o_sh;
   #pragma unroll
       for (int db = 0; db < ND; ++db)
@@ -1765,9 +1775,9 @@ hipError_t launch_pack(const PackParams &pp, int blocks, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename TQK, typename TOut, int D, int KH>
+template <typename TQK, typename TOut, int D, int KH, bool LS>
 hipError_t launch_attn_halves(const KParams &kp, int grid, hipStream_t stream) {
-  auto kernel = tree_attn_kernel<TQK, TOut, D, KH>;
+  auto kernel = tree_attn_kernel<TQK, TOut, D, KH, LS>;
   constexpr int lds = KH == 2 ? Merge<D, (int)sizeof(TQK)>::total : Lds<D, (int)sizeof(TQK)>::total + kVoteBytes;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -1776,11 +1786,18 @@ hipError_t launch_attn_halves(const KParams &kp, int grid, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename TQK, typename TOut, int D, bool LS>
+hipError_t launch_attn_lse(const KParams &kp, int grid, bool halves, hipStream_t stream) {
+  if constexpr (D <= 128)
+    if (halves) return launch_attn_halves<TQK, TOut, D, 2, LS>(kp, grid, stream);
+  return launch_attn_halves<TQK, TOut, D, 1, LS>(kp, grid, stream);
+}
+
 template <typename TQK, typename TOut, int D>
 hipError_t launch_attn(const KParams &kp, int grid, bool halves, hipStream_t stream) {
-  if constexpr (D <= 128)
-    if (halves) return launch_attn_halves<TQK, TOut, D, 2>(kp, grid, stream);
-  return launch_attn_halves<TQK, TOut, D, 1>(kp, grid, stream);
+  if constexpr (std::is_same<TQK, TOut>::value)  // bf16 and fp16: what a gradient is built for
+    if (kp.lse) return launch_attn_lse<TQK, TOut, D, true>(kp, grid, halves, stream);
+  return launch_attn_lse<TQK, TOut, D, false>(kp, grid, halves, stream);
 }
 
 }  // namespace dan
@@ -1808,8 +1825,11 @@ int64_t dan_tree_attn_workspace_size(int32_t num_kv_heads, int32_t head_dim, int
   return dan::vt_bytes(num_kv_heads, head_dim, vt_cols) + ((int64_t)num_kv_heads * (vt_cols / dan::kKeyTile) * 4 + 255) / 256 * 256;
 }
 
-int dan_tree_attn_fwd(const DanTreeAttnArgs *a, void *stream) {
-  using namespace dan;
+}  // extern "C"
+
+namespace dan {
+// dan_tree_attn_fwd, and dan_tree_attn_fwd_lse where lse is not NULL.
+int forward(const DanTreeAttnArgs *a, float *lse, void *stream) {
   g_err[0] = 0;
   if (!a) return fail(DAN_ERR_INVALID_ARGUMENT, "args is NULL");
   if (a->abi_version != DAN_TREE_ATTN_ABI_VERSION)
@@ -1830,8 +1850,8 @@ int dan_tree_attn_fwd(const DanTreeAttnArgs *a, void *stream) {
   const bool f16 = in == DAN_DTYPE_F16 && vd == DAN_DTYPE_F16 && out == DAN_DTYPE_F16;
   const bool f32 = in == DAN_DTYPE_F16 && vd == DAN_DTYPE_F32 && out == DAN_DTYPE_F32;
   const bool f8 = in == DAN_DTYPE_E4M3 && vd == DAN_DTYPE_E4M3 && out == DAN_DTYPE_BF16;
-  if (!bf16 && !f16 && !f32 && !f8)
-    return fail(DAN_ERR_UNSUPPORTED, "dtype combination q/k=%d v=%d out=%d is not built", in, vd, out);
+  if ((!bf16 && !f16 && !f32 && !f8) || (lse && !bf16 && !f16))
+    return fail(DAN_ERR_UNSUPPORTED, "dtype combination q/k=%d v=%d out=%d is not built%s", in, vd, out, lse ? " with lse" : "");
   if (a->num_work < 0 || a->num_segments < 0 || a->num_pasts < 0 || a->num_tokens < 0 || a->vt_cols < 0)
     return fail(DAN_ERR_INVALID_ARGUMENT, "negative count");
   if (a->num_work == 0 && a->num_saves)  // nothing would be launched that writes them
@@ -1916,6 +1936,7 @@ int dan_tree_attn_fwd(const DanTreeAttnArgs *a, void *stream) {
   kp.c = a->scale * 1.4426950408889634f;
   kp.q_scale = a->q_scale; kp.k_scale = a->k_scale;
   kp.units = a->units; kp.sched_off = a->sched_off; kp.num_units = (int32_t)units;
+  kp.lse = lse; kp.lse_rows = a->num_tokens;
   const int grid = a->num_slots;
 
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1945,6 +1966,19 @@ int dan_tree_attn_fwd(const DanTreeAttnArgs *a, void *stream) {
 #undef DAN_ATTN
   if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "attention launch failed: %s", hipGetErrorString(err));
   return DAN_OK;
+}
+}  // namespace dan
+
+extern "C" {
+
+int dan_tree_attn_fwd(const DanTreeAttnArgs *a, void *stream) { return dan::forward(a, nullptr, stream); }
+
+int dan_tree_attn_fwd_lse(const DanTreeAttnArgs *a, float *lse, void *stream) {
+  if (!lse) {
+    dan::g_err[0] = 0;
+    return dan::fail(DAN_ERR_INVALID_ARGUMENT, "lse is NULL");
+  }
+  return dan::forward(a, lse, stream);
 }
 
 namespace dan {

@@ -1,0 +1,706 @@
+// Gradient of tree-masked attention for gfx950 (include/dan_tree_grad.h).
+//
+// With S = scale Q K^T, P = softmax(S) over the visible keys, O = P V, and the
+// output's gradient G:
+//   delta_i = sum_d G_id O_id       dP = G V^T        dS = P * (dP - delta)
+//   dV = P^T G                      dQ = scale dS K   dK = scale dS^T Q
+// P is computed again from Q, K and the forward pass's logsumexp. Three launches:
+//   grad_rows_kernel     delta, and for fp16 a bound of |dS|;
+//   grad_keys_kernel     dK and dV: a work group holds a run of keys and walks the
+//                        query rows that see them, over all heads of the kv head;
+//   grad_queries_kernel  dQ: a work group holds query rows of the heads that share
+//                        a kv head and walks the keys that they see.
+// Each result is summed by one work group in a fixed order, so there are no atomics
+// and the results do not change from run to run. The price is that S and dP are
+// computed twice: 7 products where 5 would do.
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "dan_tree_grad.h"
+#include "tiles.h"
+
+namespace dan {
+
+int fail(int status, const char *fmt, ...);  // tree_attn.hip: sets the thread's last-error message
+extern thread_local char g_err[512];
+
+namespace {
+
+using namespace tiles;
+
+constexpr int kThreads = 256;
+constexpr int kMaxPartials = 1024;  // work groups of grad_rows_kernel, and partial maxima
+// fp16: P goes into its product times 2^14, so that the small probabilities of long rows keep their bits.
+constexpr float kPBias = 14.0f;
+constexpr int64_t kAlign = 256;
+
+// Rows (keys, queries) that a wave holds: 64, or 32 where head_dim 256 takes twice the registers. A wave
+// reads each tile of the other side from LDS once for all of them: 64 B a clock of the CU's 128 with 64 rows.
+template <int D>
+constexpr int kWaveRows = D == 256 ? 32 : 64;
+
+struct GradParams {
+  const void *q, *k, *v, *o, *g;
+  void *dq, *dk, *dv;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, g_st, g_sh, dq_st, dq_sh, dk_st, dk_sh, dv_st, dv_sh;
+  const float *lse;
+  float *stats;    // [2][H][N]: bias - lse, -delta
+  float *partial;  // [3][partials]: max |G row|^2, max |V row|^2, max |delta|
+  const DanGradKeyUnit *key_units;
+  const DanGradQueryUnit *query_units;
+  const int32_t *row_lo, *row_end;
+  const DanPastDesc *pasts;
+  int32_t num_tokens, num_heads, num_kv_heads, rep, hpw, groups, num_pasts, partials, key_rows;
+  float scale, c;  // c = scale * log2 e
+};
+
+template <typename T>
+__device__ inline T load_unit(const T *p) {
+  struct Raw {
+    uint32_t w[sizeof(T) / 4];
+  } raw;
+  const __attribute__((address_space(4))) uint32_t *src = (const __attribute__((address_space(4))) uint32_t *)p;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) raw.w[i] = __builtin_amdgcn_readfirstlane(src[i]);
+  return __builtin_bit_cast(T, raw);
+}
+
+__device__ inline float block_max(float x, float *red) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  return x;
+}
+
+// ---------------------------------------------------------------- delta
+// One pass over G and O (2 x 67 MB at 8192 rows x 32 heads x 128): a row is D / 8 lanes, 16 bytes each.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p) {
+  constexpr int L = D / 8, R = kThreads / L;
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  const int sub = threadIdx.x % L, mine = threadIdx.x / L;
+  const int64_t rows = (int64_t)p.num_tokens * p.num_heads;
+  float gmax = 0.f, vmax = 0.f, dmax = 0.f;
+  for (int64_t r = (int64_t)blockIdx.x * R + mine; r < rows; r += (int64_t)gridDim.x * R) {
+    const int64_t n = r / p.num_heads, h = r % p.num_heads;
+    const f32x8 g = unpack8<T>(load16(static_cast<const T *>(p.g) + n * p.g_st + h * p.g_sh + 8 * sub));
+    const f32x8 o = unpack8<T>(load16(static_cast<const T *>(p.o) + n * p.o_st + h * p.o_sh + 8 * sub));
+    float dot = 0.f, sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      dot = fmaf(g[i], o[i], dot);
+      if (kHalf) sq = fmaf(g[i], g[i], sq);
+    }
+#pragma unroll
+    for (int m = L / 2; m; m >>= 1) {
+      dot += __shfl_xor(dot, m);
+      if (kHalf) sq += __shfl_xor(sq, m);
+    }
+    if (sub == 0) {
+      const int64_t at = h * p.num_tokens + n;
+      p.stats[at] = (kHalf ? kPBias : 0.f) - p.lse[at];
+      p.stats[rows + at] = -dot;
+    }
+    gmax = fmaxf(gmax, sq);
+    dmax = fmaxf(dmax, fabsf(dot));
+  }
+  if constexpr (kHalf) {
+    const int64_t vrows = (int64_t)p.num_tokens * p.num_kv_heads;
+    for (int64_t r = (int64_t)blockIdx.x * R + mine; r < vrows; r += (int64_t)gridDim.x * R) {
+      const int64_t n = r / p.num_kv_heads, h = r % p.num_kv_heads;
+      const f32x8 v = unpack8<T>(load16(static_cast<const T *>(p.v) + n * p.v_st + h * p.v_sh + 8 * sub));
+      float sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+#pragma unroll
+      for (int m = L / 2; m; m >>= 1) sq += __shfl_xor(sq, m);
+      vmax = fmaxf(vmax, sq);
+    }
+    __shared__ float red[4];
+    gmax = block_max(gmax, red);
+    vmax = block_max(vmax, red);
+    dmax = block_max(dmax, red);
+    if (threadIdx.x == 0) {
+      p.partial[blockIdx.x] = gmax;
+      p.partial[p.partials + blockIdx.x] = vmax;
+      p.partial[2 * p.partials + blockIdx.x] = dmax;
+    }
+  }
+}
+
+// fp16: the power of 2 that brings every |dS| under 2^15 and keeps the rest as far above fp16's smallest
+// as it goes: |dP| <= |G row| |V row|. (A prefix's V is left out of the bound of dP, and its |delta| is in:
+// a prefix key's dP may pass it by the ratio of the norms; the clamp in dS keeps the product finite.)
+__device__ inline float ds_factor(const GradParams &p, float *red) {
+  float g = 0.f, v = 0.f, d = 0.f;
+  for (int i = threadIdx.x; i < p.partials; i += kThreads) {
+    g = fmaxf(g, p.partial[i]);
+    v = fmaxf(v, p.partial[p.partials + i]);
+    d = fmaxf(d, p.partial[2 * p.partials + i]);
+  }
+  g = block_max(g, red);
+  v = block_max(v, red);
+  d = block_max(d, red);
+  const float bound = sqrtf(g) * sqrtf(v) + d;
+  if (!(bound > 0.f && bound < INFINITY)) return 1.f;
+  const int e = min(max(14 - ilogbf(bound), -100), 100);
+  return ldexpf(1.f, e);
+}
+
+// Results of a 32x32 product whose lane holds column `lane % 32`, rows 8 (i / 4) + 4 (l / 32) + i % 4, scaled and
+// stored as the lane's row of memory: lanes l and l ^ 32 trade halves, so that each stores 16 bytes at a time.
+template <typename T>
+__device__ inline void store_column(T *row, const f32x16 &x, float f, int hl, bool valid) {
+#pragma unroll
+  for (int jp = 0; jp < 2; ++jp) {
+    const u32x2 even = pack4<T>(f32x4{x[8 * jp], x[8 * jp + 1], x[8 * jp + 2], x[8 * jp + 3]} * f);
+    const u32x2 odd = pack4<T>(f32x4{x[8 * jp + 4], x[8 * jp + 5], x[8 * jp + 6], x[8 * jp + 7]} * f);
+    // lanes below 32 get (even, the partner's even), the others (the partner's odd, odd)
+    const auto a = __builtin_amdgcn_permlane32_swap(even[0], odd[0], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(even[1], odd[1], false, false);
+    if (valid) store16(row + 8 * (2 * jp + hl), u32x4{a[0], b[0], a[1], b[1]});
+  }
+}
+
+// ---------------------------------------------------------------- dK, dV
+// Four waves: KW runs of kWaveRows keys side by side, and 4 / KW of the (32 rows, head) tiles of a step. A wave
+// keeps its keys' K and V (as operands) and dK and dV (as accumulators) in registers: 384 of 512 at head_dim 128
+// and 64 keys. Tiles of Q and G come to LDS by direct loads, a ring of steps ahead of their use.
+template <int D, int KW>
+struct KeyLds {
+  static constexpr int QW = 4 / KW;
+  static constexpr int stage = 2 * QW * Tile<D>::bytes;
+  static constexpr int ring = 4 * (stage + 1024) <= 140 * 1024 ? 4 : 3 * (stage + 1024) <= 140 * 1024 ? 3 : 2;
+  static constexpr int stats = ring * stage;          // [ring][4 waves][64 floats]
+  static constexpr int red = stats + ring * 1024;     // 16 floats
+  static constexpr int wave = 2 * kWaveRows<D> * D * 4;  // a wave's dK and dV
+  static constexpr int merge = QW > 1 ? QW / 2 * KW * wave : 0;
+  static constexpr int total = red + 64 > merge ? red + 64 : merge;
+  static_assert(total <= 160 * 1024, "LDS");
+};
+
+template <typename T, int D, int KW>
+__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads), amdgpu_waves_per_eu(1, 1)))
+void grad_keys_kernel(const GradParams p) {
+  using Tl = Tile<D>;
+  using Lds = KeyLds<D, KW>;
+  constexpr int NS = kWaveRows<D> / 32, QW = 4 / KW, NK = D / 16, ND = D / 32, NB = Lds::ring;
+  constexpr int SL = Lds::stage / 1024 / 4, TS = Tl::blocks / 4;  // direct loads of a wave a step, and a tile
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
+  const int lane = threadIdx.x & 63, hl = lane >> 5, wave = uni(threadIdx.x >> 6);
+  const int kw = wave % KW, qw = wave / KW;
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  const DanGradKeyUnit un = load_unit(p.key_units + blockIdx.x / p.num_kv_heads);
+  if (un.start < 0 || un.n <= 0 || un.start + un.n > p.num_tokens || un.key0 < 0 || un.keys <= 0 || un.keys > p.key_rows ||
+      un.key0 + un.keys > un.n || un.q_end <= un.key0 || un.q_end > un.n)
+    return;  // no such rows
+  float factor = 1.f;
+  if constexpr (kHalf) factor = ds_factor(p, reinterpret_cast<float *>(smem + Lds::red));
+
+  // The lane's keys: row 32 s + lane % 32 of the wave's. Key x is seen by the rows [x, x + see).
+  const int wkey = un.key0 + kw * kWaveRows<D>, kend = un.key0 + un.keys;
+  u32x4 kf[NS][NK], vf[NS][NK];
+  int key[NS], see[NS];
+  int top = 0, low = un.n;  // the rows below `top` see some key, those below `low` (and past the last key) all
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    key[s] = wkey + 32 * s + (lane & 31);
+    const bool valid = key[s] < kend;
+    const int64_t row = un.start + min(key[s], kend - 1);
+    const T *kr = static_cast<const T *>(p.k) + row * p.k_st + kvh * p.k_sh + 8 * hl;
+    const T *vr = static_cast<const T *>(p.v) + row * p.v_st + kvh * p.v_sh + 8 * hl;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      kf[s][kk] = load16(kr + 16 * kk);
+      vf[s][kk] = load16(vr + 16 * kk);
+    }
+    const int end = valid ? p.row_end[row] : 0;
+    see[s] = max(end - key[s], 0);
+    top = max(top, end);
+    low = min(low, end);
+  }
+#pragma unroll
+  for (int m = 32; m; m >>= 1) {
+    top = max(top, __shfl_xor(top, m));
+    low = min(low, __shfl_xor(low, m));
+  }
+  top = uni(top);
+  low = uni(low);
+
+  f32x16 dk[NS][ND], dv[NS][ND];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int db = 0; db < ND; ++db) dk[s][db] = dv[s][db] = f32x16{};
+
+  const int tiles = (un.q_end - un.key0 + 31) / 32 * p.rep, steps = (tiles + QW - 1) / QW;
+  const int64_t plane = (int64_t)p.num_heads * p.num_tokens;
+  // Step i's tiles to ring buffer b: every wave issues SL + 1 loads for every step (past the last one, and for
+  // tiles past the last, the last tile's again), so that a count of them says which have landed.
+  auto issue = [&](int i, int b) __attribute__((always_inline)) {
+    const uint32_t dst = lds + (uint32_t)(b * Lds::stage + wave * 1024);
+#pragma unroll
+    for (int j = 0; j < QW; ++j) {
+      const int t = min(i * QW + j, tiles - 1), qt = t / p.rep, head = kvh * p.rep + (t - qt * p.rep);
+      const int qb = un.key0 + 32 * qt, left = un.n - 1 - qb;  // (rows past the segment: its last row)
+      const int64_t row = un.start + qb;
+      const T *qt_at = static_cast<const T *>(p.q) + row * p.q_st + head * p.q_sh;
+      const T *gt_at = static_cast<const T *>(p.g) + row * p.g_st + head * p.g_sh;
+#pragma unroll
+      for (int x = 0; x < TS; ++x) {
+        const uint32_t m = (uint32_t)min(Tl::block_row(4 * x + wave, lane), left), byte = Tl::block_byte(4 * x + wave, lane);
+        dma16(qt_at, m * (uint32_t)(2 * p.q_st) + byte, dst + (uint32_t)((2 * j * TS + x) * 4096));
+        dma16(gt_at, m * (uint32_t)(2 * p.g_st) + byte, dst + (uint32_t)(((2 * j + 1) * TS + x) * 4096));
+      }
+      if (j == qw)
+        dma4(p.stats + head * (int64_t)p.num_tokens + row, (uint32_t)(min(lane & 31, left) * 4 + hl * (int)(plane * 4)),
+             lds + (uint32_t)(Lds::stats + b * 1024 + wave * 256));
+    }
+  };
+  const uint32_t rows_at = Tl::rows_at(lane), cols_at = Tl::cols_at(lane);
+  auto compute = [&](int i, int b) __attribute__((always_inline)) {
+    const int t = i * QW + qw;
+    if (t >= tiles) return;
+    const int qb = un.key0 + 32 * (t / p.rep);
+    if (qb >= top || qb + 31 < wkey) return;  // no row of the tile sees a key of the wave
+    const uint32_t qt = lds + (uint32_t)(b * Lds::stage + 2 * qw * Tl::bytes), gt = qt + Tl::bytes;
+    const uint32_t st = lds + (uint32_t)(Lds::stats + b * 1024 + wave * 256 + 16 * hl);
+    f32x16 sc[NS], dp[NS];
+    float nl[16];
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const f32x4 l = __builtin_bit_cast(f32x4, lds_read16(st + 32 * i4)), d = __builtin_bit_cast(f32x4, lds_read16(st + 128 + 32 * i4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        nl[4 * i4 + e] = l[e];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) dp[s][4 * i4 + e] = d[e];  // dP - delta
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) sc[s] = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const u32x4 a = Tl::read_rows(qt, rows_at, kk);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) sc[s] = mfma32<T>(a, kf[s][kk], sc[s]);
+    }
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const u32x4 a = Tl::read_rows(gt, rows_at, kk);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) dp[s] = mfma32<T>(a, vf[s][kk], dp[s]);
+    }
+    const bool full = qb >= wkey + kWaveRows<D> - 1 && qb + 32 <= low;
+    u32x4 pf[NS][2], df[NS][2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        f32x8 x, y;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          x[r] = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * ks + r], p.c, nl[8 * ks + r]));
+          y[r] = kHalf ? fminf(fmaxf(x[r] * factor * dp[s][8 * ks + r], -65504.f), 65504.f) : x[r] * dp[s][8 * ks + r];
+        }
+        if (!full) {
+          const int rel = qb + 4 * hl - key[s];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const bool seen = (uint32_t)(rel + 16 * ks + 8 * (r >> 2) + (r & 3)) < (uint32_t)see[s];
+            x[r] = seen ? x[r] : 0.f;
+            y[r] = seen ? y[r] : 0.f;
+          }
+        }
+        pf[s][ks] = pack8<T>(x);
+        df[s][ks] = pack8<T>(y);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int db = 0; db < ND; ++db) {
+        const u32x4 ga = Tl::read_cols(gt, cols_at, db, ks), qa = Tl::read_cols(qt, cols_at, db, ks);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          dv[s][db] = mfma32<T>(ga, pf[s][ks], dv[s][db]);
+          dk[s][db] = mfma32<T>(qa, df[s][ks], dk[s][db]);
+        }
+      }
+  };
+
+  if constexpr (kHalf) factor *= 1.f / 16384.f;  // P carries 2^kPBias
+#pragma unroll
+  for (int i = 0; i < NB - 1; ++i) issue(i, i);
+  int b = 0;
+  for (int i = 0; i < steps; ++i) {
+    wait_vmem<(NB - 2) * (SL + 1)>();  // step i has landed
+    barrier_lds();                     // for every wave, and every wave has left step i - 1
+    issue(i + NB - 1, b == 0 ? NB - 1 : b - 1);
+    compute(i, b);
+    b = b == NB - 1 ? 0 : b + 1;
+  }
+  wait_vmem<0>();
+  if constexpr (QW > 1) {  // the waves of the same keys add up, pairwise, over LDS
+#pragma unroll
+    for (int h = QW / 2; h; h >>= 1) {
+      barrier_lds();
+      const uint32_t at = lds + (uint32_t)((qw % h * KW + kw) * Lds::wave + lane * 16);
+      if (qw >= h && qw < 2 * h) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int db = 0; db < ND; ++db)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t to = at + (uint32_t)(((s * ND + db) * 8 + x) * 1024);
+              *(DAN_TILE_LDS f32x4 *)(uintptr_t)to = f32x4{dk[s][db][4 * x], dk[s][db][4 * x + 1], dk[s][db][4 * x + 2], dk[s][db][4 * x + 3]};
+              *(DAN_TILE_LDS f32x4 *)(uintptr_t)(to + 4096) = f32x4{dv[s][db][4 * x], dv[s][db][4 * x + 1], dv[s][db][4 * x + 2], dv[s][db][4 * x + 3]};
+            }
+      }
+      barrier_lds();
+      if (qw < h) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int db = 0; db < ND; ++db)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t from = at + (uint32_t)(((s * ND + db) * 8 + x) * 1024);
+              const f32x4 a = __builtin_bit_cast(f32x4, lds_read16(from)), c = __builtin_bit_cast(f32x4, lds_read16(from + 4096));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                dk[s][db][4 * x + e] += a[e];
+                dv[s][db][4 * x + e] += c[e];
+              }
+            }
+      }
+    }
+    if (qw > 0) return;
+  }
+  const float fv = kHalf ? 1.f / 16384.f : 1.f, fk = kHalf ? p.scale / (factor * 16384.f) : p.scale;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int64_t row = un.start + min(key[s], kend - 1);
+    T *kr = static_cast<T *>(p.dk) + row * p.dk_st + kvh * p.dk_sh, *vr = static_cast<T *>(p.dv) + row * p.dv_st + kvh * p.dv_sh;
+#pragma unroll
+    for (int db = 0; db < ND; ++db) {
+      store_column<T>(kr + 32 * db, dk[s][db], fk, hl, key[s] < kend);
+      store_column<T>(vr + 32 * db, dv[s][db], fv, hl, key[s] < kend);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- dQ
+// Four waves: hpw heads of the kv head by 4 / hpw runs of kWaveRows rows. A wave keeps its rows' Q and G and their
+// dQ in registers; tiles of 32 keys of K and V come to LDS by direct loads.
+template <int D>
+struct QueryLds {
+  static constexpr int stage = 2 * Tile<D>::bytes, ring = 4;
+  static constexpr int red = ring * stage;
+  static constexpr int total = red + 64;
+  static_assert(total <= 160 * 1024, "LDS");
+};
+
+template <typename T, int D>
+__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads), amdgpu_waves_per_eu(1, 1)))
+void grad_queries_kernel(const GradParams p) {
+  using Tl = Tile<D>;
+  using Lds = QueryLds<D>;
+  constexpr int NS = kWaveRows<D> / 32, NK = D / 16, ND = D / 32, NB = Lds::ring;
+  constexpr int TS = Tl::blocks / 4, SL = 2 * TS;
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
+  const int lane = threadIdx.x & 63, hl = lane >> 5, wave = uni(threadIdx.x >> 6);
+  const int group = blockIdx.x % p.groups, kvh = group % p.num_kv_heads, chunk = group / p.num_kv_heads;
+  const DanGradQueryUnit un = load_unit(p.query_units + blockIdx.x / p.groups);
+  if (un.start < 0 || un.n <= 0 || un.start + un.n > p.num_tokens || un.t0 < 0 || un.tq <= 0 || un.t0 + un.tq > un.n ||
+      un.tq > kWaveRows<D> * 4 / p.hpw || un.trunk < 0 || un.trunk > un.n || un.branch0 < 0 ||
+      (un.past_len > 0 && (un.past_idx < 0 || un.past_idx >= p.num_pasts)))
+    return;  // no such rows
+  float factor = 1.f;
+  if constexpr (kHalf) factor = ds_factor(p, reinterpret_cast<float *>(smem + Lds::red)) * (1.f / 16384.f);
+
+  // The keys, three runs one after the other in tiles of 32: the prefix, the trunk up to the unit's last row, and
+  // the branch rows from the first one's branch on.
+  const int tend = un.t0 + un.tq, t_hi = min(un.trunk, tend);
+  const int past_tiles = max(un.past_len + 31, 0) / 32, trunk_tiles = (t_hi + 31) / 32;
+  const int steps = past_tiles + trunk_tiles + (tend > un.trunk ? max(tend - un.branch0 + 31, 0) / 32 : 0);
+  const T *pk = nullptr, *pv = nullptr;
+  int64_t pk_st = 0, pv_st = 0;
+  if (past_tiles) {
+    const DanPastDesc pd = load_unit(p.pasts + un.past_idx);
+    if (pd.len < un.past_len) return;  // no such prefix
+    pk = static_cast<const T *>(pd.k) + kvh * pd.k_stride_head;
+    pv = static_cast<const T *>(pd.v) + kvh * pd.v_stride_head;
+    pk_st = pd.k_stride_tok;
+    pv_st = pd.v_stride_tok;
+  }
+  const T *own_k = static_cast<const T *>(p.k) + un.start * p.k_st + kvh * p.k_sh;
+  const T *own_v = static_cast<const T *>(p.v) + un.start * p.v_st + kvh * p.v_sh;
+
+  const int hig = chunk * p.hpw + wave % p.hpw, head = min(kvh * p.rep + hig, (kvh + 1) * p.rep - 1);
+  const int w0 = un.t0 + wave / p.hpw * kWaveRows<D>;
+  const bool work = hig < p.rep && w0 < tend && wave / p.hpw < 4 / p.hpw;
+  const int wlast = min(w0 + kWaveRows<D>, tend) - 1;
+  const int64_t plane = (int64_t)p.num_heads * p.num_tokens;
+  u32x4 qf[NS][NK], gf[NS][NK];
+  float nl[NS], nd[NS];
+  int row[NS], lo[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    row[s] = w0 + 32 * s + (lane & 31);
+    const int64_t r = un.start + min(row[s], tend - 1);
+    const T *qr = static_cast<const T *>(p.q) + r * p.q_st + head * p.q_sh + 8 * hl;
+    const T *gr = static_cast<const T *>(p.g) + r * p.g_st + head * p.g_sh + 8 * hl;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      qf[s][kk] = load16(qr + 16 * kk);
+      gf[s][kk] = load16(gr + 16 * kk);
+    }
+    nl[s] = p.stats[head * (int64_t)p.num_tokens + r];
+    nd[s] = p.stats[plane + head * (int64_t)p.num_tokens + r];
+    lo[s] = p.row_lo[r];
+  }
+  f32x16 dq[NS][ND];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int db = 0; db < ND; ++db) dq[s][db] = f32x16{};
+
+  auto issue = [&](int i_any, int b) __attribute__((always_inline)) {  // (past the last step: the last one's again)
+    const int i = min(i_any, steps - 1);
+    const bool past = i < past_tiles, trunk = i < past_tiles + trunk_tiles;
+    const int kb = past ? 32 * i : trunk ? 32 * (i - past_tiles) : un.branch0 + 32 * (i - past_tiles - trunk_tiles);
+    const int left = (past ? un.past_len : trunk ? t_hi : tend) - 1 - kb;
+    const int64_t k_st = past ? pk_st : p.k_st, v_st = past ? pv_st : p.v_st;
+    const T *kt = (past ? pk : own_k) + kb * k_st, *vt = (past ? pv : own_v) + kb * v_st;
+    const uint32_t dst = lds + (uint32_t)(b * Lds::stage + wave * 1024);
+#pragma unroll
+    for (int x = 0; x < TS; ++x) {
+      const uint32_t m = (uint32_t)min(Tl::block_row(4 * x + wave, lane), left), byte = Tl::block_byte(4 * x + wave, lane);
+      dma16(kt, m * (uint32_t)(2 * k_st) + byte, dst + (uint32_t)(x * 4096));
+      dma16(vt, m * (uint32_t)(2 * v_st) + byte, dst + (uint32_t)((TS + x) * 4096));
+    }
+  };
+  const uint32_t rows_at = Tl::rows_at(lane), cols_at = Tl::cols_at(lane);
+  auto compute = [&](int i, int b) __attribute__((always_inline)) {
+    const bool past = i < past_tiles, trunk = i < past_tiles + trunk_tiles;
+    const int kb = past ? 32 * i : trunk ? 32 * (i - past_tiles) : un.branch0 + 32 * (i - past_tiles - trunk_tiles);
+    if (!work || (!past && kb > wlast)) return;
+    const uint32_t kt = lds + (uint32_t)(b * Lds::stage), vt = kt + Tl::bytes;
+    f32x16 sc[NS], dp[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sc[s][r] = 0.f;
+        dp[s][r] = nd[s];
+      }
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const u32x4 a = Tl::read_rows(kt, rows_at, kk);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) sc[s] = mfma32<T>(a, qf[s][kk], sc[s]);
+    }
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const u32x4 a = Tl::read_rows(vt, rows_at, kk);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) dp[s] = mfma32<T>(a, gf[s][kk], dp[s]);
+    }
+    const bool full = past ? kb + 32 <= un.past_len : trunk && kb + 32 <= un.trunk && kb + 31 <= w0;
+    u32x4 df[NS][2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      // The row sees the keys [first, last] of this run.
+      const int first = past || trunk ? 0 : row[s] < un.trunk ? row[s] + 1 : lo[s];
+      const int last = past ? un.past_len - 1 : trunk ? min(row[s], un.trunk - 1) : row[s];
+      const uint32_t see = (uint32_t)max(last - first + 1, 0);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        f32x8 y;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * ks + r], p.c, nl[s]));
+          y[r] = kHalf ? fminf(fmaxf(x * factor * dp[s][8 * ks + r], -65504.f), 65504.f) : x * dp[s][8 * ks + r];
+        }
+        if (!full) {
+          const int rel = kb + 4 * hl - first;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) y[r] = (uint32_t)(rel + 16 * ks + 8 * (r >> 2) + (r & 3)) < see ? y[r] : 0.f;
+        }
+        df[s][ks] = pack8<T>(y);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int db = 0; db < ND; ++db) {
+        const u32x4 ka = Tl::read_cols(kt, cols_at, db, ks);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) dq[s][db] = mfma32<T>(ka, df[s][ks], dq[s][db]);
+      }
+  };
+
+#pragma unroll
+  for (int i = 0; i < NB - 1; ++i) issue(i, i);
+  int b = 0;
+  for (int i = 0; i < steps; ++i) {
+    wait_vmem<(NB - 2) * SL>();
+    barrier_lds();
+    issue(i + NB - 1, b == 0 ? NB - 1 : b - 1);
+    compute(i, b);
+    b = b == NB - 1 ? 0 : b + 1;
+  }
+  wait_vmem<0>();
+  if (!work) return;
+  const float f = kHalf ? p.scale / (factor * 16384.f) : p.scale;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    T *r = static_cast<T *>(p.dq) + (un.start + (int64_t)min(row[s], tend - 1)) * p.dq_st + head * p.dq_sh;
+#pragma unroll
+    for (int db = 0; db < ND; ++db) store_column<T>(r + 32 * db, dq[s][db], f, hl, row[s] < tend);
+  }
+}
+
+// ---------------------------------------------------------------- host
+int wave_rows(int D) { return D == 256 ? 32 : 64; }
+int heads_of_group(int rep) { return rep >= 3 ? 4 : rep; }
+
+template <typename K>
+hipError_t allow_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename T, int D, int KW>
+hipError_t launch_keys(const GradParams &p, int64_t grid, hipStream_t s) {
+  constexpr int bytes = KeyLds<D, KW>::total;
+  static const hipError_t attr = allow_lds(grad_keys_kernel<T, D, KW>, bytes);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((grad_keys_kernel<T, D, KW>), dim3((uint32_t)grid), dim3(kThreads), bytes, s, p);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_all(const GradParams &p, int64_t keys_grid, int64_t queries_grid, hipStream_t s) {
+  hipLaunchKernelGGL((grad_rows_kernel<T, D>), dim3(p.partials), dim3(kThreads), 0, s, p);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  constexpr int KW = 64 / kWaveRows<D>;  // runs of a wave's keys in the smaller unit
+  err = p.key_rows == 128 ? launch_keys<T, D, 2 * KW>(p, keys_grid, s) : launch_keys<T, D, KW>(p, keys_grid, s);
+  if (err != hipSuccess) return err;
+  constexpr int bytes = QueryLds<D>::total;
+  static const hipError_t attr = allow_lds(grad_queries_kernel<T, D>, bytes);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((grad_queries_kernel<T, D>), dim3((uint32_t)queries_grid), dim3(kThreads), bytes, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace dan
+
+extern "C" {
+
+int dan_tree_grad_abi_version(void) { return DAN_TREE_GRAD_ABI_VERSION; }
+
+int32_t dan_tree_grad_key_rows(int32_t head_dim, int32_t small) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+  return small ? 64 : 128;
+}
+
+int32_t dan_tree_grad_query_rows(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || !dan_tree_grad_key_rows(head_dim, 0)) return 0;
+  return dan::wave_rows(head_dim) * 4 / dan::heads_of_group(num_heads / num_kv_heads);
+}
+
+int64_t dan_tree_grad_workspace_size(int32_t num_heads, int32_t num_tokens) {
+  if (num_heads <= 0 || num_tokens <= 0) return 0;
+  return ((int64_t)num_heads * num_tokens * 8 + 3 * dan::kMaxPartials * 4 + dan::kAlign - 1) / dan::kAlign * dan::kAlign;
+}
+
+int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
+  using namespace dan;
+  g_err[0] = 0;
+  if (!a) return fail(DAN_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->abi_version != DAN_TREE_GRAD_ABI_VERSION)
+    return fail(DAN_ERR_VERSION, "abi_version %d, library speaks %d", a->abi_version, DAN_TREE_GRAD_ABI_VERSION);
+  const int H = a->num_heads, Hkv = a->num_kv_heads, D = a->head_dim, N = a->num_tokens;
+  if (H <= 0 || Hkv <= 0 || H % Hkv)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "num_heads %d must be a positive multiple of num_kv_heads %d", H, Hkv);
+  if (D != 64 && D != 128 && D != 256) return fail(DAN_ERR_UNSUPPORTED, "head_dim %d: only 64, 128 and 256 are built", D);
+  if (a->dtype != DAN_DTYPE_BF16 && a->dtype != DAN_DTYPE_F16) return fail(DAN_ERR_UNSUPPORTED, "dtype %d: bf16 or fp16", a->dtype);
+  if (N < 0 || a->num_key_units < 0 || a->num_query_units < 0 || a->num_pasts < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "negative count");
+  if (!(a->scale > 0.f && isfinite(a->scale) && isfinite(a->scale * 1.4426950408889634f)))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+  if (a->key_rows != dan_tree_grad_key_rows(D, 0) && a->key_rows != dan_tree_grad_key_rows(D, 1))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "key_rows %d: dan_tree_grad_key_rows", a->key_rows);
+  if (N == 0 || a->num_key_units == 0 || a->num_query_units == 0) return DAN_OK;
+  if (!a->q || !a->k || !a->v || !a->out || !a->grad || !a->lse || !a->dq || !a->dk || !a->dv || !a->key_units || !a->query_units ||
+      !a->row_lo || !a->row_end || (a->num_pasts > 0 && !a->pasts))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "NULL tensor or table pointer");
+  const int64_t need = dan_tree_grad_workspace_size(H, N);
+  if (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & (kAlign - 1)))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
+  const int64_t strides[] = {a->q_stride_tok, a->q_stride_head, a->k_stride_tok, a->k_stride_head, a->v_stride_tok, a->v_stride_head,
+                             a->o_stride_tok, a->o_stride_head, a->g_stride_tok, a->g_stride_head, a->dq_stride_tok, a->dq_stride_head,
+                             a->dk_stride_tok, a->dk_stride_head, a->dv_stride_tok, a->dv_stride_head};
+  for (int64_t s : strides)
+    if (s % 8) return fail(DAN_ERR_INVALID_ARGUMENT, "strides must keep rows 16-byte aligned");
+  const void *rows[] = {a->q, a->k, a->v, a->out, a->grad, a->dq, a->dk, a->dv};
+  for (const void *r : rows)
+    if ((uintptr_t)r & 15) return fail(DAN_ERR_INVALID_ARGUMENT, "q, k, v, out and the gradients must be 16-byte aligned");
+  // Offsets inside a tile, and between the two planes of the workspace, are kept in 32 bits.
+  for (int64_t s : {a->q_stride_tok, a->k_stride_tok, a->v_stride_tok, a->g_stride_tok})
+    if (s < 0 || s * 64 >= (int64_t(1) << 31)) return fail(DAN_ERR_UNSUPPORTED, "token stride %lld is too large", (long long)s);
+  if ((int64_t)H * N * 4 >= (int64_t(1) << 31) - 4096) return fail(DAN_ERR_UNSUPPORTED, "%d heads x %d tokens: fewer than 2^29 rows", H, N);
+
+  GradParams p;
+  p.q = a->q; p.q_st = a->q_stride_tok; p.q_sh = a->q_stride_head;
+  p.k = a->k; p.k_st = a->k_stride_tok; p.k_sh = a->k_stride_head;
+  p.v = a->v; p.v_st = a->v_stride_tok; p.v_sh = a->v_stride_head;
+  p.o = a->out; p.o_st = a->o_stride_tok; p.o_sh = a->o_stride_head;
+  p.g = a->grad; p.g_st = a->g_stride_tok; p.g_sh = a->g_stride_head;
+  p.dq = a->dq; p.dq_st = a->dq_stride_tok; p.dq_sh = a->dq_stride_head;
+  p.dk = a->dk; p.dk_st = a->dk_stride_tok; p.dk_sh = a->dk_stride_head;
+  p.dv = a->dv; p.dv_st = a->dv_stride_tok; p.dv_sh = a->dv_stride_head;
+  p.lse = a->lse;
+  p.stats = static_cast<float *>(a->workspace);
+  p.partial = p.stats + 2 * (int64_t)H * N;
+  p.key_units = a->key_units; p.query_units = a->query_units;
+  p.row_lo = a->row_lo; p.row_end = a->row_end;
+  p.pasts = a->pasts; p.num_pasts = a->num_pasts;
+  p.num_tokens = N; p.num_heads = H; p.num_kv_heads = Hkv; p.rep = H / Hkv;
+  p.hpw = heads_of_group(p.rep);
+  p.groups = Hkv * ((p.rep + p.hpw - 1) / p.hpw);
+  p.key_rows = a->key_rows;
+  const int64_t rows_a_block = kThreads / (D / 8);
+  p.partials = (int)std::min<int64_t>(kMaxPartials, ((int64_t)H * N + rows_a_block - 1) / rows_a_block);
+  p.scale = a->scale;
+  p.c = a->scale * 1.4426950408889634f;
+  const int64_t keys_grid = (int64_t)a->num_key_units * Hkv, queries_grid = (int64_t)a->num_query_units * p.groups;
+  if (keys_grid * kThreads >= (int64_t(1) << 32) || queries_grid * kThreads >= (int64_t(1) << 32))
+    return fail(DAN_ERR_UNSUPPORTED, "%lld and %lld work groups: fewer than 2^24", (long long)keys_grid, (long long)queries_grid);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto by_d = [&](auto t) {
+    using T = decltype(t);
+    return D == 64 ? launch_all<T, 64>(p, keys_grid, queries_grid, s) : D == 128 ? launch_all<T, 128>(p, keys_grid, queries_grid, s)
+                                                                                 : launch_all<T, 256>(p, keys_grid, queries_grid, s);
+  };
+  const hipError_t err = a->dtype == DAN_DTYPE_BF16 ? by_d(__bf16{}) : by_d(_Float16{});
+  if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "attention gradient launch failed: %s", hipGetErrorString(err));
+  return DAN_OK;
+}
+
+}  // extern "C"
