@@ -21,6 +21,7 @@
 #include <stdint.h>
 
 #include "dan_fp8.h"
+#include "fp8_layout.h"
 
 namespace dan {
 int fail(int status, const char *fmt, ...);  // tree_attn.hip: sets the thread's last-error message
@@ -30,7 +31,6 @@ extern thread_local char g_err[512];
 namespace dan_fp8 {
 
 constexpr int kThreads = 256;
-constexpr float kE4m3Max = 448.0f;  // torch.finfo(torch.float8_e4m3fn).max (dan/quant.py:16)
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -58,12 +58,6 @@ __device__ inline f32x8 load8<float>(const float *p) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// |x| as its fp32 bit pattern. Non-negative floats order as unsigned
-// integers and every NaN pattern lies above +inf's, so an integer max over
-// these propagates NaN as torch's amax does (dan/fused.py:88): a row holding
-// a NaN gets a NaN scale and NaN codes. (A float max would skip the NaN.)
-__device__ inline uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
-
 // max |x| over the work group (as bits), in every thread.
 __device__ inline uint32_t block_amax(uint32_t v, uint32_t *red) {
 #pragma unroll
@@ -87,13 +81,6 @@ __device__ inline uint32_t row_amax(const T *row, int cols) {
   return a;
 }
 
-// max(amax, 1e-12) / 448 from amax's bits; a NaN amax gives a NaN scale
-// (torch's clamp keeps NaN).
-__device__ inline float scale_of(uint32_t amax_bits) {
-  const float amax = __builtin_bit_cast(float, amax_bits);
-  return amax_bits > 0x7f800000u ? amax : fmaxf(amax, 1e-12f) / kE4m3Max;
-}
-
 struct Params {
   const void *x;
   int64_t x_stride;
@@ -105,14 +92,8 @@ struct Params {
 };
 
 // Byte offset of the 8 codes of row r, columns c .. c + 7 (c a multiple of 8).
-// Tiled: 256-row panels, each a run of 16 KB k-steps; a k-step is 16 blocks
-// of 16 rows x 64 bytes, row i of a block at 64 i, its 16-byte chunk j at
-// position j ^ (((i >> 1) & 3) ^ ((i >> 3) & 1)) (include/dan_fp8.h).
 __device__ inline int64_t code_offset(const Params &p, int r, int c) {
-  if (!p.tiled) return (int64_t)r * p.cols + c;
-  const int i = r & 15, chunk = (c >> 4) & 3;
-  const int pos = chunk ^ (((i >> 1) & 3) ^ ((i >> 3) & 1));
-  return ((((int64_t)(r >> 8) * p.kt + (c >> 6)) * 16 + ((r >> 4) & 15)) << 10) + 64 * i + 16 * pos + (c & 8);
+  return p.tiled ? tiled_offset(r, c, p.kt) : (int64_t)r * p.cols + c;
 }
 
 template <typename T>

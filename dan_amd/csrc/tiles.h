@@ -1,5 +1,5 @@
 // Operand types and helpers of the kernels that feed 32x32 matrix products from tiles of
-// 16-bit rows in LDS (tree_attn_grad.hip).
+// 16-bit rows in LDS, and of what stands beside them (tree_attn_grad.hip, adapt.hip, add_norm.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -65,9 +65,13 @@ template <int N>
 __device__ inline void wait_vmem() {
   static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+  asm volatile("" ::: "memory");  // reads of what has landed stay behind
 }
 // A barrier that leaves the direct loads in flight alone: their completion is counted (wait_vmem).
 __device__ inline void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A wave's own LDS reads end here (for a tile that it alone reads and refills).
+__device__ inline void barrier_wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 __device__ inline int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 template <typename T>

@@ -62,3 +62,51 @@ def attend(q, k, v, segments, layer, scale=None, grad=None):
                     term = w[:, first:, None] * y[:, None]  # [H, own keys, D]
                     r[f].index_add_(1, idx, term.view(-1, rep, len(own), d).sum(1))
     return r
+
+
+def adapt(y, x, a, b, index, scale, grad=None):
+    """Row by row, fp64: dict of out and abs_out, and with ``grad`` dx, da, db and their abs_ bounds. index: a list; negative:
+    no adapter, past the last: NaN (and no gradient)."""
+    y, x, a, b = (t.detach().double().cpu() for t in (y, x, a, b))
+    scale = scale.double().cpu().tolist() if isinstance(scale, torch.Tensor) else [scale] * len(a)
+    r = dict(out=y.clone(), abs_out=y.abs())
+    if grad is not None:
+        grad = grad.detach().double().cpu()
+        r.update({f: torch.zeros_like(t) for f, t in (("dx", x), ("da", a), ("db", b), ("abs_dx", x), ("abs_da", a), ("abs_db", b))})
+    for n, i in enumerate(index):
+        if i < 0:
+            continue
+        if i >= len(a):
+            r["out"][n] = math.nan
+            continue
+        c, h, ah = scale[i], a[i] @ x[n], a[i].abs() @ x[n].abs()
+        r["out"][n] += c * (b[i] @ h)
+        r["abs_out"][n] += abs(c) * (b[i].abs() @ ah)
+        if grad is not None:
+            g, ag = grad[n] @ b[i], grad[n].abs() @ b[i].abs()
+            r["dx"][n] = c * (g @ a[i])
+            r["abs_dx"][n] = abs(c) * (ag @ a[i].abs())
+            r["da"][i] += c * torch.outer(g, x[n])
+            r["abs_da"][i] += abs(c) * torch.outer(ag, x[n].abs())
+            r["db"][i] += c * torch.outer(grad[n], h)
+            r["abs_db"][i] += abs(c) * torch.outer(grad[n].abs(), ah)
+    return r
+
+
+def add_norm(x, residual, weight, eps=1e-6, norm="rms", grad=None, grad_stream=None):
+    """fp64: dict of stream, out, scale (of e4m3 codes), and with ``grad`` ds, dw and their abs_ bounds."""
+    s = x.detach().double().cpu()
+    if residual is not None:
+        s = s + residual.detach().double().cpu()
+    w = weight.detach().double().cpu() + (1.0 if norm == "zero_centered" else 0.0)
+    rs = 1.0 / ((s * s).mean(1, keepdim=True) + eps).sqrt()
+    hat = s * rs
+    out = hat * w
+    r = dict(stream=s, out=out, scale=out.abs().amax(1, keepdim=True).clamp(min=1e-12) / 448.0)
+    if grad is not None:
+        g = grad.detach().double().cpu()
+        gs = torch.zeros_like(s) if grad_stream is None else grad_stream.detach().double().cpu()
+        r["ds"] = rs * (w * g - hat * (w * g * hat).mean(1, keepdim=True)) + gs
+        r["abs_ds"] = rs * ((w * g).abs() + hat.abs() * (w * g * hat).abs().mean(1, keepdim=True)) + gs.abs()
+        r["dw"], r["abs_dw"] = (g * hat).sum(0), (g * hat).abs().sum(0)
+    return r
