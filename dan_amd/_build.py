@@ -1,7 +1,7 @@
 """Build recipe for the gfx950 shared library (hipcc, in-tree) and the host
-module of the decode step's calls (g++).
+modules of the plain calls (g++).
 
-    python -m dan_amd._build          # -> dan_amd/_lib/libdan_tree_attn.so, _decode_calls.so
+    python -m dan_amd._build          # -> dan_amd/_lib/libdan_tree_attn.so, _decode_calls.so, _layer_calls.so
 
 Flags:
   --offload-arch=gfx950            CDNA4 only, no other targets.
@@ -37,9 +37,8 @@ SRC_FLAGS = {"tree_attn.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"]}
 # accumulators per lane live in the accumulation registers (AGPRs).
 MFMA_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 ACC_IN_AGPRS = {"fp8_gemm.hip"}
-# The host side of the decode step's plain calls: a CPython module on torch's headers (g++).
-CALLS_SRC = os.path.join(HERE, "csrc", "decode_calls.cpp")
-CALLS_NAME = "_decode_calls.so"
+# The host side of the plain calls: CPython modules on torch's headers (g++).
+CALLS = {"_decode_calls.so": os.path.join(HERE, "csrc", "decode_calls.cpp"), "_layer_calls.so": os.path.join(HERE, "csrc", "layer_calls.cpp")}
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(OUT_DIR, "libdan_tree_attn.so")
@@ -59,7 +58,7 @@ def hipcc():
     return path
 
 
-def calls_command(out):
+def calls_command(src, out):
     import sysconfig
 
     import torch
@@ -69,7 +68,7 @@ def calls_command(out):
             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I", INCLUDE,
             *(f for d in (os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
                           sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")) for f in ("-isystem", d)),
-            CALLS_SRC, "-o", out, "-L", os.path.join(home, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-lamdhip64"]
+            src, "-o", out, "-L", os.path.join(home, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-lamdhip64"]
 
 
 def _run(cmd, verbose):
@@ -98,15 +97,16 @@ def build(out=OUT, extra=(), verbose=False):
         return [*HIPCC_FLAGS, *([] if name in ACC_IN_AGPRS else MFMA_VGPR_FORM), *SRC_FLAGS.get(name, [])]
 
     cmds = [[hipcc(), *flags(src), *extra, "-I", INCLUDE, "-c", src, "-o", obj] for src, obj in zip(SRCS, objs)]
-    calls = os.path.join(os.path.dirname(out), CALLS_NAME)
-    cmds.insert(0, calls_command(calls + ".tmp"))
+    calls = {os.path.join(os.path.dirname(out), name): src for name, src in CALLS.items()}
+    cmds = [calls_command(src, path + ".tmp") for path, src in calls.items()] + cmds
     with ThreadPoolExecutor(max_workers=min(len(cmds), max(1, (os.cpu_count() or 1)))) as pool:
         for f in [pool.submit(_run, c, verbose) for c in cmds]:
             f.result()
     tmp = out + ".tmp"
     _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", tmp], verbose)
     os.replace(tmp, out)
-    os.replace(calls + ".tmp", calls)
+    for path in calls:
+        os.replace(path + ".tmp", path)
     return out
 
 

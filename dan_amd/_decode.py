@@ -92,15 +92,19 @@ def logprobs_workspace_size(dtype, rows, vocab, top):
 def calls():
     """The host module of the plain calls (csrc/decode_calls.cpp), bound to the library. Like the
     library it has to be there: there is no fallback for a missing one."""
-    lib, path = _native.load(), os.path.join(_native.LIB_DIR, "_decode_calls.so")
+    return load_calls("_decode_calls", ("dan_paged_append", "dan_paged_attn", "dan_paged_attn_workspace_size", "dan_logprobs_fwd", "dan_logprobs_bwd",
+                                        "dan_logprobs_workspace_size", "dan_tree_attn_last_error"))
+
+
+def load_calls(name, entries):
+    """The host module ``name``, bound to the library's ``entries``."""
+    lib, path = _native.load(), os.path.join(_native.LIB_DIR, name + ".so")
     if not os.path.exists(path):
         raise RuntimeError(f"{path} is not built; run __graft_entry__.build()")
-    loader = importlib.machinery.ExtensionFileLoader("_decode_calls", path)
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_decode_calls", loader))
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
     loader.exec_module(module)
-    module.bind(*(ctypes.cast(lib[name], ctypes.c_void_p).value for name in (
-        "dan_paged_append", "dan_paged_attn", "dan_paged_attn_workspace_size", "dan_logprobs_fwd", "dan_logprobs_bwd",
-        "dan_logprobs_workspace_size", "dan_tree_attn_last_error")))
+    module.bind(*(ctypes.cast(lib[entry], ctypes.c_void_p).value for entry in entries))
     return module
 
 

@@ -39,6 +39,32 @@ EXPORTS = ("dan_tree_attn_fwd_lse", "dan_tree_attn_bwd", "dan_tree_grad_key_rows
 call_backward = _native.Entry("dan_tree_attn_bwd", DanTreeGradArgs)
 
 
+def templates(segments, q, k, v, layer, scale, plan_args):
+    """What the host module's ``attend`` takes beside q, k and v: the two argument structures as bytes, their workspaces' sizes, whether a row
+    is in no segment, and the tensors that they point to."""
+    from . import attention as A
+
+    args, pasts_host, plan = plan_args
+    (h, n, d), hkv = q.shape, k.shape[0]
+    t = tables(segments, plan, h, hkv, d, A._num_cus(q.device))
+    code, nbytes, back = A._DTYPES[q.dtype], _native.workspace_size(hkv, d, plan.vt_cols) if plan.num_work else 0, workspace_size(h, n)
+    past = plan.past_tables[layer][0]
+    device_tables = args[3]
+    units, sched_off = (device_tables[5].data_ptr(), device_tables[6].data_ptr()) if plan.num_work else (0, 0)
+    num_segments, num_pasts, num_work, tile_q, vt_cols, slots = args[5][:6]
+    forward = call_forward_lse.pack(
+        _native.ABI_VERSION, code, code, code, h, hkv, d, n, _native.f32(args[6]), *[0] * 12, 0, 0, 0, device_tables[0].data_ptr(), num_segments,
+        past.data_ptr(), num_pasts, device_tables[1].data_ptr(), num_work, device_tables[2].data_ptr(), tile_q, vt_cols, device_tables[3].data_ptr(),
+        0, 0, _native.PHASES_ALL, units, sched_off, slots, 0, 0 if pasts_host is None else pasts_host.data_ptr(), A._layout(h, hkv, d)[0] // tile_q, 0, 0, 0)
+    backward = call_backward.pack(
+        GRAD_ABI_VERSION, code, h, hkv, d, n, _native.f32(args[6]), t.key_rows, *[0] * 15, 0, *[0] * 9, t.keys, t.num_keys, t.queries, t.num_queries,
+        t.row_lo, t.row_end, past.data_ptr(), num_pasts, 0, 0)
+    pasts = tuple(x for entry in plan.past_dicts for x in entry[layer][:2])
+    # (the prefix's rows as the kernels read them, where they had to be copied, are behind past_tables)
+    refs = tuple(x for x in plan.past_tables[layer][1][0] if isinstance(x, torch.Tensor))
+    return (forward, nbytes, backward, back, not t.covered, (t.blob, past, *device_tables, *refs), pasts), (t, pasts_host)
+
+
 class _ForwardLse(_native.Entry):
     """``dan_tree_attn_fwd_lse``: the forward entry with one more argument."""
 
@@ -148,6 +174,27 @@ def tables(segments, plan, h, hkv, d, num_cus):
     t = plan.grad_tables[h, hkv, d]
     t.use()
     return t
+
+
+def attend(q, k, v, segments, layer, scale):
+    """The differentiable call: through the host module where q, k and v are read in place."""
+    from . import attention as A
+    from . import _layer
+
+    plan = getattr(segments, "tile_plan", None)
+    if plan is None or plan.num_tokens != q.shape[1] or plan.device != q.device:
+        plan = None
+    key = (layer, *q.shape[::2], k.shape[0], q.dtype, scale)
+    made = None if plan is None else plan.train_calls.get(key)
+    if made is None:
+        with torch.no_grad():
+            plan_args = A._call_args(q, k, v, segments, layer, scale, None, _native.PHASES_ALL, False, upload=False)
+        made = templates(segments, q, k, v, layer, scale, plan_args)
+        plan_args[2].train_calls[key] = made
+    call, (t, _) = made
+    t.use()
+    out = _layer.calls().attend(q, k, v, *call)
+    return TreeAttention.apply(q, k, v, segments, layer, scale) if out is None else out
 
 
 class TreeAttention(torch.autograd.Function):

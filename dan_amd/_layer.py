@@ -4,7 +4,7 @@ layer runs in front of and beside its projections, in the library that
 import ctypes
 import functools
 
-from . import _native
+from . import _decode, _native
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -31,25 +31,34 @@ class DanNormGradArgs(ctypes.Structure):
 
 class DanAdaptArgs(ctypes.Structure):
     _fields_ = [("abi_version", _i32), ("dtype", _i32), ("rows", _i32), ("n_in", _i32), ("n_out", _i32), ("rank", _i32),
-                ("adapters", _i32), ("splits", _i32), ("x", _vp), ("x_stride", _i64), ("y", _vp), ("y_stride", _i64),
+                ("adapters", _i32), ("reserved", _i32), ("x", _vp), ("x_stride", _i64), ("y", _vp), ("y_stride", _i64),
                 ("a", _vp), ("b", _vp), ("index", _vp), ("scale", _vp), ("scale_value", _f32), ("out", _vp), ("out_stride", _i64),
-                ("down", _vp)]
+                ("down", _vp), ("workspace", _vp), ("workspace_bytes", _i64)]
 
 
 class DanAdaptGradArgs(ctypes.Structure):
     _fields_ = [("abi_version", _i32), ("dtype", _i32), ("rows", _i32), ("n_in", _i32), ("n_out", _i32), ("rank", _i32),
-                ("adapters", _i32), ("splits", _i32), ("x", _vp), ("x_stride", _i64), ("g", _vp), ("g_stride", _i64),
+                ("adapters", _i32), ("reserved", _i32), ("x", _vp), ("x_stride", _i64), ("g", _vp), ("g_stride", _i64),
                 ("a", _vp), ("b", _vp), ("index", _vp), ("scale", _vp), ("scale_value", _f32), ("down", _vp),
                 ("dx", _vp), ("dx_stride", _i64), ("da", _vp), ("db", _vp), ("workspace", _vp), ("workspace_bytes", _i64)]
 
 
 EXPORTS = ("dan_add_norm", "dan_add_norm_grad", "dan_norm_grad_workspace_size", "dan_norm_abi_version",
-           "dan_adapt", "dan_adapt_grad", "dan_adapt_splits", "dan_adapt_grad_workspace_size", "dan_adapt_abi_version")
+           "dan_adapt", "dan_adapt_grad", "dan_adapt_workspace_size", "dan_adapt_grad_workspace_size", "dan_adapt_abi_version")
 
 call_norm = _native.Entry("dan_add_norm", DanNormArgs)
 call_norm_grad = _native.Entry("dan_add_norm_grad", DanNormGradArgs)
 call_adapt = _native.Entry("dan_adapt", DanAdaptArgs)
 call_adapt_grad = _native.Entry("dan_adapt_grad", DanAdaptGradArgs)
+
+
+@functools.lru_cache(maxsize=None)
+def calls():
+    """The host module of the plain calls (csrc/layer_calls.cpp), bound to the library. Like the
+    library it has to be there: there is no fallback for a missing one."""
+    return _decode.load_calls("_layer_calls", (
+        "dan_add_norm", "dan_add_norm_grad", "dan_norm_grad_workspace_size", "dan_adapt", "dan_adapt_grad", "dan_adapt_workspace_size",
+        "dan_adapt_grad_workspace_size", "dan_tree_attn_fwd_lse", "dan_tree_attn_bwd", "dan_fp8_tiled_bytes", "dan_tree_attn_last_error"))
 
 
 def _sized(name, restype, count):
@@ -64,8 +73,8 @@ def norm_grad_workspace_size(rows, cols):
 
 
 @functools.lru_cache(maxsize=1024)
-def adapt_splits(rows, n):
-    return _sized("dan_adapt_splits", _i32, 2)(rows, n)
+def adapt_workspace_size(rows, n_in, rank):
+    return _sized("dan_adapt_workspace_size", _i64, 3)(rows, n_in, rank)
 
 
 @functools.lru_cache(maxsize=1024)

@@ -34,27 +34,28 @@ def _scale_args(scale):
     return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (0, _native.f32(scale))
 
 
-def _forward(y, x, a, b, index, scale):
-    """(out, the rows' x A^T in parts)."""
+def _forward(y, x, a, b, index, scale, want_down):
+    """(out, the rows' x A^T or None)."""
     (n, n_in), n_out = x.shape, y.shape[1]
     x, y = _layer.rows_of(x), _layer.rows_of(y)
     a, b = _padded(a, b)
     r = a.shape[1]
-    splits = _layer.adapt_splits(n, n_in)
     out = torch.empty((n, n_out), dtype=x.dtype, device=x.device)
-    down = torch.empty((splits, n, _down_rank(r)), dtype=torch.float32, device=x.device)
+    down = torch.empty((n, _down_rank(r)), dtype=torch.float32, device=x.device) if want_down else None
     if n:
+        nbytes = _layer.adapt_workspace_size(n, n_in, r)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         _layer.call_adapt(
-            _native.stream(x.device), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, r, a.shape[0], splits,
+            _native.stream(x.device), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, r, a.shape[0], 0,
             x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), a.data_ptr(), b.data_ptr(), 0 if index is None else index.data_ptr(),
-            *_scale_args(scale), out.data_ptr(), n_out, down.data_ptr())
+            *_scale_args(scale), out.data_ptr(), n_out, 0 if down is None else down.data_ptr(), ws.data_ptr(), nbytes)
     return out, down
 
 
 class _Adapt(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, a, b, index, scale):
-        out, down = _forward(y, x, a, b, index, scale)
+        out, down = _forward(y, x, a, b, index, scale, True)
         ctx.save_for_backward(x, a, b, down, *(t for t in (index, scale) if isinstance(t, torch.Tensor)))
         ctx.index, ctx.scale = index is not None, None if isinstance(scale, torch.Tensor) else scale
         return out
@@ -88,7 +89,7 @@ def _backward(x, a, b, down, index, scale, g, need):
         nbytes = _layer.adapt_grad_workspace_size(n, n_in, n_out, r, count)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _layer.call_adapt_grad(
-            _native.stream(dev), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, r, count, down.shape[0],
+            _native.stream(dev), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, r, count, 0,
             x.data_ptr(), x.stride(0), g.data_ptr(), g.stride(0), a8.data_ptr(), b8.data_ptr(), 0 if index is None else index.data_ptr(),
             *_scale_args(scale), down.data_ptr(), 0 if dx is None else dx.data_ptr(), n_in, 0 if da is None else da.data_ptr(),
             0 if db is None else db.data_ptr(), ws.data_ptr(), nbytes)
@@ -114,6 +115,9 @@ def adapt(y, x, a, b, index=None, scale=1.0):
     its forward pass in the same capture, and no earlier, eager result that holds
     the graph of the same leaves is alive (where an input is such a leaf itself, that
     raises)."""
+    made = _layer.calls().adapt(y, x, a, b, index, scale)
+    if made is not None:  # a plain call
+        return made
     if not x.is_cuda:
         raise RuntimeError(f"dan_amd.adapt runs on a gfx950 GPU only; got tensors on {x.device}")
     if x.device.index != torch._C._cuda_getDevice():
@@ -156,7 +160,7 @@ def adapt(y, x, a, b, index=None, scale=1.0):
         if isinstance(scale, torch.Tensor) and scale.requires_grad:
             raise NotImplementedError("adapt has no gradient of scale")
         return _Adapt.apply(y, x, a, b, index, scale)
-    return _forward(y, x, a, b, index, scale)[0]
+    return _forward(y, x, a, b, index, scale, False)[0]
 
 
 class AdaptedLinear(nn.Module):

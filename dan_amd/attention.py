@@ -201,7 +201,7 @@ def attend_train(q, k, v, segments, layer, scale=None):
     for s in segments:
         if s.save:
             s.saved[layer] = tuple(x[:, s.start:s.start + s.save].detach().clone() for x in (k, v))
-    return _grad.TreeAttention.apply(q, k, v, segments, layer, scale)
+    return _grad.attend(q, k, v, segments, layer, scale)
 
 
 def has_tangent(*tensors):

@@ -37,10 +37,11 @@ namespace {
 using namespace tiles;
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 128;     // values of the wide side that a wave of `down` takes at a time
-constexpr int kUpCols = 256;    // columns of a work group of `up`, 64 a wave
-constexpr int kOuterCols = 128; // columns of a work group of `outer`
-constexpr int kOuterRows = 32;  // rows of a step of `outer`
+constexpr int kFewRows = 512;    // up to here the kernels for few rows
+constexpr int kChunk = 128;      // values of the wide side that a wave of `down` takes at a time
+constexpr int kUpCols = 64;      // columns of a wave of `up`
+constexpr int kOuterCols = 128;  // columns of a work group of `outer`
+constexpr int kOuterRows = 32;   // rows of a step of `outer`
 
 // c += A B of a 16x16x32 product. Lane l holds row l % 16 of A (column of B) at k = 8 (l / 16) + 0..7, and of c
 // column l % 16, rows 4 (l / 16) + 0..3.
@@ -57,20 +58,60 @@ __device__ inline int exponent_of(float m) { return m > 0.f && m < INFINITY ? -m
 
 __device__ inline int adapter_of(const int32_t *index, int n) { return index ? index[n] : 0; }
 
+// The next adapter of a tile whose lanes' rows have the adapters `idx` and are not done yet (`left`), or -1.
+__device__ inline int next_adapter(int idx, uint64_t left) { return left ? __builtin_amdgcn_readlane(idx, __builtin_ctzll(left)) : -1; }
+
 // ---------------------------------------------------------------- down: part[s][n][j] = sum over k of x[n][k] w_i[j][k]
 struct DownParams {
   const void *x, *w;  // w [adapters][rank][n]
   const int32_t *index;
-  float *part;  // [splits][rows][rank16]
+  float *part;  // [splits][rows][ranks]
   int64_t x_stride;
-  int32_t rows, n, rank, adapters, rank16, chunks;  // chunks of kChunk values a work group
+  int32_t rows, n, rank, adapters, ranks, chunks;  // ranks: 16, 32, 64 or 128; chunks of kChunk values a work group
 };
 
-// 16 F rows, a range of chunks split over the four waves. A lane loads 32 contiguous bytes of a row (128 a row
-// and four lanes) for two steps of the product; the order of k within a chunk is the same for both operands.
+// Rows as operands: 16 F of them, four steps of 32 values from k0 on. A lane loads 16 bytes, four lanes 64 of a row.
+// (Here and below every load is made, at a clamped place where there is none to make: a load under a condition of
+// its own is a branch, and waits for the ones before it. Values past the row's end become zeros in x alone.)
+template <typename T, int F>
+__device__ inline void load_rows(const T *const (&row)[F], int k0, int last, int g4, u32x4 (&to)[F][4]) {
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+#pragma unroll
+    for (int s = 0; s < 4; ++s) to[f][s] = load16(row[f] + min(k0 + 32 * s + 8 * g4, last - 8));
+  if (k0 + kChunk > last)
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (k0 + 32 * s + 8 * g4 >= last) to[f][s] = u32x4{};
+}
+// t = w x^T over one chunk, w from adapter i.
 template <typename T, int JB, int F>
-__global__ __launch_bounds__(kThreads) void down_kernel(const DownParams p) {
-  __shared__ f32x4 red[4][JB][F][64];
+__device__ inline void chunk_product(const DownParams &p, int i, int k0, int last, int l16, int g4, const u32x4 (&xf)[F][4], f32x4 (&t)[JB][F]) {
+  const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.rank * p.n;
+  u32x4 wf[JB][4];
+#pragma unroll
+  for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+    for (int s = 0; s < 4; ++s)  // (ranks past the last one: copies of it, never used)
+      wf[jb][s] = load16(w + (int64_t)min(16 * jb + l16, p.rank - 1) * p.n + min(k0 + 32 * s + 8 * g4, last - 8));
+#pragma unroll
+  for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) t[jb][f] = mfma16<T>(wf[jb][s], xf[f][s], t[jb][f]);
+}
+
+// Many rows: 32 a work group, whose W waves split the chunks and add up over LDS.
+template <int JB>
+constexpr int kDownWaves = JB <= 2 ? 16 : 8;  // (1024 threads leave 128 registers each)
+template <typename T, int JB>
+__global__ __launch_bounds__(64 * kDownWaves<JB>) void down_kernel(const DownParams p) {
+  constexpr int F = 2, W = kDownWaves<JB>;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  f32x4 *red = reinterpret_cast<f32x4 *>(smem);  // [W / 2][JB * F][64]
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
   const int n0 = blockIdx.x * 16 * F, first = blockIdx.y * p.chunks * kChunk, last = min(first + p.chunks * kChunk, p.n);
   int idx[F];
@@ -80,49 +121,31 @@ __global__ __launch_bounds__(kThreads) void down_kernel(const DownParams p) {
     const int n = n0 + 16 * f + l16;
     idx[f] = n < p.rows ? adapter_of(p.index, n) : -1;
     if (idx[f] >= p.adapters) idx[f] = -1;  // (`up` makes the row NaN)
-    xr[f] = static_cast<const T *>(p.x) + (int64_t)min(n, p.rows - 1) * p.x_stride + 16 * g4;
+    xr[f] = static_cast<const T *>(p.x) + (int64_t)min(n, p.rows - 1) * p.x_stride;
   }
   f32x4 acc[JB][F];
 #pragma unroll
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
     for (int f = 0; f < F; ++f) acc[jb][f] = f32x4{};
-  for (int k0 = first + wave * kChunk; k0 < last; k0 += 4 * kChunk) {
+  for (int k0 = first + wave * kChunk; k0 < last; k0 += W * kChunk) {
     u32x4 xf[F][4];
-#pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = 64 * (s >> 1) + 8 * (s & 1);
-        xf[f][s] = k0 + k + 16 * g4 < last ? load16(xr[f] + k0 + k) : u32x4{};
-      }
+    load_rows<T, F>(xr, k0, last, g4, xf);
     uint64_t left[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) left[f] = __ballot(idx[f] >= 0);
     for (;;) {  // each adapter of the tile
       int i = -1;
 #pragma unroll
-      for (int f = 0; f < F; ++f)
-        if (i < 0 && left[f]) i = __builtin_amdgcn_readlane(idx[f], __builtin_ctzll(left[f]));
+      for (int f = F - 1; f >= 0; --f)
+        if (left[f]) i = next_adapter(idx[f], left[f]);
       if (i < 0) break;
-      const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.rank * p.n + 16 * g4 + k0;
       f32x4 t[JB][F];
 #pragma unroll
-      for (int jb = 0; jb < JB; ++jb) {
-        u32x4 wf[4];
-        const int j = 16 * jb + l16;
+      for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int k = 64 * (s >> 1) + 8 * (s & 1);
-          wf[s] = j < p.rank && k0 + k + 16 * g4 < last ? load16(w + (int64_t)j * p.n + k) : u32x4{};
-        }
-#pragma unroll
-        for (int f = 0; f < F; ++f) {
-          t[jb][f] = f32x4{};
-#pragma unroll
-          for (int s = 0; s < 4; ++s) t[jb][f] = mfma16<T>(wf[s], xf[f][s], t[jb][f]);
-        }
-      }
+        for (int f = 0; f < F; ++f) t[jb][f] = f32x4{};
+      chunk_product<T, JB, F>(p, i, k0, last, l16, g4, xf, t);
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const bool mine = idx[f] == i;
@@ -135,162 +158,313 @@ __global__ __launch_bounds__(kThreads) void down_kernel(const DownParams p) {
     }
   }
 #pragma unroll
-  for (int jb = 0; jb < JB; ++jb)
+  for (int h = W / 2; h; h >>= 1) {  // pairs of waves, in a fixed order
+    if (h < W / 2) __syncthreads();
+    if (wave >= h && wave < 2 * h)
 #pragma unroll
-    for (int f = 0; f < F; ++f) red[wave][jb][f][lane] = acc[jb][f];
-  __syncthreads();
-  for (int x = wave; x < JB * F; x += 4) {
-    const int jb = x / F, f = x % F, n = n0 + 16 * f + l16;
-    const f32x4 sum = (red[0][jb][f][lane] + red[1][jb][f][lane]) + (red[2][jb][f][lane] + red[3][jb][f][lane]);
-    if (n < p.rows) *(DAN_TILE_GLOBAL f32x4 *)(p.part + ((int64_t)blockIdx.y * p.rows + n) * p.rank16 + 16 * jb + 4 * g4) = sum;
+      for (int x = 0; x < JB * F; ++x) red[((wave - h) * JB * F + x) * 64 + lane] = acc[x / F][x % F];
+    __syncthreads();
+    if (wave < h)
+#pragma unroll
+      for (int x = 0; x < JB * F; ++x) acc[x / F][x % F] += red[(wave * JB * F + x) * 64 + lane];
+  }
+  if (wave == 0)
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int n = n0 + 16 * f + l16;
+      if (n < p.rows)
+#pragma unroll
+        for (int jb = 0; jb < JB; ++jb)
+          *(DAN_TILE_GLOBAL f32x4 *)(p.part + ((int64_t)blockIdx.y * p.rows + n) * p.ranks + 16 * jb + 4 * g4) = acc[jb][f];
+    }
+}
+
+// Few rows: 16 a work group, whose eight waves split the tile's adapters (each row is one wave's), so that the
+// adapters' loads do not wait for each other. The wide side is split over many work groups.
+constexpr int kFewWaves = 8;
+template <typename T, int JB>
+__global__ __launch_bounds__(64 * kFewWaves) void down_few_kernel(const DownParams p) {
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
+  const int n = blockIdx.x * 16 + l16, first = blockIdx.y * p.chunks * kChunk, last = min(first + p.chunks * kChunk, p.n);
+  int idx = n < p.rows ? adapter_of(p.index, n) : -1;
+  if (idx >= p.adapters) idx = -1;  // (`up` makes the row NaN)
+  const T *xr[1] = {static_cast<const T *>(p.x) + (int64_t)min(n, p.rows - 1) * p.x_stride};
+  float *to = p.part + ((int64_t)blockIdx.y * p.rows + n) * p.ranks + 4 * g4;
+  u32x4 xf[1][4];
+  load_rows<T, 1>(xr, first, last, g4, xf);
+  if (wave == 0 && n < p.rows && idx < 0)
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb) *(DAN_TILE_GLOBAL f32x4 *)(to + 16 * jb) = f32x4{};
+  uint64_t left = __ballot(idx >= 0);
+  for (int turn = 0; left; ++turn) {
+    const int i = next_adapter(idx, left);
+    const bool mine = idx == i;
+    left &= ~__ballot(mine);
+    if (turn % kFewWaves != wave) continue;
+    f32x4 t[JB][1];
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb) t[jb][0] = f32x4{};
+    chunk_product<T, JB, 1>(p, i, first, last, l16, g4, xf, t);
+    for (int k0 = first + kChunk; k0 < last; k0 += kChunk) {
+      u32x4 more[1][4];
+      load_rows<T, 1>(xr, k0, last, g4, more);
+      chunk_product<T, JB, 1>(p, i, k0, last, l16, g4, more, t);
+    }
+    if (mine)
+#pragma unroll
+      for (int jb = 0; jb < JB; ++jb) *(DAN_TILE_GLOBAL f32x4 *)(to + 16 * jb) = t[jb][0];
   }
 }
 
 // ---------------------------------------------------------------- up: out[n][m] = y[n][m] + c_i sum over j of v[n][j] w_i[m][j]
 struct UpParams {
-  const float *part;  // [splits][rows][rank16]
+  const float *part;  // [splits][rows][ranks]
+  float *sum;         // [rows][ranks]: v, for the gradient, or NULL
   const void *w, *y;  // w [adapters][cols][rank]; y may be NULL (zeros)
   void *out;
   const int32_t *index;
   const float *scale;
   int64_t y_stride, o_stride;
-  int32_t rows, cols, rank, adapters, rank16, splits;
+  int32_t rows, cols, rank, adapters, ranks, splits, steps;  // steps of 256 columns a work group (many rows)
   float scale_value;
 };
 
-// 16 F rows by 256 columns: a wave takes 64 columns, of which a lane owns 16 contiguous ones of its row (128 bytes a
-// row and four lanes): the product's row r of block b is column 16 (r / 4) + 4 b + r % 4. The inner dimension holds
-// v's hi parts, then its lo parts, in pieces of 8: ST steps of four pieces.
-template <typename T, int ST, int F>
+// v of 16 F rows as the second product's operand: the parts added up in order, then hi and lo numbers in pieces of 8,
+// hi pieces first, at [f][step][lane] (16 bytes each). With fp16 a row is brought near 1 first, by 2^exponent_of(top).
+template <typename T, int ST, int F, int TH>
+struct Operand {
+  f32x4 v[16 * F][4 * ST];
+  u32x4 piece[F * ST * 64];
+  uint32_t top[16 * F];  // fp16: the bits of a row's largest |v|
+  __device__ void make(const UpParams &p, int n0) {
+    constexpr bool kHalf = std::is_same<T, _Float16>::value;
+    if (kHalf)
+      for (int r = threadIdx.x; r < 16 * F; r += TH) top[r] = 0u;
+    if (kHalf) __syncthreads();
+    for (int q = threadIdx.x; q < 16 * F * 4 * ST; q += TH) {
+      const int r = q / (4 * ST), j4 = q % (4 * ST), n = n0 + r;
+      const float *from = p.part + (int64_t)min(n, p.rows - 1) * p.ranks + 4 * j4;
+      const int64_t plane = (int64_t)p.rows * p.ranks;
+      f32x4 x = *(const DAN_TILE_GLOBAL f32x4 *)from;
+#pragma unroll 8
+      for (int s = 1; s < p.splits; ++s) x += *(const DAN_TILE_GLOBAL f32x4 *)(from + s * plane);
+      if (p.sum && blockIdx.x == 0 && n < p.rows) *(DAN_TILE_GLOBAL f32x4 *)(p.sum + (int64_t)n * p.ranks + 4 * j4) = x;
+      v[r][j4] = x;
+      if (kHalf) {
+        const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        atomicMax(&top[r], __builtin_bit_cast(uint32_t, m));  // (of values that are not negative: in any order)
+      }
+    }
+    __syncthreads();
+    const int r8 = p.rank / 8;
+    for (int q = threadIdx.x; q < F * ST * 64; q += TH) {
+      const int r = q / (64 * ST) * 16 + (q & 15), u = (q / 64) % ST * 4 + (q >> 4) % 4, j8 = u >= r8 ? u - r8 : u;
+      u32x4 to = {};
+      if (u < 2 * r8) {
+        f32x8 x = __builtin_shufflevector(v[r][2 * j8], v[r][2 * j8 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        if (kHalf) {
+          const int e2 = exponent_of(__builtin_bit_cast(float, top[r]));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
+        }
+        to = pack8<T>(x);
+        if (u >= r8) to = pack8<T>(x - unpack8<T>(to));
+      }
+      piece[q] = to;
+    }
+    __syncthreads();
+  }
+};
+
+// The operand of 64 columns from m0 on. Lane (l16, g4) of the result owns 8 columns from m0 + 8 g4 on and 8 from m0 + 32 +
+// 8 g4 on, so that four lanes store 64 bytes of a row: row r of block b is column 32 (b / 2) + 8 (r / 4) + 4 (b % 2) + r % 4.
+template <typename T, int ST>
+__device__ inline void load_columns(const UpParams &p, int i, int m0, int l16, int g4, u32x4 (&wf)[ST][4]) {
+  const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.cols * p.rank;
+  const int r8 = p.rank / 8;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int col = min(m0 + 32 * (b >> 1) + 8 * (l16 >> 2) + 4 * (b & 1) + (l16 & 3), p.cols - 1);
+#pragma unroll
+    for (int t = 0; t < ST; ++t) {
+      const int u = 4 * t + g4, j = u >= 2 * r8 ? 0 : 8 * (u >= r8 ? u - r8 : u);  // (past the last piece v holds zeros)
+      wf[t][b] = load16(w + (int64_t)col * p.rank + j);
+    }
+  }
+}
+
+// The factor of a row's product with adapter i.
+template <typename T>
+__device__ inline float factor_of(const UpParams &p, int i, uint32_t top) {
+  const float c = p.scale ? p.scale[i] : p.scale_value;
+  return std::is_same<T, _Float16>::value ? ldexpf(c, -exponent_of(__builtin_bit_cast(float, top))) : c;
+}
+
+// Many rows: 64 (32 at rank 128) by `steps` times 256 columns, 64 a wave. y of the next step is loaded before this one's.
+template <int ST>
+constexpr int kUpFrags = ST == 8 ? 2 : 4;
+template <typename T, int ST>
 __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
+  constexpr int F = kUpFrags<ST>;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  __shared__ Operand<T, ST, F, kThreads> op;
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
-  const int n0 = blockIdx.y * 16 * F, m0 = blockIdx.x * kUpCols + wave * 64;
-  if (m0 >= p.cols) return;
-  const int r8 = p.rank / 8, m = m0 + 16 * g4;
-  u32x4 yv[F][2];
+  const int n0 = blockIdx.y * 16 * F, first = blockIdx.x * p.steps * 4 * kUpCols + wave * kUpCols;
   int idx[F];
+  u32x4 yv[F][2];
 #pragma unroll
   for (int f = 0; f < F; ++f) {
     const int n = n0 + 16 * f + l16;
     idx[f] = n < p.rows ? adapter_of(p.index, n) : -1;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      yv[f][h] = p.y && n < p.rows && m + 8 * h < p.cols ? load16(static_cast<const T *>(p.y) + n * p.y_stride + m + 8 * h) : u32x4{};
   }
-  int have = -1;  // the adapter whose B the wave holds
-  u32x4 wf[ST][4];
+  auto load_y = [&](int m0) __attribute__((always_inline)) {
 #pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int n = n0 + 16 * f + l16;
-    if (n0 + 16 * f >= p.rows) break;
-    f32x4 acc[4];
-    {
-      const f32x8 a = unpack8<T>(yv[f][0]), b = unpack8<T>(yv[f][1]);
+    for (int f = 0; f < F; ++f) {
+      const T *row = static_cast<const T *>(p.y) + min(n0 + 16 * f + l16, p.rows - 1) * p.y_stride;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[0][e] = a[e];
-        acc[1][e] = a[4 + e];
-        acc[2][e] = b[e];
-        acc[3][e] = b[4 + e];
-      }
+      for (int h = 0; h < 2; ++h) yv[f][h] = load16(row + min(m0 + 32 * h + 8 * g4, p.cols - 8));
     }
-    uint64_t left = __ballot(idx[f] >= 0);
-    if (left) {
-      // v's pieces of this lane, as hi or lo parts
-      f32x8 v[ST];
-      float top = 0.f;
+  };
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
-        const int u = 4 * t + g4, j = 8 * (u >= r8 ? u - r8 : u);
-        v[t] = f32x8{};
-        if (u < 2 * r8 && n < p.rows)
-          for (int s = 0; s < p.splits; ++s) {
-            const float *at = p.part + ((int64_t)s * p.rows + n) * p.rank16 + j;
-            const f32x4 a = *(const DAN_TILE_GLOBAL f32x4 *)at, b = *(const DAN_TILE_GLOBAL f32x4 *)(at + 4);
-            v[t] += __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-          }
-        if (kHalf)
+  for (int f = 0; f < F; ++f) yv[f][0] = yv[f][1] = u32x4{};
+  if (p.y) load_y(first);
+  op.make(p, n0);
+  for (int step = 0; step < p.steps; ++step) {
+    const int m0 = first + step * 4 * kUpCols;
+    if (m0 >= p.cols) break;  // (at once where there are no columns: v alone is wanted)
+    f32x4 acc[F][4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[t][e]));
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x8 y = unpack8<T>(yv[f][h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[f][2 * h][e] = y[e];
+          acc[f][2 * h + 1][e] = y[4 + e];
+        }
       }
-      int e2 = 0;
-      if (kHalf) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        e2 = exponent_of(top);
-      }
-      u32x4 vf[ST];
+    if (p.y && step + 1 < p.steps) load_y(m0 + 4 * kUpCols);
+    uint64_t left[F];
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
-        f32x8 x = v[t];
-        if (kHalf)
+    for (int f = 0; f < F; ++f) left[f] = __ballot(idx[f] >= 0);
+    for (;;) {
+      int i = -1;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
-        const u32x4 hi = pack8<T>(x);
-        vf[t] = 4 * t + g4 >= r8 ? pack8<T>(x - unpack8<T>(hi)) : hi;
-      }
-      while (left) {
-        const int i = __builtin_amdgcn_readlane(idx[f], __builtin_ctzll(left));
+      for (int f = F - 1; f >= 0; --f)
+        if (left[f]) i = next_adapter(idx[f], left[f]);
+      if (i < 0) break;
+      u32x4 wf[ST][4];
+      if (i < p.adapters) load_columns<T, ST>(p, i, m0, l16, g4, wf);
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
         const bool mine = idx[f] == i;
-        left &= ~__ballot(mine);
+        const uint64_t votes = __ballot(mine);
+        if (!votes) continue;
+        left[f] &= ~votes;
         if (i >= p.adapters) {  // no such adapter
 #pragma unroll
           for (int b = 0; b < 4; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[b][e] = mine ? NAN : acc[b][e];
+            for (int e = 0; e < 4; ++e) acc[f][b][e] = mine ? NAN : acc[f][b][e];
           continue;
         }
-        if (i != have) {
-          have = i;
-          const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.cols * p.rank;
+        const float c = factor_of<T>(p, i, kHalf ? op.top[16 * f + l16] : 0u);
+        u32x4 vf[ST];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int col = m0 + 16 * (l16 >> 2) + 4 * b + (l16 & 3);
-#pragma unroll
-            for (int t = 0; t < ST; ++t) {
-              const int u = 4 * t + g4, j = 8 * (u >= r8 ? u - r8 : u);
-              wf[t][b] = u < 2 * r8 && col < p.cols ? load16(w + (int64_t)col * p.rank + j) : u32x4{};
-            }
-          }
-        }
-        const float ci = p.scale ? p.scale[i] : p.scale_value, c = kHalf ? ldexpf(ci, -e2) : ci;
+        for (int t = 0; t < ST; ++t) vf[t] = op.piece[(f * ST + t) * 64 + lane];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           f32x4 t4 = {};
 #pragma unroll
           for (int t = 0; t < ST; ++t) t4 = mfma16<T>(wf[t][b], vf[t], t4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[b][e] = mine ? fmaf(c, t4[e], acc[b][e]) : acc[b][e];
+          for (int e = 0; e < 4; ++e) acc[f][b][e] = mine ? fmaf(c, t4[e], acc[f][b][e]) : acc[f][b][e];
         }
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (n < p.rows && m + 8 * h < p.cols)
-        store16(static_cast<T *>(p.out) + n * p.o_stride + m + 8 * h, pack8<T>(__builtin_shufflevector(acc[2 * h], acc[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7)));
+    for (int f = 0; f < F; ++f) {
+      const int n = n0 + 16 * f + l16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int m = m0 + 32 * h + 8 * g4;
+        if (n < p.rows && m < p.cols)
+          store16(static_cast<T *>(p.out) + n * p.o_stride + m, pack8<T>(__builtin_shufflevector(acc[f][2 * h], acc[f][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7)));
+      }
+    }
   }
+}
+
+// Few rows: 16 by 64 columns; the waves split the tile's adapters, and the first two store.
+template <typename T, int ST>
+__global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p) {
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  __shared__ Operand<T, ST, 1, 64 * kFewWaves> op;
+  __shared__ f32x4 sums[4][64];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
+  const int n = blockIdx.y * 16 + l16, m0 = blockIdx.x * kUpCols, m = m0 + 32 * wave + 8 * g4;
+  const int idx = n < p.rows ? adapter_of(p.index, n) : -1;
+  const bool store = wave < 2 && n < p.rows && m < p.cols;
+  u32x4 yv = {};
+  if (store && p.y) yv = load16(static_cast<const T *>(p.y) + n * p.y_stride + m);
+  op.make(p, blockIdx.y * 16);
+  if (p.cols == 0) return;  // v alone is wanted
+  u32x4 vf[ST];
+#pragma unroll
+  for (int t = 0; t < ST; ++t) vf[t] = op.piece[t * 64 + lane];
+  uint64_t left = __ballot(idx >= 0);
+  for (int turn = 0; left; ++turn) {
+    const int i = next_adapter(idx, left);
+    const bool mine = idx == i;
+    left &= ~__ballot(mine);
+    if (turn % kFewWaves != wave) continue;
+    float c = NAN;  // no such adapter
+    u32x4 wf[ST][4];
+    if (i < p.adapters) {
+      load_columns<T, ST>(p, i, m0, l16, g4, wf);
+      c = factor_of<T>(p, i, kHalf ? op.top[l16] : 0u);
+    } else {
+#pragma unroll
+      for (int t = 0; t < ST; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) wf[t][b] = u32x4{};
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      f32x4 t4 = {};
+#pragma unroll
+      for (int t = 0; t < ST; ++t) t4 = mfma16<T>(wf[t][b], vf[t], t4);
+      if (mine) sums[b][lane] = t4 * c;
+    }
+  }
+  __syncthreads();
+  if (!store) return;
+  f32x8 out = unpack8<T>(yv);
+  if (idx >= 0) out += __builtin_shufflevector(sums[2 * wave][lane], sums[2 * wave + 1][lane], 0, 1, 2, 3, 4, 5, 6, 7);
+  store16(static_cast<T *>(p.out) + n * p.o_stride + m, pack8<T>(out));
 }
 
 // ---------------------------------------------------------------- outer: d_i[j][c] = c_i sum over the rows of i of v[n][j] z[n][c]
 struct OuterSide {
-  const float *part;  // v [splits][rows][rank16]
+  const float *v;  // [rows][ranks]
   const void *z;
   int64_t z_stride;
-  float *sums;  // [parts][adapters][rank * cols]
-  int32_t cols, splits, tiles;
+  float *sums;  // [parts][adapters][rank * cols], or
+  void *out;    // with one part, the result itself
+  int32_t cols, tiles;
 };
 struct OuterParams {
   OuterSide a, b;  // dA [rank][n_in] of (g, x); dB [n_out][rank] of (h, G)
   const int32_t *index;
   const float *scale;
-  int32_t rows, rank, rank16, adapters, part_rows;  // rows of a part
+  int32_t rows, rank, ranks, adapters, parts;
   float scale_value;
 };
 
-// One adapter, one part of the rows, 128 columns. The rows of the part that are the adapter's are listed in order;
-// the waves take 32 of them in turn, each through a tile of its own in LDS, from where the transposing reads make the
-// operand whose inner dimension is the rows. v's operand is loaded in place (a lane's 8 rows).
+// One adapter, 128 columns, a part of the adapter's rows, which are listed in order; the waves take 32 of them in turn,
+// each through a tile of its own in LDS, from where the transposing reads make the operand whose inner dimension is
+// the rows. v's operand is loaded in place (a lane's 8 rows).
 template <typename T, int JB>
 __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
@@ -304,23 +478,30 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
   const bool side_b = (int)blockIdx.x >= p.a.tiles;
   const OuterSide &q = side_b ? p.b : p.a;
   const int c0 = ((int)blockIdx.x - (side_b ? p.a.tiles : 0)) * kOuterCols, i = blockIdx.y, part = blockIdx.z;
-  const int r0 = part * p.part_rows, r1 = min(r0 + p.part_rows, p.rows);
 
-  int count = 0;
-  for (int base = r0; base < r1; base += kThreads) {
-    const int n = base + threadIdx.x;
-    const bool mine = n < r1 && adapter_of(p.index, n) == i;
-    const uint64_t votes = __ballot(mine);
-    __syncthreads();
-    if (lane == 0) counts[wave] = __popcll(votes);
-    __syncthreads();
-    int at = count;
-    for (int w = 0; w < wave; ++w) at += counts[w];
-    if (mine) list[at + __popcll(votes & ((1ull << lane) - 1))] = n;
-    count += counts[0] + counts[1] + counts[2] + counts[3];
+  // Each thread counts its share of the index, then knows where its rows stand among the adapter's.
+  const int share = (p.rows + kThreads - 1) / kThreads, r0 = min((int)threadIdx.x * share, p.rows), r1 = min(r0 + share, p.rows);
+  int here = 0;
+  for (int n = r0; n < r1; ++n) here += adapter_of(p.index, n) == i;
+  int before = here;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int x = __shfl_up(before, m);
+    if (lane >= m) before += x;
   }
+  if (lane == 63) counts[wave] = before;
   __syncthreads();
-  count = uni(count);
+  before -= here;
+  for (int w = 0; w < wave; ++w) before += counts[w];
+  const int total = uni(counts[0] + counts[1] + counts[2] + counts[3]);
+  const int from = (int)((int64_t)total * part / p.parts), count = (int)((int64_t)total * (part + 1) / p.parts) - from;
+  if (here)
+    for (int n = r0; n < r1; ++n)
+      if (adapter_of(p.index, n) == i) {
+        if (before >= from && before < from + count) list[before - from] = n;
+        ++before;
+      }
+  __syncthreads();
 
   f32x4 acc[JB][CB];
 #pragma unroll
@@ -328,31 +509,34 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) acc[jb][cb] = f32x4{};
   const uint32_t tile = lds + (uint32_t)(wave * Tl::bytes);
-  const T *z = static_cast<const T *>(q.z) + (int64_t)r0 * q.z_stride + c0;
+  const int row0 = count ? uni(list[0]) : 0;  // (the list rises)
+  const T *z = static_cast<const T *>(q.z) + (int64_t)row0 * q.z_stride + c0;
   const int left = min(kOuterCols, q.cols - c0);  // columns of the tile (a multiple of 8)
   for (int s0 = wave * kOuterRows; s0 < count; s0 += 4 * kOuterRows) {
     barrier_wave_lds();  // (the last step's reads of the tile)
 #pragma unroll
     for (int x = 0; x < Tl::blocks; ++x) {
       const int n = list[min(s0 + Tl::block_row(x, lane), count - 1)];
-      dma16(z, (uint32_t)(n - r0) * (uint32_t)(2 * q.z_stride) + min(Tl::block_byte(x, lane), (uint32_t)(2 * left - 16)), tile + (uint32_t)(x * 1024));
+      dma16(z, (uint32_t)(n - row0) * (uint32_t)(2 * q.z_stride) + min(Tl::block_byte(x, lane), (uint32_t)(2 * left - 16)), tile + (uint32_t)(x * 1024));
     }
+    const int rows = min(count - s0, kOuterRows);
     float v[JB][8];
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int at = s0 + 8 * g4 + e;
-      const int n = list[min(at, count - 1)];
+      const bool in = 8 * g4 + e < rows;
+      const float *at = q.v + (int64_t)list[min(s0 + 8 * g4 + e, count - 1)] * p.ranks + l16;
 #pragma unroll
-      for (int jb = 0; jb < JB; ++jb) {
-        v[jb][e] = 0.f;
-        if (at < count)
-          for (int s = 0; s < q.splits; ++s) v[jb][e] += q.part[((int64_t)s * p.rows + n) * p.rank16 + 16 * jb + l16];
-        if (kHalf) top = fmaxf(top, fabsf(v[jb][e]));
-      }
+      for (int jb = 0; jb < JB; ++jb) v[jb][e] = at[16 * jb];
+#pragma unroll
+      for (int jb = 0; jb < JB; ++jb) v[jb][e] = in ? v[jb][e] : 0.f;
     }
     int e2 = 0;
     if (kHalf) {
+#pragma unroll
+      for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[jb][e]));
 #pragma unroll
       for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
       e2 = exponent_of(top);
@@ -368,8 +552,6 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
     }
     const float back = kHalf ? ldexpf(1.f, -e2) : 1.f;
     wait_vmem<0>();
-    // (rows past the list are copies of its last one, and v is 0 there: not so where that row holds infinities)
-    const int rows = min(count - s0, kOuterRows);
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       u32x4 zf;
@@ -381,7 +563,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
         zf[2 * h] = t[0];
         zf[2 * h + 1] = t[1];
       }
-      if (rows < kOuterRows) {
+      if (rows < kOuterRows) {  // rows past the list: zeros, whatever its last row (whose copies they are) holds
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (8 * g4 + e >= rows) zf[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
@@ -402,6 +584,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
   f32x4 *red = reinterpret_cast<f32x4 *>(smem);
   const float c = p.scale ? p.scale[i] : p.scale_value;
   float *to = q.sums + ((int64_t)part * p.adapters + i) * p.rank * q.cols;
+  T *out = static_cast<T *>(q.out) + (int64_t)i * p.rank * q.cols;
 #pragma unroll
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
@@ -410,14 +593,14 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
       for (int cb = 0; cb < CB / 2; ++cb) red[(wave * (CB / 2) + cb) * 64 + lane] = acc[jb][half * (CB / 2) + cb];
       __syncthreads();
-      const f32x4 sum = (red[wave * 64 + lane] + red[(CB / 2 + wave) * 64 + lane]) + (red[(CB + wave) * 64 + lane] + red[(3 * CB / 2 + wave) * 64 + lane]);
+      const f32x4 sum = ((red[wave * 64 + lane] + red[(CB / 2 + wave) * 64 + lane]) + (red[(CB + wave) * 64 + lane] + red[(3 * CB / 2 + wave) * 64 + lane])) * c;
       const int cb = half * (CB / 2) + wave, row = 4 * g4;
-      if (side_b) {  // lane: column l16, ranks row..
-        if (c0 + 16 * cb + l16 < q.cols && 16 * jb + row < p.rank)
-          *(DAN_TILE_GLOBAL f32x4 *)(to + (int64_t)(c0 + 16 * cb + l16) * p.rank + 16 * jb + row) = sum * c;
-      } else {  // lane: rank l16, columns row..
-        if (c0 + 16 * cb + row < q.cols && 16 * jb + l16 < p.rank)
-          *(DAN_TILE_GLOBAL f32x4 *)(to + (int64_t)(16 * jb + l16) * q.cols + c0 + 16 * cb + row) = sum * c;
+      // Lane: side b: column l16, ranks row..; side a: rank l16, columns row..
+      const int col = c0 + 16 * cb + (side_b ? l16 : row), j = 16 * jb + (side_b ? row : l16);
+      const int64_t at = side_b ? (int64_t)col * p.rank + j : (int64_t)j * q.cols + col;
+      if (col < q.cols && j < p.rank) {
+        if (p.parts == 1) *(DAN_TILE_GLOBAL u32x2 *)(out + at) = pack4<T>(sum);
+        else *(DAN_TILE_GLOBAL f32x4 *)(to + at) = sum;
       }
     }
 }
@@ -451,147 +634,177 @@ struct TurnParams {
   uint16_t *at, *bt;  // [R][n_in][rank], [R][rank][n_out]
   int32_t rank, n_in, n_out, adapters, a_tiles, b_tiles;  // tiles of 64 columns an adapter
 };
-// 64 positions of the wide side and all ranks a work group.
+// 64 positions of the wide side and all ranks a work group, 16 bytes a load and a store.
 __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
-  __shared__ uint16_t tile[DAN_ADAPT_MAX_RANK][64 + 2];
+  __shared__ __attribute__((aligned(16))) uint16_t tile[DAN_ADAPT_MAX_RANK][64 + 8];
   int x = blockIdx.x;
   const bool b = x >= p.a_tiles * p.adapters;
   if (b) x -= p.a_tiles * p.adapters;
-  const int tiles = b ? p.b_tiles : p.a_tiles, i = x / tiles, c0 = x % tiles * 64, wide = b ? p.n_out : p.n_in;
+  const int tiles = b ? p.b_tiles : p.a_tiles, i = x / tiles, c0 = x % tiles * 64, wide = b ? p.n_out : p.n_in, r8 = p.rank / 8;
   const int64_t base = (int64_t)i * p.rank * wide;
-  const int cols = min(64, wide - c0);
-  for (int e = threadIdx.x; e < 64 * p.rank; e += kThreads) {  // A: columns contiguous; B: ranks
-    const int j = b ? e % p.rank : e / 64, c = b ? e / p.rank : e % 64;
-    if (c < cols) tile[j][c] = b ? p.b[base + (int64_t)(c0 + c) * p.rank + j] : p.a[base + (int64_t)j * wide + c0 + c];
+  const uint16_t *from = (b ? p.b : p.a) + base;
+  uint16_t *to = (b ? p.bt : p.at) + base;
+  const int c8 = min(64, wide - c0) / 8;  // pieces of 8 columns
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  for (int e = threadIdx.x; e < 64 * r8; e += kThreads) {
+    if (b) {  // a column's ranks are contiguous
+      const int c = e / r8, j = 8 * (e % r8);
+      const u16x8 v = __builtin_bit_cast(u16x8, load16(from + (int64_t)(c0 + min(c, 8 * c8 - 1)) * p.rank + j));
+#pragma unroll
+      for (int y = 0; y < 8; ++y) tile[j + y][c] = v[y];
+    } else {  // a rank's columns are
+      const int j = e / 8, c = 8 * (e % 8);
+      *reinterpret_cast<u32x4 *>(&tile[j][c]) = load16(from + (int64_t)j * wide + c0 + min(c, 8 * c8 - 8));
+    }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 64 * p.rank; e += kThreads) {
-    const int j = b ? e / 64 : e % p.rank, c = b ? e % 64 : e / p.rank;
-    if (c >= cols) continue;
-    if (b) p.bt[base + (int64_t)j * wide + c0 + c] = tile[j][c];
-    else p.at[base + (int64_t)(c0 + c) * p.rank + j] = tile[j][c];
+  for (int e = threadIdx.x; e < 64 * r8; e += kThreads) {
+    if (b) {
+      const int j = e / 8, c = e % 8;
+      if (c < c8) store16(to + (int64_t)j * wide + c0 + 8 * c, *reinterpret_cast<const u32x4 *>(&tile[j][8 * c]));
+    } else {
+      const int c = e / r8, j = 8 * (e % r8);
+      u16x8 v;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) v[y] = tile[j + y][c];
+      if (c < 8 * c8) store16(to + (int64_t)(c0 + c) * p.rank + j, __builtin_bit_cast(u32x4, v));
+    }
   }
 }
 
 // ---------------------------------------------------------------- host
 // Ranks as the kernels are built for: 16, 32, 64 or 128.
-int rank16(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
-int down_frags(int rows) { return rows > 512 ? 2 : 1; }
+int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
-// Parts of `down`'s sum: as many work groups as fill the chip a few times over, at least one chunk a wave.
-int splits_of(int rows, int n) {
-  const int tiles = (rows + 16 * down_frags(rows) - 1) / (16 * down_frags(rows)), chunks = (n + kChunk - 1) / kChunk;
-  return std::max(1, std::min({(1024 + tiles - 1) / tiles, (chunks + 3) / 4, 16}));
+// Parts of `down`'s sum over n: as many work groups as fill the chip, of at least a chunk a wave (many rows) or two.
+int splits_of(int rows, int n, int rank) {
+  const int chunks = (n + kChunk - 1) / kChunk;
+  if (rows <= kFewRows) return std::max(1, std::min({chunks, std::max(2, 1024 / ((rows + 15) / 16)), 32}));
+  const int tiles = (rows + 31) / 32, waves = ranks_of(rank) <= 32 ? 16 : 8;
+  return std::max(1, std::min((256 + tiles - 1) / tiles, chunks / waves));
 }
-// Parts of `outer`'s rows.
+// Parts of an adapter's rows in `outer`: enough work groups for the chip, but parts are written and read again in fp32.
 int parts_of(int rows, int n_in, int n_out, int adapters) {
   const int64_t groups = (int64_t)((n_in + kOuterCols - 1) / kOuterCols + (n_out + kOuterCols - 1) / kOuterCols) * adapters;
-  const int by_rows = (rows + 4 * kOuterRows - 1) / (4 * kOuterRows);
-  return (int)std::max<int64_t>({1, std::min<int64_t>({(2048 + groups - 1) / groups, by_rows, 16}), (rows + 8191) / 8192});
+  const int64_t by_rows = rows / (512 * (int64_t)adapters);
+  return (int)std::max<int64_t>({1, std::min<int64_t>((1024 + groups - 1) / groups, by_rows), (rows + 16383) / 16384});
 }
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 template <typename T, int JB>
 hipError_t launch_down(const DownParams &p, int splits, hipStream_t s) {
-  const int f = down_frags(p.rows);
-  const dim3 grid((p.rows + 16 * f - 1) / (16 * f), splits);
-  if (f == 2) hipLaunchKernelGGL((down_kernel<T, JB, 2>), grid, dim3(kThreads), 0, s, p);
-  else hipLaunchKernelGGL((down_kernel<T, JB, 1>), grid, dim3(kThreads), 0, s, p);
+  if (p.rows <= kFewRows) {
+    hipLaunchKernelGGL((down_few_kernel<T, JB>), dim3((p.rows + 15) / 16, splits), dim3(64 * kFewWaves), 0, s, p);
+    return hipGetLastError();
+  }
+  constexpr int W = kDownWaves<JB>, bytes = W / 2 * JB * 2 * 1024;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(down_kernel<T, JB>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((down_kernel<T, JB>), dim3((p.rows + 31) / 32, splits), dim3(64 * W), bytes, s, p);
   return hipGetLastError();
 }
 template <typename T>
 hipError_t launch_down(DownParams p, int splits, hipStream_t s) {
   const int chunks = (p.n + kChunk - 1) / kChunk;
   p.chunks = (chunks + splits - 1) / splits;
-  const int jb = p.rank16 / 16;
-  return jb <= 1 ? launch_down<T, 1>(p, splits, s) : jb <= 2 ? launch_down<T, 2>(p, splits, s) : jb <= 4 ? launch_down<T, 4>(p, splits, s) : launch_down<T, 8>(p, splits, s);
+  return p.ranks == 16 ? launch_down<T, 1>(p, splits, s) : p.ranks == 32 ? launch_down<T, 2>(p, splits, s)
+       : p.ranks == 64 ? launch_down<T, 4>(p, splits, s) : launch_down<T, 8>(p, splits, s);
 }
 
 template <typename T, int ST>
-hipError_t launch_up(const UpParams &p, hipStream_t s) {
-  const int cols = (p.cols + kUpCols - 1) / kUpCols;
-  if (p.rows > 512) hipLaunchKernelGGL((up_kernel<T, ST, 4>), dim3(cols, (p.rows + 63) / 64), dim3(kThreads), 0, s, p);
-  else hipLaunchKernelGGL((up_kernel<T, ST, 1>), dim3(cols, (p.rows + 15) / 16), dim3(kThreads), 0, s, p);
+hipError_t launch_up(UpParams p, hipStream_t s) {
+  if (p.rows <= kFewRows) {
+    hipLaunchKernelGGL((up_few_kernel<T, ST>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
+    return hipGetLastError();
+  }
+  const int tiles = (p.rows + 16 * kUpFrags<ST> - 1) / (16 * kUpFrags<ST>), cols = std::max(1, (p.cols + 4 * kUpCols - 1) / (4 * kUpCols));
+  p.steps = std::max(1, std::min(4, (int)((int64_t)tiles * cols / 768)));
+  hipLaunchKernelGGL((up_kernel<T, ST>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
   return hipGetLastError();
 }
 template <typename T>
 hipError_t launch_up(const UpParams &p, hipStream_t s) {
-  const int steps = (p.rank / 8 + 1) / 2;
-  return steps <= 1 ? launch_up<T, 1>(p, s) : steps <= 2 ? launch_up<T, 2>(p, s) : steps <= 4 ? launch_up<T, 4>(p, s) : launch_up<T, 8>(p, s);
+  return p.ranks == 16 ? launch_up<T, 1>(p, s) : p.ranks == 32 ? launch_up<T, 2>(p, s) : p.ranks == 64 ? launch_up<T, 4>(p, s) : launch_up<T, 8>(p, s);
 }
 
+// A part's list of rows in LDS, behind the tiles (16384 rows at most: parts_of).
+int list_bytes(int rows, int parts) { return ((rows + parts - 1) / parts + 1) * 4; }
 template <typename T, int JB>
-hipError_t launch_outer(const OuterParams &p, int parts, hipStream_t s) {
-  const int bytes = std::max(4 * Tile<kOuterCols>::bytes + p.part_rows * 4, 4 * (kOuterCols / 32) * 64 * 16);
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(outer_kernel<T, JB>), hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+hipError_t launch_outer(const OuterParams &p, hipStream_t s) {
+  const int bytes = 4 * Tile<kOuterCols>::bytes + list_bytes(p.rows, p.parts);
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(outer_kernel<T, JB>), hipFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024);
   if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL((outer_kernel<T, JB>), dim3(p.a.tiles + p.b.tiles, p.adapters, parts), dim3(kThreads), bytes, s, p);
+  hipLaunchKernelGGL((outer_kernel<T, JB>), dim3(p.a.tiles + p.b.tiles, p.adapters, p.parts), dim3(kThreads), bytes, s, p);
   return hipGetLastError();
 }
 template <typename T>
-hipError_t launch_outer(const OuterParams &p, int parts, hipStream_t s) {
-  const int jb = p.rank16 / 16;
-  return jb <= 1 ? launch_outer<T, 1>(p, parts, s) : jb <= 2 ? launch_outer<T, 2>(p, parts, s) : jb <= 4 ? launch_outer<T, 4>(p, parts, s) : launch_outer<T, 8>(p, parts, s);
+hipError_t launch_outer(const OuterParams &p, hipStream_t s) {
+  return p.ranks == 16 ? launch_outer<T, 1>(p, s) : p.ranks == 32 ? launch_outer<T, 2>(p, s) : p.ranks == 64 ? launch_outer<T, 4>(p, s) : launch_outer<T, 8>(p, s);
 }
 
 template <typename T>
 hipError_t forward(const DanAdaptArgs &a, hipStream_t s) {
   DownParams d;
-  d.x = a.x; d.x_stride = a.x_stride; d.w = a.a; d.index = a.index; d.part = a.down;
-  d.rows = a.rows; d.n = a.n_in; d.rank = a.rank; d.adapters = a.adapters; d.rank16 = rank16(a.rank);
-  hipError_t err = launch_down<T>(d, a.splits, s);
+  d.x = a.x; d.x_stride = a.x_stride; d.w = a.a; d.index = a.index; d.part = static_cast<float *>(a.workspace);
+  d.rows = a.rows; d.n = a.n_in; d.rank = a.rank; d.adapters = a.adapters; d.ranks = ranks_of(a.rank);
+  const int splits = splits_of(a.rows, a.n_in, a.rank);
+  hipError_t err = launch_down<T>(d, splits, s);
   if (err != hipSuccess) return err;
   UpParams u;
-  u.part = a.down; u.w = a.b; u.y = a.y; u.y_stride = a.y_stride; u.out = a.out; u.o_stride = a.out_stride; u.index = a.index; u.scale = a.scale;
-  u.rows = a.rows; u.cols = a.n_out; u.rank = a.rank; u.adapters = a.adapters; u.rank16 = rank16(a.rank); u.splits = a.splits; u.scale_value = a.scale_value;
+  u.part = d.part; u.sum = a.down; u.w = a.b; u.y = a.y; u.y_stride = a.y_stride; u.out = a.out; u.o_stride = a.out_stride;
+  u.index = a.index; u.scale = a.scale; u.scale_value = a.scale_value;
+  u.rows = a.rows; u.cols = a.n_out; u.rank = a.rank; u.adapters = a.adapters; u.ranks = d.ranks; u.splits = splits; u.steps = 1;
   return launch_up<T>(u, s);
 }
 
-// The workspace of the gradient: A^T, B^T, g's parts, and the parts of dA and dB.
+// The workspace of the gradient: A^T, B^T, g in parts and added up, and the parts of dA and dB.
 struct GradSpace {
-  int64_t at, bt, down, da, db, total;
+  int64_t at, bt, part, g, da, db, total;
   int splits, parts;
   GradSpace(int rows, int n_in, int n_out, int rank, int adapters) {
-    splits = splits_of(rows, n_out);
+    splits = splits_of(rows, n_out, rank);
     parts = parts_of(rows, n_in, n_out, adapters);
     at = 0;
     bt = align256(at + (int64_t)adapters * rank * n_in * 2);
-    down = align256(bt + (int64_t)adapters * rank * n_out * 2);
-    da = align256(down + (int64_t)splits * rows * rank16(rank) * 4);
-    db = align256(da + (int64_t)parts * adapters * rank * n_in * 4);
-    total = align256(db + (int64_t)parts * adapters * rank * n_out * 4);
+    part = align256(bt + (int64_t)adapters * rank * n_out * 2);
+    g = align256(part + (int64_t)splits * rows * ranks_of(rank) * 4);
+    da = align256(g + (int64_t)rows * ranks_of(rank) * 4);
+    const int64_t kept = parts > 1 ? parts : 0;
+    db = align256(da + kept * adapters * rank * n_in * 4);
+    total = align256(db + kept * adapters * rank * n_out * 4);
   }
 };
 
 template <typename T>
 hipError_t backward(const DanAdaptGradArgs &a, const GradSpace &w, hipStream_t s) {
   uint8_t *ws = static_cast<uint8_t *>(a.workspace);
-  TurnParams t;
-  t.a = static_cast<const uint16_t *>(a.a); t.b = static_cast<const uint16_t *>(a.b);
-  t.at = reinterpret_cast<uint16_t *>(ws + w.at); t.bt = reinterpret_cast<uint16_t *>(ws + w.bt);
-  t.rank = a.rank; t.n_in = a.n_in; t.n_out = a.n_out; t.adapters = a.adapters;
-  t.a_tiles = a.dx ? (a.n_in + 63) / 64 : 0;
-  t.b_tiles = (a.n_out + 63) / 64;
-  hipLaunchKernelGGL(turn_kernel, dim3((t.a_tiles + t.b_tiles) * a.adapters), dim3(kThreads), 0, s, t);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  DownParams d;
-  d.x = a.g; d.x_stride = a.g_stride; d.w = t.bt; d.index = a.index; d.part = reinterpret_cast<float *>(ws + w.down);
-  d.rows = a.rows; d.n = a.n_out; d.rank = a.rank; d.adapters = a.adapters; d.rank16 = rank16(a.rank);
-  if ((err = launch_down<T>(d, w.splits, s)) != hipSuccess) return err;
-  if (a.dx) {
-    UpParams u;
-    u.part = d.part; u.w = t.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride; u.index = a.index; u.scale = a.scale;
-    u.rows = a.rows; u.cols = a.n_in; u.rank = a.rank; u.adapters = a.adapters; u.rank16 = d.rank16; u.splits = w.splits; u.scale_value = a.scale_value;
+  OuterParams o;
+  o.a = {reinterpret_cast<float *>(ws + w.g), a.x, a.x_stride, reinterpret_cast<float *>(ws + w.da), a.da, a.n_in, a.da ? (a.n_in + kOuterCols - 1) / kOuterCols : 0};
+  o.b = {a.down, a.g, a.g_stride, reinterpret_cast<float *>(ws + w.db), a.db, a.n_out, a.db ? (a.n_out + kOuterCols - 1) / kOuterCols : 0};
+  o.index = a.index; o.scale = a.scale; o.scale_value = a.scale_value; o.rows = a.rows; o.rank = a.rank; o.ranks = ranks_of(a.rank);
+  o.adapters = a.adapters; o.parts = w.parts;
+  hipError_t err;
+  if (a.dx || a.da) {
+    TurnParams t;
+    t.a = static_cast<const uint16_t *>(a.a); t.b = static_cast<const uint16_t *>(a.b);
+    t.at = reinterpret_cast<uint16_t *>(ws + w.at); t.bt = reinterpret_cast<uint16_t *>(ws + w.bt);
+    t.rank = a.rank; t.n_in = a.n_in; t.n_out = a.n_out; t.adapters = a.adapters;
+    t.a_tiles = a.dx ? (a.n_in + 63) / 64 : 0;
+    t.b_tiles = (a.n_out + 63) / 64;
+    hipLaunchKernelGGL(turn_kernel, dim3((t.a_tiles + t.b_tiles) * a.adapters), dim3(kThreads), 0, s, t);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    DownParams d;
+    d.x = a.g; d.x_stride = a.g_stride; d.w = t.bt; d.index = a.index; d.part = reinterpret_cast<float *>(ws + w.part);
+    d.rows = a.rows; d.n = a.n_out; d.rank = a.rank; d.adapters = a.adapters; d.ranks = o.ranks;
+    if ((err = launch_down<T>(d, w.splits, s)) != hipSuccess) return err;
+    UpParams u;  // (without dx: no columns, the sum of the parts alone)
+    u.part = d.part; u.sum = reinterpret_cast<float *>(ws + w.g); u.w = t.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride;
+    u.index = a.index; u.scale = a.scale; u.scale_value = a.scale_value;
+    u.rows = a.rows; u.cols = a.dx ? a.n_in : 0; u.rank = a.rank; u.adapters = a.adapters; u.ranks = o.ranks; u.splits = w.splits; u.steps = 1;
     if ((err = launch_up<T>(u, s)) != hipSuccess) return err;
   }
   if (!a.da && !a.db) return hipSuccess;
-  OuterParams o;
-  o.a = {d.part, a.x, a.x_stride, reinterpret_cast<float *>(ws + w.da), a.n_in, w.splits, a.da ? (a.n_in + kOuterCols - 1) / kOuterCols : 0};
-  o.b = {a.down, a.g, a.g_stride, reinterpret_cast<float *>(ws + w.db), a.n_out, a.splits, a.db ? (a.n_out + kOuterCols - 1) / kOuterCols : 0};
-  o.index = a.index; o.scale = a.scale; o.rows = a.rows; o.rank = a.rank; o.rank16 = d.rank16; o.adapters = a.adapters;
-  o.part_rows = (a.rows + w.parts - 1) / w.parts; o.scale_value = a.scale_value;
-  if ((err = launch_outer<T>(o, w.parts, s)) != hipSuccess) return err;
+  if ((err = launch_outer<T>(o, s)) != hipSuccess || w.parts == 1) return err;
   SumParams m;
   m.a = o.a.sums; m.b = o.b.sums; m.da = a.da; m.db = a.db; m.parts = w.parts;
   m.na = a.da ? (int64_t)a.adapters * a.rank * a.n_in : 0;
@@ -612,9 +825,10 @@ int check_sizes(int dtype, int rows, int n_in, int n_out, int rank, int adapters
   if (rank <= 0 || rank % 8 || rank > DAN_ADAPT_MAX_RANK) return fail(DAN_ERR_UNSUPPORTED, "rank %d: a multiple of 8 up to %d", rank, DAN_ADAPT_MAX_RANK);
   if (adapters <= 0 || adapters > 65535) return fail(DAN_ERR_UNSUPPORTED, "%d adapters: 1 to 65535", adapters);
   if (!(isfinite(scale_value))) return fail(DAN_ERR_INVALID_ARGUMENT, "scale_value must be finite");
-  const int64_t wide = std::max(n_in, n_out), f = rows > 512 ? 64 : 16;
-  if (too_many(over(wide, kUpCols) * over(rows, f)) || too_many(over(rows, 16) * splits_of(rows, (int)wide)) ||
-      too_many((over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters * std::max(2, parts_of(rows, n_in, n_out, adapters))) ||
+  const int64_t wide = std::max(n_in, n_out);  // (`up` has the most threads by far: 2 columns of 16 rows each for few rows)
+  if (too_many(over(wide, kUpCols) * over(rows, 16) * 2) ||
+      too_many((over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters * parts_of(rows, n_in, n_out, adapters)) ||
+      too_many((over(n_in, 64) + over(n_out, 64)) * adapters) ||
       too_many(over((int64_t)adapters * rank * ((int64_t)n_in + n_out), 8 * kThreads)))
     return fail(DAN_ERR_UNSUPPORTED, "%d rows, %d to %d, %d adapters: more than one launch holds", rows, n_in, n_out, adapters);
   return DAN_OK;
@@ -628,7 +842,10 @@ extern "C" {
 
 int dan_adapt_abi_version(void) { return DAN_ADAPT_ABI_VERSION; }
 
-int32_t dan_adapt_splits(int32_t rows, int32_t n) { return rows <= 0 || n <= 0 ? 1 : dan::splits_of(rows, n); }
+int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank) {
+  if (rows <= 0 || n_in <= 0 || rank <= 0 || rank > DAN_ADAPT_MAX_RANK) return 0;
+  return (int64_t)dan::splits_of(rows, n_in, rank) * rows * dan::ranks_of(rank) * 4;
+}
 
 int64_t dan_adapt_grad_workspace_size(int32_t rows, int32_t n_in, int32_t n_out, int32_t rank, int32_t adapters) {
   using namespace dan;
@@ -643,12 +860,14 @@ int dan_adapt(const DanAdaptArgs *a, void *stream) {
   if (a->abi_version != DAN_ADAPT_ABI_VERSION)
     return fail(DAN_ERR_VERSION, "abi_version %d, library speaks %d", a->abi_version, DAN_ADAPT_ABI_VERSION);
   if (const int rc = check_sizes(a->dtype, a->rows, a->n_in, a->n_out, a->rank, a->adapters, a->scale_value)) return rc;
-  if (a->splits != dan_adapt_splits(a->rows, a->n_in)) return fail(DAN_ERR_INVALID_ARGUMENT, "splits %d: dan_adapt_splits", a->splits);
   if (a->rows == 0) return DAN_OK;
-  if (!a->x || !a->y || !a->a || !a->b || !a->out || !a->down) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL pointer");
+  if (!a->x || !a->y || !a->a || !a->b || !a->out) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL pointer");
   if (bad_rows(a->x, a->x_stride) || bad_rows(a->y, a->y_stride) || bad_rows(a->out, a->out_stride) || (a->rows > 1 && a->out_stride < a->n_out) ||
       (((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->down) & 15))
     return fail(DAN_ERR_INVALID_ARGUMENT, "rows must start 16-byte aligned, and written ones must not overlap");
+  const int64_t need = dan_adapt_workspace_size(a->rows, a->n_in, a->rank);
+  if (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & 15))
+    return fail(DAN_ERR_INVALID_ARGUMENT, "workspace needs %lld bytes, 16-byte aligned", (long long)need);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t err = a->dtype == DAN_DTYPE_BF16 ? forward<__bf16>(*a, s) : forward<_Float16>(*a, s);
   if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "adapter launch failed: %s", hipGetErrorString(err));
@@ -662,7 +881,6 @@ int dan_adapt_grad(const DanAdaptGradArgs *a, void *stream) {
   if (a->abi_version != DAN_ADAPT_ABI_VERSION)
     return fail(DAN_ERR_VERSION, "abi_version %d, library speaks %d", a->abi_version, DAN_ADAPT_ABI_VERSION);
   if (const int rc = check_sizes(a->dtype, a->rows, a->n_in, a->n_out, a->rank, a->adapters, a->scale_value)) return rc;
-  if (a->splits != dan_adapt_splits(a->rows, a->n_in)) return fail(DAN_ERR_INVALID_ARGUMENT, "splits %d: dan_adapt_splits", a->splits);
   if (a->rows == 0) return DAN_OK;
   if (!a->x || !a->g || !a->a || !a->b || !a->down) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL pointer");
   if (bad_rows(a->x, a->x_stride) || bad_rows(a->g, a->g_stride) || bad_rows(a->dx, a->dx ? a->dx_stride : 0) ||
@@ -673,9 +891,8 @@ int dan_adapt_grad(const DanAdaptGradArgs *a, void *stream) {
   if (!a->workspace || a->workspace_bytes < w.total || ((uintptr_t)a->workspace & 255))
     return fail(DAN_ERR_INVALID_ARGUMENT, "workspace needs %lld bytes, 256-byte aligned", (long long)w.total);
   // `outer` keeps a row's offset from its part's first one in 32 bits.
-  const int64_t part_rows = (a->rows + w.parts - 1) / w.parts;
-  if (part_rows * a->x_stride * 2 >= int64_t(1) << 32 || part_rows * a->g_stride * 2 >= int64_t(1) << 32)
-    return fail(DAN_ERR_UNSUPPORTED, "row strides %lld and %lld are too large", (long long)a->x_stride, (long long)a->g_stride);
+  if ((int64_t)a->rows * a->x_stride * 2 >= int64_t(1) << 32 || (int64_t)a->rows * a->g_stride * 2 >= int64_t(1) << 32)
+    return fail(DAN_ERR_UNSUPPORTED, "x and g of %d rows: fewer than 2^32 bytes from the first to the last", a->rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t err = a->dtype == DAN_DTYPE_BF16 ? backward<__bf16>(*a, w, s) : backward<_Float16>(*a, w, s);
   if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "adapter gradient launch failed: %s", hipGetErrorString(err));

@@ -11,24 +11,11 @@
 // call, Python alone / through here, us: append 12.3 / 5.8, attend in one launch 10.0 / 5.1,
 // log probabilities 14.7 / 9.8, with their gradient 98 / 62 (of which torch's engine takes 39 for
 // any gradient; in C++ the backward needs no hand-over of the interpreter's lock to its thread).
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/utils/object_ptr.h>
-
-#include <ATen/ATen.h>
-#include <ATen/TensorSubclassLikeUtils.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-
+#include "calls.h"
 #include "dan_paged.h"
 #include "dan_readout.h"
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::variable_list;
 
 // The library's entry points (bind).
 struct Library {
@@ -40,42 +27,6 @@ struct Library {
   int64_t (*logprobs_bytes)(int32_t, int32_t, int32_t, int32_t);
   const char *(*last_error)(void);
 } lib;
-
-int code_of(at::ScalarType t) {  // DanDtype, or -1
-  switch (t) {
-    case at::kBFloat16: return DAN_DTYPE_BF16;
-    case at::kHalf: return DAN_DTYPE_F16;
-    case at::kFloat: return DAN_DTYPE_F32;
-    case at::kFloat8_e4m3fn: return DAN_DTYPE_E4M3;
-    default: return -1;
-  }
-}
-bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
-
-void check(int rc, const char *name) {
-  TORCH_CHECK_WITH(Error, rc == DAN_OK, name, " failed (status ", rc, "): ", lib.last_error());
-}
-
-// A plain tensor on device `index`: nothing wraps it, and it carries no tangent.
-bool plain(const Tensor &t, int index) {
-  return t.defined() && t.is_cuda() && t.get_device() == index && t.layout() == at::kStrided && !at::isTensorSubclassLike(t) &&
-         !t.is_neg() && !t._is_zerotensor() && !t._fw_grad(0).defined();
-}
-bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
-void *at_of(const Tensor &t) { return t.defined() ? const_cast<void *>(t.const_data_ptr()) : nullptr; }  // read, or new
-
-// Rows that the kernels read in place: unit stride, 16-byte aligned.
-bool rows_ok(const Tensor &t) {
-  const int64_t es = t.element_size(), n = t.dim();
-  if (t.stride(n - 1) != 1 || !aligned(t.const_data_ptr())) return false;
-  for (int64_t i = 0; i + 1 < n; ++i)
-    if (t.stride(i) * es % 16) return false;
-  return true;
-}
-bool index_ok(const Tensor &t, int64_t n, int index) {
-  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && (n <= 1 || t.stride(0) == 1) && plain(t, index);
-}
-bool fits(int64_t x) { return x >= 0 && x <= INT32_MAX; }
 
 // The cache, table and scales of both calls.
 bool cache_ok(const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, const Tensor &table, at::ScalarType dtype, int index) {
@@ -90,20 +41,6 @@ bool cache_ok(const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor
   for (const Tensor *t : {&ks, &vs})
     if (!t->defined() || t->numel() != 1 || t->scalar_type() != at::kFloat || !plain(*t, index)) return false;
   return true;
-}
-
-// A Python argument as a tensor: undefined for None; false for anything else.
-bool tensor_of(PyObject *o, Tensor &t) {
-  if (o == Py_None) return true;
-  if (!THPVariable_Check(o)) return false;
-  t = THPVariable_Unpack(o);
-  return true;
-}
-bool grads_of(std::initializer_list<const Tensor *> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor *t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
 }
 
 // append(q, k, v, cos, sin, k_cache, v_cache, table, places, seqs, rope_rows, q_norm_weight, k_norm_weight, eps, norm, k_scale, v_scale):
@@ -183,7 +120,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   a.places = static_cast<const int32_t *>(at_of(places));
   a.seqs = static_cast<const int32_t *>(at_of(seqs));
   a.rope_rows = static_cast<const int32_t *>(at_of(rope));
-  check(lib.append(&a, c10::hip::getCurrentHIPStream(index).stream()), "dan_paged_append");
+  check(lib.append(&a, c10::hip::getCurrentHIPStream(index).stream()), "dan_paged_append", lib.last_error);
   for (const Tensor *t : {&kc, &vc})  // a backward that has saved a cache must not take the new rows for the old
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(out);
@@ -244,7 +181,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   a.table = static_cast<const int32_t *>(at_of(table)); a.table_stride = table.stride(0);
   a.lens = static_cast<const int32_t *>(at_of(lens));
   a.workspace = at_of(ws); a.workspace_bytes = need > 0 ? need : 0;
-  check(lib.attn(&a, c10::hip::getCurrentHIPStream(index).stream()), "dan_paged_attn");
+  check(lib.attn(&a, c10::hip::getCurrentHIPStream(index).stream()), "dan_paged_attn", lib.last_error);
   if (!want) return THPVariable_Wrap(out);
   THPObjectPtr x(THPVariable_Wrap(out)), y(THPVariable_Wrap(lse));
   return x && y ? PyTuple_Pack(2, x.get(), y.get()) : nullptr;
@@ -287,35 +224,10 @@ Outputs logprobs_forward(const Tensor &x, const Tensor &tokens, int64_t top, boo
   a.top_ids = static_cast<int64_t *>(at_of(o.top_ids));
   a.workspace = at_of(ws); a.workspace_bytes = need;
   a.logsumexp_rest = static_cast<float *>(at_of(o.rest));
-  check(lib.logprobs(&a, c10::hip::getCurrentHIPStream(x.get_device()).stream()), "dan_logprobs_fwd");
+  check(lib.logprobs(&a, c10::hip::getCurrentHIPStream(x.get_device()).stream()), "dan_logprobs_fwd", lib.last_error);
   return o;
 }
 
-// A backward in a stream capture whose result goes to a node that lives on a stream outside of it, as the
-// accumulator of a leaf does while an eager graph of the same leaf is alive: the engine would make that
-// stream wait for the capture, which ends the process where it is the default one.
-bool leaves_capture(int index) {
-  const auto node = torch::autograd::get_current_node();
-  if (!node) return false;
-  const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(index);
-  auto captures = [](hipStream_t s) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    return s && hipStreamIsCapturing(s, &status) == hipSuccess && status != hipStreamCaptureStatusNone;  // never the default one
-  };
-  for (const auto &edge : node->next_edges()) {
-    if (!edge.function) continue;
-    const auto to = edge.function->stream();
-    if (!to || to->device_index() != index || to->id() == here.id()) continue;
-    const c10::hip::HIPStream there(c10::Stream(c10::Stream::UNSAFE, here.unwrap().device(), to->id()));
-    if (captures(here.stream()) && !captures(there.stream())) return true;
-  }
-  return false;
-}
-
-void check_capture(int index, const char *name = "token_logprobs") {
-  TORCH_CHECK(!leaves_capture(index), name, ": a captured backward whose inputs were first used outside of the capture; "
-              "drop every earlier result that holds their graph before the capture");
-}
 // check_capture(device index, name), for a backward that runs in Python
 PyObject *py_check_capture(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -387,13 +299,9 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
       a.grad = at_of(grad); a.grad_stride = vocab;
       a.logsumexp_rest = static_cast<const float *>(at_of(saved[5]));
       // (the engine has made the gradients' device the thread's)
-      check(lib.grad(&a, c10::hip::getCurrentHIPStream(x.get_device()).stream()), "dan_logprobs_bwd");
+      check(lib.grad(&a, c10::hip::getCurrentHIPStream(x.get_device()).stream()), "dan_logprobs_bwd", lib.last_error);
     }
-    if (again) {  // a second derivative is an error where it is taken, not before
-      torch::autograd::DelayedError twice("token_logprobs is differentiable once", 1);
-      grad = twice.apply({grad.set_requires_grad(true)})[0];
-    }
-    return {grad, Tensor(), Tensor(), Tensor()};
+    return {differentiable_once(grad, again, "token_logprobs is differentiable once"), Tensor(), Tensor(), Tensor()};
   }
 };
 

@@ -115,6 +115,11 @@ def add_norm(x, residual, weight, *, eps=1e-6, norm="rms", fp8=None, out=None):
     captured into a HIP graph has its forward pass in the same capture, and no
     earlier, eager result that holds the graph of the same leaves is alive (where an
     input is such a leaf itself, that raises)."""
+    want_out = fp8 is None if out is None else bool(out)
+    made = _layer.calls().add_norm(x, residual, weight, eps, NORMS.get(norm), -1 if fp8 is None else LAYOUTS.get(fp8), want_out)
+    if made is not None:  # a plain call
+        out, stream, codes, scale = made
+        return Normed(out, x if residual is None else stream, TiledE4M3(codes, *x.shape) if fp8 == "tiled" else codes, scale)
     if not x.is_cuda:
         raise RuntimeError(f"dan_amd.add_norm runs on a gfx950 GPU only; got tensors on {x.device}")
     if x.device.index != torch._C._cuda_getDevice():
@@ -137,7 +142,6 @@ def add_norm(x, residual, weight, *, eps=1e-6, norm="rms", fp8=None, out=None):
         raise ValueError(f"weight must be [{k}] {x.dtype} on {x.device}; got {tuple(weight.shape)} {weight.dtype} on {weight.device}")
     if not 0 <= float(eps) < float("inf"):
         raise ValueError(f"eps {eps}: finite and not negative")
-    want_out = fp8 is None if out is None else bool(out)
     if fp8 is None and not want_out:
         raise ValueError("out=False without fp8: nothing is left to compute")
     inputs = [t for t in (x, residual, weight) if t is not None]

@@ -251,6 +251,7 @@ class TilePlan:
     past_uploaded: set = field(default_factory=set)  # the layers whose device table was filled by an upload
     past_filled: dict = field(default_factory=dict)  # layer -> (stream, table) of a launch with a caller's workspace that filled it
     grad_tables: dict = field(default_factory=dict)  # (heads, kv heads, head_dim) -> the backward pass's tables
+    train_calls: dict = field(default_factory=dict)  # (layer, heads, kv heads, head_dim, dtype, scale) -> what a training call of it takes
     schedules: dict = field(default_factory=dict)  # (groups, CUs) -> (units_d, sched_off_d, slots)
     tiles: dict = field(default_factory=dict)  # (heads, kv heads, head_dim) -> queries per work item that a call of this layout takes
 

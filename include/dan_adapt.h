@@ -30,7 +30,7 @@ typedef struct {
   int32_t abi_version; /* DAN_ADAPT_ABI_VERSION */
   int32_t dtype;       /* DAN_DTYPE_BF16 or DAN_DTYPE_F16: x, y, a, b, out */
   int32_t rows, n_in, n_out, rank, adapters;
-  int32_t splits;      /* dan_adapt_splits(rows, n_in): parts of the sum over n_in */
+  int32_t reserved;
   const void *x; int64_t x_stride;
   const void *y; int64_t y_stride;
   const void *a;          /* [adapters][rank][n_in] */
@@ -39,14 +39,15 @@ typedef struct {
   const float *scale;     /* [adapters]; NULL: scale_value for every adapter */
   float scale_value;
   void *out; int64_t out_stride; /* may be y itself */
-  float *down; /* [splits][rows][rank rounded up to 16, 32, 64 or 128]: x A^T, in parts; the gradient reads it again */
+  float *down; /* [rows][rank rounded up to 16, 32, 64 or 128]: x A^T, for the gradient; NULL: not wanted */
+  void *workspace; int64_t workspace_bytes; /* dan_adapt_workspace_size() bytes, 16-byte aligned */
 } DanAdaptArgs;
 
 typedef struct {
   int32_t abi_version;
   int32_t dtype;
   int32_t rows, n_in, n_out, rank, adapters;
-  int32_t splits;      /* as in the forward call */
+  int32_t reserved;
   const void *x; int64_t x_stride;
   const void *g; int64_t g_stride; /* the gradient of out (which is that of y, too) */
   const void *a, *b;
@@ -60,8 +61,8 @@ typedef struct {
 } DanAdaptGradArgs;
 
 int dan_adapt_abi_version(void);
-int32_t dan_adapt_splits(int32_t rows, int32_t n);
 /* 0: invalid arguments. */
+int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank);
 int64_t dan_adapt_grad_workspace_size(int32_t rows, int32_t n_in, int32_t n_out, int32_t rank, int32_t adapters);
 int dan_adapt(const DanAdaptArgs *args, void *stream);
 int dan_adapt_grad(const DanAdaptGradArgs *args, void *stream);
