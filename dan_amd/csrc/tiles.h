@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 namespace dan {
 namespace tiles {
@@ -33,6 +34,17 @@ __device__ inline void store16(T *p, u32x4 x) {
 }
 __device__ inline u32x4 lds_read16(uint32_t at) { return *(const DAN_TILE_LDS u32x4 *)(uintptr_t)at; }
 
+// f(integral_constant 0), .. f(integral_constant N - 1): a loop that is always laid out in full, with indices that
+// are constants, so that what they index stays in registers.
+template <int... I, typename F>
+__device__ __attribute__((always_inline)) inline void for_each(std::integer_sequence<int, I...>, F &&f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __attribute__((always_inline)) inline void static_for(F &&f) {
+  for_each(std::make_integer_sequence<int, N>{}, f);
+}
+
 // 4 or 8 fp32 values rounded to T, packed.
 template <typename T>
 __device__ inline u32x4 pack8(f32x8 x) {
@@ -59,6 +71,16 @@ __device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+
+// The same with the result in accumulation registers, for sums that live through a loop: the compiler, asked for
+// results in vector registers, would copy them there and back every time. The block waits by itself for operands that
+// an instruction before it may have written; the sum may be read by other instructions only behind settle().
+template <typename T>
+__device__ inline void mfma32_sum(f32x16 &c, u32x4 a, u32x4 b) {
+  if constexpr (std::is_same<T, __bf16>::value) asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ inline void settle(f32x16 &c) { asm volatile("s_nop 15\n\ts_nop 15" : "+a"(c)); }
 
 // s_waitcnt vmcnt(N) (expcnt and lgkmcnt left alone).
 template <int N>

@@ -49,7 +49,7 @@ struct GradParams {
   void *dq, *dk, *dv;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, g_st, g_sh, dq_st, dq_sh, dk_st, dk_sh, dv_st, dv_sh;
   const float *lse;
-  float *stats;    // [2][H][N]: bias - lse, -delta
+  float *stats;    // [2][H][N]: (bias - lse) / c, -delta
   float *partial;  // [3][partials]: max |G row|^2, max |V row|^2, max |delta|
   const DanGradKeyUnit *key_units;
   const DanGradQueryUnit *query_units;
@@ -80,6 +80,18 @@ __device__ inline float block_max(float x, float *red) {
   return x;
 }
 
+// Sum of squares over the L lanes of a row, 8 values each.
+template <typename T, int L>
+__device__ inline float row_square(u32x4 x) {
+  const f32x8 v = unpack8<T>(x);
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+#pragma unroll
+  for (int m = L / 2; m; m >>= 1) sq += __shfl_xor(sq, m);
+  return sq;
+}
+
 // ---------------------------------------------------------------- delta
 // One pass over G and O (2 x 67 MB at 8192 rows x 32 heads x 128): a row is D / 8 lanes, 16 bytes each.
 template <typename T, int D>
@@ -106,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p)
     }
     if (sub == 0) {
       const int64_t at = h * p.num_tokens + n;
-      p.stats[at] = (kHalf ? kPBias : 0.f) - p.lse[at];
+      p.stats[at] = ((kHalf ? kPBias : 0.f) - p.lse[at]) / p.c;
       p.stats[rows + at] = -dot;
     }
     gmax = fmaxf(gmax, sq);
@@ -116,13 +128,15 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p)
     const int64_t vrows = (int64_t)p.num_tokens * p.num_kv_heads;
     for (int64_t r = (int64_t)blockIdx.x * R + mine; r < vrows; r += (int64_t)gridDim.x * R) {
       const int64_t n = r / p.num_kv_heads, h = r % p.num_kv_heads;
-      const f32x8 v = unpack8<T>(load16(static_cast<const T *>(p.v) + n * p.v_st + h * p.v_sh + 8 * sub));
-      float sq = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
-#pragma unroll
-      for (int m = L / 2; m; m >>= 1) sq += __shfl_xor(sq, m);
-      vmax = fmaxf(vmax, sq);
+      vmax = fmaxf(vmax, row_square<T, L>(load16(static_cast<const T *>(p.v) + n * p.v_st + h * p.v_sh + 8 * sub)));
+    }
+    for (int i = 0; i < p.num_pasts; ++i) {
+      const DanPastDesc pd = load_unit(p.pasts + i);
+      const int64_t prows = (int64_t)pd.len * p.num_kv_heads;
+      for (int64_t r = (int64_t)blockIdx.x * R + mine; r < prows; r += (int64_t)gridDim.x * R) {
+        const int64_t n = r / p.num_kv_heads, h = r % p.num_kv_heads;
+        vmax = fmaxf(vmax, row_square<T, L>(load16(static_cast<const T *>(pd.v) + n * pd.v_stride_tok + h * pd.v_stride_head + 8 * sub)));
+      }
     }
     __shared__ float red[4];
     gmax = block_max(gmax, red);
@@ -137,8 +151,7 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p)
 }
 
 // fp16: the power of 2 that brings every |dS| under 2^15 and keeps the rest as far above fp16's smallest
-// as it goes: |dP| <= |G row| |V row|. (A prefix's V is left out of the bound of dP, and its |delta| is in:
-// a prefix key's dP may pass it by the ratio of the norms; the clamp in dS keeps the product finite.)
+// as it goes: |dP| <= |G row| |V row|.
 __device__ inline float ds_factor(const GradParams &p, float *red) {
   float g = 0.f, v = 0.f, d = 0.f;
   for (int i = threadIdx.x; i < p.partials; i += kThreads) {
@@ -170,6 +183,15 @@ __device__ inline void store_column(T *row, const f32x16 &x, float f, int hl, bo
   }
 }
 
+// 8 of a lane's 16 results, rounded and packed.
+template <typename T>
+__device__ inline u32x4 pack_part(const f32x16 &x, int first) {
+  f32x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = x[first + i];
+  return pack8<T>(y);
+}
+
 // ---------------------------------------------------------------- dK, dV
 // Four waves: KW runs of kWaveRows keys side by side, and 4 / KW of the (32 rows, head) tiles of a step. A wave
 // keeps its keys' K and V (as operands) and dK and dV (as accumulators) in registers: 384 of 512 at head_dim 128
@@ -178,9 +200,10 @@ template <int D, int KW>
 struct KeyLds {
   static constexpr int QW = 4 / KW;
   static constexpr int stage = 2 * QW * Tile<D>::bytes;
-  static constexpr int ring = 4 * (stage + 1024) <= 140 * 1024 ? 4 : 3 * (stage + 1024) <= 140 * 1024 ? 3 : 2;
-  static constexpr int stats = ring * stage;          // [ring][4 waves][64 floats]
-  static constexpr int red = stats + ring * 1024;     // 16 floats
+  static constexpr int stat_step = QW * 1024;  // [QW][4 waves][64 floats]
+  static constexpr int ring = 4 * (stage + stat_step) <= 140 * 1024 ? 4 : 3 * (stage + stat_step) <= 140 * 1024 ? 3 : 2;
+  static constexpr int stats = ring * stage;
+  static constexpr int red = stats + ring * stat_step;  // 16 floats
   static constexpr int wave = 2 * kWaveRows<D> * D * 4;  // a wave's dK and dV
   static constexpr int merge = QW > 1 ? QW / 2 * KW * wave : 0;
   static constexpr int total = red + 64 > merge ? red + 64 : merge;
@@ -193,7 +216,7 @@ void grad_keys_kernel(const GradParams p) {
   using Tl = Tile<D>;
   using Lds = KeyLds<D, KW>;
   constexpr int NS = kWaveRows<D> / 32, QW = 4 / KW, NK = D / 16, ND = D / 32, NB = Lds::ring;
-  constexpr int SL = Lds::stage / 1024 / 4, TS = Tl::blocks / 4;  // direct loads of a wave a step, and a tile
+  constexpr int TS = Tl::blocks / 4;  // direct loads of a wave a tile of Q, and of G
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
@@ -211,7 +234,7 @@ void grad_keys_kernel(const GradParams p) {
   const int wkey = un.key0 + kw * kWaveRows<D>, kend = un.key0 + un.keys;
   u32x4 kf[NS][NK], vf[NS][NK];
   int key[NS], see[NS];
-  int top = 0, low = un.n;  // the rows below `top` see some key, those below `low` (and past the last key) all
+  int low = un.n;  // the rows below it and past the last key see every key
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     key[s] = wkey + 32 * s + (lane & 31);
@@ -226,15 +249,10 @@ void grad_keys_kernel(const GradParams p) {
     }
     const int end = valid ? p.row_end[row] : 0;
     see[s] = max(end - key[s], 0);
-    top = max(top, end);
     low = min(low, end);
   }
 #pragma unroll
-  for (int m = 32; m; m >>= 1) {
-    top = max(top, __shfl_xor(top, m));
-    low = min(low, __shfl_xor(low, m));
-  }
-  top = uni(top);
+  for (int m = 32; m; m >>= 1) low = min(low, __shfl_xor(low, m));
   low = uni(low);
 
   f32x16 dk[NS][ND], dv[NS][ND];
@@ -245,111 +263,136 @@ void grad_keys_kernel(const GradParams p) {
 
   const int tiles = (un.q_end - un.key0 + 31) / 32 * p.rep, steps = (tiles + QW - 1) / QW;
   const int64_t plane = (int64_t)p.num_heads * p.num_tokens;
-  // Step i's tiles to ring buffer b: every wave issues SL + 1 loads for every step (past the last one, and for
-  // tiles past the last, the last tile's again), so that a count of them says which have landed.
-  auto issue = [&](int i, int b) __attribute__((always_inline)) {
+  // The tiles in order, a head after the other, then the next 32 rows: what the next one to load is read from.
+  const char *q_at = uniform_ptr(static_cast<const char *>(p.q) + 2 * ((int64_t)(un.start + un.key0) * p.q_st + (int64_t)kvh * p.rep * p.q_sh));
+  const char *g_at = uniform_ptr(static_cast<const char *>(p.g) + 2 * ((int64_t)(un.start + un.key0) * p.g_st + (int64_t)kvh * p.rep * p.g_sh));
+  const float *s_at = uniform_ptr(p.stats + (int64_t)kvh * p.rep * p.num_tokens + un.start + un.key0);
+  const int64_t q_next = 2 * p.q_sh, g_next = 2 * p.g_sh, s_next = p.num_tokens;  // the next head's, and the next rows' of the first one
+  const int64_t q_wrap = 64 * p.q_st - (p.rep - 1) * q_next, g_wrap = 64 * p.g_st - (p.rep - 1) * g_next, s_wrap = 32 - (p.rep - 1) * s_next;
+  int next_head = 0, next_left = un.n - 1 - un.key0, next_tile = 0;  // left: rows of the segment past the tile's first
+  const uint32_t q_row = (uint32_t)(2 * p.q_st), g_row = (uint32_t)(2 * p.g_st);
+  uint32_t bytes_at[TS];
+  int rows_of[TS];
+#pragma unroll
+  for (int x = 0; x < TS; ++x) {
+    bytes_at[x] = Tl::block_byte(4 * x + wave, lane);
+    rows_of[x] = Tl::block_row(4 * x + wave, lane);
+  }
+  // The x-th load of a step, into ring buffer b: every wave issues LOADS for every step (past the last tile, that
+  // one's again), so that a count of them says which have landed. Rows past the segment are its last row's copies.
+  constexpr int PT = 2 * TS + 1, LOADS = QW * PT;
+  auto issue = [&](auto index, int b) __attribute__((always_inline)) {
+    constexpr int j = decltype(index)::value / PT, y = decltype(index)::value % PT;
     const uint32_t dst = lds + (uint32_t)(b * Lds::stage + wave * 1024);
-#pragma unroll
-    for (int j = 0; j < QW; ++j) {
-      const int t = min(i * QW + j, tiles - 1), qt = t / p.rep, head = kvh * p.rep + (t - qt * p.rep);
-      const int qb = un.key0 + 32 * qt, left = un.n - 1 - qb;  // (rows past the segment: its last row)
-      const int64_t row = un.start + qb;
-      const T *qt_at = static_cast<const T *>(p.q) + row * p.q_st + head * p.q_sh;
-      const T *gt_at = static_cast<const T *>(p.g) + row * p.g_st + head * p.g_sh;
-#pragma unroll
-      for (int x = 0; x < TS; ++x) {
-        const uint32_t m = (uint32_t)min(Tl::block_row(4 * x + wave, lane), left), byte = Tl::block_byte(4 * x + wave, lane);
-        dma16(qt_at, m * (uint32_t)(2 * p.q_st) + byte, dst + (uint32_t)((2 * j * TS + x) * 4096));
-        dma16(gt_at, m * (uint32_t)(2 * p.g_st) + byte, dst + (uint32_t)(((2 * j + 1) * TS + x) * 4096));
-      }
-      if (j == qw)
-        dma4(p.stats + head * (int64_t)p.num_tokens + row, (uint32_t)(min(lane & 31, left) * 4 + hl * (int)(plane * 4)),
-             lds + (uint32_t)(Lds::stats + b * 1024 + wave * 256));
+    if constexpr (y < TS) {
+      dma16(q_at, (uint32_t)min(rows_of[y], next_left) * q_row + bytes_at[y], dst + (uint32_t)((2 * j * TS + y) * 4096));
+    } else if constexpr (y < 2 * TS) {
+      dma16(g_at, (uint32_t)min(rows_of[y - TS], next_left) * g_row + bytes_at[y - TS], dst + (uint32_t)(((2 * j + 1) * TS + y - TS) * 4096));
+    } else {
+      // (each wave its own copy of the tile's statistics)
+      dma4(s_at, (uint32_t)(min(lane & 31, next_left) * 4 + hl * (int)(plane * 4)), lds + (uint32_t)(Lds::stats + b * Lds::stat_step + j * 1024 + wave * 256));
+      // (selections, no branches: a step is one block of instructions)
+      const bool more = next_tile < tiles - 1, wrap = next_head == p.rep - 1;
+      next_tile += more ? 1 : 0;
+      next_head = more ? (wrap ? 0 : next_head + 1) : next_head;
+      next_left -= more && wrap ? 32 : 0;
+      q_at += more ? (wrap ? q_wrap : q_next) : 0;
+      g_at += more ? (wrap ? g_wrap : g_next) : 0;
+      s_at += more ? (wrap ? s_wrap : s_next) : 0;
     }
   };
   const uint32_t rows_at = Tl::rows_at(lane), cols_at = Tl::cols_at(lane);
-  auto compute = [&](int i, int b) __attribute__((always_inline)) {
-    const int t = i * QW + qw;
-    if (t >= tiles) return;
-    const int qb = un.key0 + 32 * (t / p.rep);
-    if (qb >= top || qb + 31 < wkey) return;  // no row of the tile sees a key of the wave
+  // A tile's four products, NK operand reads each, every read two ahead of its use:
+  //   S = K Q^T | dP = V G^T, and meanwhile P = exp2(c S) | dV += P^T G, and meanwhile dS = P dP | dK += dS^T Q.
+  // S starts at -lse / c and dP at -delta. The next step's loads go out over the first product.
+  auto compute = [&](auto masked, int qb, int b, int to) __attribute__((always_inline)) {
+    constexpr bool kMask = decltype(masked)::value;
+    constexpr int EC = 16 * NS / NK;  // elements a step
     const uint32_t qt = lds + (uint32_t)(b * Lds::stage + 2 * qw * Tl::bytes), gt = qt + Tl::bytes;
-    const uint32_t st = lds + (uint32_t)(Lds::stats + b * 1024 + wave * 256 + 16 * hl);
-    f32x16 sc[NS], dp[NS];
-    float nl[16];
+    const uint32_t st = lds + (uint32_t)(Lds::stats + b * Lds::stat_step + qw * 1024 + wave * 256 + 16 * hl);
+    f32x16 sc[NS], dp[NS], start;
+    auto read_stats = [&](uint32_t at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i4 = 0; i4 < 4; ++i4) {
-      const f32x4 l = __builtin_bit_cast(f32x4, lds_read16(st + 32 * i4)), d = __builtin_bit_cast(f32x4, lds_read16(st + 128 + 32 * i4));
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const f32x4 x = __builtin_bit_cast(f32x4, lds_read16(at + 32 * i4));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        nl[4 * i4 + e] = l[e];
-#pragma unroll
-        for (int s = 0; s < NS; ++s) dp[s][4 * i4 + e] = d[e];  // dP - delta
+        for (int e = 0; e < 4; ++e) start[4 * i4 + e] = x[e];
       }
-    }
+    };
+    u32x4 op[4 * NK], pf[NS][2], df[NS][2];
+    auto read = [&](auto index) __attribute__((always_inline)) {
+      constexpr int i = decltype(index)::value;
+      if constexpr (i < NK) op[i] = Tl::read_rows(qt, rows_at, i);
+      else if constexpr (i < 2 * NK) op[i] = Tl::read_rows(gt, rows_at, i - NK);
+      else if constexpr (i < 3 * NK) op[i] = Tl::read_cols(gt, cols_at, (i - 2 * NK) % ND, (i - 2 * NK) / ND);
+      else if constexpr (i < 4 * NK) op[i] = Tl::read_cols(qt, cols_at, (i - 3 * NK) % ND, (i - 3 * NK) / ND);
+    };
+    read_stats(st);
+    read(std::integral_constant<int, 0>{});
+    read(std::integral_constant<int, 1>{});
+    static_for<4 * NK>([&](auto index) __attribute__((always_inline)) {
+      constexpr int i = decltype(index)::value, kk = i % NK, db = kk % ND, ks = kk / ND;
+      if constexpr (i == NK - 1) read_stats(st + 128);
+      read(std::integral_constant<int, i + 2>{});
 #pragma unroll
-    for (int s = 0; s < NS; ++s) sc[s] = f32x16{};
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const u32x4 a = Tl::read_rows(qt, rows_at, kk);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) sc[s] = mfma32<T>(a, kf[s][kk], sc[s]);
-    }
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const u32x4 a = Tl::read_rows(gt, rows_at, kk);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) dp[s] = mfma32<T>(a, vf[s][kk], dp[s]);
-    }
-    const bool full = qb >= wkey + kWaveRows<D> - 1 && qb + 32 <= low;
-    u32x4 pf[NS][2], df[NS][2];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        f32x8 x, y;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          x[r] = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * ks + r], p.c, nl[8 * ks + r]));
-          y[r] = kHalf ? fminf(fmaxf(x[r] * factor * dp[s][8 * ks + r], -65504.f), 65504.f) : x[r] * dp[s][8 * ks + r];
-        }
-        if (!full) {
-          const int rel = qb + 4 * hl - key[s];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const bool seen = (uint32_t)(rel + 16 * ks + 8 * (r >> 2) + (r & 3)) < (uint32_t)see[s];
-            x[r] = seen ? x[r] : 0.f;
-            y[r] = seen ? y[r] : 0.f;
+      for (int s = 0; s < NS; ++s) {
+        if constexpr (i < NK) sc[s] = mfma32<T>(op[i], kf[s][kk], kk ? sc[s] : start);
+        else if constexpr (i < 2 * NK) dp[s] = mfma32<T>(op[i], vf[s][kk], kk ? dp[s] : start);
+        else if constexpr (i < 3 * NK) mfma32_sum<T>(dv[s][db], op[i], pf[s][ks]);
+        else mfma32_sum<T>(dk[s][db], op[i], df[s][ks]);
+      }
+      if constexpr (i < NK) {
+        static_for<LOADS>([&](auto x) __attribute__((always_inline)) {
+          if constexpr (decltype(x)::value * NK / LOADS == kk) issue(x, to);
+        });
+      } else if constexpr (i < 3 * NK) {
+        static_for<EC>([&](auto x) __attribute__((always_inline)) {
+          constexpr int e = kk * EC + decltype(x)::value, s = e / 16, r = e % 16;
+          if constexpr (i < 2 * NK) {
+            sc[s][r] = __builtin_amdgcn_exp2f(sc[s][r] * p.c);
+            if (kMask) sc[s][r] = (uint32_t)(qb + 4 * hl - key[s] + 8 * (r >> 2) + (r & 3)) < (uint32_t)see[s] ? sc[s][r] : 0.f;
+            if constexpr (r % 8 == 7) pf[s][r / 8] = pack_part<T>(sc[s], r - 7);
+          } else {
+            dp[s][r] *= kHalf ? sc[s][r] * factor : sc[s][r];
+            if (kMask) dp[s][r] = sc[s][r] != 0.f ? dp[s][r] : 0.f;  // (a hidden key's dP may be anything)
+            if constexpr (r % 8 == 7) df[s][r / 8] = pack_part<T>(dp[s], r - 7);
           }
-        }
-        pf[s][ks] = pack8<T>(x);
-        df[s][ks] = pack8<T>(y);
+        });
       }
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int db = 0; db < ND; ++db) {
-        const u32x4 ga = Tl::read_cols(gt, cols_at, db, ks), qa = Tl::read_cols(qt, cols_at, db, ks);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          dv[s][db] = mfma32<T>(ga, pf[s][ks], dv[s][db]);
-          dk[s][db] = mfma32<T>(qa, df[s][ks], dk[s][db]);
-        }
-      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
 
   if constexpr (kHalf) factor *= 1.f / 16384.f;  // P carries 2^kPBias
+  for (int i = 0; i < NB - 1; ++i) static_for<LOADS>([&](auto x) __attribute__((always_inline)) { issue(x, i); });
+  int b = 0, head = qw % p.rep, qb = un.key0 + 32 * (qw / p.rep), t = qw;  // of the wave's tile
+  // Steps up to `end`. A step past the wave's last tile sees nothing of it.
+  auto run = [&](auto masked, int &i, int end) __attribute__((always_inline)) {
+    for (; i < end; ++i) {
+      wait_vmem<(NB - 2) * LOADS>();  // step i has landed
+      barrier_lds();                  // for every wave, and every wave has left step i - 1
+      compute(masked, t < tiles ? qb : 0x3fffffff, b, b == 0 ? NB - 1 : b - 1);
+      b = b == NB - 1 ? 0 : b + 1;
+      t += QW;
+      head += QW % p.rep;
+      qb += 32 * (QW / p.rep) + (head >= p.rep ? 32 : 0);
+      head -= head >= p.rep ? p.rep : 0;
+    }
+  };
+  // The tiles that every key of the wave is seen from are a range: from the first whose rows all come after the keys.
+  const int full0 = (wkey + kWaveRows<D> - 1 - un.key0 + 31) / 32 * p.rep, full1 = max((low - un.key0) / 32, 0) * p.rep;
+  auto step_of = [&](int tile) __attribute__((always_inline)) { return min(max((tile - qw + QW - 1) / QW, 0), steps); };
+  int i = 0;
+  run(std::true_type{}, i, full0 < full1 ? step_of(full0) : steps);
+  run(std::false_type{}, i, step_of(full1));
+  run(std::true_type{}, i, steps);
 #pragma unroll
-  for (int i = 0; i < NB - 1; ++i) issue(i, i);
-  int b = 0;
-  for (int i = 0; i < steps; ++i) {
-    wait_vmem<(NB - 2) * (SL + 1)>();  // step i has landed
-    barrier_lds();                     // for every wave, and every wave has left step i - 1
-    issue(i + NB - 1, b == 0 ? NB - 1 : b - 1);
-    compute(i, b);
-    b = b == NB - 1 ? 0 : b + 1;
-  }
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int db = 0; db < ND; ++db) {
+      settle(dk[s][db]);
+      settle(dv[s][db]);
+    }
   wait_vmem<0>();
   if constexpr (QW > 1) {  // the waves of the same keys add up, pairwise, over LDS
 #pragma unroll
@@ -453,7 +496,6 @@ void grad_queries_kernel(const GradParams p) {
   const int hig = chunk * p.hpw + wave % p.hpw, head = min(kvh * p.rep + hig, (kvh + 1) * p.rep - 1);
   const int w0 = un.t0 + wave / p.hpw * kWaveRows<D>;
   const bool work = hig < p.rep && w0 < tend && wave / p.hpw < 4 / p.hpw;
-  const int wlast = min(w0 + kWaveRows<D>, tend) - 1;
   const int64_t plane = (int64_t)p.num_heads * p.num_tokens;
   u32x4 qf[NS][NK], gf[NS][NK];
   float nl[NS], nd[NS];
@@ -495,77 +537,131 @@ void grad_queries_kernel(const GradParams p) {
     }
   };
   const uint32_t rows_at = Tl::rows_at(lane), cols_at = Tl::cols_at(lane);
-  auto compute = [&](int i, int b) __attribute__((always_inline)) {
-    const bool past = i < past_tiles, trunk = i < past_tiles + trunk_tiles;
-    const int kb = past ? 32 * i : trunk ? 32 * (i - past_tiles) : un.branch0 + 32 * (i - past_tiles - trunk_tiles);
-    if (!work || (!past && kb > wlast)) return;
-    const uint32_t kt = lds + (uint32_t)(b * Lds::stage), vt = kt + Tl::bytes;
+  // A tile's three products for the wave's NS blocks of 32 rows:
+  //   S = Q K^T of each block, and over the second block's P = exp2(c S) of the first; dP = G V^T of each block, and over them P of
+  //   the second and dS = P dP of the first; dQ += dS K of both, each operand read once for them.
+  // S starts at -lse / c and dP at -delta. K's and V's operands stay for the second block.
+  auto compute = [&](auto masked, int kb, int run, uint32_t kt) __attribute__((always_inline)) {
+    constexpr bool kMask = decltype(masked)::value;
+    constexpr int EC = 16 / NK > 0 ? 16 / NK : 1;  // elements of a block a step
+    const uint32_t vt = kt + Tl::bytes;
+    int first[NS];
+    uint32_t see[NS];
+    if constexpr (kMask) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {  // the row sees `see` keys of this run, of which `first` lie past the lane's first one
+        const int at = run < 2 ? 0 : row[s] < un.trunk ? row[s] + 1 : lo[s], last = run == 0 ? un.past_len - 1 : run == 1 ? min(row[s], un.trunk - 1) : row[s];
+        first[s] = kb + 4 * hl - at;
+        see[s] = (uint32_t)max(last - at + 1, 0);
+      }
+    }
     f32x16 sc[NS], dp[NS];
+    u32x4 op[3 * NK], df[NS][2];
+    auto read = [&](auto index) __attribute__((always_inline)) {
+      constexpr int i = decltype(index)::value;
+      if constexpr (i < NK) op[i] = Tl::read_rows(kt, rows_at, i);
+      else if constexpr (i < 2 * NK) op[i] = Tl::read_rows(vt, rows_at, i - NK);
+      else if constexpr (i < 3 * NK) op[i] = Tl::read_cols(kt, cols_at, (i - 2 * NK) % ND, (i - 2 * NK) / ND);
+    };
+    auto exps = [&](auto block, auto step) __attribute__((always_inline)) {
+      constexpr int s = decltype(block)::value;
+      static_for<EC>([&](auto x) __attribute__((always_inline)) {
+        constexpr int r = decltype(step)::value * EC + decltype(x)::value;
+        sc[s][r] = __builtin_amdgcn_exp2f(sc[s][r] * p.c);
+        if (kMask) sc[s][r] = (uint32_t)(first[s] + 8 * (r >> 2) + (r & 3)) < see[s] ? sc[s][r] : 0.f;
+      });
+    };
+    auto ds = [&](auto block, auto step) __attribute__((always_inline)) {
+      constexpr int s = decltype(block)::value;
+      static_for<EC>([&](auto x) __attribute__((always_inline)) {
+        constexpr int r = decltype(step)::value * EC + decltype(x)::value;
+        dp[s][r] *= kHalf ? sc[s][r] * factor : sc[s][r];
+        if (kMask) dp[s][r] = sc[s][r] != 0.f ? dp[s][r] : 0.f;  // (a hidden key's dP may be anything)
+        if constexpr (r % 8 == 7) df[s][r / 8] = pack_part<T>(dp[s], r - 7);
+      });
+    };
+    using First = std::integral_constant<int, 0>;
+    using Second = std::integral_constant<int, NS - 1>;
+    read(First{});
+    read(std::integral_constant<int, 1>{});
+    // S and dP of the blocks, one after the other: step i is product i / NK (S of each block, then dP of each).
+    static_for<2 * NS * NK>([&](auto index) __attribute__((always_inline)) {
+      constexpr int i = decltype(index)::value, kk = i % NK, s = i / NK % NS;
+      constexpr bool kS = i < NS * NK;
+      using Step = std::integral_constant<int, kk>;
+      constexpr int at = kS ? kk : NK + kk;
+      // what a first block reads two ahead: its own operands, then (at its end) nothing or the next product's
+      if constexpr (s == 0 && kk + 2 < NK) read(std::integral_constant<int, at + 2>{});
+      if constexpr (s == NS - 1 && kk + 2 >= NK) read(std::integral_constant<int, (kS ? NK : 2 * NK) + kk + 2 - NK>{});
+      if constexpr (kS) {
+        if constexpr (kk == 0)
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+          for (int r = 0; r < 16; ++r) sc[s][r] = nl[s];
+        sc[s] = mfma32<T>(op[at], qf[s][kk], sc[s]);
+        if constexpr (s > 0) exps(First{}, Step{});
+      } else {
+        if constexpr (kk == 0)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        sc[s][r] = 0.f;
-        dp[s][r] = nd[s];
+          for (int r = 0; r < 16; ++r) dp[s][r] = nd[s];
+        dp[s] = mfma32<T>(op[at], gf[s][kk], dp[s]);
+        if constexpr (s == 0) exps(Second{}, Step{});
+        else ds(First{}, Step{});
       }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    static_for<NK>([&](auto step) __attribute__((always_inline)) { ds(Second{}, step); });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<NK>([&](auto step) __attribute__((always_inline)) {
+      constexpr int kk = decltype(step)::value;
+      read(std::integral_constant<int, 2 * NK + kk + 2>{});
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const u32x4 a = Tl::read_rows(kt, rows_at, kk);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) sc[s] = mfma32<T>(a, qf[s][kk], sc[s]);
-    }
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const u32x4 a = Tl::read_rows(vt, rows_at, kk);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) dp[s] = mfma32<T>(a, gf[s][kk], dp[s]);
-    }
-    const bool full = past ? kb + 32 <= un.past_len : trunk && kb + 32 <= un.trunk && kb + 31 <= w0;
-    u32x4 df[NS][2];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      // The row sees the keys [first, last] of this run.
-      const int first = past || trunk ? 0 : row[s] < un.trunk ? row[s] + 1 : lo[s];
-      const int last = past ? un.past_len - 1 : trunk ? min(row[s], un.trunk - 1) : row[s];
-      const uint32_t see = (uint32_t)max(last - first + 1, 0);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        f32x8 y;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(sc[s][8 * ks + r], p.c, nl[s]));
-          y[r] = kHalf ? fminf(fmaxf(x * factor * dp[s][8 * ks + r], -65504.f), 65504.f) : x * dp[s][8 * ks + r];
-        }
-        if (!full) {
-          const int rel = kb + 4 * hl - first;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) y[r] = (uint32_t)(rel + 16 * ks + 8 * (r >> 2) + (r & 3)) < see ? y[r] : 0.f;
-        }
-        df[s][ks] = pack8<T>(y);
-      }
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int db = 0; db < ND; ++db) {
-        const u32x4 ka = Tl::read_cols(kt, cols_at, db, ks);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) dq[s][db] = mfma32<T>(ka, df[s][ks], dq[s][db]);
-      }
+      for (int s = 0; s < NS; ++s) mfma32_sum<T>(dq[s][kk % ND], op[2 * NK + kk], df[s][kk / ND]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
 
 #pragma unroll
   for (int i = 0; i < NB - 1; ++i) issue(i, i);
-  int b = 0;
-  for (int i = 0; i < steps; ++i) {
+  int b = 0, i = 0;
+  auto begin = [&]() __attribute__((always_inline)) {  // of step i
     wait_vmem<(NB - 2) * SL>();
     barrier_lds();
     issue(i + NB - 1, b == 0 ? NB - 1 : b - 1);
-    compute(i, b);
+  };
+  auto next = [&]() __attribute__((always_inline)) {
+    ++i;
     b = b == NB - 1 ? 0 : b + 1;
+  };
+  if (!work) {
+    while (i < steps) {
+      begin();
+      next();
+    }
+    wait_vmem<0>();
+    return;
+  }
+  // `count` tiles of a run of keys from kb on, some hidden from a row or none.
+  auto tiles = [&](auto masked, int run, int &kb, int count) __attribute__((always_inline)) {
+    for (int n = 0; n < count; ++n) {
+      begin();
+      compute(masked, kb, run, lds + (uint32_t)(b * Lds::stage));
+      next();
+      kb += 32;
+    }
+  };
+#pragma unroll 1
+  for (int run = 0; run < 3; ++run) {
+    const int count = run == 0 ? past_tiles : run == 1 ? trunk_tiles : steps - past_tiles - trunk_tiles;
+    const int full = run == 0 ? un.past_len / 32 : run == 1 ? min(min(un.trunk, w0 + 1) / 32, count) : 0;
+    int kb = run < 2 ? 0 : un.branch0;
+    tiles(std::false_type{}, run, kb, full);
+    tiles(std::true_type{}, run, kb, count - full);
   }
   wait_vmem<0>();
-  if (!work) return;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int db = 0; db < ND; ++db) settle(dq[s][db]);
   const float f = kHalf ? p.scale / (factor * 16384.f) : p.scale;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
@@ -642,8 +738,8 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   if (D != 64 && D != 128 && D != 256) return fail(DAN_ERR_UNSUPPORTED, "head_dim %d: only 64, 128 and 256 are built", D);
   if (a->dtype != DAN_DTYPE_BF16 && a->dtype != DAN_DTYPE_F16) return fail(DAN_ERR_UNSUPPORTED, "dtype %d: bf16 or fp16", a->dtype);
   if (N < 0 || a->num_key_units < 0 || a->num_query_units < 0 || a->num_pasts < 0) return fail(DAN_ERR_INVALID_ARGUMENT, "negative count");
-  if (!(a->scale > 0.f && isfinite(a->scale) && isfinite(a->scale * 1.4426950408889634f)))
-    return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be finite and > 0");
+  // (-lse / scale has to be finite, too)
+  if (!(a->scale >= 0x1p-100f && a->scale <= 0x1p100f)) return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be from 2^-100 to 2^100");
   if (a->key_rows != dan_tree_grad_key_rows(D, 0) && a->key_rows != dan_tree_grad_key_rows(D, 1))
     return fail(DAN_ERR_INVALID_ARGUMENT, "key_rows %d: dan_tree_grad_key_rows", a->key_rows);
   if (N == 0 || a->num_key_units == 0 || a->num_query_units == 0) return DAN_OK;
