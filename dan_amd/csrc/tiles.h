@@ -80,7 +80,12 @@ __device__ inline void mfma32_sum(f32x16 &c, u32x4 a, u32x4 b) {
   if constexpr (std::is_same<T, __bf16>::value) asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
   else asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
-__device__ inline void settle(f32x16 &c) { asm volatile("s_nop 15\n\ts_nop 15" : "+a"(c)); }
+template <int N>
+__device__ inline void settle(f32x16 (&c)[N]) {
+  asm volatile("s_nop 15\n\ts_nop 15" : "+a"(c[0]));
+#pragma unroll
+  for (int i = 1; i < N; ++i) asm volatile("" : "+a"(c[i]));
+}
 
 // s_waitcnt vmcnt(N) (expcnt and lgkmcnt left alone).
 template <int N>

@@ -200,7 +200,7 @@ template <int D, int KW>
 struct KeyLds {
   static constexpr int QW = 4 / KW;
   static constexpr int stage = 2 * QW * Tile<D>::bytes;
-  static constexpr int stat_step = QW * 1024;  // [QW][4 waves][64 floats]
+  static constexpr int stat_step = 1024;  // [4 waves][64 floats]
   static constexpr int ring = 4 * (stage + stat_step) <= 140 * 1024 ? 4 : 3 * (stage + stat_step) <= 140 * 1024 ? 3 : 2;
   static constexpr int stats = ring * stage;
   static constexpr int red = stats + ring * stat_step;  // 16 floats
@@ -216,7 +216,6 @@ void grad_keys_kernel(const GradParams p) {
   using Tl = Tile<D>;
   using Lds = KeyLds<D, KW>;
   constexpr int NS = kWaveRows<D> / 32, QW = 4 / KW, NK = D / 16, ND = D / 32, NB = Lds::ring;
-  constexpr int TS = Tl::blocks / 4;  // direct loads of a wave a tile of Q, and of G
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
@@ -261,65 +260,81 @@ void grad_keys_kernel(const GradParams p) {
 #pragma unroll
     for (int db = 0; db < ND; ++db) dk[s][db] = dv[s][db] = f32x16{};
 
+  // Tiles in order: a head after the other, then the next 32 rows. A step takes QW of them; the KW waves that share one load it.
   const int tiles = (un.q_end - un.key0 + 31) / 32 * p.rep, steps = (tiles + QW - 1) / QW;
   const int64_t plane = (int64_t)p.num_heads * p.num_tokens;
-  // The tiles in order, a head after the other, then the next 32 rows: what the next one to load is read from.
-  const char *q_at = uniform_ptr(static_cast<const char *>(p.q) + 2 * ((int64_t)(un.start + un.key0) * p.q_st + (int64_t)kvh * p.rep * p.q_sh));
-  const char *g_at = uniform_ptr(static_cast<const char *>(p.g) + 2 * ((int64_t)(un.start + un.key0) * p.g_st + (int64_t)kvh * p.rep * p.g_sh));
-  const float *s_at = uniform_ptr(p.stats + (int64_t)kvh * p.rep * p.num_tokens + un.start + un.key0);
-  const int64_t q_next = 2 * p.q_sh, g_next = 2 * p.g_sh, s_next = p.num_tokens;  // the next head's, and the next rows' of the first one
-  const int64_t q_wrap = 64 * p.q_st - (p.rep - 1) * q_next, g_wrap = 64 * p.g_st - (p.rep - 1) * g_next, s_wrap = 32 - (p.rep - 1) * s_next;
-  int next_head = 0, next_left = un.n - 1 - un.key0, next_tile = 0;  // left: rows of the segment past the tile's first
+  const int rest = QW % p.rep, whole = QW / p.rep;  // from a wave's tile to its next: `rest` heads and 32 `whole` rows on
+  int next = min(qw, tiles - 1), next_head = next % p.rep, next_left = un.n - 1 - un.key0 - 32 * (next / p.rep);  // left: rows of the segment past the tile's first
+  auto tile_at = [&](const void *base, int64_t st, int64_t sh) __attribute__((always_inline)) {
+    return uniform_ptr(static_cast<const char *>(base) + 2 * ((un.start + un.key0 + 32 * (int64_t)(next / p.rep)) * st + (kvh * p.rep + next_head) * sh));
+  };
+  const char *q_at = tile_at(p.q, p.q_st, p.q_sh), *g_at = tile_at(p.g, p.g_st, p.g_sh);
+  const float *s_at = uniform_ptr(p.stats + (int64_t)(kvh * p.rep + next_head) * p.num_tokens + un.start + un.key0 + 32 * (next / p.rep));
+  const int64_t q_on = 2 * (rest * p.q_sh + 32 * whole * p.q_st), g_on = 2 * (rest * p.g_sh + 32 * whole * p.g_st), s_on = rest * (int64_t)p.num_tokens + 32 * whole;
+  const int64_t q_wrap = 2 * (32 * p.q_st - p.rep * p.q_sh), g_wrap = 2 * (32 * p.g_st - p.rep * p.g_sh), s_wrap = 32 - p.rep * (int64_t)p.num_tokens;
   const uint32_t q_row = (uint32_t)(2 * p.q_st), g_row = (uint32_t)(2 * p.g_st);
-  uint32_t bytes_at[TS];
-  int rows_of[TS];
-#pragma unroll
-  for (int x = 0; x < TS; ++x) {
-    bytes_at[x] = Tl::block_byte(4 * x + wave, lane);
-    rows_of[x] = Tl::block_row(4 * x + wave, lane);
-  }
-  // The x-th load of a step, into ring buffer b: every wave issues LOADS for every step (past the last tile, that
+  // The x-th load of a step, into ring buffer b: every wave issues LOADS for every step (past its last tile, that
   // one's again), so that a count of them says which have landed. Rows past the segment are its last row's copies.
-  constexpr int PT = 2 * TS + 1, LOADS = QW * PT;
+  constexpr int LB = Tl::blocks / KW, LOADS = 2 * LB + 1;
   auto issue = [&](auto index, int b) __attribute__((always_inline)) {
-    constexpr int j = decltype(index)::value / PT, y = decltype(index)::value % PT;
-    const uint32_t dst = lds + (uint32_t)(b * Lds::stage + wave * 1024);
-    if constexpr (y < TS) {
-      dma16(q_at, (uint32_t)min(rows_of[y], next_left) * q_row + bytes_at[y], dst + (uint32_t)((2 * j * TS + y) * 4096));
-    } else if constexpr (y < 2 * TS) {
-      dma16(g_at, (uint32_t)min(rows_of[y - TS], next_left) * g_row + bytes_at[y - TS], dst + (uint32_t)(((2 * j + 1) * TS + y - TS) * 4096));
+    constexpr int x = decltype(index)::value % LB;
+    constexpr bool kQ = decltype(index)::value < LB;
+    const uint32_t dst = lds + (uint32_t)(b * Lds::stage + 2 * qw * Tl::bytes + kw * 1024);
+    if constexpr (decltype(index)::value < 2 * LB) {
+      const uint32_t m = (uint32_t)min(Tl::block_row(kw + KW * x, lane), next_left);
+      dma16(kQ ? q_at : g_at, __umul24(m, kQ ? q_row : g_row) + Tl::block_byte(kw + KW * x, lane), dst + (uint32_t)((kQ ? 0 : Tl::bytes) + x * KW * 1024));
     } else {
       // (each wave its own copy of the tile's statistics)
-      dma4(s_at, (uint32_t)(min(lane & 31, next_left) * 4 + hl * (int)(plane * 4)), lds + (uint32_t)(Lds::stats + b * Lds::stat_step + j * 1024 + wave * 256));
+      dma4(s_at, (uint32_t)(min(lane & 31, next_left) * 4 + hl * (int)(plane * 4)), lds + (uint32_t)(Lds::stats + b * Lds::stat_step + wave * 256));
       // (selections, no branches: a step is one block of instructions)
-      const bool more = next_tile < tiles - 1, wrap = next_head == p.rep - 1;
-      next_tile += more ? 1 : 0;
-      next_head = more ? (wrap ? 0 : next_head + 1) : next_head;
-      next_left -= more && wrap ? 32 : 0;
-      q_at += more ? (wrap ? q_wrap : q_next) : 0;
-      g_at += more ? (wrap ? g_wrap : g_next) : 0;
-      s_at += more ? (wrap ? s_wrap : s_next) : 0;
+      const bool more = next + QW < tiles, wrap = more && next_head + rest >= p.rep;
+      next += more ? QW : 0;
+      next_head += (more ? rest : 0) - (wrap ? p.rep : 0);
+      next_left -= (more ? 32 * whole : 0) + (wrap ? 32 : 0);
+      q_at += (more ? q_on : 0) + (wrap ? q_wrap : 0);
+      g_at += (more ? g_on : 0) + (wrap ? g_wrap : 0);
+      s_at += (more ? s_on : 0) + (wrap ? s_wrap : 0);
     }
   };
   const uint32_t rows_at = Tl::rows_at(lane), cols_at = Tl::cols_at(lane);
   // A tile's four products, NK operand reads each, every read two ahead of its use:
   //   S = K Q^T | dP = V G^T, and meanwhile P = exp2(c S) | dV += P^T G, and meanwhile dS = P dP | dK += dS^T Q.
-  // S starts at -lse / c and dP at -delta. The next step's loads go out over the first product.
-  auto compute = [&](auto masked, int qb, int b, int to) __attribute__((always_inline)) {
+  // S starts at -lse / c and dP at -delta. With a ring of three or more the step's barrier stands before the last
+  // product: the step after has landed then and every wave has left the step before, whose buffer the loads that go
+  // out over that product fill, and the next tile's first operands are read at its end. With two buffers the barrier
+  // stands before the first product, and the next step's loads go out over it.
+  constexpr bool kEarly = NB > 2;
+  f32x16 start;    // -lse / c of the tile's rows (then -delta)
+  u32x4 ahead[2];  // the tile's first two operands
+  auto read_stats = [&](int b, int which) __attribute__((always_inline)) {
+    const uint32_t at = lds + (uint32_t)(Lds::stats + b * Lds::stat_step + wave * 256 + which * 128 + 16 * hl);
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const f32x4 x = __builtin_bit_cast(f32x4, lds_read16(at + 32 * i4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) start[4 * i4 + e] = x[e];
+    }
+  };
+  auto tile_of = [&](int b) __attribute__((always_inline)) { return lds + (uint32_t)(b * Lds::stage + 2 * qw * Tl::bytes); };
+  auto read_first = [&](int b) __attribute__((always_inline)) {
+    read_stats(b, 0);
+    ahead[0] = Tl::read_rows(tile_of(b), rows_at, 0);
+    ahead[1] = Tl::read_rows(tile_of(b), rows_at, 1);
+  };
+  auto compute = [&](auto masked, int qb, int b) __attribute__((always_inline)) {
     constexpr bool kMask = decltype(masked)::value;
     constexpr int EC = 16 * NS / NK;  // elements a step
-    const uint32_t qt = lds + (uint32_t)(b * Lds::stage + 2 * qw * Tl::bytes), gt = qt + Tl::bytes;
-    const uint32_t st = lds + (uint32_t)(Lds::stats + b * Lds::stat_step + qw * 1024 + wave * 256 + 16 * hl);
-    f32x16 sc[NS], dp[NS], start;
-    auto read_stats = [&](uint32_t at) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const f32x4 x = __builtin_bit_cast(f32x4, lds_read16(at + 32 * i4));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) start[4 * i4 + e] = x[e];
-      }
-    };
+    const int to = b == 0 ? NB - 1 : b - 1, after = b == NB - 1 ? 0 : b + 1;
+    const uint32_t qt = tile_of(b), gt = qt + Tl::bytes;
+    if constexpr (!kEarly) {
+      wait_vmem<0>();
+      barrier_lds();
+      read_first(b);
+    }
+    f32x16 sc[NS], dp[NS];
     u32x4 op[4 * NK], pf[NS][2], df[NS][2];
+    op[0] = ahead[0];
+    op[1] = ahead[1];
     auto read = [&](auto index) __attribute__((always_inline)) {
       constexpr int i = decltype(index)::value;
       if constexpr (i < NK) op[i] = Tl::read_rows(qt, rows_at, i);
@@ -327,12 +342,14 @@ void grad_keys_kernel(const GradParams p) {
       else if constexpr (i < 3 * NK) op[i] = Tl::read_cols(gt, cols_at, (i - 2 * NK) % ND, (i - 2 * NK) / ND);
       else if constexpr (i < 4 * NK) op[i] = Tl::read_cols(qt, cols_at, (i - 3 * NK) % ND, (i - 3 * NK) / ND);
     };
-    read_stats(st);
-    read(std::integral_constant<int, 0>{});
-    read(std::integral_constant<int, 1>{});
     static_for<4 * NK>([&](auto index) __attribute__((always_inline)) {
       constexpr int i = decltype(index)::value, kk = i % NK, db = kk % ND, ks = kk / ND;
-      if constexpr (i == NK - 1) read_stats(st + 128);
+      if constexpr (kEarly && i == 3 * NK) {
+        wait_vmem<(NB - 3) * LOADS>();
+        barrier_lds();
+      }
+      if constexpr (i == NK - 1) read_stats(b, 1);
+      if constexpr (kEarly && i == 4 * NK - 2) read_first(after);
       read(std::integral_constant<int, i + 2>{});
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
@@ -341,11 +358,12 @@ void grad_keys_kernel(const GradParams p) {
         else if constexpr (i < 3 * NK) mfma32_sum<T>(dv[s][db], op[i], pf[s][ks]);
         else mfma32_sum<T>(dk[s][db], op[i], df[s][ks]);
       }
-      if constexpr (i < NK) {
+      if constexpr (kEarly ? i >= 3 * NK : i < NK) {
         static_for<LOADS>([&](auto x) __attribute__((always_inline)) {
           if constexpr (decltype(x)::value * NK / LOADS == kk) issue(x, to);
         });
-      } else if constexpr (i < 3 * NK) {
+      }
+      if constexpr (i >= NK && i < 3 * NK) {
         static_for<EC>([&](auto x) __attribute__((always_inline)) {
           constexpr int e = kk * EC + decltype(x)::value, s = e / 16, r = e % 16;
           if constexpr (i < 2 * NK) {
@@ -367,16 +385,24 @@ void grad_keys_kernel(const GradParams p) {
   for (int i = 0; i < NB - 1; ++i) static_for<LOADS>([&](auto x) __attribute__((always_inline)) { issue(x, i); });
   int b = 0, head = qw % p.rep, qb = un.key0 + 32 * (qw / p.rep), t = qw;  // of the wave's tile
   // Steps up to `end`. A step past the wave's last tile sees nothing of it.
+  if constexpr (kEarly) {
+    wait_vmem<(NB - 2) * LOADS>();
+    barrier_lds();
+    read_first(0);
+  }
   auto run = [&](auto masked, int &i, int end) __attribute__((always_inline)) {
     for (; i < end; ++i) {
-      wait_vmem<(NB - 2) * LOADS>();  // step i has landed
-      barrier_lds();                  // for every wave, and every wave has left step i - 1
-      compute(masked, t < tiles ? qb : 0x3fffffff, b, b == 0 ? NB - 1 : b - 1);
+      compute(masked, t < tiles ? qb : 0x3fffffff, b);
       b = b == NB - 1 ? 0 : b + 1;
       t += QW;
       head += QW % p.rep;
       qb += 32 * (QW / p.rep) + (head >= p.rep ? 32 : 0);
       head -= head >= p.rep ? p.rep : 0;
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      settle(dk[s]);
+      settle(dv[s]);
     }
   };
   // The tiles that every key of the wave is seen from are a range: from the first whose rows all come after the keys.
@@ -386,13 +412,6 @@ void grad_keys_kernel(const GradParams p) {
   run(std::true_type{}, i, full0 < full1 ? step_of(full0) : steps);
   run(std::false_type{}, i, step_of(full1));
   run(std::true_type{}, i, steps);
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int db = 0; db < ND; ++db) {
-      settle(dk[s][db]);
-      settle(dv[s][db]);
-    }
   wait_vmem<0>();
   if constexpr (QW > 1) {  // the waves of the same keys add up, pairwise, over LDS
 #pragma unroll
@@ -521,30 +540,57 @@ void grad_queries_kernel(const GradParams p) {
 #pragma unroll
     for (int db = 0; db < ND; ++db) dq[s][db] = f32x16{};
 
-  auto issue = [&](int i_any, int b) __attribute__((always_inline)) {  // (past the last step: the last one's again)
-    const int i = min(i_any, steps - 1);
-    const bool past = i < past_tiles, trunk = i < past_tiles + trunk_tiles;
-    const int kb = past ? 32 * i : trunk ? 32 * (i - past_tiles) : un.branch0 + 32 * (i - past_tiles - trunk_tiles);
-    const int left = (past ? un.past_len : trunk ? t_hi : tend) - 1 - kb;
-    const int64_t k_st = past ? pk_st : p.k_st, v_st = past ? pv_st : p.v_st;
-    const T *kt = (past ? pk : own_k) + kb * k_st, *vt = (past ? pv : own_v) + kb * v_st;
-    const uint32_t dst = lds + (uint32_t)(b * Lds::stage + wave * 1024);
-#pragma unroll
-    for (int x = 0; x < TS; ++x) {
-      const uint32_t m = (uint32_t)min(Tl::block_row(4 * x + wave, lane), left), byte = Tl::block_byte(4 * x + wave, lane);
-      dma16(kt, m * (uint32_t)(2 * k_st) + byte, dst + (uint32_t)(x * 4096));
-      dma16(vt, m * (uint32_t)(2 * v_st) + byte, dst + (uint32_t)((TS + x) * 4096));
+  // What the next tile is loaded from: its first row, the rows of its run past that one, and the two runs still to come.
+  const int branch_left = tend > un.trunk ? tend - un.branch0 - 1 : -1;  // (-1: no such run)
+  const char *k_at = (const char *)(past_tiles ? pk : own_k), *v_at = (const char *)(past_tiles ? pv : own_v);
+  const char *k_branch = (const char *)(own_k + un.branch0 * p.k_st), *v_branch = (const char *)(own_v + un.branch0 * p.v_st);
+  if (!past_tiles && !trunk_tiles) {
+    k_at = k_branch;
+    v_at = v_branch;
+  }
+  k_at = uniform_ptr(k_at);
+  v_at = uniform_ptr(v_at);
+  uint32_t k_row = (uint32_t)(2 * (past_tiles ? pk_st : p.k_st)), v_row = (uint32_t)(2 * (past_tiles ? pv_st : p.v_st));
+  int at_run = past_tiles ? 0 : trunk_tiles ? 1 : 2, next_left = at_run == 0 ? un.past_len - 1 : at_run == 1 ? t_hi - 1 : branch_left;
+  // The x-th load of a step, into ring buffer b (past the last step: the last tile's again).
+  constexpr int LOADS = SL;
+  auto issue = [&](auto index, int b) __attribute__((always_inline)) {
+    constexpr int x = decltype(index)::value % TS;
+    constexpr bool kK = decltype(index)::value < TS;
+    const uint32_t m = (uint32_t)min(Tl::block_row(4 * x + wave, lane), next_left);
+    dma16(kK ? k_at : v_at, __umul24(m, kK ? k_row : v_row) + Tl::block_byte(4 * x + wave, lane),
+          lds + (uint32_t)(b * Lds::stage + wave * 1024 + (kK ? 0 : Tl::bytes) + x * 4096));
+    if constexpr (decltype(index)::value == LOADS - 1) {  // (selections, no branches: a step is one block of instructions)
+      const bool same = next_left >= 32, trunk = !same && at_run == 0 && trunk_tiles > 0, branch = !same && !trunk && at_run < 2 && branch_left >= 0;
+      next_left = same ? next_left - 32 : trunk ? t_hi - 1 : branch ? branch_left : next_left;
+      k_at = same ? k_at + 32 * (int64_t)k_row : trunk ? (const char *)own_k : branch ? k_branch : k_at;
+      v_at = same ? v_at + 32 * (int64_t)v_row : trunk ? (const char *)own_v : branch ? v_branch : v_at;
+      k_row = trunk || branch ? (uint32_t)(2 * p.k_st) : k_row;
+      v_row = trunk || branch ? (uint32_t)(2 * p.v_st) : v_row;
+      at_run = trunk ? 1 : branch ? 2 : at_run;
     }
   };
   const uint32_t rows_at = Tl::rows_at(lane), cols_at = Tl::cols_at(lane);
   // A tile's three products for the wave's NS blocks of 32 rows:
   //   S = Q K^T of each block, and over the second block's P = exp2(c S) of the first; dP = G V^T of each block, and over them P of
   //   the second and dS = P dP of the first; dQ += dS K of both, each operand read once for them.
-  // S starts at -lse / c and dP at -delta. K's and V's operands stay for the second block.
-  auto compute = [&](auto masked, int kb, int run, uint32_t kt) __attribute__((always_inline)) {
+  // S starts at -lse / c and dP at -delta. K's and V's operands stay for the second block. The step's barrier stands
+  // before the last product: the step after has landed then and every wave has left the step before, whose buffer the
+  // loads that go out over that product fill, and the next tile's first operands are read at its end.
+  u32x4 ahead[2];  // the tile's first two operands
+  auto read_first = [&](int b) __attribute__((always_inline)) {
+    ahead[0] = Tl::read_rows(lds + (uint32_t)(b * Lds::stage), rows_at, 0);
+    ahead[1] = Tl::read_rows(lds + (uint32_t)(b * Lds::stage), rows_at, 1);
+  };
+  auto land = [&]() __attribute__((always_inline)) {
+    wait_vmem<(NB - 3) * LOADS>();
+    barrier_lds();
+  };
+  auto compute = [&](auto masked, int kb, int run, int b) __attribute__((always_inline)) {
     constexpr bool kMask = decltype(masked)::value;
     constexpr int EC = 16 / NK > 0 ? 16 / NK : 1;  // elements of a block a step
-    const uint32_t vt = kt + Tl::bytes;
+    const int to = b == 0 ? NB - 1 : b - 1, after = b == NB - 1 ? 0 : b + 1;
+    const uint32_t kt = lds + (uint32_t)(b * Lds::stage), vt = kt + Tl::bytes;
     int first[NS];
     uint32_t see[NS];
     if constexpr (kMask) {
@@ -582,8 +628,8 @@ void grad_queries_kernel(const GradParams p) {
     };
     using First = std::integral_constant<int, 0>;
     using Second = std::integral_constant<int, NS - 1>;
-    read(First{});
-    read(std::integral_constant<int, 1>{});
+    op[0] = ahead[0];
+    op[1] = ahead[1];
     // S and dP of the blocks, one after the other: step i is product i / NK (S of each block, then dP of each).
     static_for<2 * NS * NK>([&](auto index) __attribute__((always_inline)) {
       constexpr int i = decltype(index)::value, kk = i % NK, s = i / NK % NS;
@@ -611,43 +657,43 @@ void grad_queries_kernel(const GradParams p) {
     });
     static_for<NK>([&](auto step) __attribute__((always_inline)) { ds(Second{}, step); });
     __builtin_amdgcn_sched_barrier(0);
+    land();
     static_for<NK>([&](auto step) __attribute__((always_inline)) {
       constexpr int kk = decltype(step)::value;
+      if constexpr (kk == NK - 2) read_first(after);
       read(std::integral_constant<int, 2 * NK + kk + 2>{});
 #pragma unroll
       for (int s = 0; s < NS; ++s) mfma32_sum<T>(dq[s][kk % ND], op[2 * NK + kk], df[s][kk / ND]);
+      static_for<LOADS>([&](auto x) __attribute__((always_inline)) {
+        if constexpr (decltype(x)::value * NK / LOADS == kk) issue(x, to);
+      });
       __builtin_amdgcn_sched_barrier(0);
     });
   };
 
-#pragma unroll
-  for (int i = 0; i < NB - 1; ++i) issue(i, i);
-  int b = 0, i = 0;
-  auto begin = [&]() __attribute__((always_inline)) {  // of step i
-    wait_vmem<(NB - 2) * SL>();
-    barrier_lds();
-    issue(i + NB - 1, b == 0 ? NB - 1 : b - 1);
-  };
-  auto next = [&]() __attribute__((always_inline)) {
-    ++i;
-    b = b == NB - 1 ? 0 : b + 1;
-  };
-  if (!work) {
-    while (i < steps) {
-      begin();
-      next();
+  for (int i = 0; i < NB - 1; ++i) static_for<LOADS>([&](auto x) __attribute__((always_inline)) { issue(x, i); });
+  wait_vmem<(NB - 2) * LOADS>();
+  barrier_lds();
+  int b = 0;
+  if (!work) {  // the loads and barriers alone
+    for (int i = 0; i < steps; ++i) {
+      land();
+      static_for<LOADS>([&](auto x) __attribute__((always_inline)) { issue(x, b == 0 ? NB - 1 : b - 1); });
+      b = b == NB - 1 ? 0 : b + 1;
     }
     wait_vmem<0>();
     return;
   }
+  read_first(0);
   // `count` tiles of a run of keys from kb on, some hidden from a row or none.
   auto tiles = [&](auto masked, int run, int &kb, int count) __attribute__((always_inline)) {
     for (int n = 0; n < count; ++n) {
-      begin();
-      compute(masked, kb, run, lds + (uint32_t)(b * Lds::stage));
-      next();
+      compute(masked, kb, run, b);
+      b = b == NB - 1 ? 0 : b + 1;
       kb += 32;
     }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) settle(dq[s]);
   };
 #pragma unroll 1
   for (int run = 0; run < 3; ++run) {
@@ -658,10 +704,6 @@ void grad_queries_kernel(const GradParams p) {
     tiles(std::true_type{}, run, kb, count - full);
   }
   wait_vmem<0>();
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int db = 0; db < ND; ++db) settle(dq[s][db]);
   const float f = kHalf ? p.scale / (factor * 16384.f) : p.scale;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
@@ -757,9 +799,9 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   const void *rows[] = {a->q, a->k, a->v, a->out, a->grad, a->dq, a->dk, a->dv};
   for (const void *r : rows)
     if ((uintptr_t)r & 15) return fail(DAN_ERR_INVALID_ARGUMENT, "q, k, v, out and the gradients must be 16-byte aligned");
-  // Offsets inside a tile, and between the two planes of the workspace, are kept in 32 bits.
+  // A row's bytes are multiplied in 24 bits; offsets between the two planes of the workspace are kept in 32.
   for (int64_t s : {a->q_stride_tok, a->k_stride_tok, a->v_stride_tok, a->g_stride_tok})
-    if (s < 0 || s * 64 >= (int64_t(1) << 31)) return fail(DAN_ERR_UNSUPPORTED, "token stride %lld is too large", (long long)s);
+    if (s < 0 || s >= 1 << 23) return fail(DAN_ERR_UNSUPPORTED, "token stride %lld: fewer than 2^23", (long long)s);
   if ((int64_t)H * N * 4 >= (int64_t(1) << 31) - 4096) return fail(DAN_ERR_UNSUPPORTED, "%d heads x %d tokens: fewer than 2^29 rows", H, N);
 
   GradParams p;
