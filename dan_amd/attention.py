@@ -180,7 +180,9 @@ def attend_train(q, k, v, segments, layer, scale=None):
     Prefix-cache entries are constants (one that requires grad raises); a
     segment with ``save`` > 0 keeps detached copies, as ``attend`` does. Rows of
     no segment give zeros and have no gradient. Segments must not overlap.
-    k and v of finite values: a hidden key's weight is zero, its products are not
+    ``scale`` (1 / sqrt(D) unless given): from 2^-100 to 2^100. q, k, v and the
+    output's gradient of finite
+    values: a hidden key's weight is zero, its products are not
     left out. The first call on a ``Batch`` uploads its tables, so it cannot be
     captured into a HIP graph; later ones can, forward and backward in the same
     capture and with no earlier, eager result alive that holds the graph of the
@@ -193,6 +195,8 @@ def attend_train(q, k, v, segments, layer, scale=None):
         raise NotImplementedError("attend_train has no forward-mode derivative")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"attend_train takes bf16 or fp16; got {q.dtype}")
+    if scale is not None and not 2.0 ** -100 <= scale <= 2.0 ** 100:
+        raise ValueError(f"attend_train: scale must be from 2^-100 to 2^100; got {scale}")
     if q.is_cuda and q.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(q.device):
             return attend_train(q, k, v, segments, layer, scale)

@@ -282,7 +282,7 @@ void grad_keys_kernel(const GradParams p) {
     const uint32_t dst = lds + (uint32_t)(b * Lds::stage + 2 * qw * Tl::bytes + kw * 1024);
     if constexpr (decltype(index)::value < 2 * LB) {
       const uint32_t m = (uint32_t)min(Tl::block_row(kw + KW * x, lane), next_left);
-      dma16(kQ ? q_at : g_at, __umul24(m, kQ ? q_row : g_row) + Tl::block_byte(kw + KW * x, lane), dst + (uint32_t)((kQ ? 0 : Tl::bytes) + x * KW * 1024));
+      dma16(kQ ? q_at : g_at, m * (kQ ? q_row : g_row) + Tl::block_byte(kw + KW * x, lane), dst + (uint32_t)((kQ ? 0 : Tl::bytes) + x * KW * 1024));
     } else {
       // (each wave its own copy of the tile's statistics)
       dma4(s_at, (uint32_t)(min(lane & 31, next_left) * 4 + hl * (int)(plane * 4)), lds + (uint32_t)(Lds::stats + b * Lds::stat_step + wave * 256));
@@ -558,7 +558,7 @@ void grad_queries_kernel(const GradParams p) {
     constexpr int x = decltype(index)::value % TS;
     constexpr bool kK = decltype(index)::value < TS;
     const uint32_t m = (uint32_t)min(Tl::block_row(4 * x + wave, lane), next_left);
-    dma16(kK ? k_at : v_at, __umul24(m, kK ? k_row : v_row) + Tl::block_byte(4 * x + wave, lane),
+    dma16(kK ? k_at : v_at, m * (kK ? k_row : v_row) + Tl::block_byte(4 * x + wave, lane),
           lds + (uint32_t)(b * Lds::stage + wave * 1024 + (kK ? 0 : Tl::bytes) + x * 4096));
     if constexpr (decltype(index)::value == LOADS - 1) {  // (selections, no branches: a step is one block of instructions)
       const bool same = next_left >= 32, trunk = !same && at_run == 0 && trunk_tiles > 0, branch = !same && !trunk && at_run < 2 && branch_left >= 0;
@@ -799,9 +799,9 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   const void *rows[] = {a->q, a->k, a->v, a->out, a->grad, a->dq, a->dk, a->dv};
   for (const void *r : rows)
     if ((uintptr_t)r & 15) return fail(DAN_ERR_INVALID_ARGUMENT, "q, k, v, out and the gradients must be 16-byte aligned");
-  // A row's bytes are multiplied in 24 bits; offsets between the two planes of the workspace are kept in 32.
+  // Offsets within a tile and between the two planes of the workspace are kept in 32 bits.
   for (int64_t s : {a->q_stride_tok, a->k_stride_tok, a->v_stride_tok, a->g_stride_tok})
-    if (s < 0 || s >= 1 << 23) return fail(DAN_ERR_UNSUPPORTED, "token stride %lld: fewer than 2^23", (long long)s);
+    if (s < 0 || s >= 1 << 25) return fail(DAN_ERR_UNSUPPORTED, "token stride %lld: fewer than 2^25", (long long)s);
   if ((int64_t)H * N * 4 >= (int64_t(1) << 31) - 4096) return fail(DAN_ERR_UNSUPPORTED, "%d heads x %d tokens: fewer than 2^29 rows", H, N);
 
   GradParams p;
