@@ -86,16 +86,18 @@ __device__ inline void load_rows(const T *const (&row)[F], int k0, int last, int
       for (int s = 0; s < 4; ++s)
         if (k0 + 32 * s + 8 * g4 >= last) to[f][s] = u32x4{};
 }
-// t = w x^T over one chunk, w from adapter i.
-template <typename T, int JB, int F>
-__device__ inline void chunk_product(const DownParams &p, int i, int k0, int last, int l16, int g4, const u32x4 (&xf)[F][4], f32x4 (&t)[JB][F]) {
+// One chunk of adapter i's w (ranks past the last one: copies of it, never used).
+template <typename T, int JB>
+__device__ inline void load_chunk(const DownParams &p, int i, int k0, int last, int l16, int g4, u32x4 (&wf)[JB][4]) {
   const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.rank * p.n;
-  u32x4 wf[JB][4];
 #pragma unroll
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
-    for (int s = 0; s < 4; ++s)  // (ranks past the last one: copies of it, never used)
-      wf[jb][s] = load16(w + (int64_t)min(16 * jb + l16, p.rank - 1) * p.n + min(k0 + 32 * s + 8 * g4, last - 8));
+    for (int s = 0; s < 4; ++s) wf[jb][s] = load16(w + (int64_t)min(16 * jb + l16, p.rank - 1) * p.n + min(k0 + 32 * s + 8 * g4, last - 8));
+}
+// t += w x^T over it.
+template <typename T, int JB, int F>
+__device__ inline void chunk_product(const u32x4 (&wf)[JB][4], const u32x4 (&xf)[F][4], f32x4 (&t)[JB][F]) {
 #pragma unroll
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
@@ -104,7 +106,9 @@ __device__ inline void chunk_product(const DownParams &p, int i, int k0, int las
       for (int s = 0; s < 4; ++s) t[jb][f] = mfma16<T>(wf[jb][s], xf[f][s], t[jb][f]);
 }
 
-// Many rows: 32 a work group, whose W waves split the chunks and add up over LDS.
+// Many rows: 32 a work group, whose W waves split the chunks and add up over LDS. Work groups begin at different chunks:
+// where a row's bytes are a multiple of a large power of 2, all of them at one place of their rows ask few channels of the memory.
+// Neighbours in the grid are the splits of a tile of rows, so that a die reads few of w's columns.
 template <int JB>
 constexpr int kDownWaves = JB <= 2 ? 16 : 8;  // (1024 threads leave 128 registers each)
 template <typename T, int JB>
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(64 * kDownWaves<JB>) void down_kernel(const DownPar
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   f32x4 *red = reinterpret_cast<f32x4 *>(smem);  // [W / 2][JB * F][64]
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
-  const int n0 = blockIdx.x * 16 * F, first = blockIdx.y * p.chunks * kChunk, last = min(first + p.chunks * kChunk, p.n);
+  const int n0 = blockIdx.y * 16 * F, first = blockIdx.x * p.chunks * kChunk, last = min(first + p.chunks * kChunk, p.n);
   int idx[F];
   const T *xr[F];
 #pragma unroll
@@ -128,24 +132,25 @@ __global__ __launch_bounds__(64 * kDownWaves<JB>) void down_kernel(const DownPar
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
     for (int f = 0; f < F; ++f) acc[jb][f] = f32x4{};
-  for (int k0 = first + wave * kChunk; k0 < last; k0 += W * kChunk) {
+  constexpr bool kAhead = JB < 8;  // the first adapter's w is loaded with the rows (at rank 128 the registers do not hold both)
+  const uint64_t own[F] = {__ballot(idx[0] >= 0), __ballot(idx[1] >= 0)};
+  const int i0 = own[0] ? next_adapter(idx[0], own[0]) : next_adapter(idx[1], own[1]);
+  const int begin = first + wave * kChunk, turns = (last - begin + W * kChunk - 1) / (W * kChunk);  // (0 or fewer: no chunk)
+  for (int turn = 0, at = turns > 0 ? blockIdx.y % turns : 0; turn < turns; ++turn, at = at + 1 < turns ? at + 1 : 0) {
+    const int k0 = begin + at * W * kChunk;
     u32x4 xf[F][4];
+    u32x4 wf[JB][4];
     load_rows<T, F>(xr, k0, last, g4, xf);
-    uint64_t left[F];
-#pragma unroll
-    for (int f = 0; f < F; ++f) left[f] = __ballot(idx[f] >= 0);
-    for (;;) {  // each adapter of the tile
-      int i = -1;
-#pragma unroll
-      for (int f = F - 1; f >= 0; --f)
-        if (left[f]) i = next_adapter(idx[f], left[f]);
-      if (i < 0) break;
+    if constexpr (kAhead) load_chunk<T, JB>(p, max(i0, 0), k0, last, l16, g4, wf);
+    uint64_t left[F] = {own[0], own[1]};
+    for (int i = i0; i >= 0;) {  // each adapter of the tile
+      if (!kAhead || i != i0) load_chunk<T, JB>(p, i, k0, last, l16, g4, wf);
       f32x4 t[JB][F];
 #pragma unroll
       for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
         for (int f = 0; f < F; ++f) t[jb][f] = f32x4{};
-      chunk_product<T, JB, F>(p, i, k0, last, l16, g4, xf, t);
+      chunk_product<T, JB, F>(wf, xf, t);
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const bool mine = idx[f] == i;
@@ -155,9 +160,9 @@ __global__ __launch_bounds__(64 * kDownWaves<JB>) void down_kernel(const DownPar
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[jb][f][e] += mine ? t[jb][f][e] : 0.f;
       }
+      i = left[0] ? next_adapter(idx[0], left[0]) : next_adapter(idx[1], left[1]);
     }
   }
-#pragma unroll
   for (int h = W / 2; h; h >>= 1) {  // pairs of waves, in a fixed order
     if (h < W / 2) __syncthreads();
     if (wave >= h && wave < 2 * h)
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(64 * kDownWaves<JB>) void down_kernel(const DownPar
       if (n < p.rows)
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb)
-          *(DAN_TILE_GLOBAL f32x4 *)(p.part + ((int64_t)blockIdx.y * p.rows + n) * p.ranks + 16 * jb + 4 * g4) = acc[jb][f];
+          *(DAN_TILE_GLOBAL f32x4 *)(p.part + ((int64_t)blockIdx.x * p.rows + n) * p.ranks + 16 * jb + 4 * g4) = acc[jb][f];
     }
 }
 
@@ -204,11 +209,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void down_few_kernel(const DownPara
     f32x4 t[JB][1];
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb) t[jb][0] = f32x4{};
-    chunk_product<T, JB, 1>(p, i, first, last, l16, g4, xf, t);
+    u32x4 wf[JB][4];
+    load_chunk<T, JB>(p, i, first, last, l16, g4, wf);
+    chunk_product<T, JB, 1>(wf, xf, t);
     for (int k0 = first + kChunk; k0 < last; k0 += kChunk) {
       u32x4 more[1][4];
       load_rows<T, 1>(xr, k0, last, g4, more);
-      chunk_product<T, JB, 1>(p, i, k0, last, l16, g4, more, t);
+      load_chunk<T, JB>(p, i, k0, last, l16, g4, wf);
+      chunk_product<T, JB, 1>(wf, more, t);
     }
     if (mine)
 #pragma unroll
@@ -241,17 +249,45 @@ struct Operand {
     if (kHalf)
       for (int r = threadIdx.x; r < 16 * F; r += TH) top[r] = 0u;
     if (kHalf) __syncthreads();
-    for (int q = threadIdx.x; q < 16 * F * 4 * ST; q += TH) {
-      const int r = q / (4 * ST), j4 = q % (4 * ST), n = n0 + r;
-      const float *from = p.part + (int64_t)min(n, p.rows - 1) * p.ranks + 4 * j4;
-      const int64_t plane = (int64_t)p.rows * p.ranks;
-      f32x4 x = *(const DAN_TILE_GLOBAL f32x4 *)from;
-#pragma unroll 8
-      for (int s = 1; s < p.splits; ++s) x += *(const DAN_TILE_GLOBAL f32x4 *)(from + s * plane);
-      if (p.sum && blockIdx.x == 0 && n < p.rows) *(DAN_TILE_GLOBAL f32x4 *)(p.sum + (int64_t)n * p.ranks + 4 * j4) = x;
-      v[r][j4] = x;
+    // Four parts of all of a thread's quarters of 16 bytes are loaded at a time. Where there are more threads than quarters,
+    // P of a wave's lanes share one and add up every P-th part.
+    constexpr int Q = 16 * F * 4 * ST, P = TH >= Q ? TH / Q : 1, L = 64 / P, NQ = Q * P / TH;
+    static_assert(NQ * TH == Q * P, "every thread has as many");
+    const int64_t plane = (int64_t)p.rows * p.ranks;
+    const int s0 = (threadIdx.x & 63) / L;
+    auto quad = [&](int x) { return (int)(threadIdx.x + x * TH) / 64 * L + (int)threadIdx.x % L; };
+    const float *from[NQ];
+    f32x4 sum[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      from[x] = p.part + (int64_t)min(n0 + quad(x) / (4 * ST), p.rows - 1) * p.ranks + quad(x) % (4 * ST) * 4;
+      sum[x] = f32x4{};
+    }
+    for (int s = s0; s < p.splits; s += 4 * P) {
+      f32x4 part[NQ][4];
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) part[x][y] = *(const DAN_TILE_GLOBAL f32x4 *)(from[x] + min(s + y * P, p.splits - 1) * plane);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int x = 0; x < NQ; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[x][e] += s + y * P < p.splits ? part[x][y][e] : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+#pragma unroll
+      for (int m = L; m < 64; m <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[x][e] += __shfl_xor(sum[x][e], m);
+      if (s0) continue;
+      const int r = quad(x) / (4 * ST), j4 = quad(x) % (4 * ST), n = n0 + r;
+      if (p.sum && blockIdx.x == 0 && n < p.rows) *(DAN_TILE_GLOBAL f32x4 *)(p.sum + (int64_t)n * p.ranks + 4 * j4) = sum[x];
+      v[r][j4] = sum[x];
       if (kHalf) {
-        const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        const float m = fmaxf(fmaxf(fabsf(sum[x][0]), fabsf(sum[x][1])), fmaxf(fabsf(sum[x][2]), fabsf(sum[x][3])));
         atomicMax(&top[r], __builtin_bit_cast(uint32_t, m));  // (of values that are not negative: in any order)
       }
     }
@@ -300,12 +336,12 @@ __device__ inline float factor_of(const UpParams &p, int i, uint32_t top) {
   return std::is_same<T, _Float16>::value ? ldexpf(c, -exponent_of(__builtin_bit_cast(float, top))) : c;
 }
 
-// Many rows: 64 (32 at rank 128) by `steps` times 256 columns, 64 a wave. y of the next step is loaded before this one's.
-template <int ST>
-constexpr int kUpFrags = ST == 8 ? 2 : 4;
+// Many rows: 32 by `steps` times 256 columns, 64 a wave. y of the next step is loaded before this one's. (64 rows halve the
+// loads of w, but leave two waves a SIMD instead of four: 8192 rows of 6144 columns took 53.7 us, and take 46.6.)
+constexpr int kUpFrags = 2;
 template <typename T, int ST>
 __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
-  constexpr int F = kUpFrags<ST>;
+  constexpr int F = kUpFrags;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
   __shared__ Operand<T, ST, F, kThreads> op;
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
@@ -328,6 +364,16 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
 #pragma unroll
   for (int f = 0; f < F; ++f) yv[f][0] = yv[f][1] = u32x4{};
   if (p.y) load_y(first);
+  int loaded = -1;  // the adapter that wf holds this step's columns of
+  u32x4 wf[ST][4];
+  auto load_w = [&](int i, int m0) __attribute__((always_inline)) {
+    load_columns<T, ST>(p, i, m0, l16, g4, wf);
+    loaded = i;
+  };
+  {
+    const uint64_t some = __ballot(idx[0] >= 0 && idx[0] < p.adapters);
+    if (some && first < p.cols) load_w(next_adapter(idx[0], some), first);
+  }
   op.make(p, n0);
   for (int step = 0; step < p.steps; ++step) {
     const int m0 = first + step * 4 * kUpCols;
@@ -345,6 +391,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
         }
       }
     if (p.y && step + 1 < p.steps) load_y(m0 + 4 * kUpCols);
+    if (step) loaded = -1;
     uint64_t left[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) left[f] = __ballot(idx[f] >= 0);
@@ -354,8 +401,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
       for (int f = F - 1; f >= 0; --f)
         if (left[f]) i = next_adapter(idx[f], left[f]);
       if (i < 0) break;
-      u32x4 wf[ST][4];
-      if (i < p.adapters) load_columns<T, ST>(p, i, m0, l16, g4, wf);
+      if (i < p.adapters && i != loaded) load_w(i, m0);
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const bool mine = idx[f] == i;
@@ -456,13 +502,13 @@ struct OuterSide {
 };
 struct OuterParams {
   OuterSide a, b;  // dA [rank][n_in] of (g, x); dB [n_out][rank] of (h, G)
-  const int32_t *index;
+  const int32_t *list, *starts;  // the rows in the order of their adapters, and where each adapter's begin [adapters + 1]; or NULL (one adapter, all rows)
   const float *scale;
   int32_t rows, rank, ranks, adapters, parts;
   float scale_value;
 };
 
-// One adapter, 128 columns, a part of the adapter's rows, which are listed in order; the waves take 32 of them in turn,
+// One adapter, 128 columns, a part of the adapter's rows; the waves take 32 of them in turn,
 // each through a tile of its own in LDS, from where the transposing reads make the operand whose inner dimension is
 // the rows. v's operand is loaded in place (a lane's 8 rows).
 template <typename T, int JB>
@@ -472,51 +518,31 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
   constexpr int CB = kOuterCols / 16;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
-  __shared__ int counts[4];
-  int32_t *list = reinterpret_cast<int32_t *>(smem + 4 * Tl::bytes);
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
   const bool side_b = (int)blockIdx.x >= p.a.tiles;
   const OuterSide &q = side_b ? p.b : p.a;
   const int c0 = ((int)blockIdx.x - (side_b ? p.a.tiles : 0)) * kOuterCols, i = blockIdx.y, part = blockIdx.z;
 
-  // Each thread counts its share of the index, then knows where its rows stand among the adapter's.
-  const int share = (p.rows + kThreads - 1) / kThreads, r0 = min((int)threadIdx.x * share, p.rows), r1 = min(r0 + share, p.rows);
-  int here = 0;
-  for (int n = r0; n < r1; ++n) here += adapter_of(p.index, n) == i;
-  int before = here;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int x = __shfl_up(before, m);
-    if (lane >= m) before += x;
-  }
-  if (lane == 63) counts[wave] = before;
-  __syncthreads();
-  before -= here;
-  for (int w = 0; w < wave; ++w) before += counts[w];
-  const int total = uni(counts[0] + counts[1] + counts[2] + counts[3]);
-  const int from = (int)((int64_t)total * part / p.parts), count = (int)((int64_t)total * (part + 1) / p.parts) - from;
-  if (here)
-    for (int n = r0; n < r1; ++n)
-      if (adapter_of(p.index, n) == i) {
-        if (before >= from && before < from + count) list[before - from] = n;
-        ++before;
-      }
-  __syncthreads();
-
+  const int start = p.starts ? p.starts[i] : 0, total = p.starts ? p.starts[i + 1] - start : i == 0 ? p.rows : 0;
+  const int from = start + (int)((int64_t)total * part / p.parts), count = start + (int)((int64_t)total * (part + 1) / p.parts) - from;
+  auto row_of = [&](int k) { return p.list ? p.list[from + k] : from + k; };
   f32x4 acc[JB][CB];
 #pragma unroll
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) acc[jb][cb] = f32x4{};
   const uint32_t tile = lds + (uint32_t)(wave * Tl::bytes);
-  const int row0 = count ? uni(list[0]) : 0;  // (the list rises)
+  const int row0 = count ? uni(row_of(0)) : 0;  // (an adapter's rows rise)
   const T *z = static_cast<const T *>(q.z) + (int64_t)row0 * q.z_stride + c0;
   const int left = min(kOuterCols, q.cols - c0);  // columns of the tile (a multiple of 8)
+  int next = wave * kOuterRows < count ? row_of(min(wave * kOuterRows + (lane & 31), count - 1)) : 0;
   for (int s0 = wave * kOuterRows; s0 < count; s0 += 4 * kOuterRows) {
+    const int mine = next;  // lane l: the step's row l % 32
+    next = row_of(min(s0 + 4 * kOuterRows + (lane & 31), count - 1));
     barrier_wave_lds();  // (the last step's reads of the tile)
 #pragma unroll
     for (int x = 0; x < Tl::blocks; ++x) {
-      const int n = list[min(s0 + Tl::block_row(x, lane), count - 1)];
+      const int n = __shfl(mine, Tl::block_row(x, lane));
       dma16(z, (uint32_t)(n - row0) * (uint32_t)(2 * q.z_stride) + min(Tl::block_byte(x, lane), (uint32_t)(2 * left - 16)), tile + (uint32_t)(x * 1024));
     }
     const int rows = min(count - s0, kOuterRows);
@@ -525,7 +551,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool in = 8 * g4 + e < rows;
-      const float *at = q.v + (int64_t)list[min(s0 + 8 * g4 + e, count - 1)] * p.ranks + l16;
+      const float *at = q.v + (int64_t)__shfl(mine, 8 * g4 + e) * p.ranks + l16;
 #pragma unroll
       for (int jb = 0; jb < JB; ++jb) v[jb][e] = at[16 * jb];
 #pragma unroll
@@ -632,12 +658,63 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
 struct TurnParams {
   const uint16_t *a, *b;
   uint16_t *at, *bt;  // [R][n_in][rank], [R][rank][n_out]
-  int32_t rank, n_in, n_out, adapters, a_tiles, b_tiles;  // tiles of 64 columns an adapter
+  const int32_t *index;      // NULL: no list
+  int32_t *list, *starts;    // [rows], [adapters + 1]
+  int32_t rows, rank, n_in, n_out, adapters, a_tiles, b_tiles;  // tiles of 64 columns an adapter
 };
+// The rows of adapter i, in order, at their place among all adapters' (rows of no adapter, or of one past the last, are left
+// out): each wave counts its share, then writes it.
+__device__ inline void list_rows(const TurnParams &p, int i) {
+  constexpr int W = kThreads / 64, U = 8;
+  __shared__ int before[W], here[W];
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), share = (p.rows + W * 64 - 1) / (W * 64) * 64;
+  const int r0 = min(wave * share, p.rows), r1 = min(r0 + share, p.rows);
+  auto each = [&](auto &&f) {
+    for (int r = r0; r < r1; r += U * 64) {
+      int x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = p.index[min(r + u * 64 + lane, p.rows - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(r + u * 64 + lane, r + u * 64 + lane < r1 ? x[u] : -1);
+    }
+  };
+  int below = 0, mine = 0;
+  each([&](int, int x) {
+    below += __popcll(__ballot(x >= 0 && x < i));
+    mine += __popcll(__ballot(x == i));
+  });
+  if (lane == 0) {
+    before[wave] = below;
+    here[wave] = mine;
+  }
+  __syncthreads();
+  int start = 0, to = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    start += before[w];
+    to += w < wave ? here[w] : 0;
+    total += here[w];
+  }
+  to += start;
+  if (threadIdx.x == 0) {
+    p.starts[i] = start;
+    if (i == p.adapters - 1) p.starts[i + 1] = start + total;
+  }
+  each([&](int n, int x) {
+    const uint64_t votes = __ballot(x == i);
+    if (x == i) p.list[to + __popcll(votes & ((uint64_t(1) << lane) - 1))] = n;
+    to += __popcll(votes);
+  });
+}
+
 // 64 positions of the wide side and all ranks a work group, 16 bytes a load and a store.
 __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t tile[DAN_ADAPT_MAX_RANK][64 + 8];
   int x = blockIdx.x;
+  if (p.index) {  // (first: they take longest)
+    if (x < p.adapters) return list_rows(p, x);
+    x -= p.adapters;
+  }
   const bool b = x >= p.a_tiles * p.adapters;
   if (b) x -= p.a_tiles * p.adapters;
   const int tiles = b ? p.b_tiles : p.a_tiles, i = x / tiles, c0 = x % tiles * 64, wide = b ? p.n_out : p.n_in, r8 = p.rank / 8;
@@ -687,7 +764,7 @@ int splits_of(int rows, int n, int rank) {
 int parts_of(int rows, int n_in, int n_out, int adapters) {
   const int64_t groups = (int64_t)((n_in + kOuterCols - 1) / kOuterCols + (n_out + kOuterCols - 1) / kOuterCols) * adapters;
   const int64_t by_rows = rows / (512 * (int64_t)adapters);
-  return (int)std::max<int64_t>({1, std::min<int64_t>((1024 + groups - 1) / groups, by_rows), (rows + 16383) / 16384});
+  return (int)std::max<int64_t>(1, std::min<int64_t>((1024 + groups - 1) / groups, by_rows));
 }
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
@@ -700,7 +777,7 @@ hipError_t launch_down(const DownParams &p, int splits, hipStream_t s) {
   constexpr int W = kDownWaves<JB>, bytes = W / 2 * JB * 2 * 1024;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(down_kernel<T, JB>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL((down_kernel<T, JB>), dim3((p.rows + 31) / 32, splits), dim3(64 * W), bytes, s, p);
+  hipLaunchKernelGGL((down_kernel<T, JB>), dim3(splits, (p.rows + 31) / 32), dim3(64 * W), bytes, s, p);
   return hipGetLastError();
 }
 template <typename T>
@@ -717,7 +794,7 @@ hipError_t launch_up(UpParams p, hipStream_t s) {
     hipLaunchKernelGGL((up_few_kernel<T, ST>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
     return hipGetLastError();
   }
-  const int tiles = (p.rows + 16 * kUpFrags<ST> - 1) / (16 * kUpFrags<ST>), cols = std::max(1, (p.cols + 4 * kUpCols - 1) / (4 * kUpCols));
+  const int tiles = (p.rows + 16 * kUpFrags - 1) / (16 * kUpFrags), cols = std::max(1, (p.cols + 4 * kUpCols - 1) / (4 * kUpCols));
   p.steps = std::max(1, std::min(4, (int)((int64_t)tiles * cols / 768)));
   hipLaunchKernelGGL((up_kernel<T, ST>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
   return hipGetLastError();
@@ -727,13 +804,9 @@ hipError_t launch_up(const UpParams &p, hipStream_t s) {
   return p.ranks == 16 ? launch_up<T, 1>(p, s) : p.ranks == 32 ? launch_up<T, 2>(p, s) : p.ranks == 64 ? launch_up<T, 4>(p, s) : launch_up<T, 8>(p, s);
 }
 
-// A part's list of rows in LDS, behind the tiles (16384 rows at most: parts_of).
-int list_bytes(int rows, int parts) { return ((rows + parts - 1) / parts + 1) * 4; }
 template <typename T, int JB>
 hipError_t launch_outer(const OuterParams &p, hipStream_t s) {
-  const int bytes = 4 * Tile<kOuterCols>::bytes + list_bytes(p.rows, p.parts);
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(outer_kernel<T, JB>), hipFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024);
-  if (attr != hipSuccess) return attr;
+  constexpr int bytes = 4 * Tile<kOuterCols>::bytes;
   hipLaunchKernelGGL((outer_kernel<T, JB>), dim3(p.a.tiles + p.b.tiles, p.adapters, p.parts), dim3(kThreads), bytes, s, p);
   return hipGetLastError();
 }
@@ -757,16 +830,18 @@ hipError_t forward(const DanAdaptArgs &a, hipStream_t s) {
   return launch_up<T>(u, s);
 }
 
-// The workspace of the gradient: A^T, B^T, g in parts and added up, and the parts of dA and dB.
+// The workspace of the gradient: A^T, B^T, the list of rows, g in parts and added up, and the parts of dA and dB.
 struct GradSpace {
-  int64_t at, bt, part, g, da, db, total;
+  int64_t at, bt, list, starts, part, g, da, db, total;
   int splits, parts;
   GradSpace(int rows, int n_in, int n_out, int rank, int adapters) {
     splits = splits_of(rows, n_out, rank);
     parts = parts_of(rows, n_in, n_out, adapters);
     at = 0;
     bt = align256(at + (int64_t)adapters * rank * n_in * 2);
-    part = align256(bt + (int64_t)adapters * rank * n_out * 2);
+    list = align256(bt + (int64_t)adapters * rank * n_out * 2);
+    starts = list + (int64_t)rows * 4;
+    part = align256(starts + ((int64_t)adapters + 1) * 4);
     g = align256(part + (int64_t)splits * rows * ranks_of(rank) * 4);
     da = align256(g + (int64_t)rows * ranks_of(rank) * 4);
     const int64_t kept = parts > 1 ? parts : 0;
@@ -781,24 +856,30 @@ hipError_t backward(const DanAdaptGradArgs &a, const GradSpace &w, hipStream_t s
   OuterParams o;
   o.a = {reinterpret_cast<float *>(ws + w.g), a.x, a.x_stride, reinterpret_cast<float *>(ws + w.da), a.da, a.n_in, a.da ? (a.n_in + kOuterCols - 1) / kOuterCols : 0};
   o.b = {a.down, a.g, a.g_stride, reinterpret_cast<float *>(ws + w.db), a.db, a.n_out, a.db ? (a.n_out + kOuterCols - 1) / kOuterCols : 0};
-  o.index = a.index; o.scale = a.scale; o.scale_value = a.scale_value; o.rows = a.rows; o.rank = a.rank; o.ranks = ranks_of(a.rank);
+  o.list = a.index ? reinterpret_cast<int32_t *>(ws + w.list) : nullptr; o.starts = a.index ? reinterpret_cast<int32_t *>(ws + w.starts) : nullptr;
+  o.scale = a.scale; o.scale_value = a.scale_value; o.rows = a.rows; o.rank = a.rank; o.ranks = ranks_of(a.rank);
   o.adapters = a.adapters; o.parts = w.parts;
   hipError_t err;
-  if (a.dx || a.da) {
+  {
     TurnParams t;
     t.a = static_cast<const uint16_t *>(a.a); t.b = static_cast<const uint16_t *>(a.b);
     t.at = reinterpret_cast<uint16_t *>(ws + w.at); t.bt = reinterpret_cast<uint16_t *>(ws + w.bt);
     t.rank = a.rank; t.n_in = a.n_in; t.n_out = a.n_out; t.adapters = a.adapters;
+    t.rows = a.rows; t.list = reinterpret_cast<int32_t *>(ws + w.list); t.starts = reinterpret_cast<int32_t *>(ws + w.starts);
+    t.index = a.da || a.db ? a.index : nullptr;
     t.a_tiles = a.dx ? (a.n_in + 63) / 64 : 0;
-    t.b_tiles = (a.n_out + 63) / 64;
-    hipLaunchKernelGGL(turn_kernel, dim3((t.a_tiles + t.b_tiles) * a.adapters), dim3(kThreads), 0, s, t);
+    t.b_tiles = a.dx || a.da ? (a.n_out + 63) / 64 : 0;
+    if (const int groups = (t.a_tiles + t.b_tiles + (t.index ? 1 : 0)) * a.adapters)
+      hipLaunchKernelGGL(turn_kernel, dim3(groups), dim3(kThreads), 0, s, t);
     if ((err = hipGetLastError()) != hipSuccess) return err;
+  }
+  if (a.dx || a.da) {
     DownParams d;
-    d.x = a.g; d.x_stride = a.g_stride; d.w = t.bt; d.index = a.index; d.part = reinterpret_cast<float *>(ws + w.part);
+    d.x = a.g; d.x_stride = a.g_stride; d.w = ws + w.bt; d.index = a.index; d.part = reinterpret_cast<float *>(ws + w.part);
     d.rows = a.rows; d.n = a.n_out; d.rank = a.rank; d.adapters = a.adapters; d.ranks = o.ranks;
     if ((err = launch_down<T>(d, w.splits, s)) != hipSuccess) return err;
     UpParams u;  // (without dx: no columns, the sum of the parts alone)
-    u.part = d.part; u.sum = reinterpret_cast<float *>(ws + w.g); u.w = t.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride;
+    u.part = d.part; u.sum = reinterpret_cast<float *>(ws + w.g); u.w = ws + w.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride;
     u.index = a.index; u.scale = a.scale; u.scale_value = a.scale_value;
     u.rows = a.rows; u.cols = a.dx ? a.n_in : 0; u.rank = a.rank; u.adapters = a.adapters; u.ranks = o.ranks; u.splits = w.splits; u.steps = 1;
     if ((err = launch_up<T>(u, s)) != hipSuccess) return err;
@@ -828,7 +909,7 @@ int check_sizes(int dtype, int rows, int n_in, int n_out, int rank, int adapters
   const int64_t wide = std::max(n_in, n_out);  // (`up` has the most threads by far: 2 columns of 16 rows each for few rows)
   if (too_many(over(wide, kUpCols) * over(rows, 16) * 2) ||
       too_many((over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters * parts_of(rows, n_in, n_out, adapters)) ||
-      too_many((over(n_in, 64) + over(n_out, 64)) * adapters) ||
+      too_many((over(n_in, 64) + over(n_out, 64) + 1) * adapters) ||
       too_many(over((int64_t)adapters * rank * ((int64_t)n_in + n_out), 8 * kThreads)))
     return fail(DAN_ERR_UNSUPPORTED, "%d rows, %d to %d, %d adapters: more than one launch holds", rows, n_in, n_out, adapters);
   return DAN_OK;
