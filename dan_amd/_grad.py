@@ -6,9 +6,8 @@ import functools
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _decode, _native
+from . import _decode, _layer, _native
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -179,7 +178,6 @@ def tables(segments, plan, h, hkv, d, num_cus):
 def attend(q, k, v, segments, layer, scale):
     """The differentiable call: through the host module where q, k and v are read in place."""
     from . import attention as A
-    from . import _layer
 
     plan = getattr(segments, "tile_plan", None)
     if plan is None or plan.num_tokens != q.shape[1] or plan.device != q.device:
@@ -217,7 +215,7 @@ class TreeAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_layer.once("attend_train")
     def backward(ctx, grad):
         q, k, v, out, lse = ctx.saved_tensors[:5]
         _decode.check_capture(q.device.index, "attend_train")

@@ -82,6 +82,30 @@ def adapt_grad_workspace_size(rows, n_in, n_out, rank, adapters):
     return _sized("dan_adapt_grad_workspace_size", _i64, 5)(rows, n_in, n_out, rank, adapters)
 
 
+def once(name):
+    """Marks a backward as differentiable once, as the host module's are: where a second derivative is being recorded (by
+    the gradients or by a saved input, which torch's own decorator does not look at), taking it raises."""
+    def mark(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            import torch
+
+            again = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*grads, *ctx.saved_tensors))
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            if not again:
+                return out
+            new = [i for i, t in enumerate(out) if t is not None and all(t is not g for g in grads)]
+            out = list(out)
+            if new:
+                late = torch._C._functions.DelayedError(f"{name} is differentiable once", len(new))
+                for i, t in zip(new, late(*[out[i].detach().requires_grad_() for i in new])):
+                    out[i] = t
+            return tuple(out)
+        return run
+    return mark
+
+
 def rows_of(t):
     """A 2-D tensor that the kernels read in place (unit stride, rows 16-byte aligned), or a new copy of it."""
     s0, s1 = t.stride()

@@ -11,7 +11,6 @@ import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _decode, _layer, _native
 from .attention import _DTYPES, has_tangent
@@ -61,7 +60,7 @@ class _Adapt(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_layer.once("adapt")
     def backward(ctx, g):
         saved = list(ctx.saved_tensors)
         x, a, b, down = saved[:4]
@@ -104,12 +103,13 @@ def adapt(y, x, a, b, index=None, scale=1.0):
     y: [N, n_out], a shared projection's output; x: [N, n_in], its input; a: [R,
     rank, n_in] and b: [R, n_out, rank], R adapters (all bf16 or all fp16); index:
     int32 or int64 [N], each row's adapter, in any order: negative for none (the row
-    of y as it is), past the last one gives NaN; None: the only adapter, for
-    every row. scale: a number, or fp32 [R].
+    of y as it is), past the last one gives NaN, as x's gradient; None: the only adapter,
+    for every row. scale: a number, or fp32 [R].
 
     Sums are fp32 in an order that the sizes alone fix; x a^T stays fp32, the result
     is rounded once. Rows of other adapters take no part in a row's sums, whatever
-    they hold. Ranks 1 to 128 (multiples of 8 need no copy), n_in and n_out multiples of 8.
+    they hold. Ranks 1 to 128 (multiples of 8 need no copy), n_in and n_out multiples of 8
+    up to 2^20, at most 2^20 rows.
 
     Differentiable (once) in y, x, a and b. A backward pass that is captured into a HIP graph has
     its forward pass in the same capture, and no earlier, eager result that holds
@@ -183,4 +183,4 @@ class AdaptedLinear(nn.Module):
         if isinstance(self.base, FP8Linear) and x.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("FP8Linear has no gradient of its input")
         rows = x.reshape(-1, x.shape[-1])
-        return adapt(self.base(rows), rows, self.a, self.b, index, self.scale).view(*x.shape[:-1], -1)
+        return adapt(self.base(rows), rows, self.a, self.b, index, self.scale).view(*x.shape[:-1], self.base.out_features)

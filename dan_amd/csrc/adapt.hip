@@ -532,8 +532,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) acc[jb][cb] = f32x4{};
   const uint32_t tile = lds + (uint32_t)(wave * Tl::bytes);
-  const int row0 = count ? uni(row_of(0)) : 0;  // (an adapter's rows rise)
-  const T *z = static_cast<const T *>(q.z) + (int64_t)row0 * q.z_stride + c0;
+  const T *z = static_cast<const T *>(q.z) + c0;
   const int left = min(kOuterCols, q.cols - c0);  // columns of the tile (a multiple of 8)
   int next = wave * kOuterRows < count ? row_of(min(wave * kOuterRows + (lane & 31), count - 1)) : 0;
   for (int s0 = wave * kOuterRows; s0 < count; s0 += 4 * kOuterRows) {
@@ -543,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
     for (int x = 0; x < Tl::blocks; ++x) {
       const int n = __shfl(mine, Tl::block_row(x, lane));
-      dma16(z, (uint32_t)(n - row0) * (uint32_t)(2 * q.z_stride) + min(Tl::block_byte(x, lane), (uint32_t)(2 * left - 16)), tile + (uint32_t)(x * 1024));
+      dma16_at(z + (int64_t)n * q.z_stride + min(Tl::block_byte(x, lane) / 2, (uint32_t)(left - 8)), tile + (uint32_t)(x * 1024));
     }
     const int rows = min(count - s0, kOuterRows);
     float v[JB][8];
@@ -971,9 +970,6 @@ int dan_adapt_grad(const DanAdaptGradArgs *a, void *stream) {
   const GradSpace w(a->rows, a->n_in, a->n_out, a->rank, a->adapters);
   if (!a->workspace || a->workspace_bytes < w.total || ((uintptr_t)a->workspace & 255))
     return fail(DAN_ERR_INVALID_ARGUMENT, "workspace needs %lld bytes, 256-byte aligned", (long long)w.total);
-  // `outer` keeps a row's offset from its part's first one in 32 bits.
-  if ((int64_t)a->rows * a->x_stride * 2 >= int64_t(1) << 32 || (int64_t)a->rows * a->g_stride * 2 >= int64_t(1) << 32)
-    return fail(DAN_ERR_UNSUPPORTED, "x and g of %d rows: fewer than 2^32 bytes from the first to the last", a->rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const hipError_t err = a->dtype == DAN_DTYPE_BF16 ? backward<__bf16>(*a, w, s) : backward<_Float16>(*a, w, s);
   if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "adapter gradient launch failed: %s", hipGetErrorString(err));

@@ -1974,7 +1974,7 @@ extern "C" {
 int dan_tree_attn_fwd(const DanTreeAttnArgs *a, void *stream) { return dan::forward(a, nullptr, stream); }
 
 int dan_tree_attn_fwd_lse(const DanTreeAttnArgs *a, float *lse, void *stream) {
-  if (!lse) {
+  if (!lse && (!a || a->num_tokens != 0)) {
     dan::g_err[0] = 0;
     return dan::fail(DAN_ERR_INVALID_ARGUMENT, "lse is NULL");
   }

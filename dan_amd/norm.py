@@ -10,7 +10,6 @@ There is no CPU path: CPU tensors raise.
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _decode, _layer, _native
 from .attention import _DTYPES, E4M3, has_tangent
@@ -64,7 +63,7 @@ class _AddNorm(torch.autograd.Function):
         return out if residual is None else (out, stream)
 
     @staticmethod
-    @once_differentiable
+    @_layer.once("add_norm")
     def backward(ctx, g, g_stream=None):
         s, weight, rstd = ctx.saved_tensors
         _decode.check_capture(s.device.index, "add_norm")

@@ -66,7 +66,7 @@ def attend(q, k, v, segments, layer, scale=None, grad=None):
 
 def adapt(y, x, a, b, index, scale, grad=None):
     """Row by row, fp64: dict of out and abs_out, and with ``grad`` dx, da, db and their abs_ bounds. index: a list; negative:
-    no adapter, past the last: NaN (and no gradient)."""
+    no adapter, past the last: NaN (in dx, too; no part of da and db)."""
     y, x, a, b = (t.detach().double().cpu() for t in (y, x, a, b))
     scale = scale.double().cpu().tolist() if isinstance(scale, torch.Tensor) else [scale] * len(a)
     r = dict(out=y.clone(), abs_out=y.abs())
@@ -78,6 +78,8 @@ def adapt(y, x, a, b, index, scale, grad=None):
             continue
         if i >= len(a):
             r["out"][n] = math.nan
+            if grad is not None:
+                r["dx"][n] = math.nan
             continue
         c, h, ah = scale[i], a[i] @ x[n], a[i].abs() @ x[n].abs()
         r["out"][n] += c * (b[i] @ h)
