@@ -29,7 +29,7 @@ class DanTreeGradArgs(ctypes.Structure):
                 ("dv", _vp), ("dv_stride_tok", _i64), ("dv_stride_head", _i64),
                 ("key_units", _vp), ("num_key_units", _i32), ("query_units", _vp), ("num_query_units", _i32),
                 ("row_lo", _vp), ("row_end", _vp), ("pasts", _vp), ("num_pasts", _i32),
-                ("workspace", _vp), ("workspace_bytes", _i64)]
+                ("workspace", _vp), ("workspace_bytes", _i64), ("key_splits", _i32), ("reserved", _i32)]
 
 
 EXPORTS = ("dan_tree_attn_fwd_lse", "dan_tree_attn_bwd", "dan_tree_grad_key_rows", "dan_tree_grad_query_rows",
@@ -46,7 +46,7 @@ def templates(segments, q, k, v, layer, scale, plan_args):
     args, pasts_host, plan = plan_args
     (h, n, d), hkv = q.shape, k.shape[0]
     t = tables(segments, plan, h, hkv, d, A._num_cus(q.device))
-    code, nbytes, back = A._DTYPES[q.dtype], _native.workspace_size(hkv, d, plan.vt_cols) if plan.num_work else 0, workspace_size(h, n)
+    code, nbytes, back = A._DTYPES[q.dtype], _native.workspace_size(hkv, d, plan.vt_cols) if plan.num_work else 0, workspace_size(h, hkv, d, n, t.key_splits)
     past = plan.past_tables[layer][0]
     device_tables = args[3]
     units, sched_off = (device_tables[5].data_ptr(), device_tables[6].data_ptr()) if plan.num_work else (0, 0)
@@ -57,7 +57,7 @@ def templates(segments, q, k, v, layer, scale, plan_args):
         0, 0, _native.PHASES_ALL, units, sched_off, slots, 0, 0 if pasts_host is None else pasts_host.data_ptr(), A._layout(h, hkv, d)[0] // tile_q, 0, 0, 0)
     backward = call_backward.pack(
         GRAD_ABI_VERSION, code, h, hkv, d, n, _native.f32(args[6]), t.key_rows, *[0] * 15, 0, *[0] * 9, t.keys, t.num_keys, t.queries, t.num_queries,
-        t.row_lo, t.row_end, past.data_ptr(), num_pasts, 0, 0)
+        t.row_lo, t.row_end, past.data_ptr(), num_pasts, 0, 0, t.key_splits, 0)
     pasts = tuple(x for entry in plan.past_dicts for x in entry[layer][:2])
     # (the prefix's rows as the kernels read them, where they had to be copied, are behind past_tables)
     refs = tuple(x for x in plan.past_tables[layer][1][0] if isinstance(x, torch.Tensor))
@@ -88,10 +88,25 @@ def _rows(h, hkv, d, small):
 
 
 @functools.lru_cache(maxsize=256)
-def workspace_size(h, n):
+def workspace_size(h, hkv, d, n, splits=1):
     fn = _native.load()["dan_tree_grad_workspace_size"]
-    fn.argtypes, fn.restype = [_i32, _i32], _i64
-    return fn(h, n)
+    fn.argtypes, fn.restype = [_i32] * 5, _i64
+    return fn(h, hkv, d, n, splits)
+
+
+def choose_units(lengths, h, hkv, d, num_cus):
+    """(keys of a key unit, parts of a kv head's heads) of segments of `lengths` rows.
+
+    Larger units read less of Q and G, smaller ones and parts of the heads fill the chip: each of a number of parts that
+    divides the heads evenly and gives up to two work groups a compute unit, while the longest unit keeps 16 steps (the parts
+    are written and read again in fp32)."""
+    whole, small = (int((-(-lengths // _rows(h, hkv, d, x)[0])).sum()) * hkv for x in (False, True))
+    if whole >= num_cus or not small:
+        return _rows(h, hkv, d, False)[0], 1
+    rep, at_once = h // hkv, 2 if d == 256 else 4  # tiles of a step
+    tiles = -(-int(lengths.max()) // TILE) * rep
+    parts = [s for s in range(1, rep + 1) if rep % s == 0 and small * s <= 2.25 * num_cus and (s == 1 or tiles >= 16 * at_once * s)]
+    return _rows(h, hkv, d, True)[0], max(parts, default=1)
 
 
 def build_units(segs, spans, num_tokens, key_rows, query_rows):
@@ -142,9 +157,8 @@ class Tables:
 
         self.device, n = plan.device, plan.num_tokens
         spans = [s.branches for s in segments]
-        whole, rows = _rows(h, hkv, d, False)
-        count = int((-(-plan.segs[:, 1] // whole)).sum()) * hkv
-        self.key_rows = _rows(h, hkv, d, count < num_cus)[0]
+        rows = _rows(h, hkv, d, False)[1]
+        self.key_rows, self.key_splits = choose_units(plan.segs[:, 1], h, hkv, d, num_cus)
         keys, queries, row_lo, row_end, self.covered = build_units(plan.segs, spans, n, self.key_rows, rows)
         self.num_keys, self.num_queries = len(keys), len(queries)
         self.blob = _upload(np.concatenate([keys.ravel(), queries.ravel(), row_lo, row_end]), self.device)
@@ -234,11 +248,11 @@ def _backward(ctx, q, k, v, out, lse, grad):
     if n:
         t.use()
         q, k, v, grad = (A._kernel_view(x) for x in (q, k, v, grad))
-        nbytes = workspace_size(h, n)
+        nbytes = workspace_size(h, hkv, d, n, t.key_splits)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rows = [f for x in (q, k, v, out, grad) for f in (x.data_ptr(), x.stride(1), x.stride(0))]
         grads = [f for x in (dq, dk, dv) for f in (x.data_ptr(), x.stride(1), x.stride(0))]
         call_backward(_native.stream(q.device), GRAD_ABI_VERSION, A._DTYPES[q.dtype], h, hkv, d, n, _native.f32(ctx.scale), t.key_rows,
                       *rows, lse.data_ptr(), *grads, t.keys, t.num_keys, t.queries, t.num_queries, t.row_lo, t.row_end,
-                      ctx.past[0].data_ptr(), ctx.num_pasts, ws.data_ptr(), nbytes)
+                      ctx.past[0].data_ptr(), ctx.num_pasts, ws.data_ptr(), nbytes, t.key_splits, 0)
     return tuple(x if need else None for x, need in zip((dq, dk, dv), ctx.needs_input_grad))

@@ -51,11 +51,12 @@ struct GradParams {
   const float *lse;
   float *stats;    // [2][H][N]: (bias - lse) / c, -delta
   float *partial;  // [3][partials]: max |G row|^2, max |V row|^2, max |delta|
+  float *parts;    // [splits][2][Hkv][N][D]: dK, dV
   const DanGradKeyUnit *key_units;
   const DanGradQueryUnit *query_units;
   const int32_t *row_lo, *row_end;
   const DanPastDesc *pasts;
-  int32_t num_tokens, num_heads, num_kv_heads, rep, hpw, groups, num_pasts, partials, key_rows;
+  int32_t num_tokens, num_heads, num_kv_heads, rep, hpw, groups, num_pasts, partials, key_rows, splits;
   float scale, c;  // c = scale * log2 e
 };
 
@@ -221,8 +222,10 @@ void grad_keys_kernel(const GradParams p) {
   const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
   const int lane = threadIdx.x & 63, hl = lane >> 5, wave = uni(threadIdx.x >> 6);
   const int kw = wave % KW, qw = wave / KW;
-  const int kvh = blockIdx.x % p.num_kv_heads;
-  const DanGradKeyUnit un = load_unit(p.key_units + blockIdx.x / p.num_kv_heads);
+  // A work group's unit, kv head, and part of the heads that share it.
+  const int kvh = blockIdx.x % p.num_kv_heads, part = blockIdx.x / p.num_kv_heads % p.splits;
+  const int head0 = kvh * p.rep + p.rep * part / p.splits, rep = kvh * p.rep + p.rep * (part + 1) / p.splits - head0;
+  const DanGradKeyUnit un = load_unit(p.key_units + blockIdx.x / (p.num_kv_heads * p.splits));
   if (un.start < 0 || un.n <= 0 || un.start + un.n > p.num_tokens || un.key0 < 0 || un.keys <= 0 || un.keys > p.key_rows ||
       un.key0 + un.keys > un.n || un.q_end <= un.key0 || un.q_end > un.n)
     return;  // no such rows
@@ -261,17 +264,17 @@ void grad_keys_kernel(const GradParams p) {
     for (int db = 0; db < ND; ++db) dk[s][db] = dv[s][db] = f32x16{};
 
   // Tiles in order: a head after the other, then the next 32 rows. A step takes QW of them; the KW waves that share one load it.
-  const int tiles = (un.q_end - un.key0 + 31) / 32 * p.rep, steps = (tiles + QW - 1) / QW;
+  const int tiles = (un.q_end - un.key0 + 31) / 32 * rep, steps = (tiles + QW - 1) / QW;
   const int64_t plane = (int64_t)p.num_heads * p.num_tokens;
-  const int rest = QW % p.rep, whole = QW / p.rep;  // from a wave's tile to its next: `rest` heads and 32 `whole` rows on
-  int next = min(qw, tiles - 1), next_head = next % p.rep, next_left = un.n - 1 - un.key0 - 32 * (next / p.rep);  // left: rows of the segment past the tile's first
+  const int rest = QW % rep, whole = QW / rep;  // from a wave's tile to its next: `rest` heads and 32 `whole` rows on
+  int next = min(qw, tiles - 1), next_head = next % rep, next_left = un.n - 1 - un.key0 - 32 * (next / rep);  // left: rows of the segment past the tile's first
   auto tile_at = [&](const void *base, int64_t st, int64_t sh) __attribute__((always_inline)) {
-    return uniform_ptr(static_cast<const char *>(base) + 2 * ((un.start + un.key0 + 32 * (int64_t)(next / p.rep)) * st + (kvh * p.rep + next_head) * sh));
+    return uniform_ptr(static_cast<const char *>(base) + 2 * ((un.start + un.key0 + 32 * (int64_t)(next / rep)) * st + (head0 + next_head) * sh));
   };
   const char *q_at = tile_at(p.q, p.q_st, p.q_sh), *g_at = tile_at(p.g, p.g_st, p.g_sh);
-  const float *s_at = uniform_ptr(p.stats + (int64_t)(kvh * p.rep + next_head) * p.num_tokens + un.start + un.key0 + 32 * (next / p.rep));
+  const float *s_at = uniform_ptr(p.stats + (int64_t)(head0 + next_head) * p.num_tokens + un.start + un.key0 + 32 * (next / rep));
   const int64_t q_on = 2 * (rest * p.q_sh + 32 * whole * p.q_st), g_on = 2 * (rest * p.g_sh + 32 * whole * p.g_st), s_on = rest * (int64_t)p.num_tokens + 32 * whole;
-  const int64_t q_wrap = 2 * (32 * p.q_st - p.rep * p.q_sh), g_wrap = 2 * (32 * p.g_st - p.rep * p.g_sh), s_wrap = 32 - p.rep * (int64_t)p.num_tokens;
+  const int64_t q_wrap = 2 * (32 * p.q_st - rep * p.q_sh), g_wrap = 2 * (32 * p.g_st - rep * p.g_sh), s_wrap = 32 - rep * (int64_t)p.num_tokens;
   const uint32_t q_row = (uint32_t)(2 * p.q_st), g_row = (uint32_t)(2 * p.g_st);
   // The x-th load of a step, into ring buffer b: every wave issues LOADS for every step (past its last tile, that
   // one's again), so that a count of them says which have landed. Rows past the segment are its last row's copies.
@@ -287,9 +290,9 @@ void grad_keys_kernel(const GradParams p) {
       // (each wave its own copy of the tile's statistics)
       dma4(s_at, (uint32_t)(min(lane & 31, next_left) * 4 + hl * (int)(plane * 4)), lds + (uint32_t)(Lds::stats + b * Lds::stat_step + wave * 256));
       // (selections, no branches: a step is one block of instructions)
-      const bool more = next + QW < tiles, wrap = more && next_head + rest >= p.rep;
+      const bool more = next + QW < tiles, wrap = more && next_head + rest >= rep;
       next += more ? QW : 0;
-      next_head += (more ? rest : 0) - (wrap ? p.rep : 0);
+      next_head += (more ? rest : 0) - (wrap ? rep : 0);
       next_left -= (more ? 32 * whole : 0) + (wrap ? 32 : 0);
       q_at += (more ? q_on : 0) + (wrap ? q_wrap : 0);
       g_at += (more ? g_on : 0) + (wrap ? g_wrap : 0);
@@ -304,6 +307,10 @@ void grad_keys_kernel(const GradParams p) {
   // out over that product fill, and the next tile's first operands are read at its end. With two buffers the barrier
   // stands before the first product, and the next step's loads go out over it.
   constexpr bool kEarly = NB > 2;
+  auto land = [&]() __attribute__((always_inline)) {  // (a tile that no other wave reads needs no barrier)
+    if constexpr (KW > 1) barrier_lds();
+    else barrier_wave_lds();
+  };
   f32x16 start;    // -lse / c of the tile's rows (then -delta)
   u32x4 ahead[2];  // the tile's first two operands
   auto read_stats = [&](int b, int which) __attribute__((always_inline)) {
@@ -328,7 +335,7 @@ void grad_keys_kernel(const GradParams p) {
     const uint32_t qt = tile_of(b), gt = qt + Tl::bytes;
     if constexpr (!kEarly) {
       wait_vmem<0>();
-      barrier_lds();
+      land();
       read_first(b);
     }
     f32x16 sc[NS], dp[NS];
@@ -346,7 +353,7 @@ void grad_keys_kernel(const GradParams p) {
       constexpr int i = decltype(index)::value, kk = i % NK, db = kk % ND, ks = kk / ND;
       if constexpr (kEarly && i == 3 * NK) {
         wait_vmem<(NB - 3) * LOADS>();
-        barrier_lds();
+        land();
       }
       if constexpr (i == NK - 1) read_stats(b, 1);
       if constexpr (kEarly && i == 4 * NK - 2) read_first(after);
@@ -383,11 +390,11 @@ void grad_keys_kernel(const GradParams p) {
 
   if constexpr (kHalf) factor *= 1.f / 16384.f;  // P carries 2^kPBias
   for (int i = 0; i < NB - 1; ++i) static_for<LOADS>([&](auto x) __attribute__((always_inline)) { issue(x, i); });
-  int b = 0, head = qw % p.rep, qb = un.key0 + 32 * (qw / p.rep), t = qw;  // of the wave's tile
+  int b = 0, head = qw % rep, qb = un.key0 + 32 * (qw / rep), t = qw;  // of the wave's tile
   // Steps up to `end`. A step past the wave's last tile sees nothing of it.
   if constexpr (kEarly) {
     wait_vmem<(NB - 2) * LOADS>();
-    barrier_lds();
+    land();
     read_first(0);
   }
   auto run = [&](auto masked, int &i, int end) __attribute__((always_inline)) {
@@ -395,9 +402,9 @@ void grad_keys_kernel(const GradParams p) {
       compute(masked, t < tiles ? qb : 0x3fffffff, b);
       b = b == NB - 1 ? 0 : b + 1;
       t += QW;
-      head += QW % p.rep;
-      qb += 32 * (QW / p.rep) + (head >= p.rep ? 32 : 0);
-      head -= head >= p.rep ? p.rep : 0;
+      head += QW % rep;
+      qb += 32 * (QW / rep) + (head >= rep ? 32 : 0);
+      head -= head >= rep ? rep : 0;
     }
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -406,7 +413,7 @@ void grad_keys_kernel(const GradParams p) {
     }
   };
   // The tiles that every key of the wave is seen from are a range: from the first whose rows all come after the keys.
-  const int full0 = (wkey + kWaveRows<D> - 1 - un.key0 + 31) / 32 * p.rep, full1 = max((low - un.key0) / 32, 0) * p.rep;
+  const int full0 = (wkey + kWaveRows<D> - 1 - un.key0 + 31) / 32 * rep, full1 = max((low - un.key0) / 32, 0) * rep;
   auto step_of = [&](int tile) __attribute__((always_inline)) { return min(max((tile - qw + QW - 1) / QW, 0), steps); };
   int i = 0;
   run(std::true_type{}, i, full0 < full1 ? step_of(full0) : steps);
@@ -450,10 +457,23 @@ void grad_keys_kernel(const GradParams p) {
     }
     if (qw > 0) return;
   }
+  // With several parts of the heads: fp32 sums, [part][dK, dV][kv head][row], for grad_sum_kernel.
   const float fv = kHalf ? 1.f / 16384.f : 1.f, fk = kHalf ? p.scale / (factor * 16384.f) : p.scale;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     const int64_t row = un.start + min(key[s], kend - 1);
+    if (p.splits > 1) {
+      float *kp = p.parts + ((2 * (int64_t)part * p.num_kv_heads + kvh) * p.num_tokens + row) * D + 4 * hl, *vp = kp + (int64_t)p.num_kv_heads * p.num_tokens * D;
+      if (key[s] < kend)
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            *(DAN_TILE_GLOBAL f32x4 *)(kp + 32 * db + 8 * x) = f32x4{dk[s][db][4 * x], dk[s][db][4 * x + 1], dk[s][db][4 * x + 2], dk[s][db][4 * x + 3]} * fk;
+            *(DAN_TILE_GLOBAL f32x4 *)(vp + 32 * db + 8 * x) = f32x4{dv[s][db][4 * x], dv[s][db][4 * x + 1], dv[s][db][4 * x + 2], dv[s][db][4 * x + 3]} * fv;
+          }
+      continue;
+    }
     T *kr = static_cast<T *>(p.dk) + row * p.dk_st + kvh * p.dk_sh, *vr = static_cast<T *>(p.dv) + row * p.dv_st + kvh * p.dv_sh;
 #pragma unroll
     for (int db = 0; db < ND; ++db) {
@@ -461,6 +481,23 @@ void grad_keys_kernel(const GradParams p) {
       store_column<T>(vr + 32 * db, dv[s][db], fv, hl, key[s] < kend);
     }
   }
+}
+
+// The parts of dK and dV added up in order, rounded once: 8 values a thread. Rows that no unit holds are left as they are.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grad_sum_kernel(const GradParams p, int d8) {
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, plane = (int64_t)p.num_kv_heads * p.num_tokens * d8;
+  if (at >= 2 * plane) return;
+  const int n = (int)(at / d8 % p.num_tokens), kvh = (int)(at / d8 / p.num_tokens % p.num_kv_heads);
+  if (p.row_end[n] <= 0) return;
+  const float *from = p.parts + at * 8;
+  f32x4 x = {}, y = {};
+  for (int i = 0; i < p.splits; ++i, from += 16 * plane) {
+    x += *(const DAN_TILE_GLOBAL f32x4 *)from;
+    y += *(const DAN_TILE_GLOBAL f32x4 *)(from + 4);
+  }
+  T *to = at < plane ? static_cast<T *>(p.dk) + n * p.dk_st + kvh * p.dk_sh : static_cast<T *>(p.dv) + n * p.dv_st + kvh * p.dv_sh;
+  store16(to + 8 * (at % d8), pack8<T>(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)));
 }
 
 // ---------------------------------------------------------------- dQ
@@ -739,6 +776,10 @@ hipError_t launch_all(const GradParams &p, int64_t keys_grid, int64_t queries_gr
   constexpr int KW = 64 / kWaveRows<D>;  // runs of a wave's keys in the smaller unit
   err = p.key_rows == 128 ? launch_keys<T, D, 2 * KW>(p, keys_grid, s) : launch_keys<T, D, KW>(p, keys_grid, s);
   if (err != hipSuccess) return err;
+  if (p.splits > 1) {
+    hipLaunchKernelGGL((grad_sum_kernel<T>), dim3((uint32_t)(((int64_t)p.num_kv_heads * p.num_tokens * (D / 4) + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, p, D / 8);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+  }
   constexpr int bytes = QueryLds<D>::total;
   static const hipError_t attr = allow_lds(grad_queries_kernel<T, D>, bytes);
   if (attr != hipSuccess) return attr;
@@ -763,9 +804,11 @@ int32_t dan_tree_grad_query_rows(int32_t num_heads, int32_t num_kv_heads, int32_
   return dan::wave_rows(head_dim) * 4 / dan::heads_of_group(num_heads / num_kv_heads);
 }
 
-int64_t dan_tree_grad_workspace_size(int32_t num_heads, int32_t num_tokens) {
-  if (num_heads <= 0 || num_tokens <= 0) return 0;
-  return ((int64_t)num_heads * num_tokens * 8 + 3 * dan::kMaxPartials * 4 + dan::kAlign - 1) / dan::kAlign * dan::kAlign;
+// delta and the statistics, the bound's partials; then the parts of dK and dV.
+static int64_t stats_bytes(int64_t H, int64_t N) { return (H * N * 8 + 3 * dan::kMaxPartials * 4 + dan::kAlign - 1) / dan::kAlign * dan::kAlign; }
+int64_t dan_tree_grad_workspace_size(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_tokens, int32_t key_splits) {
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 || num_tokens <= 0 || key_splits < 1 || key_splits > num_heads / num_kv_heads) return 0;
+  return stats_bytes(num_heads, num_tokens) + (key_splits > 1 ? (int64_t)key_splits * 2 * num_kv_heads * num_tokens * head_dim * 4 : 0);
 }
 
 int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
@@ -784,11 +827,12 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   if (!(a->scale >= 0x1p-100f && a->scale <= 0x1p100f)) return fail(DAN_ERR_INVALID_ARGUMENT, "scale must be from 2^-100 to 2^100");
   if (a->key_rows != dan_tree_grad_key_rows(D, 0) && a->key_rows != dan_tree_grad_key_rows(D, 1))
     return fail(DAN_ERR_INVALID_ARGUMENT, "key_rows %d: dan_tree_grad_key_rows", a->key_rows);
+  if (a->key_splits < 1 || a->key_splits > H / Hkv) return fail(DAN_ERR_INVALID_ARGUMENT, "key_splits %d: 1 to the %d heads of a kv head", a->key_splits, H / Hkv);
   if (N == 0 || a->num_key_units == 0 || a->num_query_units == 0) return DAN_OK;
   if (!a->q || !a->k || !a->v || !a->out || !a->grad || !a->lse || !a->dq || !a->dk || !a->dv || !a->key_units || !a->query_units ||
       !a->row_lo || !a->row_end || (a->num_pasts > 0 && !a->pasts))
     return fail(DAN_ERR_INVALID_ARGUMENT, "NULL tensor or table pointer");
-  const int64_t need = dan_tree_grad_workspace_size(H, N);
+  const int64_t need = dan_tree_grad_workspace_size(H, Hkv, D, N, a->key_splits);
   if (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & (kAlign - 1)))
     return fail(DAN_ERR_INVALID_ARGUMENT, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
   const int64_t strides[] = {a->q_stride_tok, a->q_stride_head, a->k_stride_tok, a->k_stride_head, a->v_stride_tok, a->v_stride_head,
@@ -823,11 +867,14 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   p.hpw = heads_of_group(p.rep);
   p.groups = Hkv * ((p.rep + p.hpw - 1) / p.hpw);
   p.key_rows = a->key_rows;
+  p.splits = a->key_splits;
+  p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(a->workspace) + stats_bytes(H, N));
   const int64_t rows_a_block = kThreads / (D / 8);
   p.partials = (int)std::min<int64_t>(kMaxPartials, ((int64_t)H * N + rows_a_block - 1) / rows_a_block);
   p.scale = a->scale;
   p.c = a->scale * 1.4426950408889634f;
-  const int64_t keys_grid = (int64_t)a->num_key_units * Hkv, queries_grid = (int64_t)a->num_query_units * p.groups;
+  const int64_t keys_grid = (int64_t)a->num_key_units * Hkv * p.splits, queries_grid = (int64_t)a->num_query_units * p.groups;
+  if ((int64_t)Hkv * N * (D / 4) >= int64_t(1) << 32) return fail(DAN_ERR_UNSUPPORTED, "%d kv heads x %d tokens: too many for one launch", Hkv, N);
   if (keys_grid * kThreads >= (int64_t(1) << 32) || queries_grid * kThreads >= (int64_t(1) << 32))
     return fail(DAN_ERR_UNSUPPORTED, "%lld and %lld work groups: fewer than 2^24", (long long)keys_grid, (long long)queries_grid);
   hipStream_t s = static_cast<hipStream_t>(stream);

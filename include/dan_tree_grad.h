@@ -70,6 +70,8 @@ typedef struct {
   const int32_t *row_lo, *row_end;
   const DanPastDesc *pasts; int32_t num_pasts;
   void *workspace; int64_t workspace_bytes; /* dan_tree_grad_workspace_size() bytes, 256-byte aligned */
+  /* Parts of the heads of a kv head that work groups of their own take for dK and dV, added up afterwards: 1 to num_heads / num_kv_heads. */
+  int32_t key_splits, reserved;
 } DanTreeGradArgs;
 
 int dan_tree_grad_abi_version(void);
@@ -78,7 +80,7 @@ int32_t dan_tree_grad_key_rows(int32_t head_dim, int32_t small);
 /* Query rows of a query unit; 0: unsupported head layout. */
 int32_t dan_tree_grad_query_rows(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
 /* Bytes of workspace (0: invalid arguments). */
-int64_t dan_tree_grad_workspace_size(int32_t num_heads, int32_t num_tokens);
+int64_t dan_tree_grad_workspace_size(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_tokens, int32_t key_splits);
 /* dan_tree_attn_fwd of bf16 or fp16 inputs, and lse [num_heads][num_tokens]
  * (fp32): log2 of the sum over a row's visible keys of 2^(score * scale * log2 e). */
 int dan_tree_attn_fwd_lse(const DanTreeAttnArgs *args, float *lse, void *stream);

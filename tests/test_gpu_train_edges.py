@@ -201,12 +201,12 @@ def test_backward_leaves_rows_of_no_unit_alone(gpu):
     args, pasts_host, _ = A._call_args(q, k, v, segs, 0, None, None, _native.PHASES_ALL, False, upload=False)
     A._launch_tree_attn(*args, None, pasts_host, launch=lambda *a: _grad.call_forward_lse(lse.data_ptr(), *a), zero=True)
     buffers = [torch.full((n + 4, x.shape[0], d), 7.0, dtype=BF16, device=gpu) for x in (q, k, v)]
-    ws = torch.empty(_grad.workspace_size(h, n), dtype=torch.uint8, device=gpu)
+    ws = torch.empty(_grad.workspace_size(h, 2, d, n, t.key_splits), dtype=torch.uint8, device=gpu)
     o = out.detach()
     _grad.call_backward(_native.stream(gpu), _grad.GRAD_ABI_VERSION, _native.DTYPE_BF16, h, 2, d, n, _native.f32(d ** -0.5), t.key_rows,
                         *[f for x in (q, k, v, o, grad) for f in (x.data_ptr(), x.stride(1), x.stride(0))], lse.data_ptr(),
                         *[f for x in buffers for f in (x.data_ptr(), x.stride(0), x.stride(1))], t.keys, t.num_keys, t.queries, t.num_queries,
-                        t.row_lo, t.row_end, segs.tile_plan.past_tables[0][0].data_ptr(), 0, ws.data_ptr(), ws.numel())
+                        t.row_lo, t.row_end, segs.tile_plan.past_tables[0][0].data_ptr(), 0, ws.data_ptr(), ws.numel(), t.key_splits, 0)
     torch.cuda.synchronize()
     inside = torch.zeros(n + 4, dtype=torch.bool, device=gpu)
     for s in segs:

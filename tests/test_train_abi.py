@@ -58,7 +58,7 @@ GRAD = dict(abi_version=1, dtype=_native.DTYPE_BF16, num_heads=4, num_kv_heads=2
             **{f: P for f in ("q", "k", "v", "out", "grad", "lse", "dq", "dk", "dv", "key_units", "query_units", "row_lo", "row_end", "workspace")},
             **{f"{t}_stride_tok": 512 for t in ("q", "k", "v", "o", "g", "dq", "dk", "dv")},
             **{f"{t}_stride_head": 64 for t in ("q", "k", "v", "o", "g", "dq", "dk", "dv")},
-            num_key_units=1, num_query_units=1, workspace_bytes=1 << 20)
+            num_key_units=1, num_query_units=1, key_splits=1, workspace_bytes=1 << 20)
 NORM = dict(abi_version=1, dtype=_native.DTYPE_BF16, rows=3, cols=64, norm=0, layout=0, eps=1e-6, x=P, x_stride=64, weight=P, out=P, out_stride=64)
 NORM_GRAD = dict(abi_version=1, dtype=_native.DTYPE_BF16, rows=3, cols=64, norm=0, s=P, s_stride=64, weight=P, rstd=P, g=P, g_stride=64, ds=P, ds_stride=64)
 ADAPT = dict(abi_version=1, dtype=_native.DTYPE_BF16, rows=3, n_in=64, n_out=32, rank=8, adapters=2, x=P, x_stride=64, y=P, y_stride=32, a=P, b=P,
@@ -70,7 +70,7 @@ ERRORS = [
         (dict(abi_version=2), VERSION, "abi_version"), (dict(num_heads=3), BAD, "num_heads"), (dict(num_kv_heads=0), BAD, "num_heads"),
         (dict(head_dim=96), UNSUPPORTED, "head_dim"), (dict(dtype=_native.DTYPE_F32), UNSUPPORTED, "dtype"), (dict(num_tokens=-1), BAD, "negative"),
         (dict(scale=float("nan")), BAD, "scale"), (dict(scale=-0.1), BAD, "scale"), (dict(scale=0.0), BAD, "scale"), (dict(scale=2.0 ** 101), BAD, "scale"),
-        (dict(key_rows=32), BAD, "key_rows"), (dict(lse=None), BAD, "NULL"), (dict(num_pasts=1), BAD, "NULL"), (dict(workspace_bytes=64), BAD, "workspace"),
+        (dict(key_rows=32), BAD, "key_rows"), (dict(key_splits=0), BAD, "key_splits"), (dict(key_splits=3), BAD, "key_splits"), (dict(lse=None), BAD, "NULL"), (dict(num_pasts=1), BAD, "NULL"), (dict(workspace_bytes=64), BAD, "workspace"),
         (dict(workspace=P + 16), BAD, "workspace"), (dict(q=P + 8), BAD, "aligned"), (dict(dk=P + 2), BAD, "aligned"), (dict(g_stride_tok=510), BAD, "strides"),
         (dict(k_stride_tok=1 << 25), UNSUPPORTED, "token stride"), (dict(v_stride_tok=-512), UNSUPPORTED, "token stride"), (dict(num_tokens=0, q=None), OK, ""))
 ] + [
@@ -115,7 +115,8 @@ def test_argument_errors_come_before_any_launch(lib, name, kw, status, needle): 
 
 def test_sizes_of_what_the_entries_do_not_take_are_0(lib):  # noqa: F811
     assert lib.dan_tree_grad_key_rows(96, 0) == 0 and lib.dan_tree_grad_query_rows(3, 2, 64) == 0 and lib.dan_tree_grad_query_rows(4, 2, 96) == 0
-    assert _grad.workspace_size(0, 5) == 0 and _grad.workspace_size(4, -1) == 0
+    assert _grad.workspace_size(0, 2, 64, 5) == 0 and _grad.workspace_size(4, 2, 64, -1) == 0
+    assert _grad.workspace_size(4, 2, 64, 5, 0) == 0 and _grad.workspace_size(4, 2, 64, 5, 3) == 0 and _grad.workspace_size(4, 2, 64, 5, 2) > _grad.workspace_size(4, 2, 64, 5)
     assert _layer.norm_grad_workspace_size(-1, 64) == 0 and _layer.norm_grad_workspace_size(4, 60) == 0
     assert _layer.adapt_workspace_size(0, 64, 16) == 0 and _layer.adapt_workspace_size(4, 64, 129) == 0
     assert _layer.adapt_grad_workspace_size(4, 60, 64, 16, 1) == 0 and _layer.adapt_grad_workspace_size(4, 64, 64, 16, 0) == 0
