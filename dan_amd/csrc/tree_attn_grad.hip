@@ -483,21 +483,22 @@ void grad_keys_kernel(const GradParams p) {
   }
 }
 
-// The parts of dK and dV added up in order, rounded once: 8 values a thread. Rows that no unit holds are left as they are.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void grad_sum_kernel(const GradParams p, int d8) {
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, plane = (int64_t)p.num_kv_heads * p.num_tokens * d8;
-  if (at >= 2 * plane) return;
-  const int n = (int)(at / d8 % p.num_tokens), kvh = (int)(at / d8 / p.num_tokens % p.num_kv_heads);
-  if (p.row_end[n] <= 0) return;
-  const float *from = p.parts + at * 8;
+// The parts of dK and dV added up in order, rounded once: 8 values a thread of one kv head's dK or dV. Rows that no unit
+// holds are left as they are.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void grad_sum_kernel(const GradParams p) {
+  constexpr int L = D / 8;
+  const int n = blockIdx.x * (kThreads / L) + threadIdx.x / L, kvh = blockIdx.y, which = blockIdx.z, column = threadIdx.x % L * 8;
+  if (n >= p.num_tokens || p.row_end[n] <= 0) return;
+  const int64_t plane = (int64_t)p.num_kv_heads * p.num_tokens * D;
+  const float *from = p.parts + which * plane + ((int64_t)kvh * p.num_tokens + n) * D + column;
   f32x4 x = {}, y = {};
-  for (int i = 0; i < p.splits; ++i, from += 16 * plane) {
+  for (int i = 0; i < p.splits; ++i, from += 2 * plane) {
     x += *(const DAN_TILE_GLOBAL f32x4 *)from;
     y += *(const DAN_TILE_GLOBAL f32x4 *)(from + 4);
   }
-  T *to = at < plane ? static_cast<T *>(p.dk) + n * p.dk_st + kvh * p.dk_sh : static_cast<T *>(p.dv) + n * p.dv_st + kvh * p.dv_sh;
-  store16(to + 8 * (at % d8), pack8<T>(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)));
+  T *to = which ? static_cast<T *>(p.dv) + n * p.dv_st + kvh * p.dv_sh : static_cast<T *>(p.dk) + n * p.dk_st + kvh * p.dk_sh;
+  store16(to + column, pack8<T>(__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)));
 }
 
 // ---------------------------------------------------------------- dQ
@@ -777,7 +778,8 @@ hipError_t launch_all(const GradParams &p, int64_t keys_grid, int64_t queries_gr
   err = p.key_rows == 128 ? launch_keys<T, D, 2 * KW>(p, keys_grid, s) : launch_keys<T, D, KW>(p, keys_grid, s);
   if (err != hipSuccess) return err;
   if (p.splits > 1) {
-    hipLaunchKernelGGL((grad_sum_kernel<T>), dim3((uint32_t)(((int64_t)p.num_kv_heads * p.num_tokens * (D / 4) + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, p, D / 8);
+    constexpr int R = kThreads / (D / 8);
+    hipLaunchKernelGGL((grad_sum_kernel<T, D>), dim3((p.num_tokens + R - 1) / R, p.num_kv_heads, 2), dim3(kThreads), 0, s, p);
     if ((err = hipGetLastError()) != hipSuccess) return err;
   }
   constexpr int bytes = QueryLds<D>::total;
@@ -874,7 +876,8 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   p.scale = a->scale;
   p.c = a->scale * 1.4426950408889634f;
   const int64_t keys_grid = (int64_t)a->num_key_units * Hkv * p.splits, queries_grid = (int64_t)a->num_query_units * p.groups;
-  if ((int64_t)Hkv * N * (D / 4) >= int64_t(1) << 32) return fail(DAN_ERR_UNSUPPORTED, "%d kv heads x %d tokens: too many for one launch", Hkv, N);
+  if (p.splits > 1 && (Hkv > 65535 || (int64_t)Hkv * N * (D / 4) >= int64_t(1) << 31))
+    return fail(DAN_ERR_UNSUPPORTED, "%d kv heads x %d tokens in parts: too many for one launch", Hkv, N);
   if (keys_grid * kThreads >= (int64_t(1) << 32) || queries_grid * kThreads >= (int64_t(1) << 32))
     return fail(DAN_ERR_UNSUPPORTED, "%lld and %lld work groups: fewer than 2^24", (long long)keys_grid, (long long)queries_grid);
   hipStream_t s = static_cast<hipStream_t>(stream);
