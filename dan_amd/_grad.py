@@ -99,7 +99,8 @@ def choose_units(lengths, h, hkv, d, num_cus):
 
     Larger units read less of Q and G, smaller ones and parts of the heads fill the chip: each of a number of parts that
     divides the heads evenly and gives up to two work groups a compute unit, while the longest unit keeps 16 steps (the parts
-    are written and read again in fp32)."""
+    are written and read again in fp32). Forward and backward pass, us: 8192 rows, 32/8 heads x 128, units of 128 / 64 keys 2264
+    / 2293, 3413 rows in four requests 314 / 252; 2000 rows, 16/2 heads x 128, 1 part / 4 parts 346 / 216; 700 rows, 8/2 x 64, 90.3 / 92.5."""
     whole, small = (int((-(-lengths // _rows(h, hkv, d, x)[0])).sum()) * hkv for x in (False, True))
     if whole >= num_cus or not small:
         return _rows(h, hkv, d, False)[0], 1

@@ -73,8 +73,8 @@ def norm_grad_workspace_size(rows, cols):
 
 
 @functools.lru_cache(maxsize=1024)
-def adapt_workspace_size(rows, n_in, rank):
-    return _sized("dan_adapt_workspace_size", _i64, 3)(rows, n_in, rank)
+def adapt_workspace_size(rows, n_in, rank, adapters):
+    return _sized("dan_adapt_workspace_size", _i64, 4)(rows, n_in, rank, adapters)
 
 
 @functools.lru_cache(maxsize=1024)

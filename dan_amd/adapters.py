@@ -42,7 +42,7 @@ def _forward(y, x, a, b, index, scale, want_down):
     out = torch.empty((n, n_out), dtype=x.dtype, device=x.device)
     down = torch.empty((n, _down_rank(r)), dtype=torch.float32, device=x.device) if want_down else None
     if n:
-        nbytes = _layer.adapt_workspace_size(n, n_in, r)
+        nbytes = _layer.adapt_workspace_size(n, n_in, r, a.shape[0])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         _layer.call_adapt(
             _native.stream(x.device), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, r, a.shape[0], 0,

@@ -14,6 +14,11 @@
 // of which there are plenty, and keeps 16 bits or more of v. fp16 numbers are first brought near 1 by a power
 // of 2 (of a row, or of a tile of rows), so that no v leaves their range.
 //
+// Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 16 us (67 MB), up 188 us (940 MB, 5.0 TB/s); gradients: down 130 us
+// (470 MB, 3.6 TB/s), up 21, outer 109 (537 MB, 4.9 TB/s) and its sum 5. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
+// and chains of index, weights and sums; 1037 rows, 5 adapters of rank 64, 4096 -> 4096, fp16: down 14, up 14, outer 26 (the same
+// chains: 1024 values instead of 4096 take down 13.4 us).
+//
 // Rows of different adapters may lie in any order. A tile of 16 rows multiplies all of them by each adapter
 // that occurs in it and keeps the rows that are its own by selection, not by adding zeros, so that an
 // adapter that holds infinities or NaN reaches no other request's rows.
@@ -37,7 +42,6 @@ namespace {
 using namespace tiles;
 
 constexpr int kThreads = 256;
-constexpr int kFewRows = 512;    // up to here the kernels for few rows
 constexpr int kChunk = 128;      // values of the wide side that a wave of `down` takes at a time
 constexpr int kUpCols = 64;      // columns of a wave of `up`
 constexpr int kOuterCols = 128;  // columns of a work group of `outer`
@@ -752,10 +756,16 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
 // Ranks as the kernels are built for: 16, 32, 64 or 128.
 int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
+// The kernels for few rows or those for many. The former take 5 us and more with every row and rank, the latter 13 us and 4 more with each
+// adapter of a tile of 32 rows. 4096 -> 4096, us, few / many: one adapter of rank 16, 256 rows 9.6 / 12.7, 512 rows 15.4 / 13.0; of rank 128,
+// 128 rows 19.8 / 22.6, 256 rows 34.6 / 23.1; 24 adapters of rank 16 in any order, 512 rows 24.9 / 53.9, 1024 rows 45.6 / 56.5; 8 of rank 64, 384 rows
+// 47.6 / 53.2, 640 rows 83.4 / 66.5. (The order of the rows is on the device alone; 5 adapters of rank 64 one behind the other, 384 rows: 26.4 / 21.4.)
+bool few(int rows, int rank, int adapters) { return rows <= (128 + 4096 / ranks_of(rank)) * (adapters > 4 ? 2 : 1); }
+
 // Parts of `down`'s sum over n: as many work groups as fill the chip, of at least a chunk a wave (many rows) or two.
-int splits_of(int rows, int n, int rank) {
+int splits_of(int rows, int n, int rank, int adapters) {
   const int chunks = (n + kChunk - 1) / kChunk;
-  if (rows <= kFewRows) return std::max(1, std::min({chunks, std::max(2, 1024 / ((rows + 15) / 16)), 32}));
+  if (few(rows, rank, adapters)) return std::max(1, std::min({chunks, std::max(2, 1024 / ((rows + 15) / 16)), 32}));
   const int tiles = (rows + 31) / 32, waves = ranks_of(rank) <= 32 ? 16 : 8;
   return std::max(1, std::min((256 + tiles - 1) / tiles, chunks / waves));
 }
@@ -769,7 +779,7 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 template <typename T, int JB>
 hipError_t launch_down(const DownParams &p, int splits, hipStream_t s) {
-  if (p.rows <= kFewRows) {
+  if (few(p.rows, p.rank, p.adapters)) {
     hipLaunchKernelGGL((down_few_kernel<T, JB>), dim3((p.rows + 15) / 16, splits), dim3(64 * kFewWaves), 0, s, p);
     return hipGetLastError();
   }
@@ -789,7 +799,7 @@ hipError_t launch_down(DownParams p, int splits, hipStream_t s) {
 
 template <typename T, int ST>
 hipError_t launch_up(UpParams p, hipStream_t s) {
-  if (p.rows <= kFewRows) {
+  if (few(p.rows, p.rank, p.adapters)) {
     hipLaunchKernelGGL((up_few_kernel<T, ST>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
     return hipGetLastError();
   }
@@ -819,7 +829,7 @@ hipError_t forward(const DanAdaptArgs &a, hipStream_t s) {
   DownParams d;
   d.x = a.x; d.x_stride = a.x_stride; d.w = a.a; d.index = a.index; d.part = static_cast<float *>(a.workspace);
   d.rows = a.rows; d.n = a.n_in; d.rank = a.rank; d.adapters = a.adapters; d.ranks = ranks_of(a.rank);
-  const int splits = splits_of(a.rows, a.n_in, a.rank);
+  const int splits = splits_of(a.rows, a.n_in, a.rank, a.adapters);
   hipError_t err = launch_down<T>(d, splits, s);
   if (err != hipSuccess) return err;
   UpParams u;
@@ -834,7 +844,7 @@ struct GradSpace {
   int64_t at, bt, list, starts, part, g, da, db, total;
   int splits, parts;
   GradSpace(int rows, int n_in, int n_out, int rank, int adapters) {
-    splits = splits_of(rows, n_out, rank);
+    splits = splits_of(rows, n_out, rank, adapters);
     parts = parts_of(rows, n_in, n_out, adapters);
     at = 0;
     bt = align256(at + (int64_t)adapters * rank * n_in * 2);
@@ -922,9 +932,9 @@ extern "C" {
 
 int dan_adapt_abi_version(void) { return DAN_ADAPT_ABI_VERSION; }
 
-int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank) {
-  if (rows <= 0 || n_in <= 0 || rank <= 0 || rank > DAN_ADAPT_MAX_RANK) return 0;
-  return (int64_t)dan::splits_of(rows, n_in, rank) * rows * dan::ranks_of(rank) * 4;
+int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank, int32_t adapters) {
+  if (rows <= 0 || n_in <= 0 || rank <= 0 || rank > DAN_ADAPT_MAX_RANK || adapters <= 0) return 0;
+  return (int64_t)dan::splits_of(rows, n_in, rank, adapters) * rows * dan::ranks_of(rank) * 4;
 }
 
 int64_t dan_adapt_grad_workspace_size(int32_t rows, int32_t n_in, int32_t n_out, int32_t rank, int32_t adapters) {
@@ -945,7 +955,7 @@ int dan_adapt(const DanAdaptArgs *a, void *stream) {
   if (bad_rows(a->x, a->x_stride) || bad_rows(a->y, a->y_stride) || bad_rows(a->out, a->out_stride) || (a->rows > 1 && a->out_stride < a->n_out) ||
       (((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->down) & 15))
     return fail(DAN_ERR_INVALID_ARGUMENT, "rows must start 16-byte aligned, and written ones must not overlap");
-  const int64_t need = dan_adapt_workspace_size(a->rows, a->n_in, a->rank);
+  const int64_t need = dan_adapt_workspace_size(a->rows, a->n_in, a->rank, a->adapters);
   if (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & 15))
     return fail(DAN_ERR_INVALID_ARGUMENT, "workspace needs %lld bytes, 16-byte aligned", (long long)need);
   hipStream_t s = static_cast<hipStream_t>(stream);

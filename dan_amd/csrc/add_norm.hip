@@ -10,6 +10,9 @@
 // squares, its largest value and its stores; y is rounded once, from fp32, also where it becomes codes. The
 // gradient reads s as it was stored (rounded to 16 bits): the two addends would be one tensor more to read,
 // and what the rounding moves is of the size of the result's own.
+//
+// Measured, warm: 8192 x 4096 in bf16 to stream and codes 38 us (235 MB, 6.1 TB/s), 7 x 4096 3.9 us (a launch, its loads, two
+// reductions); 4099 x 2048 in fp16 to stream and out 13.0 us (67 MB, 5.2 TB/s), its gradient 14.8 (67 MB, 4.5) and dw's sum 6.8.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -150,7 +153,8 @@ __global__ __launch_bounds__(kThreads) void add_norm_kernel(const NormParams p) 
     for (int c = p.cols + 8 * t; c < 64 * p.kt; c += 8 * L) *(DAN_TILE_GLOBAL u32x2 *)(p.codes + dan_fp8::tiled_offset(row, c, p.kt)) = u32x2{0u, 0u};
 }
 
-// Rows blockIdx.x, + gridDim.x, ...: each group keeps its rows' sum of dw in registers.
+// Rows blockIdx.x, + gridDim.x, ...: each group keeps its rows' sum of dw in registers, so that dw takes one pass over s and
+// G with ds, in an order that the number of rows alone fixes.
 template <typename T, int NC>
 __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const GradParams p) {
   __shared__ float sums[2][4];
@@ -239,6 +243,8 @@ hipError_t launch_norm(const NormParams &p, hipStream_t s) {
 template <typename T>
 hipError_t launch_norm(const NormParams &p, hipStream_t s) {
   const int pieces = (p.cols + 8 * kThreads - 1) / (8 * kThreads);
+  // (a wave a row needs no barrier: 8192 rows with codes, 512 columns 7.6 us against a work group's 14.1, 1024 columns 11.8 against 17.3;
+  // 7 rows of 1024 columns 3.4 against 3.3)
   if (p.cols <= 512) return launch_norm<T, 64, 1>(p, s);
   if (p.cols <= 1024) return launch_norm<T, 64, 2>(p, s);
   if (pieces <= 1) return launch_norm<T, kThreads, 1>(p, s);

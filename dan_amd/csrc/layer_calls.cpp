@@ -25,7 +25,7 @@ struct Library {
   int64_t (*norm_grad_bytes)(int32_t, int32_t);
   int (*adapt)(const DanAdaptArgs *, void *);
   int (*adapt_grad)(const DanAdaptGradArgs *, void *);
-  int64_t (*adapt_bytes)(int32_t, int32_t, int32_t);
+  int64_t (*adapt_bytes)(int32_t, int32_t, int32_t, int32_t);
   int64_t (*adapt_grad_bytes)(int32_t, int32_t, int32_t, int32_t, int32_t);
   int (*attn_lse)(const DanTreeAttnArgs *, float *, void *);
   int (*attn_grad)(const DanTreeGradArgs *, void *);
@@ -202,7 +202,7 @@ Tensor adapt_forward(const Tensor &y, const Tensor &x, const Tensor &ad, const T
     *down = at::empty({n, ranks_of(rank)}, x.options().dtype(at::kFloat).requires_grad(false));
     a.down = static_cast<float *>(at_of(*down));
   }
-  a.workspace_bytes = lib.adapt_bytes((int32_t)n, (int32_t)n_in, (int32_t)rank);
+  a.workspace_bytes = lib.adapt_bytes((int32_t)n, (int32_t)n_in, (int32_t)rank, (int32_t)ad.size(0));
   const Tensor ws = bytes(a.workspace_bytes, x);
   a.workspace = at_of(ws);
   a.abi_version = DAN_ADAPT_ABI_VERSION;

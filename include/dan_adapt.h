@@ -62,7 +62,7 @@ typedef struct {
 
 int dan_adapt_abi_version(void);
 /* 0: invalid arguments. */
-int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank);
+int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank, int32_t adapters);
 int64_t dan_adapt_grad_workspace_size(int32_t rows, int32_t n_in, int32_t n_out, int32_t rank, int32_t adapters);
 int dan_adapt(const DanAdaptArgs *args, void *stream);
 int dan_adapt_grad(const DanAdaptGradArgs *args, void *stream);

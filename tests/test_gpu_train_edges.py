@@ -288,6 +288,18 @@ def test_adapters_in_other_layouts(gpu):
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+@pytest.mark.parametrize("n,n_in,n_out,rank,count", [  # on both sides of where the kernels for many rows begin, for each rank
+    (384, 136, 72, 16, 2), (385, 136, 72, 16, 2), (769, 136, 72, 16, 5), (256, 264, 72, 32, 3), (257, 264, 72, 32, 3), (193, 600, 136, 64, 1),
+    (385, 72, 264, 40, 6), (160, 520, 264, 128, 2), (161, 520, 264, 128, 2), (321, 136, 200, 104, 9), (1100, 8, 8, 8, 1)])
+def test_where_many_rows_begin(gpu, n, n_in, n_out, rank, count, order, dtype):
+    say(f"adapt {n} rows {n_in} -> {n_out} rank {rank} x {count} {dtype} {order}")
+    args = test_gpu_adapt.make(gpu, n, n_in, n_out, rank, count, dtype, order=order)
+    y, x, a, b, index, scale, grad = args
+    test_gpu_adapt.check(test_gpu_adapt.run(*args), oracle.adapt(y, x, a, b, index.tolist(), scale, grad), dtype, ["out", "dx", "da", "db"])
+
+
 def test_many_adapters_and_few_rows_each(gpu):
     say("adapt: 300 adapters")
     args = test_gpu_adapt.make(gpu, 520, 64, 72, 8, 300, BF16)
@@ -317,7 +329,7 @@ def test_the_c_entry_writes_in_place_and_no_row_more(gpu):
         want = adapt(y, x, a, b, index, scale)
         out = torch.full((n + 3, 208), 7.0, dtype=BF16, device=gpu)
         out[:n, :200] = y
-        nbytes = _layer.adapt_workspace_size(n, 136, 16)
+        nbytes = _layer.adapt_workspace_size(n, 136, 16, 3)
         ws = torch.full((nbytes + 64,), 5, dtype=torch.uint8, device=gpu)
         _layer.call_adapt(_native.stream(gpu), _layer.ADAPT_ABI_VERSION, _native.DTYPE_BF16, n, 136, 200, 16, 3, 0, x.data_ptr(), x.stride(0),
                           out.data_ptr(), 208, a.data_ptr(), b.data_ptr(), index.data_ptr(), scale.data_ptr(), 0.0, out.data_ptr(), 208, 0, ws.data_ptr(), nbytes)

@@ -118,7 +118,7 @@ def test_sizes_of_what_the_entries_do_not_take_are_0(lib):  # noqa: F811
     assert _grad.workspace_size(0, 2, 64, 5) == 0 and _grad.workspace_size(4, 2, 64, -1) == 0
     assert _grad.workspace_size(4, 2, 64, 5, 0) == 0 and _grad.workspace_size(4, 2, 64, 5, 3) == 0 and _grad.workspace_size(4, 2, 64, 5, 2) > _grad.workspace_size(4, 2, 64, 5)
     assert _layer.norm_grad_workspace_size(-1, 64) == 0 and _layer.norm_grad_workspace_size(4, 60) == 0
-    assert _layer.adapt_workspace_size(0, 64, 16) == 0 and _layer.adapt_workspace_size(4, 64, 129) == 0
+    assert _layer.adapt_workspace_size(0, 64, 16, 1) == 0 and _layer.adapt_workspace_size(4, 64, 129, 1) == 0
     assert _layer.adapt_grad_workspace_size(4, 60, 64, 16, 1) == 0 and _layer.adapt_grad_workspace_size(4, 64, 64, 16, 0) == 0
 
 
