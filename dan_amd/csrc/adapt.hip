@@ -784,8 +784,8 @@ hipError_t launch_down(const DownParams &p, int splits, hipStream_t s) {
     return hipGetLastError();
   }
   constexpr int W = kDownWaves<JB>, bytes = W / 2 * JB * 2 * 1024;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(down_kernel<T, JB>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (attr != hipSuccess) return attr;
+  const hipError_t err = allow_lds<&down_kernel<T, JB>>(bytes);
+  if (err != hipSuccess) return err;
   hipLaunchKernelGGL((down_kernel<T, JB>), dim3(splits, (p.rows + 31) / 32), dim3(64 * W), bytes, s, p);
   return hipGetLastError();
 }

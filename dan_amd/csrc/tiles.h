@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include <type_traits>
 #include <utility>
 
@@ -106,6 +108,18 @@ __device__ inline const T *uniform_ptr(const T *p) {
   const uint64_t v = (uint64_t)(uintptr_t)p;
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
   return (const T *)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Host: lets a kernel have `bytes` of dynamic LDS, once for each device.
+template <auto kernel>
+hipError_t allow_lds(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  hipError_t err = hipGetDevice(&device);
+  if (err != hipSuccess || ((done.load(std::memory_order_relaxed) >> (device & 63)) & 1)) return err;
+  err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == hipSuccess) done.fetch_or(uint64_t(1) << (device & 63), std::memory_order_relaxed);
+  return err;
 }
 
 // Direct loads to LDS of 16 (4) bytes a lane: lane l's land at lds + 16 l (4 l). The address is a uniform

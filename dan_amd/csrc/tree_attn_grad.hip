@@ -774,16 +774,11 @@ void grad_queries_kernel(const GradParams p) {
 int wave_rows(int D) { return D == 256 ? 32 : 64; }
 int heads_of_group(int rep) { return rep >= 3 ? 4 : rep; }
 
-template <typename K>
-hipError_t allow_lds(K kernel, int bytes) {
-  return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <typename T, int D, int KW>
 hipError_t launch_keys(const GradParams &p, int64_t grid, hipStream_t s) {
   constexpr int bytes = KeyLds<D, KW>::total;
-  static const hipError_t attr = allow_lds(grad_keys_kernel<T, D, KW>, bytes);
-  if (attr != hipSuccess) return attr;
+  const hipError_t err = allow_lds<&grad_keys_kernel<T, D, KW>>(bytes);
+  if (err != hipSuccess) return err;
   hipLaunchKernelGGL((grad_keys_kernel<T, D, KW>), dim3((uint32_t)grid), dim3(kThreads), bytes, s, p);
   return hipGetLastError();
 }
@@ -802,8 +797,7 @@ hipError_t launch_all(const GradParams &p, int64_t keys_grid, int64_t queries_gr
     if ((err = hipGetLastError()) != hipSuccess) return err;
   }
   constexpr int bytes = QueryLds<D>::total;
-  static const hipError_t attr = allow_lds(grad_queries_kernel<T, D>, bytes);
-  if (attr != hipSuccess) return attr;
+  if ((err = allow_lds<&grad_queries_kernel<T, D>>(bytes)) != hipSuccess) return err;
   hipLaunchKernelGGL((grad_queries_kernel<T, D>), dim3((uint32_t)queries_grid), dim3(kThreads), bytes, s, p);
   return hipGetLastError();
 }

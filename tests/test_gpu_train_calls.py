@@ -3,8 +3,11 @@ graphs, what a second derivative and a changed input raise, and repeated runs.
 
 Results are compared bit for bit where the same kernels run on the same values, and with the fp64 oracle elsewhere
 (test_gpu_norm, test_gpu_adapt and test_gpu_attend_train derive the tolerances)."""
+import threading
+
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import test_gpu_adapt
 import test_gpu_attend_train
@@ -66,7 +69,6 @@ class _Rest:
 
 
 NAMES = ["norm", "adapt", "attend"]
-both_ways = pytest.mark.parametrize("through", ["module", "python"])
 
 
 @pytest.fixture
@@ -363,6 +365,74 @@ def test_compiled_functions_break_the_graph_and_agree(gpu):
         out = f(*leaves)
         got = [x.detach() for x in out] + list(torch.autograd.grad(out, leaves, c.grads))
         assert same(got, want)
+
+
+@ways
+@pytest.mark.parametrize("name", NAMES)
+def test_a_kept_graph_twice(gpu, name, way):
+    say(name, way, "backward twice through a kept graph")
+    c = Case(name, gpu)
+    want = c.run()
+    leaves = c.fresh()
+    out = c.call(*leaves)
+    for _ in range(2):
+        assert same(torch.autograd.grad(out, leaves, c.grads, retain_graph=True), want[len(out):])
+
+
+@ways
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_that_leave_the_gpu(gpu, name, way):
+    """What a call saves passes through torch's hooks: kept on the CPU, and made again by a checkpoint."""
+    say(name, way, "saved on the CPU, and checkpointed")
+    c = Case(name, gpu)
+    want = c.run()
+    leaves = c.fresh()
+    with torch.autograd.graph.save_on_cpu():
+        out = c.call(*leaves)
+    assert same(torch.autograd.grad(out, leaves, c.grads), want[len(out):])
+    for reentrant in (False, True):
+        leaves = c.fresh()
+        out = torch.utils.checkpoint.checkpoint(lambda *xs: tuple(c.call(*xs)), *leaves, use_reentrant=reentrant)
+        torch.autograd.backward(out, c.grads)
+        assert same([x.grad for x in leaves], want[len(out):])
+
+
+@ways
+def test_a_list_of_segments(gpu, way):
+    say("attend", way, "a plain list instead of a Batch")
+    c = Case("attend", gpu)
+    want = c.run()
+    c.segs = list(c.segs)
+    for _ in range(2):
+        assert same(c.run(), want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_two_threads_on_two_streams(gpu, name):
+    """Two programs in one process: each thread its own inputs and stream; the batch (its tables) is shared."""
+    say(name, "two threads")
+    c = Case(name, gpu)
+    want = [c.run(), c.run([x.detach().mul(0.5).requires_grad_() for x in c.leaves])]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got = c.run([x.detach().mul(0.5 if i else 1.0).requires_grad_() for x in c.leaves])
+                    torch.cuda.current_stream().synchronize()
+                    if not same(got, want[i]):
+                        bad.append(i)
+        except Exception as e:  # noqa: BLE001  -- (shown by the assertion below)
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
 
 
 def derivative(call, oracle_call, leaves, grads, weights, dtype, step):

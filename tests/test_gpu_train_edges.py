@@ -168,15 +168,15 @@ def test_scores_that_single_out_one_key(gpu, dtype):
         assert worst.max().item() <= 1, name
 
 
-def test_prefixes_with_wide_rows_and_large_offsets(gpu):
+@pytest.mark.parametrize("wide", [1 << 24, 1 << 25])
+def test_prefixes_with_wide_rows_and_large_offsets(gpu, wide):
     """A prefix whose rows lie 2^24 elements apart, and inputs whose rows do: offsets within a tile pass 2^30 bytes, and
-    those of the whole pass 2^32."""
-    say("attend_train, rows 2^24 elements apart")
-    wide = 1 << 24
+    those of the whole pass 2^32. From 2^25 on they are copied."""
+    say(f"attend_train, rows {wide} elements apart")
     q, k, v, grad, segs = test_gpu_attend_train.make(gpu, [(40, [30])], 2, 1, 64, BF16, pasts=[70])
     want = test_gpu_attend_train.train(q, k, v, grad, segs)
 
-    def spread(x):  # [heads, n, d] with token strides of 2^24
+    def spread(x):  # [heads, n, d] with token strides of `wide`
         out = torch.empty(x.shape[1] * wide, dtype=x.dtype, device=gpu).as_strided(x.shape, (x.shape[2], wide, 1))
         return out.copy_(x)
 
