@@ -15,7 +15,7 @@
 // of 2 (of a row, or of a tile of rows), so that no v leaves their range.
 //
 // Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 16 us (67 MB), up 188 us (940 MB, 5.0 TB/s); gradients: down 130 us
-// (470 MB, 3.6 TB/s), up 21, outer 109 (537 MB, 4.9 TB/s) and its sum 5. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
+// (470 MB, 3.6 TB/s), up 21, outer 95 (537 MB, 5.7 TB/s; with loads that the caches keep 108) and its sum 5. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
 // and chains of index, weights and sums; 1037 rows, 5 adapters of rank 64, 4096 -> 4096, fp16: down 14, up 14, outer 26 (the same
 // chains: 1024 values instead of 4096 take down 13.4 us).
 //

@@ -132,8 +132,8 @@ __device__ inline void dma16(const void *base, uint32_t off, uint32_t lds) {
                "s"(__builtin_amdgcn_readfirstlane(lds))
                : "memory", "m0");
 }
-__device__ inline void dma16_at(const void *from, uint32_t lds) {  // (an address of each lane)
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
+__device__ inline void dma16_at(const void *from, uint32_t lds) {  // (an address of each lane, read once: past the caches)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
 }
 __device__ inline void dma4(const void *base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(uniform_ptr((const char *)base)),
