@@ -14,8 +14,8 @@
 // of which there are plenty, and keeps 16 bits or more of v. fp16 numbers are first brought near 1 by a power
 // of 2 (of a row, or of a tile of rows), so that no v leaves their range.
 //
-// Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 16 us (67 MB), up 188 us (940 MB, 5.0 TB/s); gradients: down 130 us
-// (470 MB, 3.6 TB/s), up 21, outer 95 (537 MB, 5.7 TB/s; with loads that the caches keep 108) and its sum 5. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
+// Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 21 us (67 MB), up 205 us (940 MB, 4.6 TB/s); gradients: g and dB in one
+// pass 100 us (500 MB, 5 TB/s; in two, 130 + 83), g's parts 7, up 20, dA 19, the parts' sum 8. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
 // and chains of index, weights and sums; 1037 rows, 5 adapters of rank 64, 4096 -> 4096, fp16: down 14, up 14, outer 26 (the same
 // chains: 1024 values instead of 4096 take down 13.4 us).
 //
@@ -46,6 +46,9 @@ constexpr int kChunk = 128;      // values of the wide side that a wave of `down
 constexpr int kUpCols = 64;      // columns of a wave of `up`
 constexpr int kOuterCols = 128;  // columns of a work group of `outer`
 constexpr int kOuterRows = 32;   // rows of a step of `outer`
+// Bytes of G from which dB and g come from one pass. Backward passes of one adapter, 4096 wide, one pass / two, us: 8192 x 4096 (64 MB) 82 / 79,
+// 2048 x 28672 (112 MB) 64 / 71, 8192 x 14336 (224 MB) 107 / 148, 8192 x 28672 (448 MB) 160 / 263: what the caches keep is cheap to read twice.
+constexpr int64_t kBothBytes = 96 << 20;
 
 // c += A B of a 16x16x32 product. Lane l holds row l % 16 of A (column of B) at k = 8 (l / 16) + 0..7, and of c
 // column l % 16, rows 4 (l / 16) + 0..3.
@@ -634,12 +637,176 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
     }
 }
 
+// dB and g = G B_i for ranks up to 16 in bf16, from one pass over G: one adapter, 512 columns in four tiles, a part of the adapter's rows.
+// A wave takes 32 rows at a time, and of them a tile after the other, the next one on its way into its second buffer; from
+// LDS the tile is read twice, as `outer`'s operand and as rows. g is summed over the work group's columns alone: parts, a
+// sixteenth of G's bytes, for gather_kernel.
+constexpr int kBothTiles = 4;
+struct BothParams {
+  OuterParams o;   // its side b
+  const void *bt;  // B^T [adapters][rank][n_out]
+  float *g;        // [column tiles][rows][16]
+};
+__global__ __launch_bounds__(kThreads, 2) void both_kernel(const BothParams p) {
+  using T = __bf16;
+  using Tl = Tile<kOuterCols>;
+  constexpr int CB = kOuterCols / 16, CT = kBothTiles;
+  static_assert(CT % 2 == 0, "the buffers' turn");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
+  const OuterSide &q = p.o.b;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), l16 = lane & 15, g4 = lane >> 4;
+  const int c0 = blockIdx.x * CT * kOuterCols, i = blockIdx.y, part = blockIdx.z, last = q.cols - 8;
+  const int start = p.o.starts ? p.o.starts[i] : 0, total = p.o.starts ? p.o.starts[i + 1] - start : i == 0 ? p.o.rows : 0;
+  const int from = start + (int)((int64_t)total * part / p.o.parts), count = start + (int)((int64_t)total * (part + 1) / p.o.parts) - from;
+  auto row_of = [&](int k) { return p.o.list ? p.o.list[from + k] : from + k; };
+  // The columns' B^T as operands, behind the waves' buffers: [tile][step of 32 columns][lane].
+  u32x4 *bf = reinterpret_cast<u32x4 *>(smem + 8 * Tl::bytes);
+  {
+    static_assert(CT == 4, "a tile a wave");
+    const T *row = static_cast<const T *>(p.bt) + ((int64_t)i * p.o.rank + min(l16, p.o.rank - 1)) * q.cols;
+    u32x4 b[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) b[s] = load16(row + min(c0 + wave * kOuterCols + 32 * s + 8 * g4, last));
+#pragma unroll
+    for (int s = 0; s < 4; ++s) bf[(4 * wave + s) * 64 + lane] = c0 + wave * kOuterCols + 32 * s + 8 * g4 > last ? u32x4{} : b[s];
+    __syncthreads();
+  }
+  f32x4 acc[CT][CB];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) acc[ct][cb] = f32x4{};
+  const uint32_t tile = lds + (uint32_t)(wave * 2 * Tl::bytes);
+  auto issue = [&](int ct, int mine) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < Tl::blocks; ++x) {
+      const int64_t n = __shfl(mine, Tl::block_row(x, lane));
+      const int c = min(c0 + ct * kOuterCols + (int)(Tl::block_byte(x, lane) / 2), last);
+      dma16_at(static_cast<const T *>(q.z) + n * q.z_stride + c, tile + (uint32_t)((ct & 1) * Tl::bytes + x * 1024));
+    }
+  };
+  float vn[8];  // the next step's v
+  auto load_v = [&](int mine) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vn[e] = q.v[(int64_t)__shfl(mine, 8 * g4 + e) * p.o.ranks + l16];
+  };
+  int mine = 0, next = 0;  // lane l: the step's row l % 32, and the next step's
+  auto rows_at = [&](int s0) { return row_of(min(s0 + (lane & 31), count - 1)); };
+  if (wave * kOuterRows < count) {
+    mine = rows_at(wave * kOuterRows);
+    next = rows_at((wave + 4) * kOuterRows);
+    issue(0, mine);
+    load_v(mine);
+  }
+  for (int s0 = wave * kOuterRows; s0 < count; s0 += 4 * kOuterRows) {
+    const int rows = min(count - s0, kOuterRows), after = next;
+    f32x8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 8 * g4 + e < rows ? vn[e] : 0.f;
+    const u32x4 hi = pack8<T>(x), lo = pack8<T>(x - unpack8<T>(hi));
+    f32x4 g[2] = {};
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      wait_vmem<0>();
+      barrier_wave_lds();  // (the reads of the buffer that is filled next)
+      // (places in memory and in LDS are worked out again for each tile: kept, they would not leave registers for the sums)
+      int l = lane;
+      asm volatile("" : "+v"(mine), "+v"(l));
+      const int m16 = l & 15, h4 = l >> 4;
+      if (ct + 1 < CT) {
+        issue(ct + 1, mine);
+      } else {
+        issue(0, after);
+        load_v(after);
+        next = rows_at(s0 + 8 * kOuterRows);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t at_tile = tile + (uint32_t)((ct & 1) * Tl::bytes);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const u32x4 b = bf[(4 * ct + s) * 64 + lane];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const int r = 16 * f + m16;
+          g[f] = mfma16<T>(b, lds_read16(at_tile + (uint32_t)(r * Tl::row + (((4 * s + h4) ^ Tl::swizzle(r)) << 4))), g[f]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        u32x4 zf;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 8 * h4 + 4 * h + (m16 >> 2);
+          const uint32_t at = at_tile + (uint32_t)(r * Tl::row + (((2 * cb + ((m16 >> 1) & 1)) ^ Tl::swizzle(r)) << 4) + 8 * (m16 & 1));
+          const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((DAN_TILE_LDS i16x4 *)(uintptr_t)at));
+          zf[2 * h] = t[0];
+          zf[2 * h + 1] = t[1];
+        }
+        if (rows < kOuterRows) {  // rows past the list: zeros, whatever its last row (whose copies they are) holds
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (8 * g4 + e >= rows) zf[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+        }
+        acc[ct][cb] = mfma16<T>(lo, zf, mfma16<T>(hi, zf, acc[ct][cb]));
+        __builtin_amdgcn_sched_barrier(0);  // (reads of one block at a time: the registers hold no more)
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int64_t n = __shfl(mine, 16 * f + l16);
+      if (16 * f + l16 < rows) *(DAN_TILE_GLOBAL f32x4 *)(p.g + ((int64_t)blockIdx.x * p.o.rows + n) * 16 + 4 * g4) = g[f];
+    }
+    mine = after;
+  }
+  wait_vmem<0>();  // (the last step's loads of a next one)
+  // The waves' sums, added in order.
+  f32x4 *red = reinterpret_cast<f32x4 *>(smem);
+  const float c = p.o.scale ? p.o.scale[i] : p.o.scale_value;
+  float *to = q.sums + ((int64_t)part * p.o.adapters + i) * p.o.rank * q.cols;
+  T *out = static_cast<T *>(q.out) + (int64_t)i * p.o.rank * q.cols;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    __syncthreads();
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) red[(wave * CB + cb) * 64 + lane] = acc[ct][cb];
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int cb = half * 4 + wave, col = c0 + ct * kOuterCols + 16 * cb + l16;
+      const f32x4 sum = ((red[cb * 64 + lane] + red[(CB + cb) * 64 + lane]) + (red[(2 * CB + cb) * 64 + lane] + red[(3 * CB + cb) * 64 + lane])) * c;
+      if (col < q.cols && 4 * g4 < p.o.rank) {
+        const int64_t at = (int64_t)col * p.o.rank + 4 * g4;
+        if (p.o.parts == 1) *(DAN_TILE_GLOBAL u32x2 *)(out + at) = pack4<T>(sum);
+        else *(DAN_TILE_GLOBAL f32x4 *)(to + at) = sum;
+      }
+    }
+  }
+}
+
+// g's parts added up in order: four lanes share 16 bytes of the result. (Rows of no adapter have no parts, and nothing reads
+// what they get.)
+__global__ __launch_bounds__(kThreads) void gather_kernel(const float *parts, float *g, int rows, int tiles) {
+  const int lane = threadIdx.x & 63, share = lane >> 4;
+  const int64_t quad = ((int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * 16 + (lane & 15), quads = 4 * (int64_t)rows;
+  const float *from = parts + 4 * min(quad, quads - 1);
+  f32x4 x = {};
+#pragma unroll 8
+  for (int t = share; t < tiles; t += 4) x += *(const DAN_TILE_GLOBAL f32x4 *)(from + t * 4 * quads);
+#pragma unroll
+  for (int m = 16; m < 64; m <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], m);
+  if (share == 0 && quad < quads) *(DAN_TILE_GLOBAL f32x4 *)(g + 4 * quad) = x;
+}
+
 // The parts of dA and dB added up in order, rounded once: 8 values a thread.
 struct SumParams {
   const float *a, *b;
   void *da, *db;
   int64_t na, nb;  // values of dA, dB (multiples of 8)
-  int32_t parts;
+  int32_t parts_a, parts_b;
 };
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
@@ -650,7 +817,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
   if (at >= n) return;
   const float *from = (b ? p.b : p.a) + at;
   f32x4 x = {}, y = {};
-  for (int i = 0; i < p.parts; ++i, from += n) {
+  for (int i = 0, parts = b ? p.parts_b : p.parts_a; i < parts; ++i, from += n) {
     x += *(const DAN_TILE_GLOBAL f32x4 *)from;
     y += *(const DAN_TILE_GLOBAL f32x4 *)(from + 4);
   }
@@ -775,6 +942,12 @@ int parts_of(int rows, int n_in, int n_out, int adapters) {
   const int64_t by_rows = rows / (512 * (int64_t)adapters);
   return (int)std::max<int64_t>(1, std::min<int64_t>((1024 + groups - 1) / groups, by_rows));
 }
+// g and dB from one pass (both_kernel; fp16's powers of 2 of each step would leave it no registers): where G does not fit the caches from one pass to the next.
+bool both(int rows, int n_out, int rank) { return ranks_of(rank) == 16 && (int64_t)rows * n_out * 2 >= kBothBytes; }
+int both_tiles(int n_out) { return (n_out + kBothTiles * kOuterCols - 1) / (kBothTiles * kOuterCols); }
+int both_parts(int rows, int n_out, int adapters) {  // (two work groups fit a compute unit)
+  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / ((int64_t)both_tiles(n_out) * adapters), rows / (512 * (int64_t)adapters)));
+}
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 template <typename T, int JB>
@@ -842,20 +1015,23 @@ hipError_t forward(const DanAdaptArgs &a, hipStream_t s) {
 // The workspace of the gradient: A^T, B^T, the list of rows, g in parts and added up, and the parts of dA and dB.
 struct GradSpace {
   int64_t at, bt, list, starts, part, g, da, db, total;
-  int splits, parts;
+  int splits, parts, parts_a, parts_b;  // (parts_a, parts_b: where g and dB come from one pass)
   GradSpace(int rows, int n_in, int n_out, int rank, int adapters) {
     splits = splits_of(rows, n_out, rank, adapters);
     parts = parts_of(rows, n_in, n_out, adapters);
+    const bool one = both(rows, n_out, rank);
+    parts_a = one ? parts_of(rows, n_in, 0, adapters) : parts;
+    parts_b = one ? both_parts(rows, n_out, adapters) : parts;
     at = 0;
     bt = align256(at + (int64_t)adapters * rank * n_in * 2);
     list = align256(bt + (int64_t)adapters * rank * n_out * 2);
     starts = list + (int64_t)rows * 4;
     part = align256(starts + ((int64_t)adapters + 1) * 4);
-    g = align256(part + (int64_t)splits * rows * ranks_of(rank) * 4);
+    g = align256(part + (int64_t)std::max(splits, one ? both_tiles(n_out) : 0) * rows * ranks_of(rank) * 4);
     da = align256(g + (int64_t)rows * ranks_of(rank) * 4);
-    const int64_t kept = parts > 1 ? parts : 0;
-    db = align256(da + kept * adapters * rank * n_in * 4);
-    total = align256(db + kept * adapters * rank * n_out * 4);
+    auto kept = [&](int other) { return (int64_t)std::max({parts > 1 ? parts : 0, other > 1 ? other : 0}); };
+    db = align256(da + kept(parts_a) * adapters * rank * n_in * 4);
+    total = align256(db + kept(parts_b) * adapters * rank * n_out * 4);
   }
 };
 
@@ -882,23 +1058,44 @@ hipError_t backward(const DanAdaptGradArgs &a, const GradSpace &w, hipStream_t s
       hipLaunchKernelGGL(turn_kernel, dim3(groups), dim3(kThreads), 0, s, t);
     if ((err = hipGetLastError()) != hipSuccess) return err;
   }
-  if (a.dx || a.da) {
+  const bool one = a.db && (a.dx || a.da) && std::is_same<T, __bf16>::value && both(a.rows, a.n_out, a.rank);
+  float *g = reinterpret_cast<float *>(ws + w.g);
+  if (one) {
+    BothParams b;
+    b.o = o; b.o.parts = w.parts_b; b.bt = ws + w.bt; b.g = reinterpret_cast<float *>(ws + w.part);
+    const int tiles = both_tiles(a.n_out);
+    constexpr int bytes = 8 * Tile<kOuterCols>::bytes + kBothTiles * 4096;
+    if ((err = allow_lds<&both_kernel>(bytes)) != hipSuccess) return err;
+    hipLaunchKernelGGL(both_kernel, dim3(tiles, a.adapters, w.parts_b), dim3(kThreads), bytes, s, b);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    hipLaunchKernelGGL(gather_kernel, dim3((a.rows + 15) / 16), dim3(kThreads), 0, s, b.g, g, a.rows, tiles);
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+  } else if (a.dx || a.da) {
     DownParams d;
     d.x = a.g; d.x_stride = a.g_stride; d.w = ws + w.bt; d.index = a.index; d.part = reinterpret_cast<float *>(ws + w.part);
     d.rows = a.rows; d.n = a.n_out; d.rank = a.rank; d.adapters = a.adapters; d.ranks = o.ranks;
     if ((err = launch_down<T>(d, w.splits, s)) != hipSuccess) return err;
+  }
+  if (a.dx || (a.da && !one)) {
     UpParams u;  // (without dx: no columns, the sum of the parts alone)
-    u.part = d.part; u.sum = reinterpret_cast<float *>(ws + w.g); u.w = ws + w.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride;
+    u.part = one ? g : reinterpret_cast<float *>(ws + w.part); u.sum = one ? nullptr : g; u.w = ws + w.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride;
     u.index = a.index; u.scale = a.scale; u.scale_value = a.scale_value;
-    u.rows = a.rows; u.cols = a.dx ? a.n_in : 0; u.rank = a.rank; u.adapters = a.adapters; u.ranks = o.ranks; u.splits = w.splits; u.steps = 1;
+    u.rows = a.rows; u.cols = a.dx ? a.n_in : 0; u.rank = a.rank; u.adapters = a.adapters; u.ranks = o.ranks; u.splits = one ? 1 : w.splits; u.steps = 1;
     if ((err = launch_up<T>(u, s)) != hipSuccess) return err;
   }
   if (!a.da && !a.db) return hipSuccess;
-  if ((err = launch_outer<T>(o, s)) != hipSuccess || w.parts == 1) return err;
+  if (one) {
+    o.b.tiles = 0;
+    o.parts = w.parts_a;
+  }
+  if (o.a.tiles + o.b.tiles && (err = launch_outer<T>(o, s)) != hipSuccess) return err;
   SumParams m;
-  m.a = o.a.sums; m.b = o.b.sums; m.da = a.da; m.db = a.db; m.parts = w.parts;
-  m.na = a.da ? (int64_t)a.adapters * a.rank * a.n_in : 0;
-  m.nb = a.db ? (int64_t)a.adapters * a.rank * a.n_out : 0;
+  m.a = o.a.sums; m.b = o.b.sums; m.da = a.da; m.db = a.db;
+  m.parts_a = one ? w.parts_a : w.parts;
+  m.parts_b = one ? w.parts_b : w.parts;
+  m.na = a.da && m.parts_a > 1 ? (int64_t)a.adapters * a.rank * a.n_in : 0;
+  m.nb = a.db && m.parts_b > 1 ? (int64_t)a.adapters * a.rank * a.n_out : 0;
+  if (!m.na && !m.nb) return hipSuccess;
   hipLaunchKernelGGL(sum_kernel<T>, dim3((uint32_t)(((m.na + m.nb) / 8 + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, m);
   return hipGetLastError();
 }
@@ -917,7 +1114,7 @@ int check_sizes(int dtype, int rows, int n_in, int n_out, int rank, int adapters
   if (!(isfinite(scale_value))) return fail(DAN_ERR_INVALID_ARGUMENT, "scale_value must be finite");
   const int64_t wide = std::max(n_in, n_out);  // (`up` has the most threads by far: 2 columns of 16 rows each for few rows)
   if (too_many(over(wide, kUpCols) * over(rows, 16) * 2) ||
-      too_many((over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters * parts_of(rows, n_in, n_out, adapters)) ||
+      too_many((over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters * std::max(parts_of(rows, n_in, n_out, adapters), parts_of(rows, n_in, 0, adapters))) ||
       too_many((over(n_in, 64) + over(n_out, 64) + 1) * adapters) ||
       too_many(over((int64_t)adapters * rank * ((int64_t)n_in + n_out), 8 * kThreads)))
     return fail(DAN_ERR_UNSUPPORTED, "%d rows, %d to %d, %d adapters: more than one launch holds", rows, n_in, n_out, adapters);

@@ -300,6 +300,36 @@ def test_where_many_rows_begin(gpu, n, n_in, n_out, rank, count, order, dtype):
     test_gpu_adapt.check(test_gpu_adapt.run(*args), oracle.adapt(y, x, a, b, index.tolist(), scale, grad), dtype, ["out", "dx", "da", "db"])
 
 
+@pytest.mark.parametrize("order", ["mixed", "runs", "one"])
+@pytest.mark.parametrize("n,n_in,n_out,rank,count", [(12300, 64, 4104, 16, 3), (6200, 136, 8200, 8, 1), (49000, 72, 1032, 16, 2), (3080, 64, 16456, 13, 40)])
+def test_gradients_of_wide_outputs(gpu, n, n_in, n_out, rank, count, order):
+    """From 96 MB of G on, dB and g come from one pass over it. Against fp64 on the GPU, an adapter at a time. Sums over the
+    rows are made in fp32 by parts of at most 2^9 rows a wave, and of some tens of those: 2^-24 (2^9 + 2^6) of their magnitudes, which 2^-13 covers with what the two numbers of v leave."""
+    say(f"adapt {n} rows {n_in} -> {n_out} rank {rank} x {count} {order}")
+    g = torch.Generator(device=gpu).manual_seed(0)
+
+    def new(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g, device=gpu) * std).to(BF16)
+
+    x, y, grad, a, b = new(n, n_in), new(n, n_out), new(n, n_out), new(count, rank, n_in, std=n_in ** -0.5), new(count, n_out, rank)
+    index = torch.randint(-1, count, (n,), generator=g, device=gpu).int() if order == "mixed" else torch.arange(n, device=gpu).mul(count).div(n, rounding_mode="floor").int()
+    if order == "one":
+        index = None if count == 1 else torch.full_like(index, count - 1)
+    scale = torch.rand(count, generator=g, device=gpu) + 0.5
+    got = test_gpu_adapt.run(y, x, a, b, index, scale, grad)
+    assert all(torch.equal(p, q) for p, q in zip(got, test_gpu_adapt.run(y, x, a, b, index, scale, grad)))
+    ref = {f: torch.zeros_like(t, dtype=torch.float64) for f, t in (("dx", x), ("da", a), ("db", b))}
+    ref.update({"abs_" + f: torch.zeros_like(t) for f, t in ref.items()})
+    for i in range(count):
+        rows = torch.arange(n, device=gpu) if index is None else (index == i).nonzero()[:, 0]
+        for prefix, (xx, gg, aa, bb) in (("", (x[rows].double(), grad[rows].double(), a[i].double(), b[i].double())),
+                                         ("abs_", (x[rows].double().abs(), grad[rows].double().abs(), a[i].double().abs(), b[i].double().abs()))):
+            c, h, low = scale[i].double(), xx @ aa.T, gg @ bb
+            ref[prefix + "dx"][rows] = c * (low @ aa)
+            ref[prefix + "da"][i], ref[prefix + "db"][i] = c * (low.T @ xx), c * (gg.T @ h)
+    test_gpu_adapt.check(got[1:], {f: t.cpu() for f, t in ref.items()}, BF16, ["dx", "da", "db"])
+
+
 def test_many_adapters_and_few_rows_each(gpu):
     say("adapt: 300 adapters")
     args = test_gpu_adapt.make(gpu, 520, 64, 72, 8, 300, BF16)
