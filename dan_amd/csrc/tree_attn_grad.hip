@@ -139,14 +139,17 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p)
       p.stats[at] = ((kHalf ? kPBias : 0.f) - p.lse[at]) / p.c;
       p.stats[rows + at] = -dot;
     }
-    gmax = fmaxf(gmax, sq);
-    dmax = fmaxf(dmax, fabsf(dot));
+    if (kHalf && p.row_end[n] > 0) {  // (rows of no segment may hold anything, and their dS is never made)
+      gmax = fmaxf(gmax, sq);
+      dmax = fmaxf(dmax, fabsf(dot));
+    }
   }
   if constexpr (kHalf) {
     const int64_t vrows = (int64_t)p.num_tokens * p.num_kv_heads;
     for (int64_t r = (int64_t)blockIdx.x * R + mine; r < vrows; r += (int64_t)gridDim.x * R) {
       const int64_t n = r / p.num_kv_heads, h = r % p.num_kv_heads;
-      vmax = fmaxf(vmax, row_square<T, L>(load16(static_cast<const T *>(p.v) + n * p.v_st + h * p.v_sh + 8 * sub)));
+      const float sq = row_square<T, L>(load16(static_cast<const T *>(p.v) + n * p.v_st + h * p.v_sh + 8 * sub));
+      if (p.row_end[n] > 0) vmax = fmaxf(vmax, sq);
     }
     for (int i = 0; i < p.num_pasts; ++i) {
       const DanPastDesc pd = load_unit(p.pasts + i);

@@ -37,12 +37,16 @@ def test_rows_of_no_segment_give_zeros(gpu, dtype):
     inside = torch.zeros(q.shape[1], dtype=torch.bool, device=gpu)
     for s in segs:
         inside[s.start:s.end] = True
-    poison = [x.clone() for x in (q, k, v, grad)]
-    for x in poison:
-        x[:, ~inside] = math.nan  # what lies in the gaps reaches nothing
-    got = test_gpu_attend_train.train(*poison, segs)
-    for x in got:
-        assert (x[:, ~inside] == 0).all()
+    # what lies in the gaps reaches nothing: not the power of 2 that fp16's dS is scaled by, either
+    grad = (grad.float() * 2.0 ** -10).to(dtype)
+    want = test_gpu_attend_train.train(q, k, v, grad, segs)
+    for value in (math.nan, math.inf, 6e4):
+        poison = [x.clone() for x in (q, k, v, grad)]
+        for x in poison:
+            x[:, ~inside] = value
+        got = test_gpu_attend_train.train(*poison, segs)
+        for x, w in zip(got, want):
+            assert (x[:, ~inside] == 0).all() and torch.equal(x, w)
     test_gpu_attend_train.check(got, oracle.attend(q, k, v, segs, 0, grad=grad), dtype)
 
 
