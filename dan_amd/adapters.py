@@ -21,14 +21,6 @@ def _down_rank(r):
     return 16 if r <= 16 else 32 if r <= 32 else 64 if r <= 64 else 128
 
 
-def _padded(a, b):
-    """The adapters with their rank brought to a multiple of 8 (by zeros), dense."""
-    pad = -a.shape[1] % 8
-    if pad:
-        a, b = nn.functional.pad(a, (0, 0, 0, pad)), nn.functional.pad(b, (0, pad))
-    return _layer.dense(a), _layer.dense(b)
-
-
 def _scale_args(scale):
     return (scale.data_ptr(), 0.0) if isinstance(scale, torch.Tensor) else (0, _native.f32(scale))
 
@@ -37,7 +29,7 @@ def _forward(y, x, a, b, index, scale, want_down):
     """(out, the rows' x A^T or None)."""
     (n, n_in), n_out = x.shape, y.shape[1]
     x, y = _layer.rows_of(x), _layer.rows_of(y)
-    a, b = _padded(a, b)
+    a, b = _layer.dense(a), _layer.dense(b)
     r = a.shape[1]
     out = torch.empty((n, n_out), dtype=x.dtype, device=x.device)
     down = torch.empty((n, _down_rank(r)), dtype=torch.float32, device=x.device) if want_down else None
@@ -78,22 +70,19 @@ class _Adapt(torch.autograd.Function):
 def _backward(x, a, b, down, index, scale, g, need):
     (n, n_in), n_out, rank = x.shape, b.shape[1], a.shape[1]
     dev = x.device
-    a8, b8 = _padded(a, b)
-    r, count = a8.shape[1], a8.shape[0]
+    a, b, count = _layer.dense(a), _layer.dense(b), a.shape[0]
     new = torch.empty if n else torch.zeros
     dx = new((n, n_in), dtype=x.dtype, device=dev) if need[0] else None
-    da, db = (new(t.shape, dtype=x.dtype, device=dev) if want else None for t, want in ((a8, need[1]), (b8, need[2])))
+    da, db = (new(t.shape, dtype=x.dtype, device=dev) if want else None for t, want in ((a, need[1]), (b, need[2])))
     if n:
         x, g = _layer.rows_of(x), _layer.rows_of(g)
-        nbytes = _layer.adapt_grad_workspace_size(n, n_in, n_out, r, count)
+        nbytes = _layer.adapt_grad_workspace_size(n, n_in, n_out, rank, count)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _layer.call_adapt_grad(
-            _native.stream(dev), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, r, count, 0,
-            x.data_ptr(), x.stride(0), g.data_ptr(), g.stride(0), a8.data_ptr(), b8.data_ptr(), 0 if index is None else index.data_ptr(),
+            _native.stream(dev), _layer.ADAPT_ABI_VERSION, _DTYPES[x.dtype], n, n_in, n_out, rank, count, 0,
+            x.data_ptr(), x.stride(0), g.data_ptr(), g.stride(0), a.data_ptr(), b.data_ptr(), 0 if index is None else index.data_ptr(),
             *_scale_args(scale), down.data_ptr(), 0 if dx is None else dx.data_ptr(), n_in, 0 if da is None else da.data_ptr(),
             0 if db is None else db.data_ptr(), ws.data_ptr(), nbytes)
-    if r != rank:
-        da, db = None if da is None else da[:, :rank].contiguous(), None if db is None else db[..., :rank].contiguous()
     return dx, da, db
 
 
@@ -108,7 +97,7 @@ def adapt(y, x, a, b, index=None, scale=1.0):
 
     Sums are fp32 in an order that the sizes alone fix; x a^T stays fp32, the result
     is rounded once. Rows of other adapters take no part in a row's sums, whatever
-    they hold. Ranks 1 to 128 (multiples of 8 need no copy), n_in and n_out multiples of 8
+    they hold. Ranks 1 to 128, n_in and n_out multiples of 8
     up to 2^20, at most 2^20 rows.
 
     Differentiable (once) in y, x, a and b. A backward pass that is captured into a HIP graph has

@@ -235,12 +235,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void down_few_kernel(const DownPara
 struct UpParams {
   const float *part;  // [splits][rows][ranks]
   float *sum;         // [rows][ranks]: v, for the gradient, or NULL
-  const void *w, *y;  // w [adapters][cols][rank]; y may be NULL (zeros)
+  const void *w, *y;  // w [adapters][cols][w_rank]; y may be NULL (zeros)
   void *out;
   const int32_t *index;
   const float *scale;
   int64_t y_stride, o_stride;
-  int32_t rows, cols, rank, adapters, ranks, splits, steps;  // steps of 256 columns a work group (many rows)
+  int32_t rows, cols, rank, w_rank, adapters, ranks, splits, steps;  // w_rank: rank, or with zeros a multiple of 8; steps of 256 columns a work group (many rows)
   float scale_value;
 };
 
@@ -299,12 +299,15 @@ struct Operand {
       }
     }
     __syncthreads();
-    const int r8 = p.rank / 8;
+    const int r8 = (p.rank + 7) / 8;
     for (int q = threadIdx.x; q < F * ST * 64; q += TH) {
       const int r = q / (64 * ST) * 16 + (q & 15), u = (q / 64) % ST * 4 + (q >> 4) % 4, j8 = u >= r8 ? u - r8 : u;
       u32x4 to = {};
       if (u < 2 * r8) {
         f32x8 x = __builtin_shufflevector(v[r][2 * j8], v[r][2 * j8 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        if (p.rank % 8)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = 8 * j8 + e < p.rank ? x[e] : 0.f;
         if (kHalf) {
           const int e2 = exponent_of(__builtin_bit_cast(float, top[r]));
 #pragma unroll
@@ -321,17 +324,28 @@ struct Operand {
 
 // The operand of 64 columns from m0 on. Lane (l16, g4) of the result owns 8 columns from m0 + 8 g4 on and 8 from m0 + 32 +
 // 8 g4 on, so that four lanes store 64 bytes of a row: row r of block b is column 32 (b / 2) + 8 (r / 4) + 4 (b % 2) + r % 4.
-template <typename T, int ST>
+// WHOLE: ranks in memory are a multiple of 8, whose pieces lie 16-byte aligned; otherwise they come one number at a time, by kernels
+// of their own (in one kernel with the others they would take registers, and waves, from them).
+template <typename T, int ST, bool WHOLE>
 __device__ inline void load_columns(const UpParams &p, int i, int m0, int l16, int g4, u32x4 (&wf)[ST][4]) {
-  const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.cols * p.rank;
-  const int r8 = p.rank / 8;
+  const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.cols * p.w_rank;
+  const int r8 = (p.rank + 7) / 8;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const int col = min(m0 + 32 * (b >> 1) + 8 * (l16 >> 2) + 4 * (b & 1) + (l16 & 3), p.cols - 1);
 #pragma unroll
     for (int t = 0; t < ST; ++t) {
       const int u = 4 * t + g4, j = u >= 2 * r8 ? 0 : 8 * (u >= r8 ? u - r8 : u);  // (past the last piece v holds zeros)
-      wf[t][b] = load16(w + (int64_t)col * p.rank + j);
+      const T *at = w + (int64_t)col * p.w_rank;
+      if constexpr (WHOLE) {
+        wf[t][b] = load16(at + j);
+      } else {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        t8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = ((const DAN_TILE_GLOBAL T *)at)[min(j + e, p.rank - 1)];
+        wf[t][b] = __builtin_bit_cast(u32x4, x);  // (past the last rank v holds zeros: times a finite copy of it)
+      }
     }
   }
 }
@@ -346,7 +360,7 @@ __device__ inline float factor_of(const UpParams &p, int i, uint32_t top) {
 // Many rows: 32 by `steps` times 256 columns, 64 a wave. y of the next step is loaded before this one's. (64 rows halve the
 // loads of w, but leave two waves a SIMD instead of four: 8192 rows of 6144 columns took 53.7 us, and take 46.6.)
 constexpr int kUpFrags = 2;
-template <typename T, int ST>
+template <typename T, int ST, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
   constexpr int F = kUpFrags;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
@@ -374,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
   int loaded = -1;  // the adapter that wf holds this step's columns of
   u32x4 wf[ST][4];
   auto load_w = [&](int i, int m0) __attribute__((always_inline)) {
-    load_columns<T, ST>(p, i, m0, l16, g4, wf);
+    load_columns<T, ST, WHOLE>(p, i, m0, l16, g4, wf);
     loaded = i;
   };
   {
@@ -450,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
 }
 
 // Few rows: 16 by 64 columns; the waves split the tile's adapters, and the first two store.
-template <typename T, int ST>
+template <typename T, int ST, bool WHOLE>
 __global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p) {
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
   __shared__ Operand<T, ST, 1, 64 * kFewWaves> op;
@@ -475,7 +489,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p
     float c = NAN;  // no such adapter
     u32x4 wf[ST][4];
     if (i < p.adapters) {
-      load_columns<T, ST>(p, i, m0, l16, g4, wf);
+      load_columns<T, ST, WHOLE>(p, i, m0, l16, g4, wf);
       c = factor_of<T>(p, i, kHalf ? op.top[l16] : 0u);
     } else {
 #pragma unroll
@@ -514,6 +528,18 @@ struct OuterParams {
   int32_t rows, rank, ranks, adapters, parts;
   float scale_value;
 };
+
+// Up to 4 numbers of a column of dB whose ranks are no multiple of 4: rounded to `out`, or as sums.
+template <typename T>
+__device__ inline void store_ranks(T *out, float *sums, f32x4 x, int count) {
+  const u32x2 r = pack4<T>(x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < count) {
+      if (out) ((DAN_TILE_GLOBAL uint16_t *)out)[e] = (uint16_t)(r[e >> 1] >> 16 * (e & 1));
+      else ((DAN_TILE_GLOBAL float *)sums)[e] = x[e];
+    }
+}
 
 // One adapter, 128 columns, a part of the adapter's rows; the waves take 32 of them in turn,
 // each through a tile of its own in LDS, from where the transposing reads make the operand whose inner dimension is
@@ -631,7 +657,8 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
       const int col = c0 + 16 * cb + (side_b ? l16 : row), j = 16 * jb + (side_b ? row : l16);
       const int64_t at = side_b ? (int64_t)col * p.rank + j : (int64_t)j * q.cols + col;
       if (col < q.cols && j < p.rank) {
-        if (p.parts == 1) *(DAN_TILE_GLOBAL u32x2 *)(out + at) = pack4<T>(sum);
+        if (side_b && p.rank % 4) store_ranks<T>(p.parts == 1 ? out + at : nullptr, to + at, sum, p.rank - j);
+        else if (p.parts == 1) *(DAN_TILE_GLOBAL u32x2 *)(out + at) = pack4<T>(sum);
         else *(DAN_TILE_GLOBAL f32x4 *)(to + at) = sum;
       }
     }
@@ -778,7 +805,8 @@ __global__ __launch_bounds__(kThreads, 2) void both_kernel(const BothParams p) {
       const f32x4 sum = ((red[cb * 64 + lane] + red[(CB + cb) * 64 + lane]) + (red[(2 * CB + cb) * 64 + lane] + red[(3 * CB + cb) * 64 + lane])) * c;
       if (col < q.cols && 4 * g4 < p.o.rank) {
         const int64_t at = (int64_t)col * p.o.rank + 4 * g4;
-        if (p.o.parts == 1) *(DAN_TILE_GLOBAL u32x2 *)(out + at) = pack4<T>(sum);
+        if (p.o.rank % 4) store_ranks<T>(p.o.parts == 1 ? out + at : nullptr, to + at, sum, p.o.rank - 4 * g4);
+        else if (p.o.parts == 1) *(DAN_TILE_GLOBAL u32x2 *)(out + at) = pack4<T>(sum);
         else *(DAN_TILE_GLOBAL f32x4 *)(to + at) = sum;
       }
     }
@@ -827,7 +855,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(const SumParams p) {
 // ---------------------------------------------------------------- transposes of A [R][rank][n_in] and B [R][n_out][rank], 16-bit
 struct TurnParams {
   const uint16_t *a, *b;
-  uint16_t *at, *bt;  // [R][n_in][rank], [R][rank][n_out]
+  uint16_t *at, *bt;  // [R][n_in][rank, with zeros a multiple of 8], [R][rank][n_out]
   const int32_t *index;      // NULL: no list
   int32_t *list, *starts;    // [rows], [adapters + 1]
   int32_t rows, rank, n_in, n_out, adapters, a_tiles, b_tiles;  // tiles of 64 columns an adapter
@@ -887,14 +915,17 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
   }
   const bool b = x >= p.a_tiles * p.adapters;
   if (b) x -= p.a_tiles * p.adapters;
-  const int tiles = b ? p.b_tiles : p.a_tiles, i = x / tiles, c0 = x % tiles * 64, wide = b ? p.n_out : p.n_in, r8 = p.rank / 8;
+  const int tiles = b ? p.b_tiles : p.a_tiles, i = x / tiles, c0 = x % tiles * 64, wide = b ? p.n_out : p.n_in, r8 = (p.rank + 7) / 8;
   const int64_t base = (int64_t)i * p.rank * wide;
   const uint16_t *from = (b ? p.b : p.a) + base;
-  uint16_t *to = (b ? p.bt : p.at) + base;
+  uint16_t *to = b ? p.bt + base : p.at + (int64_t)i * 8 * r8 * wide;
   const int c8 = min(64, wide - c0) / 8;  // pieces of 8 columns
   typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-  for (int e = threadIdx.x; e < 64 * r8; e += kThreads) {
-    if (b) {  // a column's ranks are contiguous
+  for (int e = threadIdx.x; e < (b && p.rank % 8 ? 64 * p.rank : b ? 64 * r8 : 8 * p.rank); e += kThreads) {
+    if (b && p.rank % 8) {  // a column's ranks are contiguous, in pieces of no certain alignment
+      const int c = e / p.rank, j = e % p.rank;
+      tile[j][c] = from[(int64_t)(c0 + min(c, 8 * c8 - 1)) * p.rank + j];
+    } else if (b) {  // a column's ranks are contiguous
       const int c = e / r8, j = 8 * (e % r8);
       const u16x8 v = __builtin_bit_cast(u16x8, load16(from + (int64_t)(c0 + min(c, 8 * c8 - 1)) * p.rank + j));
 #pragma unroll
@@ -905,7 +936,7 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 64 * r8; e += kThreads) {
+  for (int e = threadIdx.x; e < (b ? 8 * p.rank : 64 * r8); e += kThreads) {
     if (b) {
       const int j = e / 8, c = e % 8;
       if (c < c8) store16(to + (int64_t)j * wide + c0 + 8 * c, *reinterpret_cast<const u32x4 *>(&tile[j][8 * c]));
@@ -913,8 +944,8 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
       const int c = e / r8, j = 8 * (e % r8);
       u16x8 v;
 #pragma unroll
-      for (int y = 0; y < 8; ++y) v[y] = tile[j + y][c];
-      if (c < 8 * c8) store16(to + (int64_t)(c0 + c) * p.rank + j, __builtin_bit_cast(u32x4, v));
+      for (int y = 0; y < 8; ++y) v[y] = j + y < p.rank ? tile[j + y][c] : (uint16_t)0;
+      if (c < 8 * c8) store16(to + (int64_t)(c0 + c) * 8 * r8 + j, __builtin_bit_cast(u32x4, v));
     }
   }
 }
@@ -970,20 +1001,25 @@ hipError_t launch_down(DownParams p, int splits, hipStream_t s) {
        : p.ranks == 64 ? launch_down<T, 4>(p, splits, s) : launch_down<T, 8>(p, splits, s);
 }
 
-template <typename T, int ST>
+template <typename T, int ST, bool WHOLE>
 hipError_t launch_up(UpParams p, hipStream_t s) {
   if (few(p.rows, p.rank, p.adapters)) {
-    hipLaunchKernelGGL((up_few_kernel<T, ST>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
+    hipLaunchKernelGGL((up_few_kernel<T, ST, WHOLE>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
     return hipGetLastError();
   }
   const int tiles = (p.rows + 16 * kUpFrags - 1) / (16 * kUpFrags), cols = std::max(1, (p.cols + 4 * kUpCols - 1) / (4 * kUpCols));
   p.steps = std::max(1, std::min(4, (int)((int64_t)tiles * cols / 768)));
-  hipLaunchKernelGGL((up_kernel<T, ST>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
+  hipLaunchKernelGGL((up_kernel<T, ST, WHOLE>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
   return hipGetLastError();
+}
+template <typename T, bool WHOLE>
+hipError_t launch_up(const UpParams &p, hipStream_t s) {
+  return p.ranks == 16 ? launch_up<T, 1, WHOLE>(p, s) : p.ranks == 32 ? launch_up<T, 2, WHOLE>(p, s)
+       : p.ranks == 64 ? launch_up<T, 4, WHOLE>(p, s) : launch_up<T, 8, WHOLE>(p, s);
 }
 template <typename T>
 hipError_t launch_up(const UpParams &p, hipStream_t s) {
-  return p.ranks == 16 ? launch_up<T, 1>(p, s) : p.ranks == 32 ? launch_up<T, 2>(p, s) : p.ranks == 64 ? launch_up<T, 4>(p, s) : launch_up<T, 8>(p, s);
+  return p.w_rank % 8 == 0 ? launch_up<T, true>(p, s) : launch_up<T, false>(p, s);
 }
 
 template <typename T, int JB>
@@ -1008,7 +1044,7 @@ hipError_t forward(const DanAdaptArgs &a, hipStream_t s) {
   UpParams u;
   u.part = d.part; u.sum = a.down; u.w = a.b; u.y = a.y; u.y_stride = a.y_stride; u.out = a.out; u.o_stride = a.out_stride;
   u.index = a.index; u.scale = a.scale; u.scale_value = a.scale_value;
-  u.rows = a.rows; u.cols = a.n_out; u.rank = a.rank; u.adapters = a.adapters; u.ranks = d.ranks; u.splits = splits; u.steps = 1;
+  u.rows = a.rows; u.cols = a.n_out; u.rank = u.w_rank = a.rank; u.adapters = a.adapters; u.ranks = d.ranks; u.splits = splits; u.steps = 1;
   return launch_up<T>(u, s);
 }
 
@@ -1023,7 +1059,7 @@ struct GradSpace {
     parts_a = one ? parts_of(rows, n_in, 0, adapters) : parts;
     parts_b = one ? both_parts(rows, n_out, adapters) : parts;
     at = 0;
-    bt = align256(at + (int64_t)adapters * rank * n_in * 2);
+    bt = align256(at + (int64_t)adapters * ((rank + 7) / 8 * 8) * n_in * 2);
     list = align256(bt + (int64_t)adapters * rank * n_out * 2);
     starts = list + (int64_t)rows * 4;
     part = align256(starts + ((int64_t)adapters + 1) * 4);
@@ -1080,7 +1116,7 @@ hipError_t backward(const DanAdaptGradArgs &a, const GradSpace &w, hipStream_t s
     UpParams u;  // (without dx: no columns, the sum of the parts alone)
     u.part = one ? g : reinterpret_cast<float *>(ws + w.part); u.sum = one ? nullptr : g; u.w = ws + w.at; u.y = nullptr; u.y_stride = 0; u.out = a.dx; u.o_stride = a.dx_stride;
     u.index = a.index; u.scale = a.scale; u.scale_value = a.scale_value;
-    u.rows = a.rows; u.cols = a.dx ? a.n_in : 0; u.rank = a.rank; u.adapters = a.adapters; u.ranks = o.ranks; u.splits = one ? 1 : w.splits; u.steps = 1;
+    u.rows = a.rows; u.cols = a.dx ? a.n_in : 0; u.rank = a.rank; u.w_rank = (a.rank + 7) / 8 * 8; u.adapters = a.adapters; u.ranks = o.ranks; u.splits = one ? 1 : w.splits; u.steps = 1;
     if ((err = launch_up<T>(u, s)) != hipSuccess) return err;
   }
   if (!a.da && !a.db) return hipSuccess;
@@ -1109,7 +1145,7 @@ int check_sizes(int dtype, int rows, int n_in, int n_out, int rank, int adapters
   if (rows < 0 || rows > 1 << 20) return fail(DAN_ERR_UNSUPPORTED, "rows %d: at most 2^20", rows);
   if (n_in <= 0 || n_out <= 0 || n_in % 8 || n_out % 8 || n_in > 1 << 20 || n_out > 1 << 20)
     return fail(DAN_ERR_UNSUPPORTED, "n_in %d and n_out %d: multiples of 8 up to 2^20", n_in, n_out);
-  if (rank <= 0 || rank % 8 || rank > DAN_ADAPT_MAX_RANK) return fail(DAN_ERR_UNSUPPORTED, "rank %d: a multiple of 8 up to %d", rank, DAN_ADAPT_MAX_RANK);
+  if (rank <= 0 || rank > DAN_ADAPT_MAX_RANK) return fail(DAN_ERR_UNSUPPORTED, "rank %d: 1 to %d", rank, DAN_ADAPT_MAX_RANK);
   if (adapters <= 0 || adapters > 65535) return fail(DAN_ERR_UNSUPPORTED, "%d adapters: 1 to 65535", adapters);
   if (!(isfinite(scale_value))) return fail(DAN_ERR_INVALID_ARGUMENT, "scale_value must be finite");
   const int64_t wide = std::max(n_in, n_out);  // (`up` has the most threads by far: 2 columns of 16 rows each for few rows)

@@ -290,7 +290,7 @@ PyObject *adapt(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (t->scalar_type() != dtype || !plain(*t, dev)) Py_RETURN_NONE;
   const int64_t n = x.size(0), n_in = x.size(1), n_out = y.size(1), count = a.size(0), rank = a.size(1);
   if (!rows_ok(x) || !rows_ok(y) || !dense_ok(a) || !dense_ok(b) || y.size(0) != n || a.size(2) != n_in || b.size(0) != count || b.size(1) != n_out ||
-      b.size(2) != rank || n == 0 || n > 1 << 20 || n_in == 0 || n_out == 0 || n_in % 8 || n_out % 8 || !fits(n_in) || !fits(n_out) || rank == 0 || rank % 8 ||
+      b.size(2) != rank || n == 0 || n > 1 << 20 || n_in == 0 || n_out == 0 || n_in % 8 || n_out % 8 || !fits(n_in) || !fits(n_out) || rank == 0 ||
       rank > DAN_ADAPT_MAX_RANK || count == 0 || !fits(count))
     Py_RETURN_NONE;
   if (index.defined() ? !index_ok(index, n, dev) : count != 1) Py_RETURN_NONE;

@@ -24,7 +24,7 @@ extern "C" {
 #endif
 
 #define DAN_ADAPT_ABI_VERSION 1
-#define DAN_ADAPT_MAX_RANK 128 /* ranks: multiples of 8 */
+#define DAN_ADAPT_MAX_RANK 128
 
 typedef struct {
   int32_t abi_version; /* DAN_ADAPT_ABI_VERSION */

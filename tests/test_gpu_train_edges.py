@@ -296,7 +296,10 @@ def test_adapters_in_other_layouts(gpu):
 @pytest.mark.parametrize("order", ["mixed", "runs"])
 @pytest.mark.parametrize("n,n_in,n_out,rank,count", [  # on both sides of where the kernels for many rows begin, for each rank
     (384, 136, 72, 16, 2), (385, 136, 72, 16, 2), (769, 136, 72, 16, 5), (256, 264, 72, 32, 3), (257, 264, 72, 32, 3), (193, 600, 136, 64, 1),
-    (385, 72, 264, 40, 6), (160, 520, 264, 128, 2), (161, 520, 264, 128, 2), (321, 136, 200, 104, 9), (1100, 8, 8, 8, 1)])
+    (385, 72, 264, 40, 6), (160, 520, 264, 128, 2), (161, 520, 264, 128, 2), (321, 136, 200, 104, 9), (1100, 8, 8, 8, 1),
+    # ranks that are no multiple of 8, or of 4
+    (400, 136, 200, 5, 2), (2, 840, 776, 4, 2), (1, 64, 64, 1, 1), (500, 64, 8, 1, 1), (270, 264, 72, 30, 3), (200, 64, 136, 63, 1), (170, 72, 72, 127, 2),
+    (40, 72, 136, 18, 5), (40, 136, 72, 61, 3), (30, 72, 72, 125, 2)])
 def test_where_many_rows_begin(gpu, n, n_in, n_out, rank, count, order, dtype):
     say(f"adapt {n} rows {n_in} -> {n_out} rank {rank} x {count} {dtype} {order}")
     args = test_gpu_adapt.make(gpu, n, n_in, n_out, rank, count, dtype, order=order)

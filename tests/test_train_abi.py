@@ -89,7 +89,7 @@ ERRORS = [
     (name, kw, status, needle) for name in ("dan_adapt", "dan_adapt_grad") for kw, status, needle in (
         (dict(abi_version=2), VERSION, "abi_version"), (dict(dtype=_native.DTYPE_E4M3), UNSUPPORTED, "dtype"), (dict(rows=-1), UNSUPPORTED, "rows"),
         (dict(rows=(1 << 20) + 1), UNSUPPORTED, "rows"), (dict(n_in=60), UNSUPPORTED, "n_in"), (dict(n_out=0), UNSUPPORTED, "n_out"),
-        (dict(n_in=(1 << 20) + 8), UNSUPPORTED, "n_in"), (dict(rank=4), UNSUPPORTED, "rank"), (dict(rank=136), UNSUPPORTED, "rank"),
+        (dict(n_in=(1 << 20) + 8), UNSUPPORTED, "n_in"), (dict(rank=0), UNSUPPORTED, "rank"), (dict(rank=136), UNSUPPORTED, "rank"),
         (dict(adapters=0), UNSUPPORTED, "adapters"), (dict(adapters=65536), UNSUPPORTED, "adapters"), (dict(scale_value=float("inf")), BAD, "scale_value"),
         (dict(rows=1 << 20, n_in=1 << 20), UNSUPPORTED, "launch"), (dict(x=None), BAD, "NULL"), (dict(x=P + 8), BAD, "aligned"),
         (dict(workspace=None), BAD, "workspace"), (dict(workspace_bytes=8), BAD, "workspace"), (dict(rows=0, x=None), OK, ""))
