@@ -16,7 +16,7 @@
 //
 // Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 21 us (67 MB), up 205 us (940 MB, 4.6 TB/s); gradients: g and dB in one
 // pass 100 us (500 MB, 5 TB/s; in two, 130 + 83), g's parts 7, up 20, dA 19, the parts' sum 8. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
-// and chains of index, weights and sums; 1037 rows, 5 adapters of rank 64, 4096 -> 4096, fp16: down 14, up 14, outer 26 (the same
+// and chains of index, weights and sums; 1037 rows, 5 adapters of rank 64, 4096 -> 4096, fp16: down 14, up 10.5, outer 26 (the same
 // chains: 1024 values instead of 4096 take down 13.4 us).
 //
 // Rows of different adapters may lie in any order. A tile of 16 rows multiplies all of them by each adapter
@@ -324,20 +324,24 @@ struct Operand {
 
 // The operand of 64 columns from m0 on. Lane (l16, g4) of the result owns 8 columns from m0 + 8 g4 on and 8 from m0 + 32 +
 // 8 g4 on, so that four lanes store 64 bytes of a row: row r of block b is column 32 (b / 2) + 8 (r / 4) + 4 (b % 2) + r % 4.
-// WHOLE: ranks in memory are a multiple of 8, whose pieces lie 16-byte aligned; otherwise they come one number at a time, by kernels
-// of their own (in one kernel with the others they would take registers, and waves, from them).
-template <typename T, int ST, bool WHOLE>
-__device__ inline void load_columns(const UpParams &p, int i, int m0, int l16, int g4, u32x4 (&wf)[ST][4]) {
+// Ranks in memory: kAny, one number at a time; kPieces, a multiple of 8, whose pieces lie 16-byte aligned; kFull, 32, 64 or 128, where
+// the second half of the steps (v's low parts) takes the first half's operands again. Each by kernels of its own: in one with the others
+// they would take registers, and waves, from them (rank 64, fp16, 1037 rows of 4096 columns: 10.5 us in full, 14.3 in pieces).
+enum Form { kAny, kPieces, kFull };
+template <int ST, Form FORM>
+constexpr int kColumnSteps = FORM == kFull ? ST / 2 : ST;
+template <typename T, int ST, Form FORM>
+__device__ inline void load_columns(const UpParams &p, int i, int m0, int l16, int g4, u32x4 (&wf)[kColumnSteps<ST, FORM>][4]) {
   const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.cols * p.w_rank;
   const int r8 = (p.rank + 7) / 8;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const int col = min(m0 + 32 * (b >> 1) + 8 * (l16 >> 2) + 4 * (b & 1) + (l16 & 3), p.cols - 1);
 #pragma unroll
-    for (int t = 0; t < ST; ++t) {
+    for (int t = 0; t < kColumnSteps<ST, FORM>; ++t) {
       const int u = 4 * t + g4, j = u >= 2 * r8 ? 0 : 8 * (u >= r8 ? u - r8 : u);  // (past the last piece v holds zeros)
       const T *at = w + (int64_t)col * p.w_rank;
-      if constexpr (WHOLE) {
+      if constexpr (FORM != kAny) {
         wf[t][b] = load16(at + j);
       } else {
         typedef T t8 __attribute__((ext_vector_type(8)));
@@ -360,7 +364,7 @@ __device__ inline float factor_of(const UpParams &p, int i, uint32_t top) {
 // Many rows: 32 by `steps` times 256 columns, 64 a wave. y of the next step is loaded before this one's. (64 rows halve the
 // loads of w, but leave two waves a SIMD instead of four: 8192 rows of 6144 columns took 53.7 us, and take 46.6.)
 constexpr int kUpFrags = 2;
-template <typename T, int ST, bool WHOLE>
+template <typename T, int ST, Form FORM>
 __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
   constexpr int F = kUpFrags;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
@@ -386,9 +390,9 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
   for (int f = 0; f < F; ++f) yv[f][0] = yv[f][1] = u32x4{};
   if (p.y) load_y(first);
   int loaded = -1;  // the adapter that wf holds this step's columns of
-  u32x4 wf[ST][4];
+  u32x4 wf[kColumnSteps<ST, FORM>][4];
   auto load_w = [&](int i, int m0) __attribute__((always_inline)) {
-    load_columns<T, ST, WHOLE>(p, i, m0, l16, g4, wf);
+    load_columns<T, ST, FORM>(p, i, m0, l16, g4, wf);
     loaded = i;
   };
   {
@@ -444,7 +448,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
         for (int b = 0; b < 4; ++b) {
           f32x4 t4 = {};
 #pragma unroll
-          for (int t = 0; t < ST; ++t) t4 = mfma16<T>(wf[t][b], vf[t], t4);
+          for (int t = 0; t < ST; ++t) t4 = mfma16<T>(wf[t % kColumnSteps<ST, FORM>][b], vf[t], t4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[f][b][e] = mine ? fmaf(c, t4[e], acc[f][b][e]) : acc[f][b][e];
         }
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
 }
 
 // Few rows: 16 by 64 columns; the waves split the tile's adapters, and the first two store.
-template <typename T, int ST, bool WHOLE>
+template <typename T, int ST, Form FORM>
 __global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p) {
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
   __shared__ Operand<T, ST, 1, 64 * kFewWaves> op;
@@ -487,13 +491,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p
     left &= ~__ballot(mine);
     if (turn % kFewWaves != wave) continue;
     float c = NAN;  // no such adapter
-    u32x4 wf[ST][4];
+    u32x4 wf[kColumnSteps<ST, FORM>][4];
     if (i < p.adapters) {
-      load_columns<T, ST, WHOLE>(p, i, m0, l16, g4, wf);
+      load_columns<T, ST, FORM>(p, i, m0, l16, g4, wf);
       c = factor_of<T>(p, i, kHalf ? op.top[l16] : 0u);
     } else {
 #pragma unroll
-      for (int t = 0; t < ST; ++t)
+      for (int t = 0; t < kColumnSteps<ST, FORM>; ++t)
 #pragma unroll
         for (int b = 0; b < 4; ++b) wf[t][b] = u32x4{};
     }
@@ -501,7 +505,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p
     for (int b = 0; b < 4; ++b) {
       f32x4 t4 = {};
 #pragma unroll
-      for (int t = 0; t < ST; ++t) t4 = mfma16<T>(wf[t][b], vf[t], t4);
+      for (int t = 0; t < ST; ++t) t4 = mfma16<T>(wf[t % kColumnSteps<ST, FORM>][b], vf[t], t4);
       if (mine) sums[b][lane] = t4 * c;
     }
   }
@@ -1001,25 +1005,26 @@ hipError_t launch_down(DownParams p, int splits, hipStream_t s) {
        : p.ranks == 64 ? launch_down<T, 4>(p, splits, s) : launch_down<T, 8>(p, splits, s);
 }
 
-template <typename T, int ST, bool WHOLE>
+template <typename T, int ST, Form FORM>
 hipError_t launch_up(UpParams p, hipStream_t s) {
   if (few(p.rows, p.rank, p.adapters)) {
-    hipLaunchKernelGGL((up_few_kernel<T, ST, WHOLE>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
+    hipLaunchKernelGGL((up_few_kernel<T, ST, FORM>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
     return hipGetLastError();
   }
   const int tiles = (p.rows + 16 * kUpFrags - 1) / (16 * kUpFrags), cols = std::max(1, (p.cols + 4 * kUpCols - 1) / (4 * kUpCols));
   p.steps = std::max(1, std::min(4, (int)((int64_t)tiles * cols / 768)));
-  hipLaunchKernelGGL((up_kernel<T, ST, WHOLE>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
+  hipLaunchKernelGGL((up_kernel<T, ST, FORM>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
   return hipGetLastError();
 }
-template <typename T, bool WHOLE>
+template <typename T, int ST>
 hipError_t launch_up(const UpParams &p, hipStream_t s) {
-  return p.ranks == 16 ? launch_up<T, 1, WHOLE>(p, s) : p.ranks == 32 ? launch_up<T, 2, WHOLE>(p, s)
-       : p.ranks == 64 ? launch_up<T, 4, WHOLE>(p, s) : launch_up<T, 8, WHOLE>(p, s);
+  if constexpr (ST > 1)
+    if (p.w_rank == p.ranks) return launch_up<T, ST, kFull>(p, s);
+  return p.w_rank % 8 == 0 ? launch_up<T, ST, kPieces>(p, s) : launch_up<T, ST, kAny>(p, s);
 }
 template <typename T>
 hipError_t launch_up(const UpParams &p, hipStream_t s) {
-  return p.w_rank % 8 == 0 ? launch_up<T, true>(p, s) : launch_up<T, false>(p, s);
+  return p.ranks == 16 ? launch_up<T, 1>(p, s) : p.ranks == 32 ? launch_up<T, 2>(p, s) : p.ranks == 64 ? launch_up<T, 4>(p, s) : launch_up<T, 8>(p, s);
 }
 
 template <typename T, int JB>
