@@ -7,7 +7,7 @@ fp64 restatements from the definitions:
   hidden key takes no part in any sum;
 - ``adapt``: low-rank adapters beside a shared projection, one row at a time.
 
-Where a result was made by adding up terms, its bound (what a checker multiplies by a
+Where a result was made by adding up terms, its bound (what a test multiplies by a
 rounding's size) is the same sum over the terms' magnitudes: ``abs_`` results.
 """
 import math
