@@ -97,16 +97,18 @@ def workspace_size(h, hkv, d, n, splits=1):
 def choose_units(lengths, h, hkv, d, num_cus):
     """(keys of a key unit, parts of a kv head's heads) of segments of `lengths` rows.
 
-    Larger units read less of Q and G, smaller ones and parts of the heads fill the chip: each of a number of parts that
-    divides the heads evenly and gives up to two work groups a compute unit, while the longest unit keeps 16 steps (the parts
-    are written and read again in fp32). Forward and backward pass, us: 8192 rows, 32/8 heads x 128, units of 128 / 64 keys 2264
-    / 2293, 3413 rows in four requests 314 / 252; 2000 rows, 16/2 heads x 128, 1 part / 4 parts 346 / 216; 700 rows, 8/2 x 64, 90.3 / 92.5."""
+    Larger units read less of Q and G, smaller ones and parts of the heads fill the chip, with the units of dQ behind them in
+    the same launch: of a number of parts that divides the heads evenly and gives up to one work group a compute unit, while
+    the longest unit keeps 16 steps (the parts are written and read again in fp32). Forward and backward pass, us: 8192 rows,
+    32/8 heads x 128, units of 128 / 64 keys 2264 / 2293, 3413 rows in four requests 251 / 239; 2000 rows, 16/2 heads x 128, units of 64
+    keys in 1 / 2 / 4 / 8 parts 260 / 175 / 170 / 205; 4000 rows, 16/4 x 128, 1 / 2 parts 355 / 414; 4099 rows in five requests, 16/2 x 256,
+    1 / 2 / 4 parts 371 / 372 / 409."""
     whole, small = (int((-(-lengths // _rows(h, hkv, d, x)[0])).sum()) * hkv for x in (False, True))
     if whole >= num_cus or not small:
         return _rows(h, hkv, d, False)[0], 1
     rep, at_once = h // hkv, 2 if d == 256 else 4  # tiles of a step
     tiles = -(-int(lengths.max()) // TILE) * rep
-    parts = [s for s in range(1, rep + 1) if rep % s == 0 and small * s <= 2.25 * num_cus and (s == 1 or tiles >= 16 * at_once * s)]
+    parts = [s for s in range(1, rep + 1) if rep % s == 0 and small * s <= num_cus and (s == 1 or tiles >= 16 * at_once * s)]
     return _rows(h, hkv, d, True)[0], max(parts, default=1)
 
 

@@ -4,14 +4,14 @@
 // output's gradient G:
 //   delta_i = sum_d G_id O_id       dP = G V^T        dS = P * (dP - delta)
 //   dV = P^T G                      dQ = scale dS K   dK = scale dS^T Q
-// P is computed again from Q, K and the forward pass's logsumexp. Three launches, or four:
+// P is computed again from Q, K and the forward pass's logsumexp. Two launches, or three:
 //   grad_rows_kernel     delta, and for fp16 a bound of |dS|;
-//   grad_keys_kernel     dK and dV: a work group holds a run of keys and walks the
-//                        query rows that see them, over the heads of the kv head;
+//   grad_kernel          dK and dV (grad_keys): a work group holds a run of keys and
+//                        walks the query rows that see them, over the heads of the kv
+//                        head; and dQ (grad_queries): it holds query rows of the heads
+//                        that share a kv head and walks the keys that they see;
 //   grad_sum_kernel      where few keys made several work groups share them by heads,
 //                        adds those parts up;
-//   grad_queries_kernel  dQ: a work group holds query rows of the heads that share
-//                        a kv head and walks the keys that they see.
 // Each result is summed by one work group in a fixed order, so there are no atomics
 // and the results do not change from run to run. The price is that S and dP are
 // computed twice: 7 products where 5 would do (dQ summed by atomics, or written and
@@ -19,15 +19,15 @@
 // that see 7700 keys 134 MB for each run of them).
 //
 // Measured: 8192 rows in one request of 32 branches, 32/8 heads x 128, bf16: rows 28 us
-// (134 MB, 4.8 TB/s), keys 935 us (1095 GFLOP, 1170 TFLOP/s), queries 715 us (822 GFLOP,
-// 1150 TFLOP/s), where a library's product of 16384^3 reaches 1370. The matrix unit is
+// (134 MB, 4.8 TB/s), keys and queries 1.7 ms (1917 GFLOP, 1130 TFLOP/s; in launches of
+// their own 0.94 and 0.73), where a library's product of 16384^3 reaches 1370. The matrix unit is
 // busy 57 % (keys) and 52 % (queries) of the time at about 1.95 GHz, which the power
 // holds; what it waits for is the chain from S over its exponentials to dS in each wave,
 // of which one fits a SIMD (its registers are full). With head_dim 256 every operand read
 // feeds one product instead of two, and LDS is as busy as the matrix unit: 4099 rows
-// behind 1024 keys, 16/2 heads: keys 87 us, parts' sum 12, queries 179. Batches of a few
-// thousand rows wait for their longest units: 3413 rows in four requests, 32/8 x 128, fp16:
-// keys 114 us, queries 79, where an even share of the steps would take three quarters.
+// behind 1024 keys, 16/2 heads x 256: 244 us. Batches of a few thousand rows have one to
+// four units a compute unit, and each loads, joins and stores by itself (10 us of its 50 to 100):
+// 3413 rows in four requests, 32/8 x 128, fp16: 181 us.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -71,7 +71,7 @@ struct GradParams {
   const DanGradQueryUnit *query_units;
   const int32_t *row_lo, *row_end;
   const DanPastDesc *pasts;
-  int32_t num_tokens, num_heads, num_kv_heads, rep, hpw, groups, num_pasts, partials, key_rows, splits;
+  int32_t num_tokens, num_heads, num_kv_heads, rep, hpw, groups, num_pasts, partials, key_rows, splits, key_groups;
   float scale, c;  // c = scale * log2 e
 };
 
@@ -234,20 +234,18 @@ struct KeyLds {
 };
 
 template <typename T, int D, int KW>
-__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads), amdgpu_waves_per_eu(1, 1)))
-void grad_keys_kernel(const GradParams p) {
+__device__ __forceinline__ void grad_keys(const GradParams &p, int block, uint8_t *smem) {
   using Tl = Tile<D>;
   using Lds = KeyLds<D, KW>;
   constexpr int NS = kWaveRows<D> / 32, QW = 4 / KW, NK = D / 16, ND = D / 32, NB = Lds::ring;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
   const int lane = threadIdx.x & 63, hl = lane >> 5, wave = uni(threadIdx.x >> 6);
   const int kw = wave % KW, qw = wave / KW;
   // A work group's unit, kv head, and part of the heads that share it.
-  const int kvh = blockIdx.x % p.num_kv_heads, part = blockIdx.x / p.num_kv_heads % p.splits;
+  const int kvh = block % p.num_kv_heads, part = block / p.num_kv_heads % p.splits;
   const int head0 = kvh * p.rep + p.rep * part / p.splits, rep = kvh * p.rep + p.rep * (part + 1) / p.splits - head0;
-  const DanGradKeyUnit un = load_unit(p.key_units + blockIdx.x / (p.num_kv_heads * p.splits));
+  const DanGradKeyUnit un = load_unit(p.key_units + block / (p.num_kv_heads * p.splits));
   if (un.start < 0 || un.n <= 0 || un.start + un.n > p.num_tokens || un.key0 < 0 || un.keys <= 0 || un.keys > p.key_rows ||
       un.key0 + un.keys > un.n || un.q_end <= un.key0 || un.q_end > un.n)
     return;  // no such rows
@@ -535,18 +533,16 @@ struct QueryLds {
 };
 
 template <typename T, int D>
-__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads), amdgpu_waves_per_eu(1, 1)))
-void grad_queries_kernel(const GradParams p) {
+__device__ __forceinline__ void grad_queries(const GradParams &p, int block, uint8_t *smem) {
   using Tl = Tile<D>;
   using Lds = QueryLds<D>;
   constexpr int NS = kWaveRows<D> / 32, NK = D / 16, ND = D / 32, NB = Lds::ring;
   constexpr int TS = Tl::blocks / 4, SL = 2 * TS;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds = (uint32_t)(uintptr_t)(DAN_TILE_LDS uint8_t *)smem;
   const int lane = threadIdx.x & 63, hl = lane >> 5, wave = uni(threadIdx.x >> 6);
-  const int group = blockIdx.x % p.groups, kvh = group % p.num_kv_heads, chunk = group / p.num_kv_heads;
-  const DanGradQueryUnit un = load_unit(p.query_units + blockIdx.x / p.groups);
+  const int group = block % p.groups, kvh = group % p.num_kv_heads, chunk = group / p.num_kv_heads;
+  const DanGradQueryUnit un = load_unit(p.query_units + block / p.groups);
   if (un.start < 0 || un.n <= 0 || un.start + un.n > p.num_tokens || un.t0 < 0 || un.tq <= 0 || un.t0 + un.tq > un.n ||
       un.tq > kWaveRows<D> * 4 / p.hpw || un.trunk < 0 || un.trunk > un.n || un.branch0 < 0 ||
       (un.past_len > 0 && (un.past_idx < 0 || un.past_idx >= p.num_pasts)))
@@ -773,35 +769,41 @@ void grad_queries_kernel(const GradParams p) {
   }
 }
 
+// Both in one launch: the units of dK and dV, then those of dQ, each longest first. A work group fills a compute unit, and the last
+// units of the one kind leave room for the first of the other: forward and backward pass of 3413 rows in four requests, fp16, 254 us in two
+// launches and 244 in one, of 4099 in five behind 1024 keys, 16/2 heads x 256, 429 and 379 (with fewer parts of the heads); 8192 rows take as long.
+template <typename T, int D, int KW>
+__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads), amdgpu_waves_per_eu(1, 1)))
+void grad_kernel(const GradParams p) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int block = (int)blockIdx.x - p.key_groups;
+  if (block < 0) grad_keys<T, D, KW>(p, blockIdx.x, smem);
+  else grad_queries<T, D>(p, block, smem);
+}
+
 // ---------------------------------------------------------------- host
 int wave_rows(int D) { return D == 256 ? 32 : 64; }
 int heads_of_group(int rep) { return rep >= 3 ? 4 : rep; }
 
 template <typename T, int D, int KW>
-hipError_t launch_keys(const GradParams &p, int64_t grid, hipStream_t s) {
-  constexpr int bytes = KeyLds<D, KW>::total;
-  const hipError_t err = allow_lds<&grad_keys_kernel<T, D, KW>>(bytes);
+hipError_t launch_units(const GradParams &p, int64_t grid, hipStream_t s) {
+  constexpr int bytes = std::max<int>(KeyLds<D, KW>::total, QueryLds<D>::total);
+  const hipError_t err = allow_lds<&grad_kernel<T, D, KW>>(bytes);
   if (err != hipSuccess) return err;
-  hipLaunchKernelGGL((grad_keys_kernel<T, D, KW>), dim3((uint32_t)grid), dim3(kThreads), bytes, s, p);
+  hipLaunchKernelGGL((grad_kernel<T, D, KW>), dim3((uint32_t)grid), dim3(kThreads), bytes, s, p);
   return hipGetLastError();
 }
 
 template <typename T, int D>
-hipError_t launch_all(const GradParams &p, int64_t keys_grid, int64_t queries_grid, hipStream_t s) {
+hipError_t launch_all(const GradParams &p, int64_t grid, hipStream_t s) {
   hipLaunchKernelGGL((grad_rows_kernel<T, D>), dim3(p.partials), dim3(kThreads), 0, s, p);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   constexpr int KW = 64 / kWaveRows<D>;  // runs of a wave's keys in the smaller unit
-  err = p.key_rows == 128 ? launch_keys<T, D, 2 * KW>(p, keys_grid, s) : launch_keys<T, D, KW>(p, keys_grid, s);
-  if (err != hipSuccess) return err;
-  if (p.splits > 1) {
-    constexpr int R = kThreads / (D / 8);
-    hipLaunchKernelGGL((grad_sum_kernel<T, D>), dim3((p.num_tokens + R - 1) / R, p.num_kv_heads, 2), dim3(kThreads), 0, s, p);
-    if ((err = hipGetLastError()) != hipSuccess) return err;
-  }
-  constexpr int bytes = QueryLds<D>::total;
-  if ((err = allow_lds<&grad_queries_kernel<T, D>>(bytes)) != hipSuccess) return err;
-  hipLaunchKernelGGL((grad_queries_kernel<T, D>), dim3((uint32_t)queries_grid), dim3(kThreads), bytes, s, p);
+  err = p.key_rows == 128 ? launch_units<T, D, 2 * KW>(p, grid, s) : launch_units<T, D, KW>(p, grid, s);
+  if (err != hipSuccess || p.splits == 1) return err;
+  constexpr int R = kThreads / (D / 8);
+  hipLaunchKernelGGL((grad_sum_kernel<T, D>), dim3((p.num_tokens + R - 1) / R, p.num_kv_heads, 2), dim3(kThreads), 0, s, p);
   return hipGetLastError();
 }
 
@@ -894,13 +896,14 @@ int dan_tree_attn_bwd(const DanTreeGradArgs *a, void *stream) {
   const int64_t keys_grid = (int64_t)a->num_key_units * Hkv * p.splits, queries_grid = (int64_t)a->num_query_units * p.groups;
   if (p.splits > 1 && (Hkv > 65535 || (int64_t)Hkv * N * (D / 4) >= int64_t(1) << 31))
     return fail(DAN_ERR_UNSUPPORTED, "%d kv heads x %d tokens in parts: too many for one launch", Hkv, N);
-  if (keys_grid * kThreads >= (int64_t(1) << 32) || queries_grid * kThreads >= (int64_t(1) << 32))
-    return fail(DAN_ERR_UNSUPPORTED, "%lld and %lld work groups: fewer than 2^24", (long long)keys_grid, (long long)queries_grid);
+  const int64_t grid = keys_grid + queries_grid;
+  if (grid * kThreads >= int64_t(1) << 32)
+    return fail(DAN_ERR_UNSUPPORTED, "%lld and %lld work groups: fewer than 2^24 together", (long long)keys_grid, (long long)queries_grid);
+  p.key_groups = (int)keys_grid;
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto by_d = [&](auto t) {
     using T = decltype(t);
-    return D == 64 ? launch_all<T, 64>(p, keys_grid, queries_grid, s) : D == 128 ? launch_all<T, 128>(p, keys_grid, queries_grid, s)
-                                                                                 : launch_all<T, 256>(p, keys_grid, queries_grid, s);
+    return D == 64 ? launch_all<T, 64>(p, grid, s) : D == 128 ? launch_all<T, 128>(p, grid, s) : launch_all<T, 256>(p, grid, s);
   };
   const hipError_t err = a->dtype == DAN_DTYPE_BF16 ? by_d(__bf16{}) : by_d(_Float16{});
   if (err != hipSuccess) return fail(DAN_ERR_LAUNCH, "attention gradient launch failed: %s", hipGetErrorString(err));
