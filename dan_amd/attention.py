@@ -179,7 +179,8 @@ def attend_train(q, k, v, segments, layer, scale=None):
 
     Prefix-cache entries are constants (one that requires grad raises); a
     segment with ``save`` > 0 keeps detached copies, as ``attend`` does. Rows of
-    no segment give zeros and have no gradient. Segments must not overlap.
+    no segment give zeros (also where no input needs a gradient and the call is
+    ``attend``'s) and have no gradient. Segments must not overlap.
     ``scale`` (1 / sqrt(D) unless given): from 2^-100 to 2^100. q, k, v and the
     output's gradient of finite
     values: a hidden key's weight is zero, its products are not
@@ -201,11 +202,24 @@ def attend_train(q, k, v, segments, layer, scale=None):
         with torch.cuda.device(q.device):
             return attend_train(q, k, v, segments, layer, scale)
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        return attend(q, k, v, segments, layer, scale)
+        out = attend(q, k, v, segments, layer, scale)
+        for a, b in _uncovered(segments, out.shape[1]):
+            out[:, a:b].zero_()
+        return out
     for s in segments:
         if s.save:
             s.saved[layer] = tuple(x[:, s.start:s.start + s.save].detach().clone() for x in (k, v))
     return _grad.attend(q, k, v, segments, layer, scale)
+
+
+def _uncovered(segments, n):
+    """The runs (start, end) of ``n`` packed rows that lie in no segment."""
+    runs, at = [], 0
+    for a, b in sorted((s.start, s.end) for s in segments):
+        if a > at:
+            runs.append((at, a))
+        at = max(at, b)
+    return runs + [(at, n)] if at < n else runs
 
 
 def has_tangent(*tensors):
