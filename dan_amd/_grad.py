@@ -169,16 +169,7 @@ class Tables:
         self.keys, self.queries = at, at + keys.nbytes
         self.row_lo = self.queries + queries.nbytes
         self.row_end = self.row_lo + row_lo.nbytes
-        self.stream = _native.stream(self.device)
-        self.ready = torch.cuda.Event()
-        self.ready.record(torch.cuda.current_stream(self.device))
-
-    def use(self):
-        """Orders the current stream behind the upload (a capture begins with the device idle)."""
-        if _native.stream(self.device) != self.stream and not torch.cuda.is_current_stream_capturing():
-            stream = torch.cuda.current_stream(self.device)
-            stream.wait_event(self.ready)
-            self.blob.record_stream(stream)
+        plan.fills()
 
 
 def tables(segments, plan, h, hkv, d, num_cus):
@@ -187,9 +178,7 @@ def tables(segments, plan, h, hkv, d, num_cus):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attend_train: run the batch once before a capture (its tables are uploaded then)")
         plan.grad_tables[h, hkv, d] = Tables(segments, plan, h, hkv, d, num_cus)
-    t = plan.grad_tables[h, hkv, d]
-    t.use()
-    return t
+    return plan.grad_tables[h, hkv, d]
 
 
 def attend(q, k, v, segments, layer, scale):
@@ -204,10 +193,10 @@ def attend(q, k, v, segments, layer, scale):
     if made is None:
         with torch.no_grad():
             plan_args = A._call_args(q, k, v, segments, layer, scale, None, _native.PHASES_ALL, False, upload=False)
-        made = templates(segments, q, k, v, layer, scale, plan_args)
-        plan_args[2].train_calls[key] = made
-    call, (t, _) = made
-    t.use()
+        made, plan = templates(segments, q, k, v, layer, scale, plan_args), plan_args[2]
+        plan.train_calls[key] = made
+    call, _ = made
+    plan.order(q.device)  # (behind what was uploaded on any stream: for an earlier call, another layer, or by ``attend``)
     out = _layer.calls().attend(q, k, v, *call)
     return TreeAttention.apply(q, k, v, segments, layer, scale) if out is None else out
 
@@ -249,7 +238,6 @@ def _backward(ctx, q, k, v, out, lse, grad):
     new = torch.empty if t.covered else torch.zeros  # rows of no segment have no gradient
     dq, dk, dv = (new((n, x.shape[0], d), dtype=q.dtype, device=q.device).transpose(0, 1) for x in (q, k, v))
     if n:
-        t.use()
         q, k, v, grad = (A._kernel_view(x) for x in (q, k, v, grad))
         nbytes = workspace_size(h, hkv, d, n, t.key_splits)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)

@@ -202,6 +202,9 @@ def attend_train(q, k, v, segments, layer, scale=None):
         with torch.cuda.device(q.device):
             return attend_train(q, k, v, segments, layer, scale)
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        plan = getattr(segments, "tile_plan", None)
+        if plan is not None and plan.device == q.device:
+            plan.order(q.device)
         out = attend(q, k, v, segments, layer, scale)
         for a, b in _uncovered(segments, out.shape[1]):
             out[:, a:b].zero_()
@@ -401,10 +404,14 @@ def _past_table(plan, layer, hkv, d, dtype, device, upload=True):
     if layer not in plan.past_tables:
         raw, refs = _past_descs(plan.past_dicts, plan.segs, layer, hkv, d, dtype, device)
         plan.past_hosts[layer] = raw if len(plan.past_dicts) <= _native.INLINE_PASTS else None
+        # (of 16-bit entries, which training reads, other tensors than the entry's own are copies)
+        if plan.past_dicts and dtype.itemsize == 2 and any(a is not b for a, b in zip(refs, (x for entry in plan.past_dicts for x in entry[layer][:2]))):
+            plan.fills()
         plan.past_tables[layer] = (torch.empty(raw.numel(), dtype=torch.uint8, device=device), (refs, raw))
     table, (refs, raw) = plan.past_tables[layer]
     if (upload or plan.past_hosts[layer] is None) and layer not in plan.past_uploaded:
         table.copy_(raw.pin_memory() if device.type == "cuda" else raw, non_blocking=True)
+        plan.fills()
         plan.past_uploaded.add(layer)
     return table, refs
 

@@ -254,6 +254,8 @@ class TilePlan:
     train_calls: dict = field(default_factory=dict)  # (layer, heads, kv heads, head_dim, dtype, scale) -> what a training call of it takes
     schedules: dict = field(default_factory=dict)  # (groups, CUs) -> (units_d, sched_off_d, slots)
     tiles: dict = field(default_factory=dict)  # (heads, kv heads, head_dim) -> queries per work item that a call of this layout takes
+    filled: dict = field(default_factory=dict)  # stream that fills some of these tables -> event behind that, or None
+    ordered: dict = field(default_factory=dict)  # stream -> the tables that ``order`` has seen to there
 
     @classmethod
     def build(cls, segments, num_tokens, tile_q, device):
@@ -266,6 +268,7 @@ class TilePlan:
         plan.work_d = _upload(work, device)
         plan.key_lo_d = _upload(key_lo, device)
         plan.col_seg_d = _upload(col_seg, device)
+        plan.fills()
         return plan
 
     @classmethod
@@ -286,7 +289,8 @@ class TilePlan:
             raise ValueError(f"{w} work items, {slots} slots, {len(segs)} segments or {len(starts)} branches "
                              "exceed the device planner's limits")
         dev = torch.device(device)
-        plan = cls(tile_q, num_tokens, dev, segs, None, None, None, past_dicts, None, num_work=w, num_cols=c)
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        plan = cls(tile_q, num_tokens, dev, segs, None, None, None, past_dicts, None, num_work=w, num_cols=c, filled={stream: None})
         blob = _upload(np.concatenate([segs.ravel(), starts]).astype(np.int32), dev)  # the one upload
         plan.segs_d = blob[:segs.size]
         plan.key_lo_d = torch.empty(num_tokens, dtype=torch.int32, device=dev)
@@ -305,9 +309,53 @@ class TilePlan:
             a.key_lo, a.col_seg, a.work, a.cost = (plan.key_lo_d.data_ptr(), plan.col_seg_d.data_ptr(),
                                                    plan.work_d.data_ptr(), plan.cost_d.data_ptr())
             a.units, a.sched_off = units.data_ptr(), off.data_ptr()
-            _native.plan(a, torch.cuda.current_stream(dev).cuda_stream, lib)
+            _native.plan(a, stream, lib)
         plan.schedules[(groups, num_cus)] = (units, off, slots)
         return plan
+
+    def fills(self):
+        """Notes that the current stream fills tables of the plan (before they can be found there)."""
+        if self.device.type == "cuda":
+            import torch
+
+            self.filled[torch.cuda.current_stream(self.device).cuda_stream] = None
+
+    def order(self, device):
+        """The current stream of ``device`` goes on behind the tables that other streams fill, and the allocator learns that
+        it reads them: a batch may be used on several streams, and dropped before the last of them has got there. Once
+        for each stream and table. (A capture begins with the device idle.)"""
+        import torch
+
+        from . import _native
+
+        here = _native.stream(device)
+        state = (len(self.past_tables), len(self.past_uploaded), len(self.schedules), len(self.grad_tables))
+        if self.ordered.get(here) == state or torch.cuda.is_current_stream_capturing():
+            return
+        stream = torch.cuda.current_stream(device)
+        for other, event in list(self.filled.items()):
+            event = event or self._event(other)
+            if other != here and event:
+                stream.wait_event(event)
+        tables = [self.segs_d, self.work_d, self.key_lo_d, self.col_seg_d, *(t.blob for t in list(self.grad_tables.values()))]
+        tables += [t for units, off, _ in list(self.schedules.values()) for t in (units, off)]
+        tables += [t for table, (refs, _) in list(self.past_tables.values()) for t in (table, *refs)]
+        for table in tables:
+            table.record_stream(stream)
+        self.ordered[here] = state
+
+    def _event(self, handle):
+        """An event behind what the stream has been given so far: recorded when first asked for, so that a batch of a single
+        stream pays for none. None if the stream has begun a capture since then."""
+        import torch
+
+        stream, event = torch.cuda.ExternalStream(handle, device=self.device), torch.cuda.Event()
+        with torch.cuda.stream(stream):
+            if torch.cuda.is_current_stream_capturing():
+                return None
+        event.record(stream)
+        self.filled[handle] = event
+        return event
 
     def items(self, tile):
         """Work items that the segments make with ``tile`` queries each."""
@@ -334,7 +382,9 @@ class TilePlan:
                 raise ValueError(f"this plan was scheduled on the device for {list(self.schedules)}, not {key}")
             sched, off = schedule(self.cost, groups, num_cus)
             units = unit_records(self.segs, self.work, sched, groups)
-            self.schedules[key] = (_upload(units, self.device), _upload(off, self.device), len(off) - 1)
+            tables = (_upload(units, self.device), _upload(off, self.device), len(off) - 1)
+            self.fills()
+            self.schedules[key] = tables
         return self.schedules[key]
 
     def key_tiles(self):

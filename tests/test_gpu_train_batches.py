@@ -1,5 +1,5 @@
 """attend_train over batches that change or that training and other calls share: rows of no segment where nothing needs a
-gradient.
+gradient, tables uploaded on another stream.
 
 Results are compared bit for bit with those of the same kernels on the same values."""
 import math
@@ -9,8 +9,9 @@ import torch
 import torch.utils.checkpoint
 
 import test_gpu_attend_train
-from dan_amd.attention import Batch, attend_train, segment
-from test_gpu_train_calls import same, say
+from dan_amd import workloads
+from dan_amd.attention import Batch, attend, attend_train, segment
+from test_gpu_train_calls import same, say, way, ways  # noqa: F401  -- the fixture of `ways`
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +67,127 @@ def test_gaps_under_a_reentrant_checkpoint(gpu):
     assert torch.equal(out, want[0])
     out.backward(grad)
     assert same([x.grad for x in leaves], want[1:])
+
+
+# ---------------------------------------------------------------- batches
+def entry(gpu, seed, length, dtype=BF16, heads=2, d=64, other=False):
+    g = torch.Generator().manual_seed(seed)
+    new = [torch.randn(heads, length, d, generator=g).to(dtype).to(gpu) for _ in range(2)]
+    if other:  # (rows that the kernels read from a copy)
+        new = [torch.nn.functional.pad(x, (3, 2))[..., 3:-2] for x in new]
+    return tuple(new)
+
+
+def batch(gpu, lengths, pasts):
+    segs, at = Batch(), 0
+    for (t, ls), past in zip(lengths, pasts):
+        ids = workloads.branch_ids(t, ls)
+        segs.append(segment(at, ids, past, 0, past[0][0].shape[1] if past else 0, str(gpu)))
+        at += len(ids)
+    return segs, at
+
+
+def train(q, k, v, grad, segs, layer=0):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = attend_train(*leaves, segs, layer)
+    return out.detach(), *torch.autograd.grad(out, leaves, grad)
+
+
+# ---------------------------------------------------------------- streams
+def slow(x):
+    for _ in range(150):
+        torch.mm(x, x)
+
+
+@pytest.fixture(scope="module")
+def big(gpu):
+    x = torch.randn(8192, 8192, device=gpu, dtype=BF16)
+    slow(x)
+    torch.cuda.synchronize()
+    return x
+
+
+def many(gpu, seed, count=12, other=False):
+    """(q, k, v, G, a function that makes the batch): each segment behind an entry of its own, more than a launch carries by value."""
+    lengths = [(20 + i, [3, 4]) for i in range(count)]
+    pasts = [{layer: entry(gpu, 100 * layer + i, 5 + i, other=other) for layer in range(3)} for i in range(count)]
+    n = sum(t + sum(ls) for t, ls in lengths)
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(h, n, 64, generator=g).to(BF16).to(gpu) for h in (4, 2, 2, 4)], lambda: batch(gpu, lengths, pasts)[0]
+
+
+@ways
+@pytest.mark.parametrize("other", [False, True])
+@pytest.mark.parametrize("count", [3, 12])
+def test_a_plan_made_behind_slow_work_on_another_stream(gpu, big, count, other, way):  # noqa: F811
+    """attend on one stream makes the plan and a layer's prefix table; attend_train of it and of another layer on a second stream, and
+    of the first's layers on a third, wait for what they read, with and without a gradient."""
+    say("attend_train on another stream than the plan's", count, other, way)
+    x, make = many(gpu, 3, count, other)
+    want = [train(*x, make(), layer) for layer in range(3)]
+    b, c = torch.cuda.Stream(), torch.cuda.Stream()
+    for first, a in (("grad", torch.cuda.Stream()), ("no_grad", torch.cuda.Stream()), ("grad", torch.cuda.default_stream())):
+        segs = make()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            slow(big)
+            out = [attend(*x[:3], segs, 0)]
+        with torch.cuda.stream(b):
+            if first == "grad":
+                got = [train(*x, segs, 0)]
+            else:
+                with torch.no_grad():
+                    out.append(attend_train(*x[:3], segs, 0))
+                got = []
+            slow(big)
+            got.append(train(*x, segs, 1))
+        with torch.cuda.stream(c):
+            more = [train(*x, segs, 0), train(*x, segs, 1), train(*x, segs, 2)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[0][0]) for o in out)
+        assert all(same(g, want[i]) for i, g in zip((0, 1) if first == "grad" else (1,), got))
+        assert all(same(g, w) for g, w in zip(more, want))
+
+
+@ways
+def test_a_later_layers_table_uploaded_on_another_stream(gpu, big, way):  # noqa: F811
+    say("attend_train: a later layer's prefix table behind slow work", way)
+    x, make = many(gpu, 4)
+    want = [train(*x, make(), layer) for layer in range(2)]
+    segs = make()
+    assert same(train(*x, segs, 0), want[0])
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        slow(big)
+        first = train(*x, segs, 1)  # (uploads the layer's table)
+    with torch.cuda.stream(b):
+        second = train(*x, segs, 1)
+    torch.cuda.synchronize()
+    assert same(first, want[1]) and same(second, want[1])
+
+
+@ways
+@pytest.mark.parametrize("needs", [True, False])
+def test_a_batch_dropped_before_another_stream_has_read_it(gpu, big, needs, way):  # noqa: F811
+    """Tables that were allocated on the stream of the first call, read on another one: their memory is not given away before that."""
+    say("attend_train: batch dropped behind slow work", needs, way)
+    x, make = many(gpu, 5)
+    want = train(*x, make())
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        segs = make()
+        assert same(train(*x, segs), want)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(b):
+        slow(big)
+        if needs:
+            got = train(*x, segs)
+        else:
+            with torch.no_grad():
+                got = [attend_train(*x[:3], segs, 0)]
+    del segs
+    with torch.cuda.stream(a):  # what takes the place of freed tables: zeros, which name no rows
+        zeros = [torch.zeros(s, dtype=torch.uint8, device=gpu) for s in (256, 512, 1024, 2048, 4096, 8192, 16384, 32768, 65536) for _ in range(40)]
+    torch.cuda.synchronize()
+    assert same(got, want[:len(got)]) and all((z == 0).all() for z in zeros[::40])
