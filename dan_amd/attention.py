@@ -184,8 +184,9 @@ def attend_train(q, k, v, segments, layer, scale=None):
     ``scale`` (1 / sqrt(D) unless given): from 2^-100 to 2^100. q, k, v and the
     output's gradient of finite
     values: a hidden key's weight is zero, its products are not
-    left out. The first call on a ``Batch`` uploads its tables, so it cannot be
-    captured into a HIP graph; later ones can, forward and backward in the same
+    left out. The first call on a ``Batch`` uploads its tables (and a layer's first one its
+    prefix table, where the batch has more than 8 entries or some are copied), so it is refused
+    in the capture of a HIP graph; later ones can be captured, forward and backward in the same
     capture and with no earlier, eager result alive that holds the graph of the
     same leaves (where q, k or v is such a leaf itself, that raises)."""
     from . import _grad
@@ -307,14 +308,18 @@ def _aligned(t):
     return st[-1] == 1 and t.data_ptr() % 16 == 0 and all((s * es) % 16 == 0 for s in st[:-1])
 
 
+def _in_place(t):
+    """Whether the kernel can read the tensor where it lies: aligned rows, and token strides that its 32-bit in-tile offsets hold."""
+    es, st = t.element_size(), t.stride()
+    return len(st) == 3 and st[2] == 1 and not ((st[0] | st[1]) * es | t.data_ptr()) & 15 and abs(st[1]) < 2 ** 25
+
+
 def _kernel_view(t):
     """The tensor itself when the kernel can read it in place, else a fresh
-    contiguous copy (unaligned rows, or token strides too large for the
-    kernel's 32-bit in-tile offsets). The copy is a new allocation, so its
+    contiguous copy. The copy is a new allocation, so its
     base is aligned; ``contiguous()`` would return a contiguous but
     misaligned view unchanged."""
-    es, st = t.element_size(), t.stride()
-    if len(st) == 3 and st[2] == 1 and not ((st[0] | st[1]) * es | t.data_ptr()) & 15 and abs(st[1]) < 2 ** 25:
+    if _in_place(t):
         return t
     return torch.empty_like(t, memory_format=torch.contiguous_format).copy_(t)
 

@@ -1,5 +1,5 @@
 """attend_train over batches that change or that training and other calls share: rows of no segment where nothing needs a
-gradient, tables uploaded on another stream.
+gradient, tables uploaded on another stream, first calls in a capture.
 
 Results are compared bit for bit with those of the same kernels on the same values."""
 import math
@@ -191,3 +191,55 @@ def test_a_batch_dropped_before_another_stream_has_read_it(gpu, big, needs, way)
         zeros = [torch.zeros(s, dtype=torch.uint8, device=gpu) for s in (256, 512, 1024, 2048, 4096, 8192, 16384, 32768, 65536) for _ in range(40)]
     torch.cuda.synchronize()
     assert same(got, want[:len(got)]) and all((z == 0).all() for z in zeros[::40])
+
+
+# ---------------------------------------------------------------- captures
+@ways
+@pytest.mark.parametrize("kept", [True, False])
+def test_a_refused_capture_leaves_nothing_behind(gpu, kept, way):  # noqa: F811
+    """A batch whose very first call is in a capture: refused before a table is made, since one made there would be kept on the batch
+    and never filled. What the message asks for then works."""
+    say("attend_train: first call of a new batch in a capture", kept, way)
+    x, make = many(gpu, 6, 3)
+    want = train(*x, make())
+    segs = make() if kept else list(make())
+    leaves = [t.detach().requires_grad_() for t in x[:3]]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="before a capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
+            attend_train(*leaves, segs, 0)
+    torch.cuda.synchronize()
+    assert getattr(segs, "tile_plan", None) is None
+    assert same(train(*x, segs), want)
+
+
+@ways
+@pytest.mark.parametrize("count,other,allowed", [(3, False, True), (3, True, False), (12, False, False)])
+def test_another_layers_first_call_in_a_capture(gpu, count, other, allowed, way):  # noqa: F811
+    """A layer that the warm-up left out is captured where that uploads and copies nothing, and refused otherwise; in either
+    case an eager call of it is right afterwards, before any replay, and so is each replay."""
+    say("attend_train: first call of a layer in a capture", count, other, way)
+    x, make = many(gpu, 7, count, other)
+    want = [train(*x, make(), layer) for layer in range(2)]
+    segs = make()
+    assert same(train(*x, segs, 0), want[0])
+    leaves = [t.detach().requires_grad_() for t in x[:3]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    if allowed:
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            out = attend_train(*leaves, segs, 1)
+            got = [out.detach(), *torch.autograd.grad(out, leaves, x[3])]
+    else:
+        with pytest.raises(RuntimeError, match="before a capture"):
+            with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+                attend_train(*leaves, segs, 1)
+    torch.cuda.synchronize()
+    assert same(train(*x, segs, 1), want[1])
+    if allowed:
+        for _ in range(3):
+            for t in got:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert same(got, want[1]) and same(train(*x, segs, 1), want[1])
