@@ -177,7 +177,9 @@ def attend_train(q, k, v, segments, layer, scale=None):
     fixes; P and dS are rounded to the inputs' type for the matrix core, dS
     after a power-of-2 scaling where that is fp16.
 
-    Prefix-cache entries are constants (one that requires grad raises); a
+    Prefix-cache entries are constants (one that requires grad raises). Where
+    others have taken their place since a ``Batch`` was first run, a call reads
+    those, by a plan of its own that is not kept (a new ``Batch`` keeps it). A
     segment with ``save`` > 0 keeps detached copies, as ``attend`` does. Rows of
     no segment give zeros (also where no input needs a gradient and the call is
     ``attend``'s) and have no gradient. Segments must not overlap.
@@ -191,7 +193,7 @@ def attend_train(q, k, v, segments, layer, scale=None):
     same leaves (where q, k or v is such a leaf itself, that raises)."""
     from . import _grad
 
-    if torch.is_grad_enabled() and any(x.requires_grad for s in segments if s.past for x in s.past[layer] if isinstance(x, torch.Tensor)):
+    if torch.is_grad_enabled() and any(x.requires_grad for s in segments if s.past for x in s.past.get(layer, ()) if isinstance(x, torch.Tensor)):
         raise NotImplementedError("attend_train: prefix-cache entries are constants; got one that requires grad")
     if has_tangent(q, k, v):
         raise NotImplementedError("attend_train has no forward-mode derivative")
@@ -204,7 +206,9 @@ def attend_train(q, k, v, segments, layer, scale=None):
             return attend_train(q, k, v, segments, layer, scale)
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         plan = getattr(segments, "tile_plan", None)
-        if plan is not None and plan.device == q.device:
+        if plan is not None and _replaced(segments, plan, layer, saves=True):
+            segments = list(segments)
+        elif plan is not None and plan.device == q.device:
             plan.order(q.device)
         out = attend(q, k, v, segments, layer, scale)
         for a, b in _uncovered(segments, out.shape[1]):
@@ -213,7 +217,25 @@ def attend_train(q, k, v, segments, layer, scale=None):
     for s in segments:
         if s.save:
             s.saved[layer] = tuple(x[:, s.start:s.start + s.save].detach().clone() for x in (k, v))
+    plan = getattr(segments, "tile_plan", None)
+    if plan is not None and _replaced(segments, plan, layer):
+        segments = list(segments)  # (planned for this call alone: captured calls may still read the batch's own tables)
     return _grad.attend(q, k, v, segments, layer, scale)
+
+
+def _replaced(segments, plan, layer, saves=False):
+    """Whether the segments' prefix-cache entries are others than those that ``plan``'s table of ``layer`` names, or one that is
+    read from a copy has changed. ``saves``: an entry that the batch's own segments save is about to be replaced."""
+    if len(segments) != len(plan.pasts) or any(s.past is not p or s.past_len != n if s.past else p is not None for s, (p, n) in zip(segments, plan.pasts)):
+        return True
+    if not plan.past_dicts or layer not in plan.past_tables:
+        return False
+    refs, copied = plan.past_tables[layer][1][0], plan.past_copied.get(layer, {})
+    for i, x in enumerate(x for entry in plan.past_dicts for x in entry[layer][:2]):
+        was, version = copied.get(i, (refs[i], None))
+        if x is not was or version is not None and x._version != version:
+            return True
+    return saves and any(s.past is t.saved for t in segments if t.save for s in segments if s.past)
 
 
 def _uncovered(segments, n):
@@ -407,11 +429,11 @@ def _past_table(plan, layer, hkv, d, dtype, device, upload=True):
     ``upload`` a table of at most INLINE_PASTS entries is left to the launch,
     which takes its bytes (``plan.past_hosts[layer]``) by value and fills it."""
     if layer not in plan.past_tables:
-        raw, refs = _past_descs(plan.past_dicts, plan.segs, layer, hkv, d, dtype, device)
+        raw, refs = _past_descs(plan.past_dicts, plan.segs, layer, hkv, d, dtype, device, copied=(copied := {}))
         plan.past_hosts[layer] = raw if len(plan.past_dicts) <= _native.INLINE_PASTS else None
-        # (of 16-bit entries, which training reads, other tensors than the entry's own are copies)
-        if plan.past_dicts and dtype.itemsize == 2 and any(a is not b for a, b in zip(refs, (x for entry in plan.past_dicts for x in entry[layer][:2]))):
+        if copied:
             plan.fills()
+            plan.past_copied[layer] = copied
         plan.past_tables[layer] = (torch.empty(raw.numel(), dtype=torch.uint8, device=device), (refs, raw))
     table, (refs, raw) = plan.past_tables[layer]
     if (upload or plan.past_hosts[layer] is None) and layer not in plan.past_uploaded:
@@ -421,11 +443,12 @@ def _past_table(plan, layer, hkv, d, dtype, device, upload=True):
     return table, refs
 
 
-def _past_descs(past_dicts, segs, layer, hkv, d, dtype, device, capacity=None):
+def _past_descs(past_dicts, segs, layer, hkv, d, dtype, device, capacity=None, copied=None):
     """The DanPastDesc bytes of ``layer``'s prefix-cache entries (host uint8
     tensor, ``capacity`` entries if given) and the device tensors they point
     at (kept alive by the caller); ``segs`` is the segment table, whose
-    past lengths are checked against the entries."""
+    past lengths are checked against the entries. ``copied`` takes, by its
+    place among those tensors, what an entry is read from a copy of, and its version."""
     n = len(past_dicts)
     descs = (_native.DanPastDesc * max(capacity or n, 1))()
     refs = []
@@ -450,7 +473,10 @@ def _past_descs(past_dicts, segs, layer, hkv, d, dtype, device, capacity=None):
             pk, pks = _stage_f16(pk)
             refs.append(pks)
             descs[i].k_scale = pks.data_ptr()
+        own = pk, pv
         pk, pv = _kernel_view(pk), _kernel_view(pv)
+        if copied is not None and (pk is not own[0] or pv is not own[1]):
+            copied.update({len(refs) + j: (x, None if x.is_inference() else x._version) for j, x in enumerate(own) if x is not (pk, pv)[j]})
         refs += [pk, pv]
         descs[i].k, descs[i].v = pk.data_ptr(), pv.data_ptr()
         descs[i].k_stride_head, descs[i].k_stride_tok = pk.stride(0), pk.stride(1)

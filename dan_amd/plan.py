@@ -247,6 +247,7 @@ class TilePlan:
     key_lo_d: object = None
     col_seg_d: object = None
     past_tables: dict = field(default_factory=dict)  # layer -> (device bytes, keep-alive refs)
+    past_copied: dict = field(default_factory=dict)  # layer -> {place in its refs: (what is read from a copy there, its version)}
     past_hosts: dict = field(default_factory=dict)  # layer -> the table's host bytes (None: too long to ride in a launch)
     past_uploaded: set = field(default_factory=set)  # the layers whose device table was filled by an upload
     past_filled: dict = field(default_factory=dict)  # layer -> (stream, table) of a launch with a caller's workspace that filled it
@@ -254,6 +255,7 @@ class TilePlan:
     train_calls: dict = field(default_factory=dict)  # (layer, heads, kv heads, head_dim, dtype, scale) -> what a training call of it takes
     schedules: dict = field(default_factory=dict)  # (groups, CUs) -> (units_d, sched_off_d, slots)
     tiles: dict = field(default_factory=dict)  # (heads, kv heads, head_dim) -> queries per work item that a call of this layout takes
+    pasts: list = field(default_factory=list)  # each segment's prefix-cache entry and its length (None, 0: it has none)
     filled: dict = field(default_factory=dict)  # stream that fills some of these tables -> event behind that, or None
     ordered: dict = field(default_factory=dict)  # stream -> the tables that ``order`` has seen to there
 
@@ -263,7 +265,7 @@ class TilePlan:
 
         segs, work, key_lo, cost, past_dicts, col_seg = build_tables(segments, num_tokens, tile_q)
         plan = cls(tile_q, num_tokens, torch.device(device), segs, work, key_lo, cost, past_dicts, col_seg,
-                   num_work=len(work), num_cols=len(col_seg))
+                   num_work=len(work), num_cols=len(col_seg), pasts=[(s.past, s.past_len) if s.past else (None, 0) for s in segments])
         plan.segs_d = _upload(segs, device)
         plan.work_d = _upload(work, device)
         plan.key_lo_d = _upload(key_lo, device)
@@ -290,7 +292,8 @@ class TilePlan:
                              "exceed the device planner's limits")
         dev = torch.device(device)
         stream = torch.cuda.current_stream(dev).cuda_stream
-        plan = cls(tile_q, num_tokens, dev, segs, None, None, None, past_dicts, None, num_work=w, num_cols=c, filled={stream: None})
+        plan = cls(tile_q, num_tokens, dev, segs, None, None, None, past_dicts, None, num_work=w, num_cols=c, filled={stream: None},
+                   pasts=[(s.past, s.past_len) if s.past else (None, 0) for s in segments])
         blob = _upload(np.concatenate([segs.ravel(), starts]).astype(np.int32), dev)  # the one upload
         plan.segs_d = blob[:segs.size]
         plan.key_lo_d = torch.empty(num_tokens, dtype=torch.int32, device=dev)

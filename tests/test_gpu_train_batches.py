@@ -1,5 +1,5 @@
 """attend_train over batches that change or that training and other calls share: rows of no segment where nothing needs a
-gradient, tables uploaded on another stream, first calls in a capture.
+gradient, tables uploaded on another stream, first calls in a capture, prefix-cache entries replaced between calls.
 
 Results are compared bit for bit with those of the same kernels on the same values."""
 import math
@@ -11,6 +11,7 @@ import torch.utils.checkpoint
 import test_gpu_attend_train
 from dan_amd import workloads
 from dan_amd.attention import Batch, attend, attend_train, segment
+from oracle import training as oracle
 from test_gpu_train_calls import same, say, way, ways  # noqa: F401  -- the fixture of `ways`
 
 pytestmark = pytest.mark.gpu
@@ -243,3 +244,106 @@ def test_another_layers_first_call_in_a_capture(gpu, count, other, allowed, way)
             graph.replay()
             torch.cuda.synchronize()
             assert same(got, want[1]) and same(train(*x, segs, 1), want[1])
+
+
+# ---------------------------------------------------------------- prefix-cache entries
+LENGTHS = [(40, [5, 9]), (0, [3, 4]), (7, [2])]
+
+
+@ways
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("change", ["entry", "dict", "swap", "longer", "copy"])
+def test_prefix_entries_replaced_between_calls(gpu, change, dtype, way):  # noqa: F811
+    """A batch that is run again behind other prefixes (as when each step of a training loop makes them anew) reads those."""
+    say("attend_train, prefix replaced:", change, dtype, way)
+    other = change == "copy"
+    dicts = [{0: entry(gpu, 1, 12, dtype, other=other)}, None, {0: entry(gpu, 2, 12, dtype, other=other)}]
+    segs, n = batch(gpu, LENGTHS, dicts)
+    g = torch.Generator().manual_seed(3)
+    q, k, v, grad = (torch.randn(h, n, 64, generator=g).to(dtype).to(gpu) for h in (4, 2, 2, 4))
+    first = test_gpu_attend_train.train(q, k, v, grad, segs)
+    if change == "entry":
+        segs[0].past[0] = entry(gpu, 5, 12, dtype)
+    elif change == "dict":
+        segs[0].past = {0: entry(gpu, 5, 12, dtype)}
+    elif change == "swap":
+        segs[0].past, segs[2].past = segs[2].past, segs[0].past
+    elif change == "longer":
+        segs[0].past, segs[0].past_len = {0: entry(gpu, 5, 33, dtype)}, 33
+    else:
+        segs[0].past[0][0].mul_(0.5)
+        segs[2].past[0][1].add_(1)
+    fresh, _ = batch(gpu, LENGTHS, [s.past for s in segs])
+    want = test_gpu_attend_train.train(q, k, v, grad, fresh)
+    assert not torch.equal(want[0], first[0])
+    for _ in range(2):
+        assert same(test_gpu_attend_train.train(q, k, v, grad, segs), want)
+        with torch.no_grad():
+            assert torch.equal(attend_train(q, k, v, segs, 0), want[0])
+    test_gpu_attend_train.check(want, oracle.attend(q, k, v, segs, 0, grad=grad), dtype)
+
+
+@ways
+def test_an_entry_that_the_batch_itself_saves(gpu, way):  # noqa: F811
+    """A segment behind another one's saved rows: each call reads the rows that it has saved, not an earlier call's, in each layer."""
+    say("attend_train, a prefix that the batch saves", way)
+
+    def make():
+        segs, n = batch(gpu, [(20, [5]), (9, [4, 3])], [None, None])
+        segs[0].save = 13
+        segs[1].past, segs[1].past_len = segs[0].saved, 13
+        return segs, n
+
+    segs, n = make()
+    g = torch.Generator().manual_seed(3)
+    sets = [[torch.randn(h, n, 64, generator=g).to(BF16).to(gpu) for h in (4, 2, 2, 4)] for _ in range(3)]
+    want = [train(*x, make()[0], 0) for x in sets]
+    for _ in range(2):
+        for layer in (0, 1):
+            for x, w in zip(sets, want):
+                assert same(train(*x, segs, layer), w)
+    for x, w in zip(sets, want):
+        assert torch.equal(attend_train(*x[:3], segs, 0), w[0])
+
+
+@pytest.mark.parametrize("change", ["dict", "grown"])
+def test_a_batch_changed_before_another_layers_first_call(gpu, change):
+    say("attend_train, batch changed before another layer:", change)
+    dicts = [{i: entry(gpu, 1 + i, 12) for i in range(2)}, None, None]
+    segs, n = batch(gpu, LENGTHS[:2], dicts)
+    g = torch.Generator().manual_seed(3)
+    x = [torch.randn(h, n + 9, 64, generator=g).to(BF16).to(gpu) for h in (4, 2, 2, 4)]
+    train(*x, segs, 0)
+    if change == "dict":
+        segs[0].past, segs[0].past_len = {i: entry(gpu, 5 + i, 20) for i in range(2)}, 20
+    else:
+        segs.append(segment(n, workloads.branch_ids(*LENGTHS[2]), None, 0, 0, str(gpu)))
+    for layer in (1, 0):
+        want = train(*x, Batch(segs), layer)
+        assert same(train(*x, segs, layer), want) and torch.equal(attend_train(*x[:3], segs, layer), want[0])
+
+
+def test_a_captured_step_keeps_its_entries(gpu):
+    """A call behind replaced entries leaves the tables alone that a captured step reads."""
+    say("attend_train, captured behind entries that are replaced")
+    segs, n = batch(gpu, LENGTHS, [{0: entry(gpu, 1, 12)}, None, {0: entry(gpu, 2, 12)}])
+    g = torch.Generator().manual_seed(3)
+    x = [torch.randn(h, n, 64, generator=g).to(BF16).to(gpu) for h in (4, 2, 2, 4)]
+    want = train(*x, segs)
+    leaves = [t.detach().requires_grad_() for t in x[:3]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = attend_train(*leaves, segs, 0)
+        got = [out.detach(), *torch.autograd.grad(out, leaves, x[3])]
+    kept = segs[0].past[0]
+    for i in range(3):
+        segs[0].past[0] = entry(gpu, 10 + i, 12)
+        other = train(*x, segs)
+        assert not torch.equal(other[0], want[0])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(got, want)
+    segs[0].past[0] = kept
+    assert same(train(*x, segs), want)
