@@ -98,7 +98,8 @@ def adapt(y, x, a, b, index=None, scale=1.0):
     Sums are fp32 in an order that the sizes alone fix; x a^T stays fp32, the result
     is rounded once. Rows of other adapters take no part in a row's sums, whatever
     they hold. Ranks 1 to 128, n_in and n_out multiples of 8
-    up to 2^20, at most 2^20 rows.
+    up to 2^20, at most 2^20 rows and 65535 adapters; rows * max(n_in, n_out) below
+    2^39, and for the gradient R * (n_in + n_out) below 2^30, that times rank below 2^35.
 
     Differentiable (once) in y, x, a and b. A backward pass that is captured into a HIP graph has
     its forward pass in the same capture, and no earlier, eager result that holds

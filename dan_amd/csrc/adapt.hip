@@ -1005,15 +1005,29 @@ hipError_t launch_down(DownParams p, int splits, hipStream_t s) {
        : p.ranks == 64 ? launch_down<T, 4>(p, splits, s) : launch_down<T, 8>(p, splits, s);
 }
 
+// The grid of `up`, and the steps of a work group (many rows).
+struct UpGrid {
+  int x, y, threads, steps;
+  UpGrid(int rows, int cols, int rank, int adapters) : steps(1) {
+    if (few(rows, rank, adapters)) {
+      x = std::max(1, (cols + kUpCols - 1) / kUpCols);
+      y = (rows + 15) / 16;
+      threads = 64 * kFewWaves;
+      return;
+    }
+    const int groups = std::max(1, (cols + 4 * kUpCols - 1) / (4 * kUpCols));
+    y = (rows + 16 * kUpFrags - 1) / (16 * kUpFrags);
+    steps = std::max(1, std::min(4, (int)((int64_t)y * groups / 768)));
+    x = (groups + steps - 1) / steps;
+    threads = kThreads;
+  }
+};
 template <typename T, int ST, Form FORM>
 hipError_t launch_up(UpParams p, hipStream_t s) {
-  if (few(p.rows, p.rank, p.adapters)) {
-    hipLaunchKernelGGL((up_few_kernel<T, ST, FORM>), dim3(std::max(1, (p.cols + kUpCols - 1) / kUpCols), (p.rows + 15) / 16), dim3(64 * kFewWaves), 0, s, p);
-    return hipGetLastError();
-  }
-  const int tiles = (p.rows + 16 * kUpFrags - 1) / (16 * kUpFrags), cols = std::max(1, (p.cols + 4 * kUpCols - 1) / (4 * kUpCols));
-  p.steps = std::max(1, std::min(4, (int)((int64_t)tiles * cols / 768)));
-  hipLaunchKernelGGL((up_kernel<T, ST, FORM>), dim3((cols + p.steps - 1) / p.steps, tiles), dim3(kThreads), 0, s, p);
+  const UpGrid g(p.rows, p.cols, p.rank, p.adapters);
+  p.steps = g.steps;
+  if (few(p.rows, p.rank, p.adapters)) hipLaunchKernelGGL((up_few_kernel<T, ST, FORM>), dim3(g.x, g.y), dim3(g.threads), 0, s, p);
+  else hipLaunchKernelGGL((up_kernel<T, ST, FORM>), dim3(g.x, g.y), dim3(g.threads), 0, s, p);
   return hipGetLastError();
 }
 template <typename T, int ST>
@@ -1142,7 +1156,7 @@ hipError_t backward(const DanAdaptGradArgs &a, const GradSpace &w, hipStream_t s
 }
 
 // A launch holds fewer than 2^32 threads.
-bool too_many(int64_t groups) { return groups * kThreads >= int64_t(1) << 32; }
+bool too_many(int64_t groups, int threads = kThreads) { return groups * threads >= int64_t(1) << 32; }
 int64_t over(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
 int check_sizes(int dtype, int rows, int n_in, int n_out, int rank, int adapters, float scale_value) {
@@ -1153,12 +1167,18 @@ int check_sizes(int dtype, int rows, int n_in, int n_out, int rank, int adapters
   if (rank <= 0 || rank > DAN_ADAPT_MAX_RANK) return fail(DAN_ERR_UNSUPPORTED, "rank %d: 1 to %d", rank, DAN_ADAPT_MAX_RANK);
   if (adapters <= 0 || adapters > 65535) return fail(DAN_ERR_UNSUPPORTED, "%d adapters: 1 to 65535", adapters);
   if (!(isfinite(scale_value))) return fail(DAN_ERR_INVALID_ARGUMENT, "scale_value must be finite");
-  const int64_t wide = std::max(n_in, n_out);  // (`up` has the most threads by far: 2 columns of 16 rows each for few rows)
-  if (too_many(over(wide, kUpCols) * over(rows, 16) * 2) ||
-      too_many((over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters * std::max(parts_of(rows, n_in, n_out, adapters), parts_of(rows, n_in, 0, adapters))) ||
-      too_many((over(n_in, 64) + over(n_out, 64) + 1) * adapters) ||
-      too_many(over((int64_t)adapters * rank * ((int64_t)n_in + n_out), 8 * kThreads)))
-    return fail(DAN_ERR_UNSUPPORTED, "%d rows, %d to %d, %d adapters: more than one launch holds", rows, n_in, n_out, adapters);
+  // (`up` has the most threads by far: one for 2 values, or with many rows for 32 to 128. `down` has 2^26 at most.)
+  const UpGrid up(rows, std::max(n_in, n_out), rank, adapters);
+  if (too_many((int64_t)up.x * up.y, up.threads))
+    return fail(DAN_ERR_UNSUPPORTED, "%d rows of %d columns: more than one launch holds (2^39 values)", rows, std::max(n_in, n_out));
+  return DAN_OK;
+}
+// And of the gradient, whose other launches grow with the adapters.
+int check_grad_sizes(int rows, int n_in, int n_out, int rank, int adapters) {
+  const int64_t groups = (over(n_in, kOuterCols) + over(n_out, kOuterCols)) * adapters;
+  if (too_many(groups * std::max(parts_of(rows, n_in, n_out, adapters), parts_of(rows, n_in, 0, adapters))) ||
+      too_many((over(n_in, 64) + over(n_out, 64) + 1) * adapters) || too_many(over((int64_t)adapters * rank * ((int64_t)n_in + n_out), 8 * kThreads)))
+    return fail(DAN_ERR_UNSUPPORTED, "%d adapters of rank %d, %d to %d: more than one launch holds (columns 2^30, numbers 2^35)", adapters, rank, n_in, n_out);
   return DAN_OK;
 }
 bool bad_rows(const void *p, int64_t stride) { return ((uintptr_t)p & 15) || stride % 8 || stride < 0; }
@@ -1177,7 +1197,9 @@ int64_t dan_adapt_workspace_size(int32_t rows, int32_t n_in, int32_t rank, int32
 
 int64_t dan_adapt_grad_workspace_size(int32_t rows, int32_t n_in, int32_t n_out, int32_t rank, int32_t adapters) {
   using namespace dan;
-  if (rows <= 0 || check_sizes(DAN_DTYPE_BF16, rows, n_in, n_out, rank, adapters, 0.f) != DAN_OK) return 0;
+  if (rows <= 0 || check_sizes(DAN_DTYPE_BF16, rows, n_in, n_out, rank, adapters, 0.f) != DAN_OK ||
+      check_grad_sizes(rows, n_in, n_out, rank, adapters) != DAN_OK)
+    return 0;
   return GradSpace(rows, n_in, n_out, rank, adapters).total;
 }
 
@@ -1209,6 +1231,7 @@ int dan_adapt_grad(const DanAdaptGradArgs *a, void *stream) {
   if (a->abi_version != DAN_ADAPT_ABI_VERSION)
     return fail(DAN_ERR_VERSION, "abi_version %d, library speaks %d", a->abi_version, DAN_ADAPT_ABI_VERSION);
   if (const int rc = check_sizes(a->dtype, a->rows, a->n_in, a->n_out, a->rank, a->adapters, a->scale_value)) return rc;
+  if (const int rc = check_grad_sizes(a->rows, a->n_in, a->n_out, a->rank, a->adapters)) return rc;
   if (a->rows == 0) return DAN_OK;
   if (!a->x || !a->g || !a->a || !a->b || !a->down) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL pointer");
   if (bad_rows(a->x, a->x_stride) || bad_rows(a->g, a->g_stride) || bad_rows(a->dx, a->dx ? a->dx_stride : 0) ||

@@ -26,6 +26,10 @@ extern "C" {
 #define DAN_ADAPT_ABI_VERSION 1
 #define DAN_ADAPT_MAX_RANK 128
 
+/* Sizes: rows to 2^20, n_in and n_out multiples of 8 to 2^20, ranks to 128, 65535 adapters; together, as far as one launch
+ * goes: rows * max(n_in, n_out) below 2^39, and for the gradient adapters * (n_in + n_out) below 2^30 and that times rank
+ * below 2^35. */
+
 typedef struct {
   int32_t abi_version; /* DAN_ADAPT_ABI_VERSION */
   int32_t dtype;       /* DAN_DTYPE_BF16 or DAN_DTYPE_F16: x, y, a, b, out */

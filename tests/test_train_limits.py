@@ -1,13 +1,16 @@
-"""What training calls decide on the host, without a GPU: rows of no segment, and what a capture may begin with."""
+"""What training calls decide on the host, without a GPU: rows of no segment, what a capture may begin with, and
+which sizes a launch holds."""
+import ctypes
 import itertools
 
 import pytest
 
 import torch
 
-from dan_amd import _grad, _native, workloads
+from dan_amd import _grad, _layer, _native, workloads
 from dan_amd.attention import Batch, _uncovered, segment
 from dan_amd.plan import TilePlan
+from test_abi import lib  # noqa: F401  -- the library fixture
 
 
 @pytest.mark.parametrize("spans", [[], [(0, 9)], [(2, 9)], [(0, 4), (4, 9)], [(6, 9), (1, 3)], [(0, 3), (5, 6), (8, 11)], [(3, 3), (4, 9)], [(2, 7), (3, 5)]])
@@ -47,3 +50,30 @@ def test_what_a_capture_may_begin_with():
             assert not _grad.capturable(plan, 0, layout)
             plan.past_uploaded.add(0)
         assert _grad.capturable(plan, 0, layout) and not _grad.capturable(plan, 1, layout)
+
+
+P = 4096  # an aligned address that no call reads
+
+
+def adapt_args(cls, rows, n_in, n_out, rank, adapters):
+    a = cls()
+    a.abi_version, a.dtype, a.scale_value = _layer.ADAPT_ABI_VERSION, _native.DTYPE_BF16, 1.0
+    a.rows, a.n_in, a.n_out, a.rank, a.adapters = rows, n_in, n_out, rank, adapters
+    return a  # (x is missing: sizes that are taken end there)
+
+
+@pytest.mark.parametrize("rows,n_in,n_out,rank,adapters,forward,gradient", [
+    # up to what a launch of the kernels for many rows holds, a thread for 128 values
+    (1 << 20, 8, 8192, 16, 1, True, True), (1 << 19, 4096, 28672, 64, 8, True, True), (131072, 64, 65536, 16, 3, True, True),
+    (1 << 20, 1 << 18, 8, 8, 1, True, True), (1 << 20, 8, (1 << 19) - 1024, 1, 1, True, True), (1 << 20, 8, 1 << 19, 1, 1, False, False),
+    (1 << 20, 1 << 20, 32, 8, 1, False, False), (1 << 19, 8, (1 << 20) - 1024, 1, 1, True, True), (1 << 19, 8, 1 << 20, 1, 1, False, False),
+    # few rows: a thread for 2 values, always held
+    (640, 1 << 20, 1 << 20, 16, 1, True, True), (768, 1 << 20, 1 << 20, 16, 5, True, True),
+    # many adapters are the gradient's limit
+    (64, 8192, 28672, 1, 65535, True, False), (64, 8192, 4096, 1, 65535, True, True), (64, 8192, 8192, 128, 16383, True, True), (64, 8192, 8192, 128, 16400, True, False)])
+def test_adapts_sizes(lib, rows, n_in, n_out, rank, adapters, forward, gradient):  # noqa: F811
+    for name, cls, taken in (("dan_adapt", _layer.DanAdaptArgs, forward), ("dan_adapt_grad", _layer.DanAdaptGradArgs, gradient)):
+        a = adapt_args(cls, rows, n_in, n_out, rank, adapters)
+        assert lib[name](ctypes.byref(a), None) == (_native.ERR_INVALID_ARGUMENT if taken else _native.ERR_UNSUPPORTED)
+        assert ("NULL" if taken else "one launch") in _native.last_error(lib)
+    assert (_layer.adapt_grad_workspace_size(rows, n_in, n_out, rank, adapters) > 0) == gradient
