@@ -97,7 +97,9 @@ def adapt(y, x, a, b, index=None, scale=1.0):
 
     Sums are fp32 in an order that the sizes alone fix; x a^T stays fp32, the result
     is rounded once. Rows of other adapters take no part in a row's sums, whatever
-    they hold. Ranks 1 to 128, n_in and n_out multiples of 8
+    they hold. An infinite x a^T (G b in the gradients) gives the formula's infinities;
+    an infinity in b (and where the gradients multiply by them, in a, x or G)
+    gives an infinity or NaN. Ranks 1 to 128, n_in and n_out multiples of 8
     up to 2^20, at most 2^20 rows and 65535 adapters; rows * max(n_in, n_out) below
     2^39, and for the gradient R * (n_in + n_out) below 2^30, that times rank below 2^35.
 

@@ -11,7 +11,7 @@
 //
 // The values between two products (h, g) stay fp32 in memory and enter the second product as the sum of two
 // 16-bit numbers, v = hi + lo, side by side along the product's inner dimension: it costs matrix operations,
-// of which there are plenty, and keeps 16 bits or more of v. fp16 numbers are first brought near 1 by a power
+// of which there are plenty, and keeps 16 bits or more of v; an infinite v is hi alone. fp16 numbers are first brought near 1 by a power
 // of 2 (of a row, or of a tile of rows), so that no v leaves their range.
 //
 // Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 21 us (67 MB), up 205 us (940 MB, 4.6 TB/s); gradients: g and dB in one
@@ -60,6 +60,17 @@ __device__ inline f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// What 8 values leave of themselves when they are rounded to `hi`; zeros where that is infinite, whose sum with them it stays.
+template <typename T>
+__device__ inline u32x4 low_part(f32x8 x, u32x4 hi) {
+  x -= unpack8<T>(hi);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = fabsf(x[e]) < INFINITY ? x[e] : 0.f;
+  return pack8<T>(x);
+}
+// |x|, or 0 for infinities and NaN: they have no part in a power of 2.
+__device__ inline float finite_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+
 // The power of 2 (as its exponent) that brings m into [1, 2); 0 for zeros, infinities and NaN.
 __device__ inline int exponent_of(float m) { return m > 0.f && m < INFINITY ? -max(ilogbf(m), -126) : 0; }
 
@@ -79,7 +90,8 @@ struct DownParams {
 
 // Rows as operands: 16 F of them, four steps of 32 values from k0 on. A lane loads 16 bytes, four lanes 64 of a row.
 // (Here and below every load is made, at a clamped place where there is none to make: a load under a condition of
-// its own is a branch, and waits for the ones before it. Values past the row's end become zeros in x alone.)
+// its own is a branch, and waits for the ones before it. Values past the row's end become zeros in x and in w: either's last ones
+// may be infinite.)
 template <typename T, int F>
 __device__ inline void load_rows(const T *const (&row)[F], int k0, int last, int g4, u32x4 (&to)[F][4]) {
 #pragma unroll
@@ -101,6 +113,12 @@ __device__ inline void load_chunk(const DownParams &p, int i, int k0, int last, 
   for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
     for (int s = 0; s < 4; ++s) wf[jb][s] = load16(w + (int64_t)min(16 * jb + l16, p.rank - 1) * p.n + min(k0 + 32 * s + 8 * g4, last - 8));
+  if (k0 + kChunk > last)
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (k0 + 32 * s + 8 * g4 >= last) wf[jb][s] = u32x4{};
 }
 // t += w x^T over it.
 template <typename T, int JB, int F>
@@ -294,7 +312,7 @@ struct Operand {
       if (p.sum && blockIdx.x == 0 && n < p.rows) *(DAN_TILE_GLOBAL f32x4 *)(p.sum + (int64_t)n * p.ranks + 4 * j4) = sum[x];
       v[r][j4] = sum[x];
       if (kHalf) {
-        const float m = fmaxf(fmaxf(fabsf(sum[x][0]), fabsf(sum[x][1])), fmaxf(fabsf(sum[x][2]), fabsf(sum[x][3])));
+        const float m = fmaxf(fmaxf(finite_size(sum[x][0]), finite_size(sum[x][1])), fmaxf(finite_size(sum[x][2]), finite_size(sum[x][3])));
         atomicMax(&top[r], __builtin_bit_cast(uint32_t, m));  // (of values that are not negative: in any order)
       }
     }
@@ -314,7 +332,7 @@ struct Operand {
           for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], e2);
         }
         to = pack8<T>(x);
-        if (u >= r8) to = pack8<T>(x - unpack8<T>(to));
+        if (u >= r8) to = low_part<T>(x, to);
       }
       piece[q] = to;
     }
@@ -598,7 +616,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
       for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[jb][e]));
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_size(v[jb][e]));
 #pragma unroll
       for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
       e2 = exponent_of(top);
@@ -610,7 +628,7 @@ __global__ __launch_bounds__(kThreads) void outer_kernel(const OuterParams p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = kHalf ? ldexpf(v[jb][e], e2) : v[jb][e];
       hi[jb] = pack8<T>(x);
-      lo[jb] = pack8<T>(x - unpack8<T>(hi[jb]));
+      lo[jb] = low_part<T>(x, hi[jb]);
     }
     const float back = kHalf ? ldexpf(1.f, -e2) : 1.f;
     wait_vmem<0>();
@@ -735,7 +753,7 @@ __global__ __launch_bounds__(kThreads, 2) void both_kernel(const BothParams p) {
     f32x8 x;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 8 * g4 + e < rows ? vn[e] : 0.f;
-    const u32x4 hi = pack8<T>(x), lo = pack8<T>(x - unpack8<T>(hi));
+    const u32x4 hi = pack8<T>(x), lo = low_part<T>(x, hi);
     f32x4 g[2] = {};
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {

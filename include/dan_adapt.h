@@ -9,7 +9,9 @@
  *
  * x [N, n_in] is the projection's input, y [N, n_out] its output, A_i [rank,
  * n_in], B_i [n_out, rank]. A negative index: no adapter (out = y). An index
- * past the last adapter gives NaN.
+ * past the last adapter gives NaN. An infinite x A^T (or G B) gives the formula's
+ * infinities; an infinity that is itself a factor of it (in B, and for the gradients
+ * in A, x or G) gives an infinity or NaN.
  *
  * Conventions as in dan_tree_attn.h: device memory of the caller, rows of unit
  * stride that start 16 bytes aligned, 0 on success, dan_tree_attn_last_error().
