@@ -1,4 +1,9 @@
-"""adapt and its gradient on infinities between the two products. Tolerances as in test_gpu_adapt."""
+"""adapt and its gradient on values far apart from each other, and on infinities between the two products.
+
+A value v between the two products enters the second one as the sum of two 16-bit numbers. In fp16 it is multiplied before by a power of
+2 that is one for a row (out, dx) or a tile of 32 rows (the gradients of a and b) and brings the largest |v| to 2^14 or
+above: 2^-25 of a number that is 2^-20 of the largest's size is 2^-25 / 2^(14 - 20) = 2^-19 of it, and what is above that
+scale has 22 bits. test_gpu_adapt's tolerance (2^-13 of the sum of magnitudes) holds for it as it stands."""
 import math
 
 import pytest
@@ -15,6 +20,57 @@ BF16, FP16 = torch.bfloat16, torch.float16
 
 def say(*a):
     print("[gpu-case]", *a, flush=True)
+
+
+# ---------------------------------------------------------------- values far apart
+@pytest.mark.parametrize("rank", [5, 16, 64, 128])
+@pytest.mark.parametrize("n", [40, 600])
+def test_fp16_rows_of_very_different_size(gpu, n, rank):
+    """Rows whose G is 2^20 times the others', and whose x (or the other way round) is zero in the columns looked at: those columns'
+    gradients are sums of the small rows' products alone."""
+    say("adapt fp16, rows of very different size", n, rank)
+    y, x, a, b, _, _, grad = test_gpu_adapt.make(gpu, n, 136, 200, rank, 1, FP16)
+    a, big = a * 0.25, torch.arange(n, device=gpu) % 8 == 3
+    for name in ("da", "db"):
+        z, w = x.clone(), grad.clone()
+        if name == "da":  # g of the large rows reaches the last 8 columns of a alone
+            w[big], w[~big] = w[big] * 2.0 ** 8, w[~big] * 2.0 ** -12
+            z[big, :-8], z[big, -8:] = 0, z[big, -8:] * 2.0 ** -12
+            z[~big] *= 2.0 ** 6
+        else:  # h of the large rows reaches the last 8 rows of b alone
+            z[big], z[~big] = z[big] * 2.0 ** 8, z[~big] * 2.0 ** -12
+            w[big, :-8], w[big, -8:] = 0, w[big, -8:] * 2.0 ** -12
+            w[~big] *= 2.0 ** 8
+        ref = oracle.adapt(y, z, a, b, [0] * n, 0.5, w)
+        small = ref[name][0, :, :-8] if name == "da" else ref[name][0, :-8]
+        assert small.abs().mean() > 2 ** -9 and all(r.isfinite().all() for r in ref.values())
+        test_gpu_adapt.check(test_gpu_adapt.run(y, z, a, b, None, 0.5, w), ref, FP16, ["out", "dx", "da", "db"])
+
+
+@pytest.mark.parametrize("rank", [5, 16, 64, 128])
+@pytest.mark.parametrize("n", [40, 600])
+def test_fp16_ranks_of_very_different_size(gpu, n, rank):
+    """Ranks whose h is 2^20 times the others' and that some rows of b (or whose g and columns of a) leave out."""
+    say("adapt fp16, ranks of very different size", n, rank)
+    y, x, a, b, _, _, grad = test_gpu_adapt.make(gpu, n, 136, 200, rank, 1, FP16)
+    big = torch.arange(rank, device=gpu) % 4 == 1
+    y = y * 0
+    for name in ("out", "dx"):
+        p, q, w, z = a.clone(), b.clone() * 0.25, grad.clone(), x.clone()
+        if name == "out":
+            p[0, big], p[0, ~big] = p[0, big] * 2.0 ** 9, p[0, ~big] * 2.0 ** -11
+            q[0, :-8, big], q[0, -8:, big] = 0, q[0, -8:, big] * 2.0 ** -9
+            q[0, :, ~big] *= 2.0 ** 9
+            w *= 2.0 ** -10
+        else:
+            q[0, :, big], q[0, :, ~big] = q[0, :, big] * 2.0 ** 7, q[0, :, ~big] * 2.0 ** -13
+            p[0, big, :-8], p[0, big, -8:] = 0, p[0, big, -8:] * 2.0 ** -9
+            p[0, ~big] *= 2.0 ** 11
+            z *= 2.0 ** -10
+        ref = oracle.adapt(y, z, p, q, [0] * n, 0.5, w)
+        small = ref[name][:, :-8]
+        assert small.abs().mean() > 2 ** -9 and all(r.abs().max() < 65504 for r in ref.values())
+        test_gpu_adapt.check(test_gpu_adapt.run(y, z, p, q, None, 0.5, w), ref, FP16, ["out", "dx", "da", "db"])
 
 
 # ---------------------------------------------------------------- infinities
