@@ -304,6 +304,9 @@ int dan_add_norm(const DanNormArgs *a, void *stream) {
     return fail(DAN_ERR_INVALID_ARGUMENT, "layout %d: 0 (rows) or 1 (tiled)", a->layout);
   if (a->rows == 0) return DAN_OK;
   if (!a->x || !a->weight || (!a->out && !a->codes) || (a->codes && !a->scale)) return fail(DAN_ERR_INVALID_ARGUMENT, "NULL pointer");
+  // (a work group each row, also those of the last panel; up to 1024 columns four rows share one)
+  if (a->codes && a->layout == DAN_FP8_LAYOUT_TILED && a->cols > 1024 && a->rows > (1 << 24) - 256)
+    return fail(DAN_ERR_INVALID_ARGUMENT, "rows %d: at most 2^24 - 256 with %d columns in the tiled layout", a->rows, a->cols);
   if (a->codes && a->cols % 16) return fail(DAN_ERR_UNSUPPORTED, "cols %d: a multiple of 16 for codes", a->cols);
   if (bad_rows(a->x, a->x_stride, a->rows, a->cols, false) || (a->residual && bad_rows(a->residual, a->residual_stride, a->rows, a->cols, false)) ||
       (a->stream && bad_rows(a->stream, a->stream_stride, a->rows, a->cols, true)) ||

@@ -174,7 +174,7 @@ PyObject *add_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
   if (x.dim() != 2 || !is16(x.scalar_type()) || !plain(x, index) || !rows_ok(x)) Py_RETURN_NONE;
   const int64_t n = x.size(0), k = x.size(1);
-  if (n == 0 || n >= 1 << 24 || k == 0 || k > DAN_NORM_MAX_COLS || k % (f.layout < 0 ? 8 : 16)) Py_RETURN_NONE;
+  if (n == 0 || n >= 1 << 24 || (f.layout == DAN_FP8_LAYOUT_TILED && k > 1024 && n > (1 << 24) - 256) || k == 0 || k > DAN_NORM_MAX_COLS || k % (f.layout < 0 ? 8 : 16)) Py_RETURN_NONE;
   if (residual.defined() && (residual.sizes() != x.sizes() || residual.scalar_type() != x.scalar_type() || !plain(residual, index) || !rows_ok(residual)))
     Py_RETURN_NONE;
   if (weight.dim() != 1 || weight.size(0) != k || weight.scalar_type() != x.scalar_type() || !plain(weight, index) || !dense_ok(weight)) Py_RETURN_NONE;

@@ -107,7 +107,8 @@ def add_norm(x, residual, weight, *, eps=1e-6, norm="rms", fp8=None, out=None):
     The norm is of the fp32 sum; ``out`` and the codes are each rounded once, from
     fp32. ``out`` defaults to whether ``fp8`` is None; True gives both, as a
     projection with adapters needs them. K: a multiple of 8 (16 with ``fp8``), at
-    most 16384; fewer than 2^24 rows.
+    most 16384; fewer than 2^24 rows (with ``fp8`` "tiled" and
+    more than 1024 columns at most 2^24 - 256).
 
     Without ``fp8`` the result is differentiable (once) in x, residual and weight;
     the gradient takes the sum as ``stream`` holds it. A backward pass that is
@@ -133,8 +134,8 @@ def add_norm(x, residual, weight, *, eps=1e-6, norm="rms", fp8=None, out=None):
     n, k = x.shape
     if k % (8 if fp8 is None else 16) or not 0 < k <= _layer.MAX_COLS:
         raise ValueError(f"K {k}: a multiple of {8 if fp8 is None else 16} up to {_layer.MAX_COLS}")
-    if n >= 1 << 24:
-        raise ValueError(f"{n} rows: fewer than 2^24")
+    if n >= 1 << 24 or fp8 == "tiled" and k > 1024 and n > (1 << 24) - 256:
+        raise ValueError(f"{n} rows: fewer than 2^24, at most 2^24 - 256 with tiled codes of more than 1024 columns")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} on {residual.device} must be as x")
     if weight.shape != (k,) or weight.dtype != x.dtype or weight.device != x.device:

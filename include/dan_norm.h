@@ -31,7 +31,7 @@ enum { DAN_NORM_RMS = 0, DAN_NORM_ZERO_CENTERED = 1 };
 typedef struct {
   int32_t abi_version; /* DAN_NORM_ABI_VERSION */
   int32_t dtype;       /* DAN_DTYPE_BF16 or DAN_DTYPE_F16: x, residual, weight, stream, out */
-  int32_t rows, cols;  /* cols: a multiple of 8 (16 with codes), at most DAN_NORM_MAX_COLS */
+  int32_t rows, cols;  /* rows: below 2^24 (at most 2^24 - 256 with tiled codes of more than 1024 columns); cols: a multiple of 8 (16 with codes), at most DAN_NORM_MAX_COLS */
   int32_t norm;        /* DAN_NORM_* */
   int32_t layout;      /* of codes: DAN_FP8_LAYOUT_ROWS or DAN_FP8_LAYOUT_TILED (dan_fp8.h) */
   float eps;           /* finite, >= 0 */

@@ -77,3 +77,16 @@ def test_adapts_sizes(lib, rows, n_in, n_out, rank, adapters, forward, gradient)
         assert lib[name](ctypes.byref(a), None) == (_native.ERR_INVALID_ARGUMENT if taken else _native.ERR_UNSUPPORTED)
         assert ("NULL" if taken else "one launch") in _native.last_error(lib)
     assert (_layer.adapt_grad_workspace_size(rows, n_in, n_out, rank, adapters) > 0) == gradient
+
+
+@pytest.mark.parametrize("rows,cols,layout,taken", [
+    ((1 << 24) - 1, 4096, 0, True), ((1 << 24) - 256, 4096, 1, True), ((1 << 24) - 255, 4096, 1, False), ((1 << 24) - 1, 1040, 1, False), ((1 << 24) - 1, 1024, 1, True)])
+def test_add_norms_rows(lib, rows, cols, layout, taken):  # noqa: F811
+    """With tiled codes whole panels of 256 rows are launched, a work group each row (four up to 1024 columns): 2^24 of them are more than a
+    launch holds. (What is taken ends at its weight's alignment.)"""
+    a = _layer.DanNormArgs()
+    a.abi_version, a.dtype, a.rows, a.cols, a.eps, a.layout = _layer.NORM_ABI_VERSION, _native.DTYPE_BF16, rows, cols, 1e-6, layout
+    a.x = a.codes = a.scale = P
+    a.weight, a.x_stride = P + 2, cols
+    assert lib.dan_add_norm(ctypes.byref(a), None) == _native.ERR_INVALID_ARGUMENT
+    assert ("aligned" if taken else "2^24 - 256") in _native.last_error(lib)
