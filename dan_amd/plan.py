@@ -352,10 +352,14 @@ class TilePlan:
         stream pays for none. None if the stream has begun a capture since then."""
         import torch
 
-        stream, event = torch.cuda.ExternalStream(handle, device=self.device), torch.cuda.Event()
-        with torch.cuda.stream(stream):
-            if torch.cuda.is_current_stream_capturing():
-                return None
+        event = torch.cuda.Event()
+        if not handle:  # the default stream, which no capture takes (a stream made from its handle would be a new one)
+            stream = torch.cuda.default_stream(self.device)
+        else:
+            stream = torch.cuda.ExternalStream(handle, device=self.device)
+            with torch.cuda.stream(stream):
+                if torch.cuda.is_current_stream_capturing():
+                    return None
         event.record(stream)
         self.filled[handle] = event
         return event
