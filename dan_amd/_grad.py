@@ -169,6 +169,7 @@ class Tables:
         self.keys, self.queries = at, at + keys.nbytes
         self.row_lo = self.queries + queries.nbytes
         self.row_end = self.row_lo + row_lo.nbytes
+        plan.make_spare(ctypes.sizeof(_native.DanPastDesc) * max(len(plan.past_dicts), 1))
         plan.fills()
 
 
@@ -188,7 +189,8 @@ def capturable(plan, layer, layout):
         return False
     if layer in plan.past_tables:
         return plan.past_hosts[layer] is not None or layer in plan.past_uploaded
-    return len(plan.past_dicts) <= _native.INLINE_PASTS and all(A._in_place(x) for entry in plan.past_dicts for x in entry[layer][:2])
+    return (len(plan.past_dicts) <= _native.INLINE_PASTS and (not plan.past_dicts or layer in plan.spare)
+            and all(A._in_place(x) for entry in plan.past_dicts for x in entry[layer][:2]))
 
 
 def attend(q, k, v, segments, layer, scale):

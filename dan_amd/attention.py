@@ -187,8 +187,8 @@ def attend_train(q, k, v, segments, layer, scale=None):
     output's gradient of finite
     values: a hidden key's weight is zero, its products are not
     left out. The first call on a ``Batch`` uploads its tables (and a layer's first one its
-    prefix table, where the batch has more than 8 entries or some are copied), so it is refused
-    in the capture of a HIP graph; later ones can be captured, forward and backward in the same
+    prefix table, where the batch has more than 8 entries, some are copied, or the
+    first call had none of the layer's), so it is refused in the capture of a HIP graph; later ones can be captured, forward and backward in the same
     capture and with no earlier, eager result alive that holds the graph of the
     same leaves (where q, k or v is such a leaf itself, that raises)."""
     from . import _grad
@@ -432,9 +432,11 @@ def _past_table(plan, layer, hkv, d, dtype, device, upload=True):
         raw, refs = _past_descs(plan.past_dicts, plan.segs, layer, hkv, d, dtype, device, copied=(copied := {}))
         plan.past_hosts[layer] = raw if len(plan.past_dicts) <= _native.INLINE_PASTS else None
         if copied:
-            plan.fills()
             plan.past_copied[layer] = copied
-        plan.past_tables[layer] = (torch.empty(raw.numel(), dtype=torch.uint8, device=device), (refs, raw))
+        table = plan.spare.pop(layer) if layer in plan.spare else torch.empty(raw.numel(), dtype=torch.uint8, device=device)
+        if device.type == "cuda":  # (another stream may write the table only behind what its memory was used for here)
+            plan.filled[_native.stream(device)] = None
+        plan.past_tables[layer] = (table, (refs, raw))
     table, (refs, raw) = plan.past_tables[layer]
     if (upload or plan.past_hosts[layer] is None) and layer not in plan.past_uploaded:
         table.copy_(raw.pin_memory() if device.type == "cuda" else raw, non_blocking=True)

@@ -256,7 +256,8 @@ class TilePlan:
     schedules: dict = field(default_factory=dict)  # (groups, CUs) -> (units_d, sched_off_d, slots)
     tiles: dict = field(default_factory=dict)  # (heads, kv heads, head_dim) -> queries per work item that a call of this layout takes
     pasts: list = field(default_factory=list)  # each segment's prefix-cache entry and its length (None, 0: it has none)
-    filled: dict = field(default_factory=dict)  # stream that fills some of these tables -> event behind that, or None
+    spare: dict = field(default_factory=dict)  # layer -> an empty table for its prefix entries (``past_tables``)
+    filled: dict = field(default_factory=dict)  # stream that allocates or fills some of these tables -> event behind that, or None
     ordered: dict = field(default_factory=dict)  # stream -> the tables that ``order`` has seen to there
 
     @classmethod
@@ -317,11 +318,21 @@ class TilePlan:
         return plan
 
     def fills(self):
-        """Notes that the current stream fills tables of the plan (before they can be found there)."""
+        """Notes that the current stream allocates or fills tables of the plan (before they can be found there)."""
         if self.device.type == "cuda":
             import torch
 
-            self.filled[torch.cuda.current_stream(self.device).cuda_stream] = None
+            index = torch.cuda.current_device() if self.device.index is None else self.device.index
+            self.filled[torch._C._cuda_getCurrentRawStream(index)] = None
+
+    def make_spare(self, nbytes):
+        """Tables of ``nbytes`` for the layers that the prefix-cache entries hold and that have none yet, so that one whose first call is
+        in a capture has a table that shares no memory with the graph's other calls."""
+        import torch
+
+        layers = set.intersection(*map(set, self.past_dicts)) - set(self.past_tables) if self.past_dicts else ()
+        rows = torch.empty((len(layers), -(-nbytes // 256) * 256), dtype=torch.uint8, device=self.device)
+        self.spare = {layer: row[:nbytes] for layer, row in zip(layers, rows)}
 
     def order(self, device):
         """The current stream of ``device`` goes on behind the tables that other streams fill, and the allocator learns that

@@ -169,6 +169,38 @@ def test_a_later_layers_table_uploaded_on_another_stream(gpu, big, way):  # noqa
 
 
 @ways
+@pytest.mark.parametrize("count", [3, 12])
+def test_a_table_in_memory_that_its_stream_still_uses(gpu, big, count, way):  # noqa: F811
+    """A prefix table takes memory that was given back on its stream, where work that uses it may still be to come: a call on another
+    stream, which writes the table (3 entries) or reads it (12), comes behind that work."""
+    say("attend_train: a layer's table in memory still in use", count, way)
+    x, make = many(gpu, 8, count)
+    want = [train(*x, make(), layer) for layer in range(2)]
+    segs = make()
+    b, c = torch.cuda.Stream(), torch.cuda.Stream()
+    nbytes = segs_table_bytes(segs)
+    with torch.cuda.stream(b):
+        assert same(train(*x, segs, 0), want[0])
+        segs.tile_plan.spare.clear()  # (or the layer's table would be there already)
+        small = [torch.full((nbytes,), i % 251, dtype=torch.uint8, device=gpu) for i in range(512)]  # (also the holes that were there)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(b):
+        slow(big)
+        copies = [t.clone() for t in small[::2]]
+        del small[::2]
+        first = train(*x, segs, 1)
+    with torch.cuda.stream(c):
+        second = train(*x, segs, 1)
+    torch.cuda.synchronize()
+    assert same(first, want[1]) and same(second, want[1])
+    assert all((t == 2 * i % 251).all() for i, t in enumerate(copies))
+
+
+def segs_table_bytes(segs):
+    return max(72 * len(segs), 512)  # a DanPastDesc each, and what the allocator rounds to
+
+
+@ways
 @pytest.mark.parametrize("needs", [True, False])
 def test_a_batch_dropped_before_another_stream_has_read_it(gpu, big, needs, way):  # noqa: F811
     """Tables that were allocated on the stream of the first call, read on another one: their memory is not given away before that."""

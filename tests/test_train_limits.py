@@ -38,12 +38,16 @@ def test_what_a_capture_may_begin_with():
     plan = make(3, aligned)
     assert not _grad.capturable(plan, 0, layout)  # the backward pass's tables are missing
     plan.grad_tables[layout] = None
+    assert not _grad.capturable(plan, 0, layout)  # a prefix table in the capture's own memory
+    plan.make_spare(3 * 72)
+    assert set(plan.spare) == {0, 1} and all(t.shape == (3 * 72,) for t in plan.spare.values())
     assert _grad.capturable(plan, 0, layout) and not _grad.capturable(plan, 0, (8, 2, 64))
     odd = torch.zeros(2, 3, 65, dtype=torch.bfloat16)[..., 1:]
     copied = make(1, (aligned[0], odd))
     long = make(_native.INLINE_PASTS + 1, aligned)
     for plan in (copied, long):
         plan.grad_tables[layout] = None
+        plan.make_spare(72 * len(plan.past_dicts))
         assert not _grad.capturable(plan, 0, layout)
         plan.past_tables[0], plan.past_hosts[0] = None, None if plan is long else 0
         if plan is long:
