@@ -175,7 +175,8 @@ def attend_train(q, k, v, segments, layer, scale=None):
     (dan_amd/csrc/tree_attn_grad.hip). A kv head's gradients are summed over
     the heads that share it. Sums are fp32 in an order that the batch alone
     fixes; P and dS are rounded to the inputs' type for the matrix core, dS
-    after a power-of-2 scaling where that is fp16.
+    after a power-of-2 scaling where that is fp16 (one for the batch, from the
+    finite values: what is far below the batch's largest |dS| keeps fewer bits).
 
     Prefix-cache entries are constants (one that requires grad raises). Where
     others have taken their place since a ``Batch`` was first run, a call reads

@@ -96,6 +96,9 @@ __device__ inline float block_max(float x, float *red) {
   return x;
 }
 
+// The larger of two sizes; an infinite or NaN one has no part in fp16's power of 2, whose batch other segments share.
+__device__ inline float finite_max(float top, float x) { return x < INFINITY ? fmaxf(top, x) : top; }
+
 // Sum of squares over the L lanes of a row, 8 values each.
 template <typename T, int L>
 __device__ inline float row_square(u32x4 x) {
@@ -140,8 +143,8 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p)
       p.stats[rows + at] = -dot;
     }
     if (kHalf && p.row_end[n] > 0) {  // (rows of no segment may hold anything, and their dS is never made)
-      gmax = fmaxf(gmax, sq);
-      dmax = fmaxf(dmax, fabsf(dot));
+      gmax = finite_max(gmax, sq);
+      dmax = finite_max(dmax, fabsf(dot));
     }
   }
   if constexpr (kHalf) {
@@ -149,14 +152,14 @@ __global__ __launch_bounds__(kThreads) void grad_rows_kernel(const GradParams p)
     for (int64_t r = (int64_t)blockIdx.x * R + mine; r < vrows; r += (int64_t)gridDim.x * R) {
       const int64_t n = r / p.num_kv_heads, h = r % p.num_kv_heads;
       const float sq = row_square<T, L>(load16(static_cast<const T *>(p.v) + n * p.v_st + h * p.v_sh + 8 * sub));
-      if (p.row_end[n] > 0) vmax = fmaxf(vmax, sq);
+      if (p.row_end[n] > 0) vmax = finite_max(vmax, sq);
     }
     for (int i = 0; i < p.num_pasts; ++i) {
       const DanPastDesc pd = load_unit(p.pasts + i);
       const int64_t prows = (int64_t)pd.len * p.num_kv_heads;
       for (int64_t r = (int64_t)blockIdx.x * R + mine; r < prows; r += (int64_t)gridDim.x * R) {
         const int64_t n = r / p.num_kv_heads, h = r % p.num_kv_heads;
-        vmax = fmaxf(vmax, row_square<T, L>(load16(static_cast<const T *>(pd.v) + n * pd.v_stride_tok + h * pd.v_stride_head + 8 * sub)));
+        vmax = finite_max(vmax, row_square<T, L>(load16(static_cast<const T *>(pd.v) + n * pd.v_stride_tok + h * pd.v_stride_head + 8 * sub)));
       }
     }
     __shared__ float red[4];
@@ -184,7 +187,7 @@ __device__ inline float ds_factor(const GradParams &p, float *red) {
   v = block_max(v, red);
   d = block_max(d, red);
   const float bound = sqrtf(g) * sqrtf(v) + d;
-  if (!(bound > 0.f && bound < INFINITY)) return 1.f;
+  if (!(bound > 0.f)) return 1.f;
   const int e = min(max(14 - ilogbf(bound), -100), 100);
   return ldexpf(1.f, e);
 }
