@@ -132,6 +132,36 @@ __device__ inline void chunk_product(const u32x4 (&wf)[JB][4], const u32x4 (&xf)
       for (int s = 0; s < 4; ++s) t[jb][f] = mfma16<T>(wf[jb][s], xf[f][s], t[jb][f]);
 }
 
+// Both, for ranks up to 128, whose w fills the registers: zeros past the row's end (as load_chunk makes them) a rank block at a time,
+// in a chunk that has any. (Behind all of w's loads they would hold all of it at once: 4096 rows, 4096 -> 4096, rank 128, 61.3 us, and 57.4 so.)
+template <typename T, int JB, int F>
+__device__ inline void chunk_at_once(const DownParams &p, int i, int k0, int last, int l16, int g4, const u32x4 (&xf)[F][4], f32x4 (&t)[JB][F]) {
+  const T *w = static_cast<const T *>(p.w) + (int64_t)i * p.rank * p.n;
+  if (k0 + kChunk <= last) {
+    u32x4 wf[JB][4];
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) wf[jb][s] = load16(w + (int64_t)min(16 * jb + l16, p.rank - 1) * p.n + k0 + 32 * s + 8 * g4);
+    chunk_product<T, JB, F>(wf, xf, t);
+    return;
+  }
+#pragma unroll
+  for (int jb = 0; jb < JB; ++jb) {
+    u32x4 wf[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) wf[s] = load16(w + (int64_t)min(16 * jb + l16, p.rank - 1) * p.n + min(k0 + 32 * s + 8 * g4, last - 8));
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (k0 + 32 * s + 8 * g4 >= last) wf[s] = u32x4{};
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) t[jb][f] = mfma16<T>(wf[s], xf[f][s], t[jb][f]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Many rows: 32 a work group, whose W waves split the chunks and add up over LDS. Work groups begin at different chunks:
 // where a row's bytes are a multiple of a large power of 2, all of them at one place of their rows ask few channels of the memory.
 // Neighbours in the grid are the splits of a tile of rows, so that a die reads few of w's columns.
@@ -170,13 +200,14 @@ __global__ __launch_bounds__(64 * kDownWaves<JB>) void down_kernel(const DownPar
     if constexpr (kAhead) load_chunk<T, JB>(p, max(i0, 0), k0, last, l16, g4, wf);
     uint64_t left[F] = {own[0], own[1]};
     for (int i = i0; i >= 0;) {  // each adapter of the tile
-      if (!kAhead || i != i0) load_chunk<T, JB>(p, i, k0, last, l16, g4, wf);
+      if (kAhead && i != i0) load_chunk<T, JB>(p, i, k0, last, l16, g4, wf);
       f32x4 t[JB][F];
 #pragma unroll
       for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
         for (int f = 0; f < F; ++f) t[jb][f] = f32x4{};
-      chunk_product<T, JB, F>(wf, xf, t);
+      if constexpr (kAhead) chunk_product<T, JB, F>(wf, xf, t);
+      else chunk_at_once<T, JB, F>(p, i, k0, last, l16, g4, xf, t);
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const bool mine = idx[f] == i;
