@@ -335,27 +335,27 @@ class TilePlan:
         self.spare = {layer: row[:nbytes] for layer, row in zip(layers, rows)}
 
     def order(self, device):
-        """The current stream of ``device`` goes on behind the tables that other streams fill, and the allocator learns that
-        it reads them: a batch may be used on several streams, and dropped before the last of them has got there. Once
-        for each stream and table. (A capture begins with the device idle.)"""
+        """The current stream of ``device`` goes on behind the tables that other streams allocate or fill, and the allocator learns
+        that it reads them: a batch may be used on several streams, and dropped before the last of them has got there.
+        Once for each stream and table. (A capture begins with the device idle.)"""
         import torch
 
         from . import _native
 
         here = _native.stream(device)
-        state = (len(self.past_tables), len(self.past_uploaded), len(self.schedules), len(self.grad_tables))
+        state = (len(self.filled), len(self.past_tables), len(self.past_uploaded), len(self.schedules), len(self.grad_tables))
         if self.ordered.get(here) == state or torch.cuda.is_current_stream_capturing():
             return
-        stream = torch.cuda.current_stream(device)
-        for other, event in list(self.filled.items()):
-            event = event or self._event(other)
-            if other != here and event:
-                stream.wait_event(event)
-        tables = [self.segs_d, self.work_d, self.key_lo_d, self.col_seg_d, *(t.blob for t in list(self.grad_tables.values()))]
-        tables += [t for units, off, _ in list(self.schedules.values()) for t in (units, off)]
-        tables += [t for table, (refs, _) in list(self.past_tables.values()) for t in (table, *refs)]
-        for table in tables:
-            table.record_stream(stream)
+        if others := [other for other in list(self.filled) if other != here]:
+            stream = torch.cuda.current_stream(device)
+            for other in others:
+                if event := self.filled[other] or self._event(other):
+                    stream.wait_event(event)
+            tables = [self.segs_d, self.work_d, self.key_lo_d, self.col_seg_d, *(t.blob for t in list(self.grad_tables.values()))]
+            tables += [t for units, off, _ in list(self.schedules.values()) for t in (units, off)]
+            tables += [t for table, (refs, _) in list(self.past_tables.values()) for t in (table, *refs)]
+            for table in tables:
+                table.record_stream(stream)
         self.ordered[here] = state
 
     def _event(self, handle):
