@@ -18,7 +18,7 @@
 // Measured, 8192 rows, one adapter of rank 16, 4096 -> 28672: down 21 us (67 MB), up 205 us (940 MB, 4.6 TB/s); gradients: g and dB in one
 // pass 100 us (500 MB, 5 TB/s; in two, 130 + 83), g's parts 7, up 20, dA 19, the parts' sum 8. 64 rows of 24 adapters, 4096 -> 4096: 5 + 5 us, launches
 // and chains of index, weights and sums; 1037 rows, 5 adapters of rank 64, 4096 -> 4096, fp16: down 14, up 10.5, outer 26 (the same
-// chains: 1024 values instead of 4096 take down 13.4 us).
+// chains: 1024 values instead of 4096 take down 13.4 us). Gradients of 2 rows of rank 4, 4096 -> 4096: six launches of 2.5 to 5 us each.
 //
 // Rows of different adapters may lie in any order. A tile of 16 rows multiplies all of them by each adapter
 // that occurs in it and keeps the rows that are its own by selection, not by adding zeros, so that an
@@ -517,7 +517,9 @@ __global__ __launch_bounds__(kThreads) void up_kernel(const UpParams p) {
   }
 }
 
-// Few rows: 16 by 64 columns; the waves split the tile's adapters, and the first two store.
+// Few rows: 16 by 64 columns; the waves split the tile's adapters, and the first two store. (Ranks from 65 on that are no multiple of 8 take
+// 1.3 KB of scratch memory a lane for the numbers that they read one at a time: 100 rows of 4 adapters, 4096 -> 4096, rank 100 in 100 us, rank
+// 104 in 14.)
 template <typename T, int ST, Form FORM>
 __global__ __launch_bounds__(64 * kFewWaves) void up_few_kernel(const UpParams p) {
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
@@ -595,6 +597,8 @@ __device__ inline void store_ranks(T *out, float *sums, f32x4 x, int count) {
     }
 }
 
+// (fp16's sums of a tile beside those of all rows fill the registers of one wave a SIMD from rank 33 on, bf16's own from 65; fp16's from 65 on
+// keep 97 of them in scratch memory: 1037 rows of 5 adapters, 4096 -> 4096, the whole gradient at rank 64 56 us, bf16 44, at 128 114 and 83.)
 // One adapter, 128 columns, a part of the adapter's rows; the waves take 32 of them in turn,
 // each through a tile of its own in LDS, from where the transposing reads make the operand whose inner dimension is
 // the rows. v's operand is loaded in place (a lane's 8 rows).
@@ -1120,7 +1124,7 @@ hipError_t forward(const DanAdaptArgs &a, hipStream_t s) {
 // The workspace of the gradient: A^T, B^T, the list of rows, g in parts and added up, and the parts of dA and dB.
 struct GradSpace {
   int64_t at, bt, list, starts, part, g, da, db, total;
-  int splits, parts, parts_a, parts_b;  // (parts_a, parts_b: where g and dB come from one pass)
+  int splits, parts, parts_a, parts_b;  // (parts_a, parts_b: where g and dB come from one pass, which fp16's size holds, too: it is asked for without a type)
   GradSpace(int rows, int n_in, int n_out, int rank, int adapters) {
     splits = splits_of(rows, n_out, rank, adapters);
     parts = parts_of(rows, n_in, n_out, adapters);

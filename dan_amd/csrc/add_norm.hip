@@ -11,8 +11,9 @@
 // gradient reads s as it was stored (rounded to 16 bits): the two addends would be one tensor more to read,
 // and what the rounding moves is of the size of the result's own.
 //
-// Measured, warm: 8192 x 4096 in bf16 to stream and codes 38 us (235 MB, 6.1 TB/s), 7 x 4096 3.9 us (a launch, its loads, two
-// reductions); 4099 x 2048 in fp16 to stream and out 13.0 us (67 MB, 5.2 TB/s), its gradient 14.8 (67 MB, 4.5) and dw's sum 6.8.
+// Measured, warm: 8192 x 4096 in bf16 to stream and codes 38 us (235 MB, 6.1 TB/s), to tiled codes 43, 7 x 4096 3.9 us (a launch, its
+// loads, two reductions; tiled 4.0); 4096 x 14336 to stream and out 149 us (470 MB, 3.2 TB/s: above 8192 columns a row's values fill the
+// registers of one wave a SIMD, as they do in the gradient); 4099 x 2048 in fp16 to stream and out 13.0 us (67 MB, 5.2 TB/s), its gradient 14.8 (67 MB, 4.5) and dw's sum 6.8.
 #include <hip/hip_runtime.h>
 
 #include <math.h>

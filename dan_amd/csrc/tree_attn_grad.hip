@@ -12,22 +12,26 @@
 //                        that share a kv head and walks the keys that they see;
 //   grad_sum_kernel      where few keys made several work groups share them by heads,
 //                        adds those parts up;
-// Each result is summed by one work group in a fixed order, so there are no atomics
+// Each result, or part of one, is summed by one work group in a fixed order, and parts are
+// added up in order, so there are no atomics
 // and the results do not change from run to run. The price is that S and dP are
 // computed twice: 7 products where 5 would do (dQ summed by atomics, or written and
 // read again in fp32 for every run of keys, would cost 8192 rows of 32 heads x 128
-// that see 7700 keys 134 MB for each run of them).
+// that see 7700 keys 134 MB for each run of them). Parts of dK and dV cost their
+// bytes twice, in fp32 (2 D numbers a row, kv head and part): 2000 rows of 2 kv heads
+// x 128 in 4 parts 16 MB, written and read again.
 //
 // Measured: 8192 rows in one request of 32 branches, 32/8 heads x 128, bf16: rows 28 us
 // (134 MB, 4.8 TB/s), keys and queries 1.7 ms (1917 GFLOP, 1130 TFLOP/s; in launches of
 // their own 0.94 and 0.73), where a library's product of 16384^3 reaches 1370. The matrix unit is
 // busy 57 % (keys) and 52 % (queries) of the time at about 1.95 GHz, which the power
 // holds; what it waits for is the chain from S over its exponentials to dS in each wave,
-// of which one fits a SIMD (its registers are full). With head_dim 256 every operand read
+// of which one fits a SIMD (its registers are full; what is needed once in front of or behind a loop,
+// 18 to 54 of them, is kept in scratch memory at head_dim 128 and 256, but for bf16's larger unit of 256). With head_dim 256 every operand read
 // feeds one product instead of two, and LDS is as busy as the matrix unit: 4099 rows
-// behind 1024 keys, 16/2 heads x 256: 244 us. Batches of a few thousand rows have one to
+// behind 1024 keys, 16/2 heads x 256: 241 us. Batches of a few thousand rows have one to
 // four units a compute unit, and each loads, joins and stores by itself (10 us of its 50 to 100):
-// 3413 rows in four requests, 32/8 x 128, fp16: 181 us.
+// 3413 rows in four requests, 32/8 x 128, fp16: 180 us.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
