@@ -191,7 +191,10 @@ def attend_train(q, k, v, segments, layer, scale=None):
     prefix table, where the batch has more than 8 entries, some are copied, or the
     first call had none of the layer's), so it is refused in the capture of a HIP graph; later ones can be captured, forward and backward in the same
     capture and with no earlier, eager result alive that holds the graph of the
-    same leaves (where q, k or v is such a leaf itself, that raises)."""
+    same leaves (where q, k or v is such a leaf itself, that raises). Under
+    ``torch.compile`` the call is left to eager execution."""
+    if torch.compiler.is_compiling():
+        return torch.compiler.disable(attend_train)(q, k, v, segments, layer, scale)
     from . import _grad
 
     if torch.is_grad_enabled() and any(x.requires_grad for s in segments if s.past for x in s.past.get(layer, ()) if isinstance(x, torch.Tensor)):

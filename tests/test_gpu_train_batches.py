@@ -379,3 +379,23 @@ def test_a_captured_step_keeps_its_entries(gpu):
         assert same(got, want)
     segs[0].past[0] = kept
     assert same(train(*x, segs), want)
+
+
+@pytest.mark.parametrize("needs", [True, False])
+def test_compiled_over_gaps_and_replaced_entries(gpu, needs):
+    """torch.compile leaves the call to eager execution, with everything that it looks at on the host."""
+    say("attend_train under torch.compile, eager backend", needs)
+    segs, n = batch(gpu, LENGTHS, [{0: entry(gpu, 1, 12)}, None, {0: entry(gpu, 2, 12)}])
+    g = torch.Generator().manual_seed(3)
+    x = [torch.randn(h, n + 5, 64, generator=g).to(BF16).to(gpu) for h in (4, 2, 2, 4)]
+    torch._dynamo.reset()
+    f = torch.compile(lambda q, k, v: attend_train(q * 1, k * 1, v * 1, segs, 0) * 1, backend="eager")
+    for seed in (1, 1, 7, 8):  # (the first call makes the batch's tables)
+        segs[0].past[0] = entry(gpu, seed, 12)
+        want = train(*x, Batch(segs))
+        poison(want[0])
+        leaves = [t.detach().requires_grad_(needs) for t in x[:3]]
+        out = f(*leaves)
+        assert torch.equal(out, want[0]) and (out[:, n:] == 0).all()
+        if needs:
+            assert same(torch.autograd.grad(out, leaves, x[3]), want[1:])
