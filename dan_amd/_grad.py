@@ -180,17 +180,26 @@ def tables(segments, plan, h, hkv, d, num_cus):
     return plan.grad_tables[h, hkv, d]
 
 
-def capturable(plan, layer, layout):
-    """Whether a first call of ``layer`` and a head layout (heads, kv heads, head_dim) finds every table on the device. What a capture
-    uploads or copies is there only once the graph has run: tables kept from it would be read before."""
+BEFORE_CAPTURE = "attend_train: run the batch once before a capture (its tables are uploaded then)"
+
+
+def planned(plan, layer):
+    """Whether a first call of ``layer`` finds the forward pass's tables on the device. What a capture uploads or copies is there only
+    once the graph has run: tables kept from it would be read before."""
     from . import attention as A
 
-    if plan is None or layout not in plan.grad_tables:
+    if plan is None:
         return False
     if layer in plan.past_tables:
         return plan.past_hosts[layer] is not None or layer in plan.past_uploaded
-    return (len(plan.past_dicts) <= _native.INLINE_PASTS and (not plan.past_dicts or layer in plan.spare)
-            and all(A._in_place(x) for entry in plan.past_dicts for x in entry[layer][:2]))
+    return len(plan.past_dicts) <= _native.INLINE_PASTS and all(A._in_place(x) for entry in plan.past_dicts for x in entry[layer][:2])
+
+
+def capturable(plan, layer, layout):
+    """Whether a first training call of ``layer`` and a head layout (heads, kv heads, head_dim) does, and finds the backward pass's, and a
+    prefix table that shares no memory with the graph's other calls."""
+    return (planned(plan, layer) and layout in plan.grad_tables
+            and (not plan.past_dicts or layer in plan.past_tables or layer in plan.spare))
 
 
 def attend(q, k, v, segments, layer, scale):
@@ -204,7 +213,7 @@ def attend(q, k, v, segments, layer, scale):
     made = None if plan is None else plan.train_calls.get(key)
     if made is None:
         if q.is_cuda and torch.cuda.is_current_stream_capturing() and not capturable(plan, layer, (q.shape[0], k.shape[0], q.shape[-1])):
-            raise RuntimeError("attend_train: run the batch once before a capture (its tables are uploaded then)")
+            raise RuntimeError(BEFORE_CAPTURE)
         with torch.no_grad():
             plan_args = A._call_args(q, k, v, segments, layer, scale, None, _native.PHASES_ALL, False, upload=False)
         made, plan = templates(segments, q, k, v, layer, scale, plan_args), plan_args[2]

@@ -211,8 +211,12 @@ def attend_train(q, k, v, segments, layer, scale=None):
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         plan = getattr(segments, "tile_plan", None)
         if plan is not None and _replaced(segments, plan, layer, saves=True):
-            segments = list(segments)
-        elif plan is not None and plan.device == q.device:
+            segments, plan = list(segments), None
+        if plan is not None and (plan.device != q.device or plan.num_tokens != q.shape[1]):
+            plan = None
+        if q.is_cuda and torch.cuda.is_current_stream_capturing() and not _grad.planned(plan, layer):
+            raise RuntimeError(_grad.BEFORE_CAPTURE)
+        if plan is not None:
             plan.order(q.device)
         out = attend(q, k, v, segments, layer, scale)
         for a, b in _uncovered(segments, out.shape[1]):

@@ -229,14 +229,15 @@ def test_a_batch_dropped_before_another_stream_has_read_it(gpu, big, needs, way)
 # ---------------------------------------------------------------- captures
 @ways
 @pytest.mark.parametrize("kept", [True, False])
-def test_a_refused_capture_leaves_nothing_behind(gpu, kept, way):  # noqa: F811
+@pytest.mark.parametrize("needs", [True, False])
+def test_a_refused_capture_leaves_nothing_behind(gpu, needs, kept, way):  # noqa: F811
     """A batch whose very first call is in a capture: refused before a table is made, since one made there would be kept on the batch
     and never filled. What the message asks for then works."""
-    say("attend_train: first call of a new batch in a capture", kept, way)
+    say("attend_train: first call of a new batch in a capture", needs, kept, way)
     x, make = many(gpu, 6, 3)
     want = train(*x, make())
     segs = make() if kept else list(make())
-    leaves = [t.detach().requires_grad_() for t in x[:3]]
+    leaves = [t.detach().requires_grad_(needs) for t in x[:3]]
     torch.cuda.synchronize()
     with pytest.raises(RuntimeError, match="before a capture"):
         with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
@@ -353,6 +354,36 @@ def test_a_batch_changed_before_another_layers_first_call(gpu, change):
     for layer in (1, 0):
         want = train(*x, Batch(segs), layer)
         assert same(train(*x, segs, layer), want) and torch.equal(attend_train(*x[:3], segs, layer), want[0])
+
+
+def test_captured_without_a_gradient(gpu):
+    """Behind attend's plan, rows of no segment among the others; a second layer of the same batch."""
+    say("attend_train, captured without a gradient")
+    segs, n = batch(gpu, LENGTHS, [{i: entry(gpu, 1 + i, 12) for i in range(2)}, None, None])
+    g = torch.Generator().manual_seed(3)
+    x = [torch.randn(h, n + 7, 64, generator=g).to(BF16).to(gpu) for h in (4, 2, 2, 4)]
+    want = [train(*x, Batch(segs), layer)[0] for layer in range(2)]
+    attend(*x[:3], segs, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        got = [attend_train(*x[:3], segs, layer) for layer in range(2)]
+    for _ in range(3):
+        for t in got:
+            t.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(got, want)
+        assert torch.equal(train(*x, segs, 1)[0], want[1])
+    many_x, make = many(gpu, 9)
+    segs = make()
+    attend(*many_x[:3], segs, 0)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="before a capture"):  # (another layer's table would be uploaded)
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
+            attend_train(*many_x[:3], segs, 1)
+    torch.cuda.synchronize()
+    assert torch.equal(attend_train(*many_x[:3], segs, 1), train(*many_x, make(), 1)[0])
 
 
 def test_a_captured_step_keeps_its_entries(gpu):
